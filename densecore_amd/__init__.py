@@ -10,6 +10,8 @@ missing.
 from .configs import (CONFIGS, TYPE_F16, TYPE_F32, TYPE_NAMES, TYPE_Q4_0, TYPE_Q4_K, TYPE_Q5_K,  # noqa: F401
                       TYPE_Q6_K, TYPE_Q8_0, TYPE_Q8_0_RS, TYPE_Q8_K, Config, by_index)
 from ._lib import (GGUF, KV_BLOCK_SIZE, PagedKVCache, kv_attention_workspace_size, kv_slot_bytes,  # noqa: F401
+                   kv_compact_workspace_size, kv_fork_workspace_size, kv_tree_attention_workspace_size,
+                   beam_select, beam_select_workspace_size,
                    DcqError, LIB_PATH, block_size, block_sums_per_row, build, dequantize_rows,  # noqa: F401
                    dot_rows, ffn_gate_up, ffn_gate_up_workspace_size, lib, mul_mat, mul_mat_add,
                    mul_mat_add_workspace_size, mul_mat_ex, mul_mat_noalloc, NOALLOC_SCRATCH_BYTES, probe_stream_read,
@@ -27,4 +29,6 @@ __all__ = [
     "PATH_GEMV", "PATH_MMQ", "TYPE_F32", "TYPE_F16", "TYPE_Q4_0", "TYPE_Q8_0", "TYPE_Q4_K", "TYPE_Q5_K",
     "TYPE_Q6_K", "TYPE_Q8_K", "TYPE_Q8_0_RS",
     "TYPE_NAMES", "KV_BLOCK_SIZE", "PagedKVCache", "kv_slot_bytes", "kv_attention_workspace_size",
+    "kv_tree_attention_workspace_size", "kv_fork_workspace_size", "kv_compact_workspace_size", "beam_select",
+    "beam_select_workspace_size",
 ]

@@ -19,6 +19,9 @@ SYMBOLS = [
     "dcq_gguf_open", "dcq_gguf_close", "dcq_gguf_tensor_count", "dcq_gguf_find_tensor", "dcq_gguf_tensor_info",
     "dcq_gguf_get_int", "dcq_gguf_get_str", "dcq_gguf_load_tensor",
     "dcq_kv_slot_bytes", "dcq_kv_write", "dcq_kv_gather", "dcq_kv_attention_workspace_size", "dcq_kv_attention",
+    "dcq_kv_tree_attention_workspace_size", "dcq_kv_tree_attention", "dcq_kv_write_path",
+    "dcq_kv_fork_workspace_size", "dcq_kv_fork", "dcq_kv_compact_workspace_size", "dcq_kv_compact",
+    "dcq_beam_select_workspace_size", "dcq_beam_select",
     "dcq_probe_stream_read",  # include/dcq_probe.h: measurement aid
 ]
 
@@ -92,6 +95,18 @@ def lib():
             "dcq_kv_attention_workspace_size": (sz, [i32, i32, i32, i64, i64]),
             "dcq_kv_attention": (i32, [i32, vp, vp, i64, i32, i32, vp, i64, i32, i32, i32, vp, sz, vp, vp, sz,
                                        i64, i64, ctypes.c_float, vp, sz, vp, sz, vp]),
+            "dcq_kv_tree_attention_workspace_size": (sz, [i32, i32, i32, i64, i64, i64]),
+            "dcq_kv_tree_attention": (i32, [i32, vp, vp, i64, i32, i32, vp, i64, i64, vp, i64, vp, vp, i32, i32, i32,
+                                            vp, sz, vp, vp, sz, i64, i64, ctypes.c_float, vp, sz, vp, sz, vp]),
+            "dcq_kv_write_path": (i32, [i32, vp, vp, i64, i32, i64, vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, sz, sz,
+                                        i64, i64, vp]),
+            "dcq_kv_fork_workspace_size": (sz, [i64, i64, i64]),
+            "dcq_kv_fork": (i32, [i32, vp, vp, i64, i32, i64, vp, i64, i64, vp, i64, vp, i64, vp, vp, i64, vp, vp, vp,
+                                  vp, sz, vp]),
+            "dcq_kv_compact_workspace_size": (sz, [i64]),
+            "dcq_kv_compact": (i32, [i32, vp, vp, i64, i32, i64, vp, i64, i64, vp, i64, vp, vp, i64, vp, vp, vp, sz, vp]),
+            "dcq_beam_select_workspace_size": (sz, [i64, i32, i64, i32]),
+            "dcq_beam_select": (i32, [i32, vp, sz, i64, i32, i64, vp, i32, vp, vp, vp, vp, sz, vp]),
             "dcq_probe_stream_read": (i32, [vp, sz, i32, i32, vp, vp]),
         }
         for name, (res, args) in sig.items():
@@ -147,12 +162,12 @@ def mul_mat_workspace_size(wt, m, k):
 # below take one fast path of plain attribute reads and leave every message to the slow one, tensors
 # pass as integer addresses, and nothing calls into the library that is not the call itself
 # (dcq_mul_mat with preallocated tensors: 10.2 -> 6.4 us a call, 3.5 of them the library's and HIP's).
-_torch = _raw_stream = _F32 = _U8 = None
+_torch = _raw_stream = _F32 = _U8 = _I32 = None
 
 
 def _t():
     """torch, imported at first use (the metadata calls work without it)."""
-    global _torch, _raw_stream, _F32, _U8
+    global _torch, _raw_stream, _F32, _U8, _I32
     if _torch is None:
         import torch
         get_stream, get_device = (getattr(torch._C, n, None) for n in ("_cuda_getCurrentRawStream", "_cuda_getDevice"))
@@ -160,7 +175,7 @@ def _t():
             _raw_stream = lambda: get_stream(get_device())  # noqa: E731
         else:
             _raw_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
-        _F32, _U8, _torch = torch.float32, torch.uint8, torch
+        _F32, _U8, _I32, _torch = torch.float32, torch.uint8, torch.int32, torch
     return _torch
 
 
@@ -222,6 +237,31 @@ def _u8(name, t, ndim=(1, 2)):
     except (AttributeError, IndexError):
         pass
     _need(name, t, _t().uint8, ndim)
+
+
+def _i32(name, t, ndim=(1,)):
+    try:
+        if t.dtype is _I32 and t.is_cuda and t.dim() in ndim and t.stride(-1) == 1:
+            return
+    except (AttributeError, IndexError):
+        pass
+    _need(name, t, _t().int32, ndim)
+
+
+def _shape(name, t, shape):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _packed(name, t, shape):
+    _shape(name, t, shape)
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+
+
+def _row_stride(t):
+    """Elements between the rows of a 2-D tensor (its width where there is one row, whose stride means nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def quantize_rows(vdt, x, out=None, stream=None):
@@ -552,9 +592,197 @@ class PagedKVCache:
             out.stride(0) * 4, _ptr(workspace), ws_bytes, _stream(stream)))
         return out
 
+    # ---- search: several sequences per call, their block tables int32 [S, T] (rows may be strided)
+    def _arenas(self):
+        nbytes = self.n_blocks * self.n_layer * KV_BLOCK_SIZE * self.slot_bytes
+        if self.k.numel() < nbytes or self.v.numel() < nbytes:
+            raise ValueError(f"arenas of {self.k.numel()} and {self.v.numel()} bytes, {self.n_blocks} blocks need {nbytes}")
+        return _ptr(self.k), _ptr(self.v)
+
+    def tree_attention(self, layer, tables, past, max_past, q, k_cur, v_cur, scale, mask=None, n_draft=None, out=None,
+                       workspace=None, stream=None):
+        """Attention of the drafted tokens of S sequences, N rows each: q [S * N, n_head * head_dim], k_cur / v_cur
+        [S * N, row_elems] fp32 -> out like q. past int32 [S] cached positions (max_past: no fewer than any),
+        mask int64 [S, N, (N + 63) // 64], bit i of row j set where token j sees drafted token i (None: i <= j),
+        n_draft int32 [S] drafted tokens of the N (None: all). Rows that see nothing, or past n_draft, are zeros."""
+        torch = _torch or _t()
+        for name, t in (("q", q), ("k_cur", k_cur), ("v_cur", v_cur)):
+            _f32(name, t)
+        _i32("tables", tables, (2,))
+        _i32("past", past)
+        s, rows = tables.shape[0], q.shape[0]
+        n = rows // s if s else 0
+        if s == 0 or n == 0 or rows != s * n:
+            raise ValueError(f"q: {rows} rows of {s} sequences")
+        if q.shape[1] % self.head_dim:
+            raise ValueError(f"q: {q.shape[1]} values per row are no heads of {self.head_dim}")
+        n_head = q.shape[1] // self.head_dim
+        _shape("k_cur", k_cur, (rows, self.row_elems))
+        _shape("v_cur", v_cur, (rows, self.row_elems))
+        if _row_stride(k_cur) != _row_stride(v_cur):
+            raise ValueError(f"k_cur and v_cur must share a row stride (the ABI takes one): "
+                             f"{k_cur.stride(0)} != {v_cur.stride(0)}")
+        _packed("past", past, (s,))
+        if mask is not None:
+            _need("mask", mask, torch.int64, (3,))
+            _packed("mask", mask, (s, n, (n + 63) // 64))
+        if n_draft is not None:
+            _i32("n_draft", n_draft)
+            _packed("n_draft", n_draft, (s,))
+        if out is None:
+            out = torch.empty((rows, q.shape[1]), dtype=torch.float32, device=q.device)
+        _f32("out", out)
+        _shape("out", out, q.shape)
+        if workspace is None:
+            need = kv_tree_attention_workspace_size(n_head, self.n_head_kv, self.head_dim, s, n, max_past)
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        k, v = self._arenas()
+        _check("dcq_kv_tree_attention", lib().dcq_kv_tree_attention(
+            self.cache_type, k, v, self.n_blocks, self.n_layer, layer, _ptr(tables), _row_stride(tables),
+            tables.shape[1], _ptr(past), max_past, _ptr(n_draft), _ptr(mask), n_head, self.n_head_kv, self.head_dim,
+            _ptr(q), _row_stride(q) * 4, _ptr(k_cur), _ptr(v_cur), _row_stride(k_cur) * 4, s, n, scale, _ptr(out),
+            _row_stride(out) * 4, _ptr(workspace), _nbytes(workspace), _stream(stream)))
+        return out
+
+    def write_path(self, tables, past, path, n_path, k_cur, v_cur, stream=None):
+        """The accepted tokens' rows into the cache, every layer: place j < n_path[b] (int32 [S]; None: all P) of
+        path int32 [S, P] names a drafted token, whose rows of k_cur / v_cur [n_layer, S * N, row_elems] go to
+        position past[b] + j of sequence b."""
+        for name, t in (("k_cur", k_cur), ("v_cur", v_cur)):
+            _f32(name, t, (3,))
+        _i32("tables", tables, (2,))
+        _i32("past", past)
+        _i32("path", path, (2,))
+        s, rows = tables.shape[0], k_cur.shape[1]
+        n = rows // s if s else 0
+        if s == 0 or n == 0 or rows != s * n:
+            raise ValueError(f"k_cur: {rows} rows of {s} sequences")
+        _shape("k_cur", k_cur, (self.n_layer, rows, self.row_elems))
+        _shape("v_cur", v_cur, k_cur.shape)
+        strides = [(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if rows > 1 else self.row_elems)
+                   for t in (k_cur, v_cur)]
+        if strides[0] != strides[1]:
+            raise ValueError(f"k_cur and v_cur must share their strides (the ABI takes one): {strides[0]} != {strides[1]}")
+        _packed("past", past, (s,))
+        _shape("path", path, (s, path.shape[1]))
+        if n_path is not None:
+            _i32("n_path", n_path)
+            _packed("n_path", n_path, (s,))
+        k, v = self._arenas()
+        _check("dcq_kv_write_path", lib().dcq_kv_write_path(
+            self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, _ptr(tables), _row_stride(tables),
+            tables.shape[1], _ptr(past), _ptr(path), _row_stride(path), path.shape[1], _ptr(n_path), _ptr(k_cur),
+            _ptr(v_cur), strides[0][0] * 4, strides[0][1] * 4, s, n, _stream(stream)))
+
+    def fork(self, tables, lengths, parents, refs, tables_out=None, lengths_out=None, refs_out=None, missing=None,
+             workspace=None, stream=None):
+        """The C sequences that continue sequences parents int32 [C] of the S in tables / lengths: shared pages, a
+        copy of a partial last page where two would write into it. refs int32 [n_blocks] counts each page's
+        holders. Returns (tables [C, T], lengths [C], refs, missing [1]: the copies that found no free page)."""
+        torch = _torch or _t()
+        _i32("tables", tables, (2,))
+        for name, t in (("lengths", lengths), ("parents", parents), ("refs", refs)):
+            _i32(name, t)
+        (s, width), c = tables.shape, parents.shape[0]
+        _packed("lengths", lengths, (s,))
+        _packed("parents", parents, (c,))
+        _packed("refs", refs, (self.n_blocks,))
+        made = []
+        for name, t, shape in (("tables_out", tables_out, (c, width)), ("lengths_out", lengths_out, (c,)),
+                               ("refs_out", refs_out, (self.n_blocks,)), ("missing", missing, (1,))):
+            if t is None:
+                t = torch.empty(shape, dtype=torch.int32, device=tables.device)
+            _i32(name, t, (len(shape),))
+            (_shape if len(shape) == 2 else _packed)(name, t, shape)
+            made.append(t)
+        if workspace is None:
+            workspace = torch.empty(max(kv_fork_workspace_size(self.n_blocks, s, c), 256), dtype=torch.uint8,
+                                    device=tables.device)
+        k, v = self._arenas()
+        _check("dcq_kv_fork", lib().dcq_kv_fork(
+            self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, _ptr(tables), _row_stride(tables),
+            width, _ptr(lengths), s, _ptr(parents), c, _ptr(refs), _ptr(made[0]), _row_stride(made[0]), _ptr(made[1]),
+            _ptr(made[2]), _ptr(made[3]), _ptr(workspace), _nbytes(workspace), _stream(stream)))
+        return tuple(made)
+
+    def compact(self, tables, lengths, refs, tables_out=None, refs_out=None, n_live=None, workspace=None, stream=None):
+        """The pages in use (refs > 0) to the front of the arenas. Returns (tables [S, T] with the moved pages'
+        new numbers, refs in their new places, n_live [1])."""
+        torch = _torch or _t()
+        _i32("tables", tables, (2,))
+        for name, t in (("lengths", lengths), ("refs", refs)):
+            _i32(name, t)
+        s, width = tables.shape
+        _packed("lengths", lengths, (s,))
+        _packed("refs", refs, (self.n_blocks,))
+        made = []
+        for name, t, shape in (("tables_out", tables_out, (s, width)), ("refs_out", refs_out, (self.n_blocks,)),
+                               ("n_live", n_live, (1,))):
+            if t is None:
+                t = torch.empty(shape, dtype=torch.int32, device=tables.device)
+            _i32(name, t, (len(shape),))
+            (_shape if len(shape) == 2 else _packed)(name, t, shape)
+            made.append(t)
+        if workspace is None:
+            workspace = torch.empty(max(kv_compact_workspace_size(self.n_blocks), 256), dtype=torch.uint8,
+                                    device=tables.device)
+        k, v = self._arenas()
+        _check("dcq_kv_compact", lib().dcq_kv_compact(
+            self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, _ptr(tables), _row_stride(tables),
+            width, _ptr(lengths), s, _ptr(refs), _ptr(made[0]), _row_stride(made[0]), _ptr(made[1]), _ptr(made[2]),
+            _ptr(workspace), _nbytes(workspace), _stream(stream)))
+        return tuple(made)
+
 
 def kv_attention_workspace_size(n_head, n_head_kv, head_dim, n_tokens, n_past):
     return int(lib().dcq_kv_attention_workspace_size(n_head, n_head_kv, head_dim, n_tokens, n_past))
+
+
+def kv_tree_attention_workspace_size(n_head, n_head_kv, head_dim, n_seqs, n_tokens, max_past):
+    return int(lib().dcq_kv_tree_attention_workspace_size(n_head, n_head_kv, head_dim, n_seqs, n_tokens, max_past))
+
+
+def kv_fork_workspace_size(n_blocks, n_seqs, n_children):
+    return int(lib().dcq_kv_fork_workspace_size(n_blocks, n_seqs, n_children))
+
+
+def kv_compact_workspace_size(n_blocks):
+    return int(lib().dcq_kv_compact_workspace_size(n_blocks))
+
+
+# ---------------------------------------------------------------- beam search's selection
+def beam_select_workspace_size(n_batch, n_beams, vocab, n_out):
+    return int(lib().dcq_beam_select_workspace_size(n_batch, n_beams, vocab, n_out))
+
+
+def beam_select(logits, beam_scores, n_out, scores=None, parents=None, tokens=None, workspace=None, stream=None):
+    """The n_out best continuations of each request: logits fp32 or fp16 [B * W, V], beam_scores fp32 [B, W] ->
+    (scores fp32, parents int32: rows b * W + w, tokens int32), each [B, n_out], best first, ties to the lower
+    beam, then token; -inf, -1, -1 where there are no more."""
+    torch = _torch or _t()
+    half = getattr(logits, "dtype", None) is torch.float16
+    _need("logits", logits, torch.float16 if half else torch.float32, (2,))
+    _f32("beam_scores", beam_scores)
+    b, w = beam_scores.shape
+    _packed("beam_scores", beam_scores, (b, w))
+    vocab = logits.shape[1]
+    _shape("logits", logits, (b * w, vocab))
+    made = []
+    for name, t, dtype in (("scores", scores, torch.float32), ("parents", parents, torch.int32),
+                           ("tokens", tokens, torch.int32)):
+        if t is None:
+            t = torch.empty((b, n_out), dtype=dtype, device=logits.device)
+        _need(name, t, dtype, (2,))
+        _packed(name, t, (b, n_out))
+        made.append(t)
+    if workspace is None:
+        workspace = torch.empty(max(beam_select_workspace_size(b, w, vocab, n_out), 256), dtype=torch.uint8,
+                                device=logits.device)
+    _check("dcq_beam_select", lib().dcq_beam_select(
+        1 if half else 0, _ptr(logits), _row_stride(logits) * (2 if half else 4), b, w, vocab, _ptr(beam_scores), n_out,
+        _ptr(made[0]), _ptr(made[1]), _ptr(made[2]), _ptr(workspace), _nbytes(workspace), _stream(stream)))
+    return tuple(made)
 
 
 # ---------------------------------------------------------------- measurement aid (include/dcq_probe.h)

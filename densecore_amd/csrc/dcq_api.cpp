@@ -13,6 +13,7 @@
 #include "../../include/dcq.h"
 #include "dcq_common.h"
 #include "dcq_kernels.h"
+#include "dcq_search.h"
 
 namespace dcq {
 
@@ -176,6 +177,30 @@ int validate_arena(int ct, const void* arena, int64_t n_blocks, int n_layer, int
     if (row_elems <= 0 || row_elems % 32 || row_elems > ((int64_t)1 << 24)) return DCQ_ERR_BAD_SHAPE;
     if (!aligned(arena, 16)) return DCQ_ERR_MISALIGNED;
     return DCQ_OK;
+}
+
+// Whether the byte ranges [a, a + an) and [b, b + bn) meet.
+bool overlap(const void* a, int64_t an, const void* b, int64_t bn) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return an > 0 && bn > 0 && x < y + (uintptr_t)bn && y < x + (uintptr_t)an;
+}
+
+// int32 rows [n][width], `stride` entries apart: their extent in bytes.
+int64_t rows_bytes(int64_t n, int64_t stride, int64_t width) { return n > 0 ? ((n - 1) * stride + width) * 4 : 0; }
+
+// Block tables of several sequences.
+int validate_tables(const int32_t* tables, int64_t table_stride, int64_t n_table, int64_t n_seqs) {
+    if (n_seqs <= 0 || n_seqs > 65535 || n_table < 0 || n_table > ((int64_t)1 << 24)) return DCQ_ERR_BAD_SHAPE;
+    if (n_table > 0 && !tables) return DCQ_ERR_INVALID_ARG;
+    if (n_table > 0 && n_seqs > 1 && (table_stride < n_table || table_stride > INT32_MAX)) return DCQ_ERR_INVALID_ARG;
+    return aligned(tables, 4) ? DCQ_OK : DCQ_ERR_MISALIGNED;
+}
+
+// A workspace of `need` bytes.
+int validate_workspace(const void* workspace, size_t workspace_bytes, size_t need) {
+    if (!need) return DCQ_OK;
+    if (!workspace || workspace_bytes < need) return DCQ_ERR_WORKSPACE;
+    return aligned(workspace, 256) ? DCQ_OK : DCQ_ERR_MISALIGNED;
 }
 
 }  // namespace
@@ -693,6 +718,222 @@ int dcq_kv_attention(int cache_type, const void* k_arena, const void* v_arena, i
         block_table, nt, n_head, n_head_kv, head_dim, q, (int64_t)(q_stride_bytes / 4), k_cur, v_cur,
         (int64_t)(kv_stride_bytes / 4), (int)n_tokens, (int)n_past, scale, out, (int64_t)(out_stride_bytes / 4),
         workspace, workspace_bytes, (hipStream_t)stream));
+}
+
+static int validate_tree_shape(int n_head, int n_head_kv, int head_dim, int64_t n_seqs, int64_t n_tokens,
+                               int64_t max_past) {
+    const int rc = validate_attention_shape(n_head, n_head_kv, head_dim, n_tokens, max_past);
+    if (rc) return rc;
+    // rows whose merge fits a grid
+    if (n_tokens > 1024 || n_seqs <= 0 || n_seqs > 65535 || n_seqs * n_tokens * n_head > ((int64_t)1 << 27))
+        return DCQ_ERR_BAD_SHAPE;
+    return DCQ_OK;
+}
+
+size_t dcq_kv_tree_attention_workspace_size(int n_head, int n_head_kv, int head_dim, int64_t n_seqs,
+                                            int64_t n_tokens, int64_t max_past) {
+    if (validate_tree_shape(n_head, n_head_kv, head_dim, n_seqs, n_tokens, max_past)) return 0;
+    return tree_workspace_bytes(head_dim, n_head, n_head_kv, (int)n_seqs, (int)n_tokens, (int)max_past);
+}
+
+int dcq_kv_tree_attention(int cache_type, const void* k_arena, const void* v_arena, int64_t n_blocks, int n_layer,
+                          int layer, const int32_t* tables, int64_t table_stride, int64_t n_table,
+                          const int32_t* past, int64_t max_past, const int32_t* n_draft, const uint64_t* mask,
+                          int n_head, int n_head_kv, int head_dim, const float* q, size_t q_stride_bytes,
+                          const float* k_cur, const float* v_cur, size_t kv_stride_bytes, int64_t n_seqs,
+                          int64_t n_tokens, float scale, float* out, size_t out_stride_bytes, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+    const int64_t row_elems = (int64_t)n_head_kv * head_dim;
+    int rc = validate_tree_shape(n_head, n_head_kv, head_dim, n_seqs, n_tokens, max_past);
+    if (rc) return rc;
+    if ((rc = validate_arena(cache_type, k_arena, n_blocks, n_layer, layer, row_elems))) return rc;
+    if ((rc = validate_arena(cache_type, v_arena, n_blocks, n_layer, layer, row_elems))) return rc;
+    if ((rc = validate_tables(tables, table_stride, n_table, n_seqs))) return rc;
+    if (!past || !q || !k_cur || !v_cur || !out) return DCQ_ERR_INVALID_ARG;
+    if (!(scale == scale) || scale == INFINITY || scale == -INFINITY) return DCQ_ERR_INVALID_ARG;
+    const size_t q_row = (size_t)n_head * head_dim * 4, kv_row = (size_t)row_elems * 4;
+    if (q_stride_bytes < q_row || kv_stride_bytes < kv_row || out_stride_bytes < q_row) return DCQ_ERR_INVALID_ARG;
+    if (q_stride_bytes > INT32_MAX || kv_stride_bytes > ((size_t)1 << 27) || out_stride_bytes > INT32_MAX)
+        return DCQ_ERR_INVALID_ARG;
+    if (!aligned(q, 16) || !aligned(k_cur, 16) || !aligned(v_cur, 16) || !aligned(out, 4) || !aligned(past, 4) ||
+        !aligned(n_draft, 4) || !aligned(mask, 8))
+        return DCQ_ERR_MISALIGNED;
+    if (q_stride_bytes % 16 || kv_stride_bytes % 16 || out_stride_bytes % 4) return DCQ_ERR_MISALIGNED;
+    const int64_t rows = n_seqs * n_tokens;
+    const int64_t out_bytes = (rows - 1) * (int64_t)out_stride_bytes + (int64_t)q_row;
+    const int64_t kv_bytes = (rows - 1) * (int64_t)kv_stride_bytes + (int64_t)kv_row;
+    if (overlap(out, out_bytes, q, (rows - 1) * (int64_t)q_stride_bytes + (int64_t)q_row) ||
+        overlap(out, out_bytes, k_cur, kv_bytes) || overlap(out, out_bytes, v_cur, kv_bytes))
+        return DCQ_ERR_INVALID_ARG;
+    const size_t need = tree_workspace_bytes(head_dim, n_head, n_head_kv, (int)n_seqs, (int)n_tokens, (int)max_past);
+    if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
+    if ((rc = check_device())) return rc;
+    TreeArgs a{};
+    a.k_arena = static_cast<const uint8_t*>(k_arena), a.v_arena = static_cast<const uint8_t*>(v_arena);
+    a.n_blocks = (int)n_blocks, a.n_layer = n_layer, a.layer = layer;
+    a.sb = (int64_t)dcq_kv_slot_bytes(cache_type, row_elems);
+    a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table;
+    a.past = past, a.max_past = (int)max_past, a.n_draft = n_draft;
+    a.mask = mask, a.words = (int)((n_tokens + 63) / 64);
+    a.q = q, a.q_stride = (int64_t)(q_stride_bytes / 4);
+    a.k_cur = k_cur, a.v_cur = v_cur, a.kv_stride = (int64_t)(kv_stride_bytes / 4);
+    a.out = out, a.out_stride = (int64_t)(out_stride_bytes / 4);
+    a.n_seqs = (int)n_seqs, a.n_tokens = (int)n_tokens, a.n_head = n_head, a.n_head_kv = n_head_kv;
+    a.scale_log2e = scale * 1.4426950408889634f;
+    return hip_status(launch_tree_attention(cache_type, head_dim, a, workspace, (hipStream_t)stream));
+}
+
+int dcq_kv_write_path(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer,
+                      int64_t row_elems, const int32_t* tables, int64_t table_stride, int64_t n_table,
+                      const int32_t* past, const int32_t* path, int64_t path_stride, int64_t max_path,
+                      const int32_t* n_path, const float* k_cur, const float* v_cur, size_t layer_stride_bytes,
+                      size_t kv_stride_bytes, int64_t n_seqs, int64_t n_tokens, void* stream) {
+    int rc = validate_arena(cache_type, k_arena, n_blocks, n_layer, 0, row_elems);
+    if (rc) return rc;
+    if ((rc = validate_arena(cache_type, v_arena, n_blocks, n_layer, 0, row_elems))) return rc;
+    if ((rc = validate_tables(tables, table_stride, n_table, n_seqs))) return rc;
+    if (n_layer > 65535 || n_tokens <= 0 || n_tokens > 65535 || max_path < 0 || max_path > 65535 ||
+        n_seqs * max_path > INT32_MAX)
+        return DCQ_ERR_BAD_SHAPE;
+    if (max_path == 0) return DCQ_OK;
+    if (!past || !path || !k_cur || !v_cur) return DCQ_ERR_INVALID_ARG;
+    if (n_seqs > 1 && path_stride < max_path) return DCQ_ERR_INVALID_ARG;
+    if (kv_stride_bytes < (size_t)row_elems * 4) return DCQ_ERR_INVALID_ARG;
+    if (n_layer > 1 && layer_stride_bytes < kv_stride_bytes * (size_t)(n_seqs * n_tokens - 1) + (size_t)row_elems * 4)
+        return DCQ_ERR_INVALID_ARG;
+    if (!aligned(k_cur, 16) || !aligned(v_cur, 16) || kv_stride_bytes % 16 || layer_stride_bytes % 16 ||
+        !aligned(past, 4) || !aligned(path, 4) || !aligned(n_path, 4))
+        return DCQ_ERR_MISALIGNED;
+    if ((rc = check_device())) return rc;
+    PathArgs a{};
+    a.ct = cache_type;
+    a.k_arena = static_cast<uint8_t*>(k_arena), a.v_arena = static_cast<uint8_t*>(v_arena);
+    a.n_blocks = (int)n_blocks, a.n_layer = n_layer, a.row_elems = row_elems;
+    a.sb = (int64_t)dcq_kv_slot_bytes(cache_type, row_elems);
+    a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table;
+    a.past = past, a.path = path, a.path_stride = path_stride, a.n_path = n_path, a.max_path = (int)max_path;
+    a.k_cur = k_cur, a.v_cur = v_cur;
+    a.layer_stride = (int64_t)(layer_stride_bytes / 4), a.kv_stride = (int64_t)(kv_stride_bytes / 4);
+    a.n_seqs = (int)n_seqs, a.n_tokens = (int)n_tokens;
+    return hip_status(launch_path_write(a, (hipStream_t)stream));
+}
+
+// Arguments that forks and compaction share.
+static int validate_pages(int cache_type, const void* k_arena, const void* v_arena, int64_t n_blocks, int n_layer,
+                          int64_t row_elems, const int32_t* tables, int64_t table_stride, int64_t n_table,
+                          const int32_t* lengths, int64_t n_seqs, const int32_t* refs) {
+    int rc = validate_arena(cache_type, k_arena, n_blocks, n_layer, 0, row_elems);
+    if (rc) return rc;
+    if ((rc = validate_arena(cache_type, v_arena, n_blocks, n_layer, 0, row_elems))) return rc;
+    if ((rc = validate_tables(tables, table_stride, n_table, n_seqs))) return rc;
+    if (n_table <= 0 || n_blocks > ((int64_t)1 << 24)) return DCQ_ERR_BAD_SHAPE;
+    if (!lengths || !refs) return DCQ_ERR_INVALID_ARG;
+    return aligned(lengths, 4) && aligned(refs, 4) ? DCQ_OK : DCQ_ERR_MISALIGNED;
+}
+
+size_t dcq_kv_fork_workspace_size(int64_t n_blocks, int64_t n_seqs, int64_t n_children) {
+    if (n_blocks <= 0 || n_seqs <= 0 || n_children <= 0 || n_children > 4096) return 0;
+    return fork_workspace_bytes(n_children);
+}
+
+int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer, int64_t row_elems,
+                const int32_t* tables, int64_t table_stride, int64_t n_table, const int32_t* lengths, int64_t n_seqs,
+                const int32_t* parents, int64_t n_children, const int32_t* refs, int32_t* tables_out,
+                int64_t tables_out_stride, int32_t* lengths_out, int32_t* refs_out, int32_t* missing,
+                void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = validate_pages(cache_type, k_arena, v_arena, n_blocks, n_layer, row_elems, tables, table_stride, n_table,
+                            lengths, n_seqs, refs);
+    if (rc) return rc;
+    if (n_children <= 0 || n_children > 4096) return DCQ_ERR_BAD_SHAPE;
+    if (!parents || !tables_out || !lengths_out || !refs_out || !missing) return DCQ_ERR_INVALID_ARG;
+    if (n_children > 1 && (tables_out_stride < n_table || tables_out_stride > INT32_MAX)) return DCQ_ERR_INVALID_ARG;
+    if (!aligned(parents, 4) || !aligned(tables_out, 4) || !aligned(lengths_out, 4) || !aligned(refs_out, 4) ||
+        !aligned(missing, 4))
+        return DCQ_ERR_MISALIGNED;
+    const struct { const void* p; int64_t n; } in[] = {{tables, rows_bytes(n_seqs, table_stride, n_table)},
+                                                       {lengths, n_seqs * 4}, {parents, n_children * 4},
+                                                       {refs, n_blocks * 4}},
+        out[] = {{tables_out, rows_bytes(n_children, tables_out_stride, n_table)}, {lengths_out, n_children * 4},
+                 {refs_out, n_blocks * 4}, {missing, 4}};
+    for (const auto& o : out)
+        for (const auto& i : in)
+            if (overlap(o.p, o.n, i.p, i.n)) return DCQ_ERR_INVALID_ARG;
+    if ((rc = validate_workspace(workspace, workspace_bytes, fork_workspace_bytes(n_children)))) return rc;
+    if ((rc = check_device())) return rc;
+    ForkArgs a{};
+    a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table, a.lengths = lengths, a.n_seqs = (int)n_seqs;
+    a.parents = parents, a.n_children = (int)n_children, a.refs = refs, a.n_blocks = (int)n_blocks;
+    a.tables_out = tables_out, a.tables_out_stride = tables_out_stride, a.lengths_out = lengths_out;
+    a.refs_out = refs_out, a.missing = missing;
+    const int64_t page = (int64_t)dcq_kv_slot_bytes(cache_type, row_elems) * DCQ_KV_BLOCK_SIZE * n_layer;
+    return hip_status(launch_fork(a, k_arena, v_arena, page, workspace, (hipStream_t)stream));
+}
+
+size_t dcq_kv_compact_workspace_size(int64_t n_blocks) {
+    return n_blocks > 0 && n_blocks <= ((int64_t)1 << 24) ? compact_workspace_bytes(n_blocks) : 0;
+}
+
+int dcq_kv_compact(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer, int64_t row_elems,
+                   const int32_t* tables, int64_t table_stride, int64_t n_table, const int32_t* lengths,
+                   int64_t n_seqs, const int32_t* refs, int32_t* tables_out, int64_t tables_out_stride,
+                   int32_t* refs_out, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = validate_pages(cache_type, k_arena, v_arena, n_blocks, n_layer, row_elems, tables, table_stride, n_table,
+                            lengths, n_seqs, refs);
+    if (rc) return rc;
+    if (!tables_out || !refs_out || !n_live) return DCQ_ERR_INVALID_ARG;
+    if (n_seqs > 1 && (tables_out_stride < n_table || tables_out_stride > INT32_MAX)) return DCQ_ERR_INVALID_ARG;
+    if (!aligned(tables_out, 4) || !aligned(refs_out, 4) || !aligned(n_live, 4)) return DCQ_ERR_MISALIGNED;
+    const struct { const void* p; int64_t n; } in[] = {{tables, rows_bytes(n_seqs, table_stride, n_table)},
+                                                       {lengths, n_seqs * 4}, {refs, n_blocks * 4}},
+        out[] = {{tables_out, rows_bytes(n_seqs, tables_out_stride, n_table)}, {refs_out, n_blocks * 4}, {n_live, 4}};
+    for (const auto& o : out)
+        for (const auto& i : in)
+            if (overlap(o.p, o.n, i.p, i.n)) return DCQ_ERR_INVALID_ARG;
+    if ((rc = validate_workspace(workspace, workspace_bytes, compact_workspace_bytes(n_blocks)))) return rc;
+    if ((rc = check_device())) return rc;
+    CompactArgs a{};
+    a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table, a.lengths = lengths, a.n_seqs = (int)n_seqs;
+    a.refs = refs, a.n_blocks = (int)n_blocks, a.tables_out = tables_out, a.tables_out_stride = tables_out_stride;
+    a.refs_out = refs_out, a.n_live = n_live;
+    const int64_t page = (int64_t)dcq_kv_slot_bytes(cache_type, row_elems) * DCQ_KV_BLOCK_SIZE * n_layer;
+    return hip_status(launch_compact(a, k_arena, v_arena, page, workspace, (hipStream_t)stream));
+}
+
+static int validate_beam_shape(int64_t n_batch, int n_beams, int64_t vocab, int n_out) {
+    if (n_batch <= 0 || n_beams <= 0 || n_beams > kBeamMaxBeams || n_batch > 65535 / n_beams || vocab <= 0 ||
+        vocab > ((int64_t)1 << 24) || n_out <= 0 || n_out > 64)
+        return DCQ_ERR_BAD_SHAPE;
+    return DCQ_OK;
+}
+
+size_t dcq_beam_select_workspace_size(int64_t n_batch, int n_beams, int64_t vocab, int n_out) {
+    if (validate_beam_shape(n_batch, n_beams, vocab, n_out)) return 0;
+    return beam_workspace_bytes(n_batch, n_beams, (int)vocab, n_out);
+}
+
+int dcq_beam_select(int type, const void* logits, size_t stride_bytes, int64_t n_batch, int n_beams, int64_t vocab,
+                    const float* beam_scores, int n_out, float* scores, int32_t* parents, int32_t* tokens,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+    if (type != DCQ_TYPE_F32 && type != DCQ_TYPE_F16) return DCQ_ERR_UNSUPPORTED;
+    int rc = validate_beam_shape(n_batch, n_beams, vocab, n_out);
+    if (rc) return rc;
+    if (!logits || !beam_scores || !scores || !parents || !tokens) return DCQ_ERR_INVALID_ARG;
+    const size_t size = type == DCQ_TYPE_F32 ? 4 : 2;
+    if (stride_bytes < (size_t)vocab * size || stride_bytes > INT32_MAX) return DCQ_ERR_INVALID_ARG;
+    if (!aligned(logits, size) || stride_bytes % size || !aligned(beam_scores, 4) || !aligned(scores, 4) ||
+        !aligned(parents, 4) || !aligned(tokens, 4))
+        return DCQ_ERR_MISALIGNED;
+    const int64_t rows = n_batch * n_beams, x_bytes = (rows - 1) * (int64_t)stride_bytes + vocab * (int64_t)size;
+    for (const void* o : {(const void*)scores, (const void*)parents, (const void*)tokens})
+        if (overlap(o, n_batch * n_out * 4, logits, x_bytes) || overlap(o, n_batch * n_out * 4, beam_scores, rows * 4))
+            return DCQ_ERR_INVALID_ARG;
+    const size_t need = beam_workspace_bytes(n_batch, n_beams, (int)vocab, n_out);
+    if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
+    if ((rc = check_device())) return rc;
+    BeamArgs a{};
+    a.x = logits, a.stride = (int64_t)(stride_bytes / size), a.n_beams = n_beams, a.vocab = (int)vocab;
+    a.beam = beam_scores, a.n_out = n_out, a.scores = scores, a.parents = parents, a.tokens = tokens;
+    return hip_status(launch_beam_select(type, a, n_batch, workspace, (hipStream_t)stream));
 }
 
 }  // extern "C"

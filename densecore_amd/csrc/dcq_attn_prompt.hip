@@ -61,10 +61,6 @@
 namespace dcq {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kBlk = 32;        // keys per block
 constexpr int kRows = 128;      // query rows per workgroup
@@ -91,31 +87,6 @@ struct __align__(16) PromptSmem {
     float ks[2][4], ev[2][4], vi[2][4];  // per 8 keys: 2^ek, ev (or kWide), 2^-ev
     float ks1[2][kBlk], ev1[2][kBlk];    // per key, only of wide groups: 2^ek, ev
 };
-
-// The exponent field that normalises magnitudes up to m: m * pow2(268 - E) is in [2^14, 2^15).
-__device__ __forceinline__ int norm_exp(uint32_t bits) {
-    return max((int)(bits >> 23), 30);  // below 2^-97 (zeros too): the floor's exponent
-}
-__device__ __forceinline__ float pow2_bits(int e) { return __uint_as_float((uint32_t)e << 23); }
-
-// four consecutive fp32 values (already scaled) -> the f16 pieces
-__device__ __forceinline__ void split4(const float x0, const float x1, const float x2, const float x3, f16x4& h,
-                                       f16x4& l) {
-    const f16x2 h0 = __builtin_convertvector((f32x2){x0, x1}, f16x2);
-    const f16x2 h1 = __builtin_convertvector((f32x2){x2, x3}, f16x2);
-    const f16x2 l0 = __builtin_convertvector((f32x2){x0 - (float)h0[0], x1 - (float)h0[1]}, f16x2);
-    const f16x2 l1 = __builtin_convertvector((f32x2){x2 - (float)h1[0], x3 - (float)h1[1]}, f16x2);
-    h = __builtin_shufflevector(h0, h1, 0, 1, 2, 3);
-    l = __builtin_shufflevector(l0, l1, 0, 1, 2, 3);
-}
-
-// Transposing LDS read, per 16 lanes: lane j gives the address of elements 4 (j % 4) .. + 3 of row j / 4
-// of a 4 x 16 matrix and receives column j.
-__device__ __forceinline__ f16x4 lds_transposed(const _Float16* src) {
-    typedef short i16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
-    return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)src));
-}
 
 // One staging thread's E elements of a K (V) row, as loaded: fp32 words of a current row, or the
 // slot's words (Q8_0: E / 4 words of quants and the block's scale; F16: E / 2 words).

@@ -1,0 +1,331 @@
+// dcq_pages.hip — the pages of the paged KV cache between two steps of a search: the accepted path's rows
+// into their slots, forks of sequences, and compaction. All of it moves bytes; the plans are whole numbers.
+//
+// A page is block b of both arenas: n_layer * 16 slots in a row, a multiple of 16 bytes. refs[b] counts the
+// sequences (of this call or not) that hold page b; a page is free where refs[b] <= 0. Sequence i holds the
+// first ceil(length / 16) entries of its table row; entries outside [0, n_blocks) hold nothing.
+//
+// Kernels:
+//   path_write_kernel    accepted token rows of every layer into their sequences' slots (bytes of kv_write)
+//   fork_count_kernel    the children's tables, and the counts without the parents' and with the children's
+//   fork_plan_kernel     who keeps a partial last page, who gets a copy and where; one workgroup
+//   compact_plan_kernel  the holes among the first n_live pages and the pages that move there; one workgroup
+//   compact_map_kernel   the tables and counts after the move
+//   copy_pages_kernel    whole pages (from, to) of both arenas
+#include <algorithm>
+
+#include "dcq_common.h"
+#include "dcq_kernels.h"
+#include "dcq_kv_row.h"
+#include "dcq_search.h"
+
+namespace dcq {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / 64;
+
+__device__ __forceinline__ int pages_of_length(int length, int n_table) {
+    return min((int)(((int64_t)max(length, 0) + kKvBlock - 1) / kKvBlock), n_table);
+}
+
+// ---------------------------------------------------------------- accepted paths
+// One workgroup per (accepted token, layer, arena).
+__global__ void __launch_bounds__(256) path_write_kernel(PathArgs a) {
+    const int seq = blockIdx.x / a.max_path, j = blockIdx.x % a.max_path, layer = blockIdx.y;
+    const int n = a.n_path ? a.n_path[seq] : a.max_path;
+    const int tok = a.path[(int64_t)seq * a.path_stride + j];
+    const int past = a.past[seq];
+    if (j >= n || tok < 0 || tok >= a.n_tokens || past < 0) return;
+    const int64_t pos = (int64_t)past + j;
+    if (pos / kKvBlock >= a.n_table) return;
+    const int blk = a.tables[(int64_t)seq * a.table_stride + pos / kKvBlock];
+    if (blk < 0 || blk >= a.n_blocks) return;
+    uint8_t* arena = blockIdx.z ? a.v_arena : a.k_arena;
+    const float* cur = blockIdx.z ? a.v_cur : a.k_cur;
+    const float* x = cur + (int64_t)layer * a.layer_stride + ((int64_t)seq * a.n_tokens + tok) * a.kv_stride;
+    uint8_t* dst = const_cast<uint8_t*>(kv_slot(arena, blk, a.n_layer, layer, (int)(pos % kKvBlock), a.sb));
+    kv_encode_row(a.ct, dst, x, a.row_elems);
+}
+
+hipError_t launch_path_write(const PathArgs& a, hipStream_t st) {
+    const int64_t wgs = (int64_t)a.n_seqs * a.max_path;
+    if (wgs > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(path_write_kernel, dim3((unsigned)wgs, (unsigned)a.n_layer, 2), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- whole pages
+// plan[0] pairs (from, to) at plan[2 + 2 i]: pieces of 16 KB, dealt to the workgroups in turn.
+constexpr int kPiece = 16384;
+__global__ void __launch_bounds__(256) copy_pages_kernel(uint8_t* k_arena, uint8_t* v_arena, const int32_t* plan,
+                                                         int64_t page_bytes) {
+    const int64_t per_page = (page_bytes + kPiece - 1) / kPiece;
+    const int64_t pieces = 2 * per_page * plan[0];
+    for (int64_t i = blockIdx.x; i < pieces; i += gridDim.x) {
+        const int64_t unit = i / per_page, at = (i % per_page) * kPiece;
+        const int64_t from = plan[2 + 2 * (unit / 2)], to = plan[3 + 2 * (unit / 2)];
+        uint8_t* arena = unit % 2 ? v_arena : k_arena;
+        const uint8_t* src = arena + from * page_bytes + at;
+        uint8_t* dst = arena + to * page_bytes + at;
+        const int64_t left = page_bytes - at;
+        uint4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int o = 16 * ((int)threadIdx.x + 256 * u);
+            if (o < left) w[u] = ld16(src + o);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int o = 16 * ((int)threadIdx.x + 256 * u);
+            if (o < left) *reinterpret_cast<uint4*>(dst + o) = w[u];
+        }
+    }
+}
+
+static hipError_t launch_copy_pages(void* k_arena, void* v_arena, const int32_t* plan, int64_t max_pages,
+                                    int64_t page_bytes, hipStream_t st) {
+    const int64_t pieces = 2 * max_pages * ((page_bytes + kPiece - 1) / kPiece);
+    const unsigned grid = (unsigned)std::min<int64_t>(pieces, 8 * (int64_t)cu_count());
+    hipLaunchKernelGGL(copy_pages_kernel, dim3(grid), dim3(256), 0, st, static_cast<uint8_t*>(k_arena),
+                       static_cast<uint8_t*>(v_arena), plan, page_bytes);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- scans of a plan's workgroup
+// The thread's offset among the flags of the workgroup's threads, in thread order, and their number.
+struct Scan {
+    int before, total;
+};
+__device__ __forceinline__ Scan block_scan(bool flag, int* counts /* kPlanWaves */) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint64_t set = __ballot(flag);
+    __syncthreads();  // counts of the scan before are read
+    if (lane == 0) counts[wave] = __popcll(set);
+    __syncthreads();
+    Scan s{(int)__popcll(set & ((1ull << lane) - 1)), 0};
+#pragma unroll
+    for (int k = 0; k < kPlanWaves; ++k) {
+        const int c = counts[k];
+        s.before += k < wave ? c : 0;
+        s.total += c;
+    }
+    return s;
+}
+
+// ---------------------------------------------------------------- forks
+// The counts: refs_out = refs - one for each page a sequence holds + one for each page a child takes over, and
+// the children's tables and lengths. The part of one (sequence or child, table entry).
+template <class Add>
+__device__ __forceinline__ void fork_count_entry(const ForkArgs& a, int row, int at, Add add) {
+    if (row < a.n_seqs) {
+        const int page = a.tables[(int64_t)row * a.table_stride + at];
+        if (at < pages_of_length(a.lengths[row], a.n_table) && page >= 0 && page < a.n_blocks) add(page, -1);
+        return;
+    }
+    const int child = row - a.n_seqs, parent = a.parents[child];
+    const bool known = parent >= 0 && parent < a.n_seqs;
+    const int length = known ? min(max(a.lengths[parent], 0), a.n_table * kKvBlock) : 0;
+    int page = -1;
+    if (at < pages_of_length(length, a.n_table)) {
+        page = a.tables[(int64_t)parent * a.table_stride + at];
+        if (page >= 0 && page < a.n_blocks) add(page, 1);
+    }
+    a.tables_out[(int64_t)child * a.tables_out_stride + at] = page;
+    if (at == 0) a.lengths_out[child] = length;
+}
+
+__global__ void __launch_bounds__(256) fork_refs_kernel(const int32_t* refs, int32_t* refs_out, int n_blocks) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n_blocks) refs_out[i] = refs[i];
+}
+
+__global__ void __launch_bounds__(256) fork_count_kernel(ForkArgs a) {
+    const int64_t entries = (int64_t)(a.n_seqs + a.n_children) * a.n_table;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256)
+        fork_count_entry(a, (int)(i / a.n_table), (int)(i % a.n_table),
+                         [&](int page, int by) { atomicAdd(a.refs_out + page, by); });
+}
+
+// LDS: the counts are in LDS, and this workgroup does the counting too (few pages and entries). Otherwise
+// refs_out holds the counts already.
+template <bool LDS>
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
+    extern __shared__ int32_t lds[];
+    __shared__ int counts[kPlanWaves];
+    const int tid = threadIdx.x;
+    int32_t* tails = lds;                                        // [n_children]: partial last page, or -1
+    int32_t* fresh = lds + a.n_children;                         // [n_children]: the copy's page, by its rank
+    int32_t* refs = LDS ? lds + 2 * a.n_children : a.refs_out;  // [n_blocks]
+    if (LDS) {
+        for (int i = tid; i < a.n_blocks; i += kPlanThreads) refs[i] = a.refs[i];
+        __syncthreads();
+        const int entries = (a.n_seqs + a.n_children) * a.n_table;
+        for (int i = tid; i < entries; i += kPlanThreads)
+            fork_count_entry(a, i / a.n_table, i % a.n_table, [&](int page, int by) { atomicAdd(refs + page, by); });
+    }
+    for (int i = tid; i < a.n_children; i += kPlanThreads) {
+        const int parent = a.parents[i];
+        int tail = -1;
+        if (parent >= 0 && parent < a.n_seqs) {
+            const int length = min(max(a.lengths[parent], 0), a.n_table * kKvBlock);
+            if (length % kKvBlock) tail = a.tables[(int64_t)parent * a.table_stride + length / kKvBlock];
+            if (tail >= a.n_blocks) tail = -1;
+        }
+        tails[i] = tail;
+    }
+    __syncthreads();
+    // ---- a child keeps its partial page if all who hold it are children that would write into it, and it is
+    // the first of them; the others get copies, ranked in the children's order
+    int copies = 0;
+    for (int i0 = 0; i0 < a.n_children; i0 += kPlanThreads) {
+        const int i = i0 + tid, tail = i < a.n_children ? tails[i] : -1;
+        bool copy = false;
+        if (tail >= 0) {
+            int users = 0;
+            bool first = true;
+            for (int k = 0; k < a.n_children; ++k) {
+                const bool same = tails[k] == tail;
+                users += same;
+                first &= !(same && k < i);
+            }
+            copy = !(first && refs[tail] == users);
+        }
+        const Scan s = block_scan(copy, counts);
+        if (i < a.n_children) a.rank[i] = copy ? copies + s.before : -1;
+        copies += s.total;
+    }
+    // ---- as many free pages, the lowest first
+    int found = 0;
+    for (int i0 = 0; i0 < a.n_blocks && found < copies; i0 += kPlanThreads) {
+        const int i = i0 + tid;
+        const bool free = i < a.n_blocks && refs[i] <= 0;
+        const Scan s = block_scan(free, counts);
+        if (free && found + s.before < copies) fresh[found + s.before] = i;
+        found += s.total;
+    }
+    found = min(found, copies);
+    __syncthreads();
+    // ---- the copies' pages into tables, counts and the copy list
+    for (int i = tid; i < a.n_children; i += kPlanThreads) {
+        const int rank = a.rank[i];
+        if (rank < 0) continue;
+        const int page = rank < found ? fresh[rank] : -1;
+        a.tables_out[(int64_t)i * a.tables_out_stride + a.lengths[a.parents[i]] / kKvBlock] = page;
+        atomicAdd(refs + tails[i], -1);
+        if (page >= 0) {
+            refs[page] = 1;
+            a.plan[2 + 2 * rank] = tails[i];
+            a.plan[3 + 2 * rank] = page;
+        }
+    }
+    if (tid == 0) {
+        a.plan[0] = found;
+        a.missing[0] = copies - found;
+    }
+    if (LDS) {
+        __syncthreads();
+        for (int i = tid; i < a.n_blocks; i += kPlanThreads) a.refs_out[i] = refs[i];
+    }
+}
+
+// Workspace: rank [n_children], then the plan (its length, a spare word, the pairs).
+size_t fork_workspace_bytes(int64_t n_children) {
+    return (size_t)round_up(n_children * 4, 256) + (size_t)round_up((2 + 2 * n_children) * 4, 256);
+}
+
+hipError_t launch_fork(ForkArgs a, void* k_arena, void* v_arena, int64_t page_bytes, void* ws, hipStream_t st) {
+    a.rank = static_cast<int32_t*>(ws);
+    a.plan = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(ws) + round_up((int64_t)a.n_children * 4, 256));
+    const int64_t entries = (int64_t)(a.n_seqs + a.n_children) * a.n_table;
+    const size_t lds = 2 * (size_t)a.n_children * 4;
+    // one workgroup does it all while the counts fit in LDS and its threads have few entries to see; beyond, the
+    // counting alone takes longer than the two launches it then gets
+    if (2 * a.n_children + a.n_blocks <= 12288 && entries <= 32768) {
+        hipLaunchKernelGGL((fork_plan_kernel<true>), dim3(1), dim3(kPlanThreads), lds + (size_t)a.n_blocks * 4, st, a);
+    } else {
+        hipLaunchKernelGGL(fork_refs_kernel, dim3((unsigned)((a.n_blocks + 255) / 256)), dim3(256), 0, st, a.refs,
+                           a.refs_out, a.n_blocks);
+        const int64_t wgs = std::min<int64_t>((entries + 255) / 256, 4 * (int64_t)cu_count());
+        hipLaunchKernelGGL(fork_count_kernel, dim3((unsigned)wgs), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((fork_plan_kernel<false>), dim3(1), dim3(kPlanThreads), lds, st, a);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    return launch_copy_pages(k_arena, v_arena, a.plan, a.n_children, page_bytes, st);
+}
+
+// ---------------------------------------------------------------- compaction
+// rank [n_blocks]: of a page that moves, its place in the plan.
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs a) {
+    __shared__ int counts[kPlanWaves];
+    const int tid = threadIdx.x;
+    int live = 0;
+    for (int i = tid; i < a.n_blocks; i += kPlanThreads) live += a.refs[i] > 0;
+    live = (int)lanes_sum<64>((float)live);
+    if ((tid & 63) == 0) counts[tid >> 6] = live;
+    __syncthreads();
+    live = 0;
+#pragma unroll
+    for (int k = 0; k < kPlanWaves; ++k) live += counts[k];
+    int holes = 0, movers = 0;
+    for (int i0 = 0; i0 < a.n_blocks; i0 += kPlanThreads) {
+        const int i = i0 + tid;
+        const bool used = i < a.n_blocks && a.refs[i] > 0;
+        const bool hole = i < live && !used, moves = used && i >= live;
+        // a step's pages are below live, above, or (one step) on both sides
+        if (i0 < live) {
+            const Scan s = block_scan(hole, counts);
+            if (hole) a.plan[3 + 2 * (holes + s.before)] = i;
+            holes += s.total;
+        }
+        if (i0 + kPlanThreads > live) {
+            const Scan s = block_scan(moves, counts);
+            if (moves) {
+                a.plan[2 + 2 * (movers + s.before)] = i;
+                a.rank[i] = movers + s.before;
+            }
+            movers += s.total;
+        }
+    }
+    if (tid == 0) a.plan[0] = movers, a.plan[1] = live, a.n_live[0] = live;
+}
+
+__global__ void __launch_bounds__(256) compact_map_kernel(CompactArgs a) {
+    const int live = a.plan[1];
+    const int64_t entries = (int64_t)a.n_seqs * a.n_table;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries + a.n_blocks; i += (int64_t)gridDim.x * 256) {
+        if (i < entries) {
+            const int row = (int)(i / a.n_table), at = (int)(i % a.n_table);
+            int page = a.tables[(int64_t)row * a.table_stride + at];
+            if (at < pages_of_length(a.lengths[row], a.n_table) && page >= live && page < a.n_blocks && a.refs[page] > 0)
+                page = a.plan[3 + 2 * a.rank[page]];
+            a.tables_out[(int64_t)row * a.tables_out_stride + at] = page;
+        } else {
+            const int page = (int)(i - entries), n = a.refs[page];
+            if (page < live ? n > 0 : n <= 0) {
+                a.refs_out[page] = n;
+            } else if (page >= live) {  // moves: the pair's counts; a hole's comes from its pair
+                a.refs_out[a.plan[3 + 2 * a.rank[page]]] = n;
+                a.refs_out[page] = 0;
+            }
+        }
+    }
+}
+
+size_t compact_workspace_bytes(int64_t n_blocks) {
+    return (size_t)round_up(n_blocks * 4, 256) + (size_t)round_up((2 + n_blocks) * 4, 256);
+}
+
+hipError_t launch_compact(CompactArgs a, void* k_arena, void* v_arena, int64_t page_bytes, void* ws, hipStream_t st) {
+    a.rank = static_cast<int32_t*>(ws);
+    a.plan = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(ws) + round_up((int64_t)a.n_blocks * 4, 256));
+    hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+    const int64_t items = (int64_t)a.n_seqs * a.n_table + a.n_blocks;
+    const int64_t wgs = std::min<int64_t>((items + 255) / 256, 4 * (int64_t)cu_count());
+    hipLaunchKernelGGL(compact_map_kernel, dim3((unsigned)wgs), dim3(256), 0, st, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.n_blocks < 2) return e;
+    return launch_copy_pages(k_arena, v_arena, a.plan, a.n_blocks / 2, page_bytes, st);
+}
+
+}  // namespace dcq

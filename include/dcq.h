@@ -349,6 +349,89 @@ int dcq_kv_attention(int cache_type, const void* k_arena, const void* v_arena, i
                      size_t kv_stride_bytes, int64_t n_tokens, int64_t n_past, float scale, float* out,
                      size_t out_stride_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Search over the paged cache: drafted trees, accepted paths, forks, compaction, beams ----
+ * No counterpart in the reference, whose cache serves one continuation per sequence. Several sequences per
+ * call: tables is int32 [n_seqs][n_table] with rows table_stride entries apart, and past, n_draft, lengths,
+ * refs and the like are int32 device arrays, so that a step needs nothing back on the host. What a device
+ * array holds out of its range is not an error (the host cannot see it): it is clamped or skipped as each
+ * call says, and no access leaves the arrays. All results are the same from run to run. Layers, arenas,
+ * types and alignment as above; no output may overlap an input. */
+
+/* Attention of one layer for the drafted tokens of n_seqs sequences. Sequence b has past[b] cached positions
+ * (below 0 counts as 0, above max_past as max_past) and n_draft[b] drafted tokens (clamped to 0 .. n_tokens;
+ * NULL: n_tokens each). Their rows of q, k_cur, v_cur and out are b * n_tokens + 0 .. n_draft[b] - 1. Token j
+ * attends every cached position of its sequence, and drafted token i where bit i % 64 of
+ * mask[b][j][i / 64] is set (uint64, (n_tokens + 63) / 64 words per token, 8-byte aligned; NULL: i <= j):
+ * the ancestors of j in the tree, j itself among them if its bit is set. Bits of tokens from n_draft[b] on
+ * count as 0. A cached position whose page is missing from the table, or outside [0, n_blocks), is a row of
+ * zeros that is attended, as in dcq_kv_attention. A token that sees nothing, all of whose scores are
+ * -infinity, or that is not drafted (j >= n_draft[b]) gets zeros. What a token does not see has no influence
+ * on it, infinities and NaN included. head_dim 64, 128 or 256; n_tokens <= 1024; max_past <= 2^24.
+ * Precision: as dcq_kv_attention (fp32 sums and weights; products of at least 22 bits of each operand).
+ * The workspace (256-byte aligned) holds the partial results of key splits; 0 needs none. */
+size_t dcq_kv_tree_attention_workspace_size(int n_head, int n_head_kv, int head_dim, int64_t n_seqs,
+                                            int64_t n_tokens, int64_t max_past);
+int dcq_kv_tree_attention(int cache_type, const void* k_arena, const void* v_arena, int64_t n_blocks, int n_layer,
+                          int layer, const int32_t* tables, int64_t table_stride, int64_t n_table,
+                          const int32_t* past, int64_t max_past, const int32_t* n_draft, const uint64_t* mask,
+                          int n_head, int n_head_kv, int head_dim, const float* q, size_t q_stride_bytes,
+                          const float* k_cur, const float* v_cur, size_t kv_stride_bytes, int64_t n_seqs,
+                          int64_t n_tokens, float scale, float* out, size_t out_stride_bytes, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* The accepted tokens of each sequence into the cache, K and V of every layer: place j < n_path[b] (NULL:
+ * max_path) of path[b] names a drafted token t, whose rows k_cur / v_cur[layer][b * n_tokens + t] go to
+ * position past[b] + j in the bytes of dcq_kv_write. Layers lie layer_stride_bytes apart, rows
+ * kv_stride_bytes. A place whose token is outside 0 .. n_tokens - 1, or whose position is negative, past
+ * the table or on a page outside [0, n_blocks), is skipped. Two places must not have one position (two
+ * sequences share pages only before past[b]). */
+int dcq_kv_write_path(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer,
+                      int64_t row_elems, const int32_t* tables, int64_t table_stride, int64_t n_table,
+                      const int32_t* past, const int32_t* path, int64_t path_stride, int64_t max_path,
+                      const int32_t* n_path, const float* k_cur, const float* v_cur, size_t layer_stride_bytes,
+                      size_t kv_stride_bytes, int64_t n_seqs, int64_t n_tokens, void* stream);
+
+/* The sequences of the next step from those of the last one. Child i continues sequence parents[i]: its length,
+ * and its pages, shared. refs[p] counts the sequences that hold page p (a sequence of length n holds its first
+ * (n + 15) / 16 table entries; entries outside [0, n_blocks) hold nothing): refs_out = refs without the
+ * n_seqs sequences and with the n_children children. A last page that is not full would be written by all
+ * who hold it, so it stays with the first child that has it, if no full page of a child and no sequence
+ * beyond this call holds it; each other child gets a copy of it (every layer, K and V) on a free page
+ * (refs_out <= 0; the lowest pages, in the order of the children). Where the free pages do not suffice, the
+ * children that are left have -1 there, and *missing is their number (0 otherwise). tables_out
+ * [n_children][n_table] has -1 past each child's pages. A child whose parent is outside 0 .. n_seqs - 1 is
+ * empty; lengths count as 0 .. 16 * n_table. n_children <= 4096. */
+size_t dcq_kv_fork_workspace_size(int64_t n_blocks, int64_t n_seqs, int64_t n_children);
+int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer, int64_t row_elems,
+                const int32_t* tables, int64_t table_stride, int64_t n_table, const int32_t* lengths, int64_t n_seqs,
+                const int32_t* parents, int64_t n_children, const int32_t* refs, int32_t* tables_out,
+                int64_t tables_out_stride, int32_t* lengths_out, int32_t* refs_out, int32_t* missing,
+                void* workspace, size_t workspace_bytes, void* stream);
+
+/* The n_live pages in use (refs > 0) to the front of the arenas: of those at n_live and above, the lowest
+ * goes to the lowest free page below n_live, the next to the next, K and V of every layer; pages below
+ * n_live stay. tables_out: the tables with the pages that the sequences hold renamed, other entries as they
+ * are; refs_out: the counts in their new places, 0 where a page left. Every sequence that holds a page must
+ * be in the tables. */
+size_t dcq_kv_compact_workspace_size(int64_t n_blocks);
+int dcq_kv_compact(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer, int64_t row_elems,
+                   const int32_t* tables, int64_t table_stride, int64_t n_table, const int32_t* lengths,
+                   int64_t n_seqs, const int32_t* refs, int32_t* tables_out, int64_t tables_out_stride,
+                   int32_t* refs_out, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Beam search's selection. logits: F32 or F16, rows b * n_beams + w of vocab elements, stride_bytes apart (a
+ * multiple of the element's size). Candidate (w, t) of request b scores beam_scores[b][w] + log softmax of the
+ * row at t, with the row's sum in 64 bits and scores compared in 64; scores / parents / tokens [n_batch][n_out]
+ * receive the best of each request in falling order, ties by the lower w, then the lower t: the score rounded to
+ * fp32, the row b * n_beams + w, and t. A logit of -infinity rules a token out; a row whose logits hold a NaN
+ * or +infinity, or are all -infinity, and a beam whose score is not finite have no continuations; where fewer
+ * than n_out are left, the rest is -infinity, -1, -1. n_beams <= 256, n_out <= 64, n_batch * n_beams <= 65535,
+ * vocab <= 2^24. Workspace 256-byte aligned. */
+size_t dcq_beam_select_workspace_size(int64_t n_batch, int n_beams, int64_t vocab, int n_out);
+int dcq_beam_select(int type, const void* logits, size_t stride_bytes, int64_t n_batch, int n_beams, int64_t vocab,
+                    const float* beam_scores, int n_out, float* scores, int32_t* parents, int32_t* tokens,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
