@@ -8,8 +8,8 @@
 
 namespace dcq {
 
-// dcq_tree.hip: drafted tokens of several sequences over their cached keys. rep, tiles, splits, kps, rows,
-// units and the workspace pointers are the launcher's.
+// dcq_tree.hip: drafted tokens of several sequences over their cached keys. rep .. units and what follows is
+// the launcher's.
 struct TreeArgs {
     const uint8_t* k_arena;
     const uint8_t* v_arena;
@@ -31,7 +31,7 @@ struct TreeArgs {
     int64_t out_stride;
     int n_seqs, n_tokens, n_head, n_head_kv;
     float scale_log2e;
-    int rep, tiles, splits, kps, units;
+    int rep, tiles, tiles16, splits, kps, units, draft_wgs;
     int64_t rows;  // n_seqs * n_tokens * n_head
     float* ws_o;   // [splits][rows][HD]
     float* ws_ml;  // [splits][rows][2]

@@ -14,6 +14,10 @@
 //   V: a lane holds dims 64 u + 4 (lane % 16) + 0..3 of the keys whose weights it has; output tile (u, e) is
 //      made of the dims 64 u + 4 m + e, so that its A operand is in the lane, one byte permute per two keys.
 //
+// Many query rows of a KV head (tree_block_kernel): as many rows as a workgroup has waves x 32 share the keys,
+// which go through LDS in blocks, decoded once. 32 x 32 tiles, S^T and O^T as above; V^T comes by transposing
+// LDS reads. Drafted keys, a small part, are the other kernel's work, in workgroups of the same launch.
+//
 // Arithmetic. F16 and Q8_0 slots are multiplied on the f16 matrix instructions (16 x the fp32 ones' rate):
 // q and p', fp32, are split into two f16 pieces of 22 bits (q under an exponent per row, p' times 2^7), an
 // F16 slot is one exact piece, and a Q8_0 value d * q, a product of 11 and 7 bits, is exactly the two pieces
@@ -32,9 +36,11 @@
 namespace dcq {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTile = 16;          // query rows of a tile
 constexpr int kTreeWaves = 4;      // waves of a workgroup, a share of the keys each
+constexpr int kRowsPerWave = 32;   // of the block kernel
 constexpr float kPieces = 128.0f;  // of the weights in O: 2^15 at most before the reference is raised
 
 template <int CT>
@@ -290,9 +296,10 @@ __device__ __forceinline__ float slot_value(const uint8_t* head, int e) {
     }
 }
 
+template <int W>
 struct TreeSmem {
-    float o[kTreeWaves][kTile][68];  // 64 dims of the waves' sums; pitch: 16-byte aligned, 4 banks apart
-    float m[kTreeWaves][kTile], l[kTreeWaves][kTile];
+    float o[W][kTile][68];  // 64 dims of the waves' sums; pitch: 16-byte aligned, 4 banks apart
+    float m[W][kTile], l[W][kTile];
     uint32_t again;  // rows to compute again
 };
 
@@ -301,6 +308,7 @@ struct TreeJob {
     int seq, h_kv, row0, n_rows, n_draft, past;
     int k_begin, k_end;  // cached keys
     bool drafts;         // and the drafted ones
+    int slot;            // of the partial results
 };
 
 __device__ __forceinline__ int page_of(const TreeArgs& a, int seq, int lb) {
@@ -314,10 +322,10 @@ __device__ __forceinline__ bool draft_seen(const TreeArgs& a, int seq, int tok, 
     return (a.mask[((int64_t)seq * a.n_tokens + tok) * a.words + i / 64] >> (i % 64)) & 1;
 }
 
-// One row again, key by key in fp32, by the whole workgroup: each wave takes every fourth key, its lanes dims
-// lane + 64 u. Leaves the row's m and l in sm.m[0][0], sm.l[0][0] and returns the thread's dim of O (tid < HD).
-template <int CT, int HD>
-__device__ __forceinline__ float tree_row_again(const TreeArgs& a, const TreeJob& w, TreeSmem& sm, int row) {
+// One row again, key by key in fp32, by the whole workgroup of W waves: each takes every W-th key, its lanes dims
+// lane + 64 u. The result goes to the output or the partial results.
+template <int CT, int HD, int W>
+__device__ __forceinline__ void tree_row_again(const TreeArgs& a, const TreeJob& w, TreeSmem<W>& sm, int row) {
     constexpr int U = HD / 64;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int tok = row / a.rep, h = w.h_kv * a.rep + row % a.rep;
@@ -338,7 +346,7 @@ __device__ __forceinline__ float tree_row_again(const TreeArgs& a, const TreeJob
         for (int u = 0; u < U; ++u) acc[u] = fmaf(p, v[u], acc[u] * c);
         m = mn;
     };
-    for (int t = w.k_begin + wave; t < w.k_end; t += kTreeWaves) {
+    for (int t = w.k_begin + wave; t < w.k_end; t += W) {
         const int blk = page_of(a, w.seq, t / kKvBlock);
         float k[U], v[U];
         const int64_t off = (((int64_t)max(blk, 0) * a.n_layer + a.layer) * kKvBlock + t % kKvBlock) * a.sb + hb;
@@ -349,7 +357,7 @@ __device__ __forceinline__ float tree_row_again(const TreeArgs& a, const TreeJob
         }
         add(k, v);
     }
-    for (int t = wave; w.drafts && t < w.n_draft; t += kTreeWaves) {
+    for (int t = wave; w.drafts && t < w.n_draft; t += W) {
         if (!draft_seen(a, w.seq, tok, t)) continue;
         const int64_t off = ((int64_t)w.seq * a.n_tokens + t) * a.kv_stride + (int64_t)w.h_kv * HD;
         float k[U], v[U];
@@ -365,47 +373,30 @@ __device__ __forceinline__ float tree_row_again(const TreeArgs& a, const TreeJob
     __syncthreads();
     float mx = -INFINITY, ls = 0.0f, o = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kTreeWaves; ++k) mx = fmaxf(mx, sm.m[k][0]);
+    for (int k = 0; k < W; ++k) mx = fmaxf(mx, sm.m[k][0]);
 #pragma unroll
-    for (int k = 0; k < kTreeWaves; ++k) {
+    for (int k = 0; k < W; ++k) {
         const float c = ref_factor(sm.m[k][0], sm.l[k][0], mx);
         ls += sm.l[k][0] * c;
         if (tid < HD) o += so[k * HD + tid] * c;
     }
+    const int64_t tr = (int64_t)w.seq * a.n_tokens + tok, wr = (int64_t)w.slot * a.rows + tr * a.n_head + h;
+    if (tid < HD) {
+        if (a.splits == 1)
+            a.out[tr * a.out_stride + (int64_t)h * HD + tid] = ls != 0.0f ? o / ls : 0.0f;
+        else
+            a.ws_o[wr * HD + tid] = o;
+    }
+    if (a.splits > 1 && tid == 0) a.ws_ml[2 * wr] = mx, a.ws_ml[2 * wr + 1] = ls;
     __syncthreads();
-    if (tid == 0) sm.m[0][0] = mx, sm.l[0][0] = ls;
-    __syncthreads();
-    return o;
 }
 
-// A tile of 16 rows over a share of the keys. Grid: (unit, tile) pairs with the tiles of a unit on one XCD
-// (workgroup id % 8) one after another, as they read the same keys; unit = (sequence, split, KV head).
-template <int CT, int HD>
-__global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) {
+// A tile of 16 rows over a share of the keys, by a workgroup of W waves (HIST: cached keys too).
+template <int CT, int HD, int W, bool HIST>
+__device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, TreeSmem<W>& sm) {
     constexpr int U = HD / 64, CK = tree_chunk<CT>(), NP = CK / kKvBlock;
-    __shared__ TreeSmem sm;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, n = lane & 15;
-    TreeJob w;
-    int split, tile;
-    {
-        const int id = blockIdx.x, turn = id / (8 * a.tiles), rest = id % (8 * a.tiles);
-        const int unit = turn * 8 + rest % 8;
-        tile = rest / 8;
-        if (unit >= a.units) return;
-        w.h_kv = unit % a.n_head_kv;
-        split = unit / a.n_head_kv % a.splits;
-        w.seq = unit / a.n_head_kv / a.splits;
-    }
-    w.past = min(max(a.past[w.seq], 0), a.max_past);
-    w.n_draft = a.n_draft ? min(max(a.n_draft[w.seq], 0), a.n_tokens) : a.n_tokens;
-    w.n_rows = w.n_draft * a.rep;
-    w.row0 = tile * kTile;
-    const int n_split = max((w.past + a.kps - 1) / a.kps, 1);
-    if (split >= n_split || (w.row0 >= w.n_rows && a.splits > 1)) return;  // the merge writes such rows' zeros
-    w.k_begin = split * a.kps;
-    w.k_end = w.row0 < w.n_rows ? min(w.past, w.k_begin + a.kps) : 0;
-    w.drafts = split == n_split - 1 && w.row0 < w.n_rows;
 
     // ---- the lane's query row
     const int row = w.row0 + n;
@@ -427,7 +418,7 @@ __global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) 
     const uint32_t head = (uint32_t)(a.sb / a.n_head_kv) * w.h_kv;
     const uint32_t sb = (uint32_t)a.sb, off_k = n * sb + head, off_v = 4 * g * sb + head;
     const int c0 = w.k_begin / CK + wave, c1 = (w.k_end + CK - 1) / CK;
-    if (c0 < c1) {
+    if (HIST && c0 < c1) {
         constexpr int S = CT == kTypeF32 ? HD / 16 : HD / 32;
         f16x8 qh[CT == kTypeF32 ? 1 : S], ql[CT == kTypeF32 ? 1 : S];
         f32x4 qf[CT == kTypeF32 ? S : 1];
@@ -474,9 +465,9 @@ __global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) 
         for (int j = 0; j < NP; ++j) t.load_k(j, a.k_arena + page_bytes(pages[j]), off_k, g);
 #pragma unroll
         for (int j = 0; j < NP; ++j) t.load_v(j, a.v_arena + page_bytes(pages[j]), off_v, sb, n);
-        for (int c = c0; c < c1; c += kTreeWaves) {
-            const bool more = c + kTreeWaves < c1;
-            if (more) pages_of(c + kTreeWaves, next);
+        for (int c = c0; c < c1; c += W) {
+            const bool more = c + W < c1;
+            if (more) pages_of(c + W, next);
             const int left = w.k_end - c * CK;  // keys of the step, if fewer than CK
             bool whole = left >= CK;
 #pragma unroll
@@ -532,7 +523,7 @@ __global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) 
 #pragma unroll
         for (int s = 0; s < S; ++s) qf[s] = load_q(16 * s + 4 * g);
         const uint32_t rs = (uint32_t)(a.kv_stride * 4);
-        for (int k0 = 16 * wave; k0 < w.n_draft; k0 += 16 * kTreeWaves) {
+        for (int k0 = 16 * wave; k0 < w.n_draft; k0 += 16 * W) {
             const int left = w.n_draft - k0;
             const int64_t base = ((int64_t)w.seq * a.n_tokens + k0) * a.kv_stride + (int64_t)w.h_kv * HD;
             TreeKeys<kTypeF32, HD> t;
@@ -558,7 +549,7 @@ __global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) 
         }
     }
 
-    // ---- the waves' sums together, 64 dims at a time: thread -> row tid / 16, 4 dims
+    // ---- the waves' sums together, 64 dims at a time: thread (of the first 256) -> row tid / 16, 4 dims
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     if (lane < kTile) sm.m[wave][lane] = m, sm.l[wave][lane] = l;
@@ -566,20 +557,20 @@ __global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) 
     __syncthreads();
     float mx = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kTreeWaves; ++k) mx = fmaxf(mx, sm.m[k][n]);
+    for (int k = 0; k < W; ++k) mx = fmaxf(mx, sm.m[k][n]);
     const float c = ref_factor(m, l, mx) * (1.0f / kPieces);
-    const int r = tid >> 4, d4 = 4 * (tid & 15), orow = w.row0 + r;
+    const int r = (tid >> 4) % kTile, d4 = 4 * (tid & 15), orow = w.row0 + r;
     float rm = -INFINITY, rl = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kTreeWaves; ++k) rm = fmaxf(rm, sm.m[k][r]);
+    for (int k = 0; k < W; ++k) rm = fmaxf(rm, sm.m[k][r]);
 #pragma unroll
-    for (int k = 0; k < kTreeWaves; ++k) rl += sm.l[k][r] * ref_factor(sm.m[k][r], sm.l[k][r], rm);
-    const bool live = orow < w.n_rows, direct = a.splits == 1;
+    for (int k = 0; k < W; ++k) rl += sm.l[k][r] * ref_factor(sm.m[k][r], sm.l[k][r], rm);
+    const bool live = tid < 16 * kTile && orow < w.n_rows, direct = a.splits == 1;
     const int otok = orow / a.rep, oh = w.h_kv * a.rep + orow % a.rep;
-    const int64_t trow = (int64_t)w.seq * a.n_tokens + otok, wrow = (int64_t)split * a.rows + trow * a.n_head + oh;
+    const int64_t trow = (int64_t)w.seq * a.n_tokens + otok, wrow = (int64_t)w.slot * a.rows + trow * a.n_head + oh;
     auto store4 = [&](int d, f32x4 v) {
         if (direct) {
-            if (otok < a.n_tokens) {
+            if (tid < 16 * kTile && otok < a.n_tokens) {
                 float* out = a.out + trow * a.out_stride + (int64_t)oh * HD + d;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) out[e] = live && rl != 0.0f ? v[e] / rl : 0.0f;
@@ -601,7 +592,7 @@ __global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) 
         __syncthreads();
         f32x4 v = *reinterpret_cast<const f32x4*>(&sm.o[0][r][d4]);
 #pragma unroll
-        for (int k = 1; k < kTreeWaves; ++k) v += *reinterpret_cast<const f32x4*>(&sm.o[k][r][d4]);
+        for (int k = 1; k < W; ++k) v += *reinterpret_cast<const f32x4*>(&sm.o[k][r][d4]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) bad |= !(fabsf(v[e]) < INFINITY);
         store4(64 * u + d4, v);
@@ -609,21 +600,312 @@ __global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) 
     if (!direct && live && d4 == 0) a.ws_ml[2 * wrow] = rm, a.ws_ml[2 * wrow + 1] = rl;
     if (bad && live) atomicOr(&sm.again, 1u << r);
     __syncthreads();
-    for (uint32_t again = sm.again; again; again &= again - 1) {
-        const int rr = __builtin_ctz(again), arow = w.row0 + rr;
-        const float v = tree_row_again<CT, HD>(a, w, sm, arow);
-        const float am = sm.m[0][0], al = sm.l[0][0];
-        const int at = arow / a.rep, ah = w.h_kv * a.rep + arow % a.rep;
-        const int64_t tr = (int64_t)w.seq * a.n_tokens + at, wr = (int64_t)split * a.rows + tr * a.n_head + ah;
-        if (tid < HD) {
-            if (direct)
-                a.out[tr * a.out_stride + (int64_t)ah * HD + tid] = al != 0.0f ? v / al : 0.0f;
-            else
-                a.ws_o[wr * HD + tid] = v;
+    for (uint32_t again = sm.again; again; again &= again - 1)
+        tree_row_again<CT, HD, W>(a, w, sm, w.row0 + __builtin_ctz(again));
+}
+
+__device__ __forceinline__ void tree_job(const TreeArgs& a, TreeJob& w, int seq) {
+    w.seq = seq;
+    w.past = min(max(a.past[seq], 0), a.max_past);
+    w.n_draft = a.n_draft ? min(max(a.n_draft[seq], 0), a.n_tokens) : a.n_tokens;
+    w.n_rows = w.n_draft * a.rep;
+}
+
+// Grid: (unit, tile) pairs with the tiles of a unit on one XCD (workgroup id % 8) one after another, as they
+// read the same keys; unit = (sequence, split, KV head).
+template <int CT, int HD>
+__global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) {
+    __shared__ TreeSmem<kTreeWaves> sm;
+    TreeJob w;
+    const int id = blockIdx.x, turn = id / (8 * a.tiles), rest = id % (8 * a.tiles), unit = turn * 8 + rest % 8;
+    if (unit >= a.units) return;
+    w.h_kv = unit % a.n_head_kv;
+    w.slot = unit / a.n_head_kv % a.splits;
+    tree_job(a, w, unit / a.n_head_kv / a.splits);
+    w.row0 = rest / 8 * kTile;
+    const int n_split = max((w.past + a.kps - 1) / a.kps, 1);
+    if (w.slot >= n_split || (w.row0 >= w.n_rows && a.splits > 1)) return;  // the merge writes such rows' zeros
+    w.k_begin = w.slot * a.kps;
+    w.k_end = w.row0 < w.n_rows ? min(w.past, w.k_begin + a.kps) : 0;
+    w.drafts = w.slot == n_split - 1 && w.row0 < w.n_rows;
+    tree_tile<CT, HD, kTreeWaves, true>(a, w, sm);
+}
+
+// ---------------------------------------------------------------- many rows
+// A block of 8 W keys in LDS, as f16 pieces (F16 slots: one).
+template <int CT, int HD, int W>
+struct __align__(16) TreeBlock {
+    static constexpr int NPC = CT == kTypeQ8_0 ? 2 : 1;
+    // pitches: K rows are read 16 bytes per lane down a column of 32 rows (4 banks apart); V rows four
+    // at a time, 64 bytes each (16 banks apart)
+    static constexpr int KP = HD + 8, VP = HD + 32;
+    _Float16 k[2][NPC][8 * W][KP];  // [buffer][piece][key][dim]
+    _Float16 v[2][NPC][8 * W][VP];
+};
+
+// E elements of a slot's head piece from element e0, as loaded, and their way into LDS.
+template <int CT, int E>
+struct TreeRaw;
+template <int E>
+struct TreeRaw<kTypeF16, E> {
+    uint4 w[E / 8];
+    __device__ __forceinline__ void load(const uint8_t* head, int e0) {
+#pragma unroll
+        for (int j = 0; j < E / 8; ++j) w[j] = ld16(head + 2 * e0 + 16 * j);
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < E / 8; ++j) w[j] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ void store(_Float16* h, _Float16*) const {
+#pragma unroll
+        for (int j = 0; j < E / 8; ++j) *reinterpret_cast<uint4*>(h + 8 * j) = w[j];
+    }
+};
+template <int E>
+struct TreeRaw<kTypeQ8_0, E> {
+    uint32_t w[E / 4], d;
+    __device__ __forceinline__ void load(const uint8_t* head, int e0) {
+        const uint8_t* b = head + e0 / 32 * 34;
+        d = ldu16(b);
+        __builtin_memcpy(w, b + 2 + e0 % 32, E);  // 2-byte aligned
+    }
+    __device__ __forceinline__ void clear() { d = 0u; }
+    __device__ __forceinline__ void store(_Float16* h, _Float16* l) const {
+        const f16x2 dd = as_f16x2(d | d << 16);
+#pragma unroll
+        for (int j = 0; j < E / 8; ++j) {
+            Pieces p[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                p[t] = q8_pieces(int8_pair(__builtin_amdgcn_perm(0u, w[2 * j + t / 2], t % 2 ? 0x0c030c02u : 0x0c010c00u)), dd);
+            *reinterpret_cast<f16x8*>(h + 8 * j) = as_f16x8(as_u32(p[0].h), as_u32(p[1].h), as_u32(p[2].h), as_u32(p[3].h));
+            *reinterpret_cast<f16x8*>(l + 8 * j) = as_f16x8(as_u32(p[0].l), as_u32(p[1].l), as_u32(p[2].l), as_u32(p[3].l));
         }
-        if (!direct && tid == 0) a.ws_ml[2 * wr] = am, a.ws_ml[2 * wr + 1] = al;
+    }
+};
+
+// 32 W rows of a KV head over a share of its cached keys (slots 1 ..), or 16 rows over the drafted keys (slot 0:
+// the first draft_wgs workgroups).
+template <int CT, int HD, int W>
+__global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(TreeArgs a) {
+    using Block = TreeBlock<CT, HD, W>;
+    constexpr int E = HD / 8;    // elements per staging thread: key tid / 8 of the block
+    constexpr int KS = HD / 16;  // k-steps of the score product
+    constexpr int NT = HD / 32;  // 32-dim tiles of the output
+    constexpr int NPC = Block::NPC;
+    __shared__ union {
+        Block b;
+        TreeSmem<W> t;
+    } sm;
+    __shared__ uint32_t again[W];
+    TreeJob w;
+    int id = blockIdx.x;
+    if (id < a.draft_wgs) {
+        const int per_seq = a.n_head_kv * a.tiles16;
+        tree_job(a, w, id / per_seq);
+        w.h_kv = id % per_seq / a.tiles16;
+        w.row0 = id % a.tiles16 * kTile;
+        w.k_begin = w.k_end = 0;
+        w.drafts = true;
+        w.slot = 0;
+        if (w.row0 < w.n_rows) tree_tile<kTypeF32, HD, W, false>(a, w, sm.t);
+        return;
+    }
+    id -= a.draft_wgs;
+    const int turn = id / (8 * a.tiles), rest = id % (8 * a.tiles), unit = turn * 8 + rest % 8;
+    if (unit >= a.units) return;
+    w.h_kv = unit % a.n_head_kv;
+    w.slot = unit / a.n_head_kv % (a.splits - 1) + 1;
+    tree_job(a, w, unit / a.n_head_kv / (a.splits - 1));
+    w.row0 = rest / 8 * (kRowsPerWave * W);
+    w.k_begin = (w.slot - 1) * a.kps;
+    w.k_end = min(w.past, w.k_begin + a.kps);
+    w.drafts = false;
+    if (w.k_begin >= w.k_end || w.row0 >= w.n_rows) return;
+
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int p = lane >> 5, c32 = lane & 31;
+
+    // ---- the lane's query row: pieces of q * scale * log2(e) at dims 16 s + 8 p .. + 7
+    const int r0 = w.row0 + kRowsPerWave * wave, row = r0 + c32;
+    const bool q_ok = row < w.n_rows;
+    const int tok = q_ok ? row / a.rep : 0, h = w.h_kv * a.rep + (q_ok ? row % a.rep : 0);
+    const int64_t trow = (int64_t)w.seq * a.n_tokens + tok;
+    f16x8 qh[KS], ql[KS];
+    float qsc;
+    {
+        const float* qp = a.q + trow * a.q_stride + (int64_t)h * HD + 8 * p;
+        f32x4 t[KS][2];
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                t[s][k] = *reinterpret_cast<const f32x4*>(qp + 16 * s + 4 * k) * (q_ok ? a.scale_log2e : 0.0f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(t[s][k][e]));
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const int ex = norm_exp(__float_as_uint(mx));
+        const float f = pow2_bits(268 - ex);
+        qsc = pow2_bits(ex - 14);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            f16x4 h0, l0, h1, l1;
+            split4(t[s][0][0] * f, t[s][0][1] * f, t[s][0][2] * f, t[s][0][3] * f, h0, l0);
+            split4(t[s][1][0] * f, t[s][1][1] * f, t[s][1][2] * f, t[s][1][3] * f, h1, l1);
+            qh[s] = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+            ql[s] = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+
+    // ---- staging: a block's loads are issued before the products of the block before, and stored after them
+    constexpr int BK = 8 * W;  // keys of a block
+    const int skey = tid >> 3, se0 = E * (tid & 7);
+    const int64_t head = a.sb / a.n_head_kv * w.h_kv;
+    TreeRaw<CT, E> rk, rv;
+    auto page_at = [&](int kb) { return kb + skey < w.k_end ? page_of(a, w.seq, (kb + skey) / kKvBlock) : -1; };
+    auto load_block = [&](int kb, int blk) {  // zeros for missing pages and past the last key
+        if (blk >= 0) {
+            const int64_t off = (((int64_t)blk * a.n_layer + a.layer) * kKvBlock + (kb + skey) % kKvBlock) * a.sb + head;
+            rk.load(a.k_arena + off, se0);
+            rv.load(a.v_arena + off, se0);
+        } else {
+            rk.clear();
+            rv.clear();
+        }
+    };
+    auto store_block = [&](int buf) {
+        rk.store(&sm.b.k[buf][0][skey][se0], &sm.b.k[buf][NPC - 1][skey][se0]);
+        rv.store(&sm.b.v[buf][0][skey][se0], &sm.b.v[buf][NPC - 1][skey][se0]);
+    };
+
+    f32x16 o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[t][v] = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // l: this lane's keys only, until the end
+
+    load_block(w.k_begin, page_at(w.k_begin));
+    int blk_next = page_at(w.k_begin + BK);
+    store_block(0);
+    __syncthreads();
+    int buf = 0;
+    for (int kb = w.k_begin; kb < w.k_end; kb += BK, buf ^= 1) {
+        const bool more = kb + BK < w.k_end;
+        if (more) {
+            load_block(kb + BK, blk_next);
+            blk_next = page_at(kb + 2 * BK);
+        }
+        if (r0 < w.n_rows) {
+#pragma unroll 1
+            for (int sub = 0; sub < BK && kb + sub < w.k_end; sub += 32) {
+                // ---- S^T = K Q^T, the small products apart
+                f32x16 sc, hi;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) sc[v] = 0.0f, hi[v] = 0.0f;
+                const _Float16* kh = &sm.b.k[buf][0][sub + c32][8 * p];
+                const _Float16* kl = &sm.b.k[buf][NPC - 1][sub + c32][8 * p];
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const f16x8 fh = *reinterpret_cast<const f16x8*>(kh + 16 * s);
+                    if constexpr (NPC == 2) {
+                        const f16x8 fl = *reinterpret_cast<const f16x8*>(kl + 16 * s);
+                        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl, qh[s], sc, 0, 0, 0);
+                    }
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fh, ql[s], sc, 0, 0, 0);
+                    hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(fh, qh[s], hi, 0, 0, 0);
+                }
+#pragma unroll
+                for (int v = 0; v < 16; ++v) sc[v] += hi[v];
+
+                // ---- the online softmax of the lane's row over its 16 keys, 8 (i / 4) + 4 p + i % 4
+                const int left = w.k_end - kb - sub;
+                if (left < 32) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (8 * (i >> 2) + 4 * p + (i & 3) >= left) sc[i] = -INFINITY;
+                }
+                float mx = sc[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * qsc;
+                if (__any(mx > m + 8.0f)) {
+                    const float m_new = mx > m + 8.0f ? __builtin_ceilf(mx) : m;
+                    const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+                    l *= alpha;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) o[t][v] *= alpha;
+                    m = m_new;
+                }
+                const float ref = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qsc, ref));
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) l += (sc[i] + sc[i + 1]) + (sc[i + 2] + sc[i + 3]);
+
+                // ---- O^T += V^T P^T: step s takes the lane's weights i = 8s .. 8s + 7, keys 16s + 4p + 0..3
+                // and 16s + 8 + 4p + 0..3
+                const int vrow = sub + 4 * p + ((lane & 15) >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                f16x8 ph[2], pl[2];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    f16x4 h0, l0, h1, l1;
+                    split4(sc[8 * s] * kPieces, sc[8 * s + 1] * kPieces, sc[8 * s + 2] * kPieces, sc[8 * s + 3] * kPieces,
+                           h0, l0);
+                    split4(sc[8 * s + 4] * kPieces, sc[8 * s + 5] * kPieces, sc[8 * s + 6] * kPieces,
+                           sc[8 * s + 7] * kPieces, h1, l1);
+                    ph[s] = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    pl[s] = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        f16x8 f[NPC];
+#pragma unroll
+                        for (int u = 0; u < NPC; ++u) {
+                            const f16x4 a0 = lds_transposed(&sm.b.v[buf][u][16 * s + vrow][32 * t + vcol]);
+                            const f16x4 a1 = lds_transposed(&sm.b.v[buf][u][16 * s + 8 + vrow][32 * t + vcol]);
+                            f[u] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                        }
+                        if constexpr (NPC == 2)
+                            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[1], ph[s], o[t], 0, 0, 0);
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], pl[s], o[t], 0, 0, 0);
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], ph[s], o[t], 0, 0, 0);
+                    }
+            }
+        }
+        if (more) store_block(buf ^ 1);
         __syncthreads();
     }
+    l += __shfl_xor(l, 32, 64);
+
+    // ---- partial results: dims 32t + 8j + 4p + 0..3 of the lane's row
+    bool bad = !(l < INFINITY);
+    const int64_t wrow = (int64_t)w.slot * a.rows + trow * a.n_head + h;
+    float* orow = a.ws_o + wrow * HD;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x4 x = {o[t][4 * j], o[t][4 * j + 1], o[t][4 * j + 2], o[t][4 * j + 3]};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad |= !(fabsf(x[e]) < INFINITY);
+            if (q_ok) *reinterpret_cast<f32x4*>(orow + 32 * t + 8 * j + 4 * p) = x * (1.0f / kPieces);
+        }
+    if (q_ok && p == 0) a.ws_ml[2 * wrow] = m, a.ws_ml[2 * wrow + 1] = l;
+    const uint64_t set = __ballot(bad && q_ok);
+    if (lane == 0) again[wave] = (uint32_t)set | (uint32_t)(set >> 32);
+    __syncthreads();
+#pragma unroll 1
+    for (int k = 0; k < W; ++k)
+        for (uint32_t x = again[k]; x; x &= x - 1)
+            tree_row_again<CT, HD, W>(a, w, sm.t, w.row0 + kRowsPerWave * k + __builtin_ctz(x));
 }
 
 // The merge of a sequence's splits: M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L, zeros for a row
@@ -641,7 +923,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, int hd) {
     const int h = (int)(row % a.n_head), seq = (int)(trow / a.n_tokens), tok = (int)(trow % a.n_tokens);
     const int past = min(max(a.past[seq], 0), a.max_past);
     const int n_draft = a.n_draft ? min(max(a.n_draft[seq], 0), a.n_tokens) : a.n_tokens;
-    const int n_split = tok < n_draft ? max((past + a.kps - 1) / a.kps, 1) : 0;
+    const int n_hist = (past + a.kps - 1) / a.kps;
+    const int n_split = tok < n_draft ? (a.draft_wgs ? n_hist + 1 : max(n_hist, 1)) : 0;
     float m = -INFINITY, l = 0.0f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = p; s0 < n_split; s0 += P * NS) {
@@ -680,11 +963,12 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, int hd) {
 
 // ---------------------------------------------------------------- host side
 struct TreePlan {
+    int block_waves;  // 0: the 16-row kernel
     int tiles, splits, kps;
 };
 
 // Key splits: workgroups until about three per CU have work, 128 keys (a step of each wave) at the least.
-static TreePlan tree_plan(int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
+static TreePlan tree_plan16(int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
     TreePlan p{};
     p.tiles = (n_tokens * (n_head / n_head_kv) + kTile - 1) / kTile;
     const int64_t base = (int64_t)p.tiles * n_head_kv * n_seqs, want = std::max<int64_t>(1, (3 * cu_count() + base - 1) / base);
@@ -693,11 +977,28 @@ static TreePlan tree_plan(int n_head, int n_head_kv, int n_seqs, int n_tokens, i
     return p;
 }
 
+static TreePlan tree_plan(int ct, int hd, int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
+    const int rows = n_tokens * (n_head / n_head_kv);
+    if (ct == kTypeF32 || rows <= 16 || max_past < 256) return tree_plan16(n_head, n_head_kv, n_seqs, n_tokens, max_past);
+    TreePlan p{};
+    p.block_waves = rows > 128 && hd <= 128 ? 8 : 4;
+    p.tiles = (rows + kRowsPerWave * p.block_waves - 1) / (kRowsPerWave * p.block_waves);
+    const int64_t base = (int64_t)p.tiles * n_head_kv * n_seqs, wgs = p.block_waves == 8 ? cu_count() : 2 * cu_count();
+    const int64_t want = std::max<int64_t>(1, (wgs + base - 1) / base);
+    p.kps = (int)std::max<int64_t>(256, round_up((max_past + want - 1) / want, 64));
+    p.splits = 1 + (max_past + p.kps - 1) / p.kps;
+    return p;
+}
+
+static size_t tree_partial_bytes(const TreePlan& p, int hd, int64_t rows) {
+    return p.splits <= 1 ? 0 : (size_t)(round_up(p.splits * rows * hd * 4, 256) + round_up(p.splits * rows * 2 * 4, 256));
+}
+
+// Of the larger plan: the query does not know the cache type.
 size_t tree_workspace_bytes(int hd, int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
-    const TreePlan p = tree_plan(n_head, n_head_kv, n_seqs, n_tokens, max_past);
-    if (p.splits <= 1) return 0;
-    const int64_t rows = (int64_t)p.splits * n_seqs * n_tokens * n_head;
-    return round_up(rows * hd * 4, 256) + round_up(rows * 2 * 4, 256);
+    const int64_t rows = (int64_t)n_seqs * n_tokens * n_head;
+    return std::max(tree_partial_bytes(tree_plan(kTypeF32, hd, n_head, n_head_kv, n_seqs, n_tokens, max_past), hd, rows),
+                    tree_partial_bytes(tree_plan(kTypeF16, hd, n_head, n_head_kv, n_seqs, n_tokens, max_past), hd, rows));
 }
 
 template <int P>
@@ -706,23 +1007,41 @@ static void launch_tree_merge(const TreeArgs& a, int hd, hipStream_t st) {
     hipLaunchKernelGGL((tree_merge_kernel<P>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a, hd);
 }
 
+template <int CT, int HD>
+static void launch_tree_t(const TreeArgs& a, int block_waves, int wgs, hipStream_t st) {
+    if constexpr (CT != kTypeF32) {
+        if constexpr (HD <= 128) {
+            if (block_waves == 8) {
+                hipLaunchKernelGGL((tree_block_kernel<CT, HD, 8>), dim3(wgs), dim3(512), 0, st, a);
+                return;
+            }
+        }
+        if (block_waves == 4) {
+            hipLaunchKernelGGL((tree_block_kernel<CT, HD, 4>), dim3(wgs), dim3(256), 0, st, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((tree_attn_kernel<CT, HD>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
+}
+
 hipError_t launch_tree_attention(int ct, int hd, TreeArgs a, void* ws, hipStream_t st) {
-    const TreePlan p = tree_plan(a.n_head, a.n_head_kv, a.n_seqs, a.n_tokens, a.max_past);
+    const TreePlan p = tree_plan(ct, hd, a.n_head, a.n_head_kv, a.n_seqs, a.n_tokens, a.max_past);
     a.rep = a.n_head / a.n_head_kv;
     a.tiles = p.tiles, a.splits = p.splits, a.kps = p.kps;
     a.rows = (int64_t)a.n_seqs * a.n_tokens * a.n_head;
-    const int64_t units = (int64_t)a.n_seqs * p.splits * a.n_head_kv;
-    const int64_t wgs = (units + 7) / 8 * 8 * p.tiles;
+    a.tiles16 = (a.n_tokens * a.rep + kTile - 1) / kTile;
+    const int64_t drafts = p.block_waves ? (int64_t)a.n_seqs * a.n_head_kv * a.tiles16 : 0;
+    const int64_t units = (int64_t)a.n_seqs * (p.block_waves ? p.splits - 1 : p.splits) * a.n_head_kv;
+    const int64_t wgs = drafts + (units + 7) / 8 * 8 * p.tiles;
     if (wgs > INT32_MAX || a.rows * (hd / 4) * 32 > (int64_t)INT32_MAX * 256) return hipErrorInvalidValue;
-    a.units = (int)units;
+    a.units = (int)units, a.draft_wgs = (int)drafts;
     if (p.splits > 1) {
         a.ws_o = static_cast<float*>(ws);
         a.ws_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round_up(p.splits * a.rows * hd * 4, 256));
     }
-    const dim3 grid((unsigned)wgs);
-#define DCQ_TREE_CASE(C, H)                                                                           \
-    if (ct == C && hd == H) {                                                                         \
-        hipLaunchKernelGGL((tree_attn_kernel<C, H>), grid, dim3(64 * kTreeWaves), 0, st, a);          \
+#define DCQ_TREE_CASE(C, H)                                         \
+    if (ct == C && hd == H) {                                       \
+        launch_tree_t<C, H>(a, p.block_waves, (int)wgs, st);        \
     } else
     DCQ_TREE_CASE(kTypeQ8_0, 128)
     DCQ_TREE_CASE(kTypeQ8_0, 64)

@@ -132,6 +132,9 @@ TREES = [
     (33, [2500], 8, 8, 64),                   # long, no group
     (3, [6000, 10], 8, 2, 128),               # many key splits, and a sequence with one
     (40, [1029], 16, 4, 256),
+    (64, [1500, 300], 8, 2, 128),             # 256 rows
+    (100, [257, 4100, 0], 3, 1, 128),         # 300 rows
+    (9, [3001], 32, 8, 128),                  # 36 rows: a wave of four
 ]
 
 
@@ -157,10 +160,11 @@ def test_tree_attention_ragged_drafts_and_rows_that_see_nothing(KV, dev, ct, hea
 
 @pytest.mark.parametrize("ct", CACHE_TYPES)
 @pytest.mark.parametrize("n,hd", [(3, 128), (40, 128), (30, 64), (20, 256)])
-def test_tree_attention_missing_pages_are_zero_rows(KV, dev, ct, n, hd):
+@pytest.mark.parametrize("past,width", [(200, 11), (900, 50)])
+def test_tree_attention_missing_pages_are_zero_rows(KV, dev, ct, n, hd, past, width):
     """Table entries of -1, and positions past the table's end, are keys of score 0 and value 0."""
-    t = Tree(KV, ct, n, [200, 90], 8, 2, hd, seed=3, holes=[(0, 1), (0, 5), (1, 0)])
-    t.tables = np.ascontiguousarray(t.tables[:, :11])
+    t = Tree(KV, ct, n, [past, 90], 8, 2, hd, seed=3, holes=[(0, 1), (0, 5), (1, 0)])
+    t.tables = np.ascontiguousarray(t.tables[:, :width])
     empty = np.zeros((0, 2 * hd), np.float32)
     t.hist = [[KV.gather(ct, a, t.n_layer, t.layer, t.tables[b], p, empty).reshape(p, 2, hd) for a in t.arena]
               for b, p in enumerate(t.pasts)]
@@ -189,10 +193,11 @@ def test_tree_attention_past_is_clamped(KV, dev):
 
 @pytest.mark.parametrize("ct", CACHE_TYPES)
 @pytest.mark.parametrize("n,heads,kv,hd", [(6, 8, 2, 128), (40, 8, 2, 128), (30, 4, 1, 64), (20, 8, 2, 256)])
-def test_tree_attention_hidden_infinities_and_nan(KV, dev, ct, n, heads, kv, hd):
+@pytest.mark.parametrize("past", [200, 777])
+def test_tree_attention_hidden_infinities_and_nan(KV, dev, ct, n, heads, kv, hd, past):
     """Drafted rows full of infinities and NaN reach only the rows that see them; a NaN beyond the drafted
     tokens reaches none."""
-    t = Tree(KV, ct, n, [70, 200], heads, kv, hd, seed=7, drafts=[n, n - 2])
+    t = Tree(KV, ct, n, [70, past], heads, kv, hd, seed=7, drafts=[n, n - 2])
     t.seen[:, 2:, 1] = False
     t.seen[:, :, 3] = False
     t.kc[:, 1], t.vc[:, 1] = np.nan, np.inf
@@ -205,10 +210,11 @@ def test_tree_attention_hidden_infinities_and_nan(KV, dev, ct, n, heads, kv, hd)
 
 @pytest.mark.parametrize("ct", [F32, F16])
 @pytest.mark.parametrize("n,heads,kv,hd", [(4, 8, 2, 128), (40, 8, 2, 128), (20, 8, 2, 64), (20, 8, 1, 256)])
-def test_tree_attention_infinities_in_the_cache(KV, dev, ct, n, heads, kv, hd):
+@pytest.mark.parametrize("past", [150, 1100])
+def test_tree_attention_infinities_in_the_cache(KV, dev, ct, n, heads, kv, hd, past):
     """As in the arithmetic of the definition: an infinite V element gives its dim that infinity, one of K a weight
     of 0 or NaN by the sign of the score, a NaN gives NaN."""
-    t = Tree(KV, ct, n, [150], heads, kv, hd, seed=8, n_layer=1)
+    t = Tree(KV, ct, n, [past], heads, kv, hd, seed=8, n_layer=1)
     dt = np.float32 if ct == F32 else np.float16
     k, v = (a.view(dt).reshape(t.n_blocks, 16, kv, hd) for a in t.arena)
     page = t.tables[0]
@@ -216,7 +222,7 @@ def test_tree_attention_infinities_in_the_cache(KV, dev, ct, n, heads, kv, hd):
     k[page[4], 1, kv - 1, 5] = np.inf
     t.q[0, :n // 2, heads // kv * (kv - 1):, 5] = -np.abs(t.q[0, :n // 2, heads // kv * (kv - 1):, 5])  # scores of -inf
     empty = np.zeros((0, kv * hd), np.float32)
-    t.hist = [[KV.gather(ct, a, 1, 0, page, 150, empty).reshape(150, kv, hd) for a in t.arena]]
+    t.hist = [[KV.gather(ct, a, 1, 0, page, past, empty).reshape(past, kv, hd) for a in t.arena]]
     out = t.run(dev)
     with np.errstate(invalid="ignore"):
         ref = S.tree_attention(t.q[0], *t.hist[0], t.kc[0], t.vc[0], t.seen[0], t.scale)[0]
