@@ -239,29 +239,46 @@ def _u8(name, t, ndim=(1, 2)):
     _need(name, t, _t().uint8, ndim)
 
 
-def _i32(name, t, ndim=(1,)):
-    try:
-        if t.dtype is _I32 and t.is_cuda and t.dim() in ndim and t.stride(-1) == 1:
-            return
-    except (AttributeError, IndexError):
-        pass
-    _need(name, t, _t().int32, ndim)
+def _plain(t, dtype, shape):
+    """Whether t is a packed GPU tensor of this type and shape: the one test of a usual argument, where _checked
+    takes the unusual ones (a call of the search functions has six to twelve tensors)."""
+    return t.dtype is dtype and t.is_cuda and t.shape == shape and t.is_contiguous()
 
 
-def _shape(name, t, shape):
-    if tuple(t.shape) != tuple(shape):
+def _checked(name, t, dtype, shape, rows=False):
+    """Raise ValueError unless t is a GPU tensor of this type and shape, packed, or with `rows` of packed rows."""
+    _need(name, t, dtype, (len(shape),))
+    if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-
-
-def _packed(name, t, shape):
-    _shape(name, t, shape)
-    if not t.is_contiguous():
+    if not rows and not t.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
 
 
-def _row_stride(t):
-    """Elements between the rows of a 2-D tensor (its width where there is one row, whose stride means nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _rows_of(name, t, dtype, shape):
+    """_checked for rows; the elements between them (the width where there is one row, whose stride means nothing)."""
+    if _plain(t, dtype, shape):
+        return shape[1]
+    _checked(name, t, dtype, shape, rows=True)
+    return t.stride(0) if shape[0] > 1 else shape[1]
+
+
+def _table_shape(name, t):
+    """The two sizes of a 2-D argument that the other arguments' shapes follow from."""
+    try:
+        a, b = t.shape
+    except (AttributeError, ValueError):
+        _need(name, t, _t().int32, (2,))
+        raise
+    return a, b
+
+
+def _made(name, t, dtype, shape, device, rows=False):
+    """An output of this type and shape: the caller's, checked, or a new one."""
+    if t is None:
+        return _torch.empty(shape, dtype=dtype, device=device)
+    if not _plain(t, dtype, shape):
+        _checked(name, t, dtype, shape, rows)
+    return t
 
 
 def quantize_rows(vdt, x, out=None, stream=None):
@@ -594,10 +611,10 @@ class PagedKVCache:
 
     # ---- search: several sequences per call, their block tables int32 [S, T] (rows may be strided)
     def _arenas(self):
-        nbytes = self.n_blocks * self.n_layer * KV_BLOCK_SIZE * self.slot_bytes
-        if self.k.numel() < nbytes or self.v.numel() < nbytes:
-            raise ValueError(f"arenas of {self.k.numel()} and {self.v.numel()} bytes, {self.n_blocks} blocks need {nbytes}")
-        return _ptr(self.k), _ptr(self.v)
+        k, v, nbytes = self.k, self.v, self.n_blocks * self.n_layer * KV_BLOCK_SIZE * self.slot_bytes
+        if k.numel() < nbytes or v.numel() < nbytes:
+            raise ValueError(f"arenas of {k.numel()} and {v.numel()} bytes, {self.n_blocks} blocks need {nbytes}")
+        return k.data_ptr(), v.data_ptr()
 
     def tree_attention(self, layer, tables, past, max_past, q, k_cur, v_cur, scale, mask=None, n_draft=None, out=None,
                        workspace=None, stream=None):
@@ -606,74 +623,82 @@ class PagedKVCache:
         mask int64 [S, N, (N + 63) // 64], bit i of row j set where token j sees drafted token i (None: i <= j),
         n_draft int32 [S] drafted tokens of the N (None: all). Rows that see nothing, or past n_draft, are zeros."""
         torch = _torch or _t()
-        for name, t in (("q", q), ("k_cur", k_cur), ("v_cur", v_cur)):
-            _f32(name, t)
-        _i32("tables", tables, (2,))
-        _i32("past", past)
-        s, rows = tables.shape[0], q.shape[0]
+        s, width = _table_shape("tables", tables)
+        rows, q_width = q_shape = _table_shape("q", q)
         n = rows // s if s else 0
-        if s == 0 or n == 0 or rows != s * n:
+        if n == 0 or rows != s * n:
             raise ValueError(f"q: {rows} rows of {s} sequences")
-        if q.shape[1] % self.head_dim:
-            raise ValueError(f"q: {q.shape[1]} values per row are no heads of {self.head_dim}")
-        n_head = q.shape[1] // self.head_dim
-        _shape("k_cur", k_cur, (rows, self.row_elems))
-        _shape("v_cur", v_cur, (rows, self.row_elems))
-        if _row_stride(k_cur) != _row_stride(v_cur):
+        n_head = q_width // self.head_dim
+        if n_head * self.head_dim != q_width:
+            raise ValueError(f"q: {q_width} values per row are no heads of {self.head_dim}")
+        cur = (rows, self.row_elems)
+        table_stride = _rows_of("tables", tables, _I32, (s, width))
+        q_stride = _rows_of("q", q, _F32, q_shape)
+        kv_stride = _rows_of("k_cur", k_cur, _F32, cur)
+        if _rows_of("v_cur", v_cur, _F32, cur) != kv_stride:
             raise ValueError(f"k_cur and v_cur must share a row stride (the ABI takes one): "
                              f"{k_cur.stride(0)} != {v_cur.stride(0)}")
-        _packed("past", past, (s,))
+        if not _plain(past, _I32, (s,)):
+            _checked("past", past, _I32, (s,))
         if mask is not None:
-            _need("mask", mask, torch.int64, (3,))
-            _packed("mask", mask, (s, n, (n + 63) // 64))
-        if n_draft is not None:
-            _i32("n_draft", n_draft)
-            _packed("n_draft", n_draft, (s,))
+            shape = (s, n, (n + 63) // 64)
+            if not _plain(mask, torch.int64, shape):
+                _checked("mask", mask, torch.int64, shape)
+        if n_draft is not None and not _plain(n_draft, _I32, (s,)):
+            _checked("n_draft", n_draft, _I32, (s,))
         if out is None:
-            out = torch.empty((rows, q.shape[1]), dtype=torch.float32, device=q.device)
-        _f32("out", out)
-        _shape("out", out, q.shape)
+            out = torch.empty(q_shape, dtype=_F32, device=q.device)
+        out_stride = _rows_of("out", out, _F32, q_shape)
         if workspace is None:
             need = kv_tree_attention_workspace_size(n_head, self.n_head_kv, self.head_dim, s, n, max_past)
             if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+                workspace = torch.empty(need, dtype=_U8, device=q.device)
         k, v = self._arenas()
-        _check("dcq_kv_tree_attention", lib().dcq_kv_tree_attention(
-            self.cache_type, k, v, self.n_blocks, self.n_layer, layer, _ptr(tables), _row_stride(tables),
-            tables.shape[1], _ptr(past), max_past, _ptr(n_draft), _ptr(mask), n_head, self.n_head_kv, self.head_dim,
-            _ptr(q), _row_stride(q) * 4, _ptr(k_cur), _ptr(v_cur), _row_stride(k_cur) * 4, s, n, scale, _ptr(out),
-            _row_stride(out) * 4, _ptr(workspace), _nbytes(workspace), _stream(stream)))
+        status = lib().dcq_kv_tree_attention(
+            self.cache_type, k, v, self.n_blocks, self.n_layer, layer, tables.data_ptr(), table_stride, width,
+            past.data_ptr(), max_past, _ptr(n_draft), _ptr(mask), n_head, self.n_head_kv, self.head_dim, q.data_ptr(),
+            q_stride * 4, k_cur.data_ptr(), v_cur.data_ptr(), kv_stride * 4, s, n, scale, out.data_ptr(), out_stride * 4,
+            _ptr(workspace), _nbytes(workspace), _stream(stream))
+        if status:
+            raise DcqError("dcq_kv_tree_attention", status)
         return out
 
     def write_path(self, tables, past, path, n_path, k_cur, v_cur, stream=None):
         """The accepted tokens' rows into the cache, every layer: place j < n_path[b] (int32 [S]; None: all P) of
         path int32 [S, P] names a drafted token, whose rows of k_cur / v_cur [n_layer, S * N, row_elems] go to
         position past[b] + j of sequence b."""
-        for name, t in (("k_cur", k_cur), ("v_cur", v_cur)):
-            _f32(name, t, (3,))
-        _i32("tables", tables, (2,))
-        _i32("past", past)
-        _i32("path", path, (2,))
-        s, rows = tables.shape[0], k_cur.shape[1]
+        _torch or _t()
+        s, width = _table_shape("tables", tables)
+        rows = k_cur.shape[1] if getattr(k_cur, "ndim", 0) == 3 else 0
         n = rows // s if s else 0
-        if s == 0 or n == 0 or rows != s * n:
+        if n == 0 or rows != s * n:
             raise ValueError(f"k_cur: {rows} rows of {s} sequences")
-        _shape("k_cur", k_cur, (self.n_layer, rows, self.row_elems))
-        _shape("v_cur", v_cur, k_cur.shape)
-        strides = [(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if rows > 1 else self.row_elems)
-                   for t in (k_cur, v_cur)]
-        if strides[0] != strides[1]:
-            raise ValueError(f"k_cur and v_cur must share their strides (the ABI takes one): {strides[0]} != {strides[1]}")
-        _packed("past", past, (s,))
-        _shape("path", path, (s, path.shape[1]))
-        if n_path is not None:
-            _i32("n_path", n_path)
-            _packed("n_path", n_path, (s,))
+        elems = self.row_elems
+        shape = (self.n_layer, rows, elems)
+        if _plain(k_cur, _F32, shape) and _plain(v_cur, _F32, shape):
+            layer_stride, kv_stride = rows * elems, elems
+        else:
+            _checked("k_cur", k_cur, _F32, shape, rows=True)
+            _checked("v_cur", v_cur, _F32, shape, rows=True)
+            strides = [(t.stride(0) if self.n_layer > 1 else 0, t.stride(1) if rows > 1 else elems) for t in (k_cur, v_cur)]
+            if strides[0] != strides[1]:
+                raise ValueError(f"k_cur and v_cur must share their strides (the ABI takes one): "
+                                 f"{strides[0]} != {strides[1]}")
+            layer_stride, kv_stride = strides[0]
+        table_stride = _rows_of("tables", tables, _I32, (s, width))
+        path_shape = _table_shape("path", path)
+        path_stride = _rows_of("path", path, _I32, (s, path_shape[1]))
+        if not _plain(past, _I32, (s,)):
+            _checked("past", past, _I32, (s,))
+        if n_path is not None and not _plain(n_path, _I32, (s,)):
+            _checked("n_path", n_path, _I32, (s,))
         k, v = self._arenas()
-        _check("dcq_kv_write_path", lib().dcq_kv_write_path(
-            self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, _ptr(tables), _row_stride(tables),
-            tables.shape[1], _ptr(past), _ptr(path), _row_stride(path), path.shape[1], _ptr(n_path), _ptr(k_cur),
-            _ptr(v_cur), strides[0][0] * 4, strides[0][1] * 4, s, n, _stream(stream)))
+        status = lib().dcq_kv_write_path(
+            self.cache_type, k, v, self.n_blocks, self.n_layer, elems, tables.data_ptr(), table_stride, width,
+            past.data_ptr(), path.data_ptr(), path_stride, path_shape[1], _ptr(n_path), k_cur.data_ptr(),
+            v_cur.data_ptr(), layer_stride * 4, kv_stride * 4, s, n, _stream(stream))
+        if status:
+            raise DcqError("dcq_kv_write_path", status)
 
     def fork(self, tables, lengths, parents, refs, tables_out=None, lengths_out=None, refs_out=None, missing=None,
              workspace=None, stream=None):
@@ -681,58 +706,53 @@ class PagedKVCache:
         copy of a partial last page where two would write into it. refs int32 [n_blocks] counts each page's
         holders. Returns (tables [C, T], lengths [C], refs, missing [1]: the copies that found no free page)."""
         torch = _torch or _t()
-        _i32("tables", tables, (2,))
-        for name, t in (("lengths", lengths), ("parents", parents), ("refs", refs)):
-            _i32(name, t)
-        (s, width), c = tables.shape, parents.shape[0]
-        _packed("lengths", lengths, (s,))
-        _packed("parents", parents, (c,))
-        _packed("refs", refs, (self.n_blocks,))
-        made = []
-        for name, t, shape in (("tables_out", tables_out, (c, width)), ("lengths_out", lengths_out, (c,)),
-                               ("refs_out", refs_out, (self.n_blocks,)), ("missing", missing, (1,))):
-            if t is None:
-                t = torch.empty(shape, dtype=torch.int32, device=tables.device)
-            _i32(name, t, (len(shape),))
-            (_shape if len(shape) == 2 else _packed)(name, t, shape)
-            made.append(t)
+        s, width = _table_shape("tables", tables)
+        c, blocks = len(parents), (self.n_blocks,)
+        table_stride = _rows_of("tables", tables, _I32, (s, width))
+        for name, t, shape in (("lengths", lengths, (s,)), ("parents", parents, (c,)), ("refs", refs, blocks)):
+            if not _plain(t, _I32, shape):
+                _checked(name, t, _I32, shape)
+        device = refs.device
+        tables_out = _made("tables_out", tables_out, _I32, (c, width), device, rows=True)
+        lengths_out = _made("lengths_out", lengths_out, _I32, (c,), device)
+        refs_out = _made("refs_out", refs_out, _I32, blocks, device)
+        missing = _made("missing", missing, _I32, (1,), device)
         if workspace is None:
-            workspace = torch.empty(max(kv_fork_workspace_size(self.n_blocks, s, c), 256), dtype=torch.uint8,
-                                    device=tables.device)
+            workspace = torch.empty(max(kv_fork_workspace_size(self.n_blocks, s, c), 256), dtype=_U8, device=device)
         k, v = self._arenas()
-        _check("dcq_kv_fork", lib().dcq_kv_fork(
-            self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, _ptr(tables), _row_stride(tables),
-            width, _ptr(lengths), s, _ptr(parents), c, _ptr(refs), _ptr(made[0]), _row_stride(made[0]), _ptr(made[1]),
-            _ptr(made[2]), _ptr(made[3]), _ptr(workspace), _nbytes(workspace), _stream(stream)))
-        return tuple(made)
+        status = lib().dcq_kv_fork(
+            self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, tables.data_ptr(), table_stride, width,
+            lengths.data_ptr(), s, parents.data_ptr(), c, refs.data_ptr(), tables_out.data_ptr(),
+            tables_out.stride(0) if c > 1 else width, lengths_out.data_ptr(), refs_out.data_ptr(), missing.data_ptr(),
+            workspace.data_ptr(), _nbytes(workspace), _stream(stream))
+        if status:
+            raise DcqError("dcq_kv_fork", status)
+        return tables_out, lengths_out, refs_out, missing
 
     def compact(self, tables, lengths, refs, tables_out=None, refs_out=None, n_live=None, workspace=None, stream=None):
         """The pages in use (refs > 0) to the front of the arenas. Returns (tables [S, T] with the moved pages'
         new numbers, refs in their new places, n_live [1])."""
         torch = _torch or _t()
-        _i32("tables", tables, (2,))
-        for name, t in (("lengths", lengths), ("refs", refs)):
-            _i32(name, t)
-        s, width = tables.shape
-        _packed("lengths", lengths, (s,))
-        _packed("refs", refs, (self.n_blocks,))
-        made = []
-        for name, t, shape in (("tables_out", tables_out, (s, width)), ("refs_out", refs_out, (self.n_blocks,)),
-                               ("n_live", n_live, (1,))):
-            if t is None:
-                t = torch.empty(shape, dtype=torch.int32, device=tables.device)
-            _i32(name, t, (len(shape),))
-            (_shape if len(shape) == 2 else _packed)(name, t, shape)
-            made.append(t)
+        s, width = _table_shape("tables", tables)
+        blocks = (self.n_blocks,)
+        table_stride = _rows_of("tables", tables, _I32, (s, width))
+        for name, t, shape in (("lengths", lengths, (s,)), ("refs", refs, blocks)):
+            if not _plain(t, _I32, shape):
+                _checked(name, t, _I32, shape)
+        device = refs.device
+        tables_out = _made("tables_out", tables_out, _I32, (s, width), device, rows=True)
+        refs_out = _made("refs_out", refs_out, _I32, blocks, device)
+        n_live = _made("n_live", n_live, _I32, (1,), device)
         if workspace is None:
-            workspace = torch.empty(max(kv_compact_workspace_size(self.n_blocks), 256), dtype=torch.uint8,
-                                    device=tables.device)
+            workspace = torch.empty(max(kv_compact_workspace_size(self.n_blocks), 256), dtype=_U8, device=device)
         k, v = self._arenas()
-        _check("dcq_kv_compact", lib().dcq_kv_compact(
-            self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, _ptr(tables), _row_stride(tables),
-            width, _ptr(lengths), s, _ptr(refs), _ptr(made[0]), _row_stride(made[0]), _ptr(made[1]), _ptr(made[2]),
-            _ptr(workspace), _nbytes(workspace), _stream(stream)))
-        return tuple(made)
+        status = lib().dcq_kv_compact(
+            self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, tables.data_ptr(), table_stride, width,
+            lengths.data_ptr(), s, refs.data_ptr(), tables_out.data_ptr(), tables_out.stride(0) if s > 1 else width,
+            refs_out.data_ptr(), n_live.data_ptr(), workspace.data_ptr(), _nbytes(workspace), _stream(stream))
+        if status:
+            raise DcqError("dcq_kv_compact", status)
+        return tables_out, refs_out, n_live
 
 
 def kv_attention_workspace_size(n_head, n_head_kv, head_dim, n_tokens, n_past):
@@ -761,28 +781,27 @@ def beam_select(logits, beam_scores, n_out, scores=None, parents=None, tokens=No
     (scores fp32, parents int32: rows b * W + w, tokens int32), each [B, n_out], best first, ties to the lower
     beam, then token; -inf, -1, -1 where there are no more."""
     torch = _torch or _t()
-    half = getattr(logits, "dtype", None) is torch.float16
-    _need("logits", logits, torch.float16 if half else torch.float32, (2,))
-    _f32("beam_scores", beam_scores)
-    b, w = beam_scores.shape
-    _packed("beam_scores", beam_scores, (b, w))
-    vocab = logits.shape[1]
-    _shape("logits", logits, (b * w, vocab))
-    made = []
-    for name, t, dtype in (("scores", scores, torch.float32), ("parents", parents, torch.int32),
-                           ("tokens", tokens, torch.int32)):
-        if t is None:
-            t = torch.empty((b, n_out), dtype=dtype, device=logits.device)
-        _need(name, t, dtype, (2,))
-        _packed(name, t, (b, n_out))
-        made.append(t)
+    b, w = _table_shape("beam_scores", beam_scores)
+    rows, vocab = shape = _table_shape("logits", logits)
+    half = logits.dtype is torch.float16
+    if rows != b * w:
+        raise ValueError(f"logits: {rows} rows of {b} requests of {w} beams")
+    stride = _rows_of("logits", logits, torch.float16 if half else _F32, shape)
+    if not _plain(beam_scores, _F32, (b, w)):
+        _checked("beam_scores", beam_scores, _F32, (b, w))
+    device, out = logits.device, (b, n_out)
+    scores = _made("scores", scores, _F32, out, device)
+    parents = _made("parents", parents, _I32, out, device)
+    tokens = _made("tokens", tokens, _I32, out, device)
     if workspace is None:
-        workspace = torch.empty(max(beam_select_workspace_size(b, w, vocab, n_out), 256), dtype=torch.uint8,
-                                device=logits.device)
-    _check("dcq_beam_select", lib().dcq_beam_select(
-        1 if half else 0, _ptr(logits), _row_stride(logits) * (2 if half else 4), b, w, vocab, _ptr(beam_scores), n_out,
-        _ptr(made[0]), _ptr(made[1]), _ptr(made[2]), _ptr(workspace), _nbytes(workspace), _stream(stream)))
-    return tuple(made)
+        workspace = torch.empty(max(beam_select_workspace_size(b, w, vocab, n_out), 256), dtype=_U8, device=device)
+    status = lib().dcq_beam_select(
+        1 if half else 0, logits.data_ptr(), stride * (2 if half else 4), b, w, vocab, beam_scores.data_ptr(), n_out,
+        scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), _nbytes(workspace),
+        _stream(stream))
+    if status:
+        raise DcqError("dcq_beam_select", status)
+    return scores, parents, tokens
 
 
 # ---------------------------------------------------------------- measurement aid (include/dcq_probe.h)

@@ -7,8 +7,8 @@
 //                      2^ref sum 2^(x log2 e - ref), and its n_out largest logits (their order is the scores')
 //   beam_join_kernel   per request: lse of each row in 64 bits, and the n_out best of the chunks' candidates
 //                      by their 64-bit scores
-// A chunk's largest are found without sorting it: the n_out-th largest of the maxima of 64 groups of threads
-// is a bound that n_out elements reach at least and few others do; those are ranked against each other.
+// A chunk's largest are found without sorting it: just below the n_out-th largest of the maxima of 64 groups of
+// threads lies a bound that n_out elements reach at least and few others do; those are ranked against each other.
 #include <algorithm>
 
 #include "dcq_common.h"
@@ -22,27 +22,32 @@ constexpr int kBeamCap = 1024;  // candidates that are ranked; more (ties) are t
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLog2eLow = (float)(1.4426950408889634 - (double)kLog2e);
 
-// Order of logits, then of indices from the lowest: larger key first. 0 is no candidate's.
+__device__ __forceinline__ uint32_t order_bits(float x) {  // larger for larger x; -0 below 0
+    const uint32_t b = __float_as_uint(x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float order_value(uint32_t o) {
+    return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+// Order of logits, then of indices (beam << 24 | token) from the lowest: larger key first. 0 is no candidate's.
 __device__ __forceinline__ uint64_t beam_key(float x, uint32_t idx) {
-    const uint32_t b = __float_as_uint(x + 0.0f);  // -0 as 0
-    return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - idx);
+    return (uint64_t)order_bits(x + 0.0f) << 32 | (0xFFFFFFFFu - idx);  // -0 as 0
 }
-__device__ __forceinline__ float key_logit(uint64_t key) {
-    const uint32_t b = (uint32_t)(key >> 32);
-    return __uint_as_float(b & 0x80000000u ? b & 0x7FFFFFFFu : ~b);
-}
+__device__ __forceinline__ float key_logit(uint64_t key) { return order_value((uint32_t)(key >> 32)); }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
 
-// The n-th largest (n <= 64) of the 64 values in a wave's lanes.
-__device__ __forceinline__ float lanes_nth_largest(float v, int n) {
-    const int lane = threadIdx.x & 63;
-    int rank = 0;
+// A bound that n (<= 64) of the values in a wave's 64 lanes reach: the n-th largest to 20 bits (its sign,
+// exponent and 11 bits, the rest as low as can be), found bit by bit with one comparison each. No more exact: a
+// bound a thousandth lower lets a few candidates more through.
+__device__ __forceinline__ float lanes_bound(float v, int n) {
+    const uint32_t o = order_bits(v);
+    uint32_t t = 0;
 #pragma unroll
-    for (int k = 0; k < 64; ++k) {
-        const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), k));
-        rank += o > v || (o == v && k < lane);
+    for (int b = 31; b >= 12; --b) {
+        const uint32_t with = t | 1u << b;
+        if ((int)__popcll(__ballot(o >= with)) >= n) t = with;
     }
-    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), __ffsll((unsigned long long)__ballot(rank == n - 1)) - 1));
+    return t < 0x00800000u ? -INFINITY : order_value(t);  // below the finite ones
 }
 
 template <class T, int EPT>
@@ -56,6 +61,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t row = blockIdx.y;
     const int chunk = blockIdx.x;
+    const uint32_t beam = (uint32_t)(row % a.n_beams) << 24;
     const T* x = static_cast<const T*>(a.x) + row * a.stride;
     // the same elements to a thread whatever the row's alignment: rows of equal logits have equal sums
     float e[NV][V];
@@ -76,14 +82,10 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
         }
     }
     float tmax = -INFINITY;
-    bool any_nan = false;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            tmax = fmaxf(tmax, e[j][k]);
-            any_nan |= e[j][k] != e[j][k];
-        }
+        for (int k = 0; k < V; ++k) tmax = fmaxf(tmax, e[j][k]);
     const float qmax = lanes_max<4>(tmax);
     if (lane % 4 == 0) gmax[tid / 4] = qmax;
     const float wm = lanes_max<64>(tmax);
@@ -91,40 +93,34 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
     if (tid == 0) count = 0;
     __syncthreads();
     const float top = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-    double ref = 0.0, part[2] = {0.0, 0.0};
-    if (fabsf(top) < 65536.0f) {
+    // exp x = 2^ref 2^(x log2 e - ref) (1 + ln 2 low): the product rounded, and what that left, to first order.
+    // ref is 0 for all logits but far ones, and then a multiple of 64, so that a term is the same number in
+    // whatever chunk it is
+    const float far = top * kLog2e;
+    const float ref = fabsf(far) < 64.0f || top == -INFINITY ? 0.0f : 64.0f * rintf(far * (1.0f / 64.0f));
+    double part[2] = {0.0, 0.0};
+    {
 #pragma clang fp contract(off)
-        // 2^(x log2 e) = 2^n 2^f, n whole, x log2 e to 2^-24 in two parts, so that a term is the same number in
-        // whatever chunk it is
-        const float n_top = floorf(top * kLog2e), cut = top - 150.0f;
-        ref = n_top;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const float y = e[j][k], hi = y * kLog2e, lo = fmaf(y, kLog2eLow, fmaf(y, kLog2e, -hi));
-                const float f = __builtin_amdgcn_fractf(hi), n = hi - f;
-                const float p = __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f + lo), (int)(n - n_top));
-                part[k % 2] += (double)(y < cut ? 0.0f : p);  // NaN stays
+                const float y = e[j][k], hi = y * kLog2e;
+                // in bounds where the first order says nothing, and a number beside -infinity
+                const float lo = __builtin_amdgcn_fmed3f(fmaf(y, kLog2eLow, fmaf(y, kLog2e, -hi)), -0.5f, 0.5f);
+                const float t = __builtin_amdgcn_exp2f(hi - ref);
+                part[k % 2] += (double)fmaf(t * lo, 0.693147181f, t);
             }
-    } else if (top != -INFINITY) {
-        ref = (double)top * 1.4426950408889634;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int k = 0; k < V; ++k) part[k % 2] += (double)__builtin_amdgcn_exp2f((e[j][k] - top) * kLog2e);
-    } else if (__any(any_nan)) {
-        part[0] = (double)NAN;
     }
     double sum = part[0] + part[1];
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s, 64);
     if (lane == 0) wsum[wave] = sum;
 
-    // ---- elements no smaller than the n_out-th largest group maximum
-    const float bound = lanes_nth_largest(gmax[lane], a.n_out);
+    // ---- elements no smaller than the bound on the groups' maxima
+    const float bound = lanes_bound(gmax[lane], a.n_out);
     const int64_t list = row * a.chunks + chunk;
-    auto index_of = [&](int j, int k) { return (uint32_t)((v0 + j * kBeamThreads) * V + k); };
+    auto index_of = [&](int j, int k) { return beam | (uint32_t)((v0 + j * kBeamThreads) * V + k); };
     if (tmax >= bound && tmax > -INFINITY) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -173,35 +169,42 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
     }
 }
 
-// A candidate before another: the higher score, then the lower beam * vocab + token.
+// A candidate before another: the higher score, then the lower beam << 24 | token.
 struct BeamPick {
     double score;
-    int64_t at;
+    uint32_t at;
     __device__ __forceinline__ bool before(const BeamPick& o) const {
         return score > o.score || (score == o.score && at < o.at);
     }
 };
 
-__global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(BeamArgs a) {
+constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / 64;
+__global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
+    constexpr int NK = 4;  // candidates of a thread that wait in registers
     __shared__ BeamPick picks[kBeamCap];
     __shared__ double lse[kBeamMaxBeams], base[kBeamMaxBeams];
     __shared__ float gmax[64];
-    __shared__ BeamPick wbest[4];
+    __shared__ BeamPick wbest[kJoinWaves];
     __shared__ int count;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t req = blockIdx.x, row0 = req * a.n_beams;
+    const int per_beam = a.chunks * a.n_out, total = a.n_beams * per_beam;
+    const uint64_t* cand = a.cand + row0 * per_beam;
+    uint64_t mine[NK];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) mine[k] = tid + k * kJoinThreads < total ? cand[tid + k * kJoinThreads] : 0;
     // ---- lse of each row; base is NaN for a beam without continuations
-    for (int w = wave; w < a.n_beams; w += 4) {
+    for (int w = wave; w < a.n_beams; w += kJoinWaves) {
         const int64_t list = (row0 + w) * a.chunks;
         double m = -(double)INFINITY;
         for (int c = lane; c < a.chunks; c += 64)
-            if (a.stat_sum[list + c] != 0.0) m = fmax(m, a.stat_ref[list + c]);
+            if (a.stat_sum[list + c] != 0.0) m = fmax(m, (double)a.stat_ref[list + c]);
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) m = fmax(m, __shfl_xor(m, k, 64));
         double s = 0.0;
         for (int c = lane; c < a.chunks; c += 64) {
             const double sc = a.stat_sum[list + c];
-            s += sc == 0.0 ? 0.0 : sc * exp2(a.stat_ref[list + c] - m);
+            s += sc == 0.0 ? 0.0 : ldexp(sc, (int)fmax((double)a.stat_ref[list + c] - m, -4096.0));
         }
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k, 64);
@@ -214,37 +217,36 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(BeamArgs a) {
     }
     if (tid == 0) count = 0;
     __syncthreads();
-    const int lists = a.n_beams * a.chunks;
-    const uint64_t* cand = a.cand + row0 * a.chunks * a.n_out;
-    auto pick_of = [&](int w, uint64_t key) {
-        return BeamPick{base[w] + ((double)key_logit(key) - lse[w]), (int64_t)w * a.vocab + key_index(key)};
+    auto pick_of = [&](uint64_t key) {
+        const uint32_t at = key_index(key), w = at >> 24;
+        return BeamPick{base[w] + ((double)key_logit(key) - lse[w]), at};
     };
-    // ---- a bound as in the chunks, on the lists' first candidates (rounded down to fp32: no higher)
+    // every candidate, those in registers first
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+            if (mine[k]) f(pick_of(mine[k]));
+        for (int i = tid + NK * kJoinThreads; i < total; i += kJoinThreads)
+            if (const uint64_t key = cand[i]) f(pick_of(key));
+    };
+    // ---- a bound as in the chunks, on the largest score of 64 groups of threads (rounded down to fp32: no higher)
     float tmax = -INFINITY;
-    for (int i = tid; i < lists; i += kBeamThreads) {
-        const uint64_t key = cand[(int64_t)i * a.n_out];
-        if (key) tmax = fmaxf(tmax, __double2float_rd(pick_of(i / a.chunks, key).score));
-    }
-    const float qmax = lanes_max<4>(tmax);
-    if (lane % 4 == 0) gmax[tid / 4] = qmax;
+    each([&](const BeamPick& p) { tmax = fmaxf(tmax, __double2float_rd(p.score)); });
+    const float gm = lanes_max<16>(tmax);
+    if (lane % 16 == 0) gmax[tid / 16] = gm;
     __syncthreads();
-    const double bound = lanes_nth_largest(gmax[lane], a.n_out);
-    for (int i = tid; i < lists; i += kBeamThreads) {
-        for (int r = 0; r < a.n_out; ++r) {
-            const uint64_t key = cand[(int64_t)i * a.n_out + r];
-            if (!key) break;
-            const BeamPick p = pick_of(i / a.chunks, key);
-            if (!(p.score >= bound)) break;  // a list is in order; NaN: a beam without continuations
-            const int at = atomicAdd(&count, 1);
-            if (at < kBeamCap) picks[at] = p;
-        }
-    }
+    const double bound = lanes_bound(gmax[lane], a.n_out);
+    each([&](const BeamPick& p) {
+        if (!(p.score >= bound)) return;  // NaN: of a beam without continuations
+        const int at = atomicAdd(&count, 1);
+        if (at < kBeamCap) picks[at] = p;
+    });
     __syncthreads();
     auto put = [&](int r, const BeamPick& p) {
         const int64_t o = req * a.n_out + r;
         a.scores[o] = (float)p.score;
-        a.parents[o] = (int32_t)(row0 + p.at / a.vocab);
-        a.tokens[o] = (int32_t)(p.at % a.vocab);
+        a.parents[o] = (int32_t)(row0 + (p.at >> 24));
+        a.tokens[o] = (int32_t)(p.at & 0xFFFFFFu);
     };
     auto put_none = [&](int r) {
         const int64_t o = req * a.n_out + r;
@@ -252,33 +254,30 @@ __global__ void __launch_bounds__(kBeamThreads) beam_join_kernel(BeamArgs a) {
     };
     const int n = count;
     if (n <= kBeamCap) {
-        for (int i = tid; i < n; i += kBeamThreads) {
+        for (int i = tid; i < n; i += kJoinThreads) {
             const BeamPick p = picks[i];
             int rank = 0;
             for (int k = 0; k < n; ++k) rank += picks[k].before(p);
             if (rank < a.n_out) put(rank, p);
         }
-        for (int i = n + tid; i < a.n_out; i += kBeamThreads) put_none(i);
+        for (int i = n + tid; i < a.n_out; i += kJoinThreads) put_none(i);
         return;
     }
-    BeamPick last{INFINITY, -1};
+    BeamPick last{INFINITY, 0};
     for (int r = 0; r < a.n_out; ++r) {
-        BeamPick mine{-INFINITY, INT64_MAX};
-        for (int64_t i = tid; i < (int64_t)lists * a.n_out; i += kBeamThreads) {
-            const uint64_t key = cand[i];
-            if (!key) continue;
-            const BeamPick p = pick_of((int)(i / a.n_out / a.chunks), key);
-            if (last.before(p) && p.before(mine)) mine = p;
-        }
+        BeamPick best{-INFINITY, 0xFFFFFFFFu};
+        each([&](const BeamPick& p) {
+            if (last.before(p) && p.before(best)) best = p;
+        });
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) {
-            const BeamPick o{__shfl_xor(mine.score, k, 64), (int64_t)__shfl_xor((long long)mine.at, k, 64)};
-            if (o.before(mine)) mine = o;
+            const BeamPick o{__shfl_xor(best.score, k, 64), (uint32_t)__shfl_xor((int)best.at, k, 64)};
+            if (o.before(best)) best = o;
         }
-        if (lane == 0) wbest[wave] = mine;
+        if (lane == 0) wbest[wave] = best;
         __syncthreads();
         last = wbest[0];
-        for (int k = 1; k < 4; ++k)
+        for (int k = 1; k < kJoinWaves; ++k)
             if (wbest[k].before(last)) last = wbest[k];
         if (tid == 0) put(r, last);  // more than kBeamCap candidates: there is one in every round
         __syncthreads();
@@ -298,7 +297,7 @@ static BeamPlan beam_plan(int64_t rows, int vocab) {
 
 size_t beam_workspace_bytes(int64_t n_batch, int n_beams, int vocab, int n_out) {
     const int64_t lists = n_batch * n_beams * beam_plan(n_batch * n_beams, vocab).chunks;
-    return (size_t)(2 * round_up(lists * 8, 256) + round_up(lists * n_out * 8, 256));
+    return (size_t)(round_up(lists * 8, 256) + round_up(lists * 4, 256) + round_up(lists * n_out * 8, 256));
 }
 
 hipError_t launch_beam_select(int type, BeamArgs a, int64_t n_batch, void* ws, hipStream_t st) {
@@ -308,8 +307,8 @@ hipError_t launch_beam_select(int type, BeamArgs a, int64_t n_batch, void* ws, h
     const int64_t lists = rows * p.chunks;
     uint8_t* w = static_cast<uint8_t*>(ws);
     a.stat_sum = reinterpret_cast<double*>(w);
-    a.stat_ref = reinterpret_cast<double*>(w + round_up(lists * 8, 256));
-    a.cand = reinterpret_cast<uint64_t*>(w + 2 * round_up(lists * 8, 256));
+    a.stat_ref = reinterpret_cast<float*>(w + round_up(lists * 8, 256));
+    a.cand = reinterpret_cast<uint64_t*>(w + round_up(lists * 8, 256) + round_up(lists * 4, 256));
     const dim3 grid((unsigned)p.chunks, (unsigned)rows);
     if (type == kTypeF32 && p.ept == 32)
         hipLaunchKernelGGL((beam_chunk_kernel<float, 32>), grid, dim3(kBeamThreads), 0, st, a);
@@ -321,7 +320,7 @@ hipError_t launch_beam_select(int type, BeamArgs a, int64_t n_batch, void* ws, h
         hipLaunchKernelGGL((beam_chunk_kernel<_Float16, 8>), grid, dim3(kBeamThreads), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)n_batch), dim3(kBeamThreads), 0, st, a);
+    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)n_batch), dim3(kJoinThreads), 0, st, a);
     return hipGetLastError();
 }
 

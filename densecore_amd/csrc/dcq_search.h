@@ -113,7 +113,7 @@ struct BeamArgs {
     int32_t* tokens;
     int chunks;  // from here on the launcher's
     double* stat_sum;
-    double* stat_ref;
+    float* stat_ref;
     uint64_t* cand;  // [rows][chunks][n_out]
 };
 size_t beam_workspace_bytes(int64_t n_batch, int n_beams, int vocab, int n_out);
