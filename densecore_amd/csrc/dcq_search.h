@@ -31,7 +31,7 @@ struct TreeArgs {
     int64_t out_stride;
     int n_seqs, n_tokens, n_head, n_head_kv;
     float scale_log2e;
-    int rep, tiles, tiles16, splits, kps, units, draft_wgs;
+    int rep, tiles, tiles16, splits, kps, units, hist_wgs, draft_wgs;
     int64_t rows;  // n_seqs * n_tokens * n_head
     float* ws_o;   // [splits][rows][HD]
     float* ws_ml;  // [splits][rows][2]

@@ -43,6 +43,11 @@ constexpr int kTreeWaves = 4;      // waves of a workgroup, a share of the keys 
 constexpr int kRowsPerWave = 32;   // of the block kernel
 constexpr float kPieces = 128.0f;  // of the weights in O: 2^15 at most before the reference is raised
 
+// An empty use: the operand of a matrix instruction stays in its registers until here, so that no result is put
+// over it.
+__device__ __forceinline__ void keep(f32x4 x) { asm volatile("" ::"v"(x)); }
+__device__ __forceinline__ void keep(f16x8 x) { asm volatile("" ::"v"(x)); }
+
 template <int CT>
 constexpr int tree_chunk() { return CT == kTypeF32 ? 16 : 32; }  // keys of a wave's step
 
@@ -238,16 +243,24 @@ struct TreeKeys<kTypeF32, HD> {
             a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][2], q[s][2], a, 0, 0, 0);
             b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][3], q[s][3], b, 0, 0, 0);
         }
+#pragma unroll
+        for (int s = 0; s < S; ++s) keep(k[s]), keep(q[s]);
         return a + b;
     }
     __device__ __forceinline__ void weigh(const float (&p)[4], f32x4 (&o)[U][4]) const {
+        const f32x4 w = (f32x4){p[0], p[1], p[2], p[3]} * kPieces;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    o[u][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][u][e], p[i] * kPieces, o[u][e], 0, 0, 0);
+                    o[u][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][u][e], w[i], o[u][e], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int u = 0; u < U; ++u) keep(v[i][u]);
+        keep(w);
     }
 };
 
@@ -311,9 +324,13 @@ struct TreeJob {
     int slot;            // of the partial results
 };
 
+// The page of a sequence's logical block (uniform), negative where there is none. A scalar load: its wait is
+// not the vector loads', which are in flight beside it.
 __device__ __forceinline__ int page_of(const TreeArgs& a, int seq, int lb) {
     if (a.n_table <= 0) return -1;
-    const int blk = a.tables[(int64_t)seq * a.table_stride + min(lb, a.n_table - 1)];
+    typedef __attribute__((address_space(4))) const int32_t* ScalarPtr;
+    lb = __builtin_amdgcn_readfirstlane(lb);
+    const int blk = *(ScalarPtr)(a.tables + ((int64_t)seq * a.table_stride + min(lb, a.n_table - 1)));
     return lb < a.n_table && blk < a.n_blocks ? blk : -1;
 }
 
@@ -455,7 +472,7 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
         int pages[NP], next[NP];
         auto pages_of = [&](int c, int (&p)[NP]) {
 #pragma unroll
-            for (int j = 0; j < NP; ++j) p[j] = __builtin_amdgcn_readfirstlane(page_of(a, w.seq, c * NP + j));
+            for (int j = 0; j < NP; ++j) p[j] = page_of(a, w.seq, c * NP + j);
         };
         auto page_bytes = [&](int blk) {  // a missing page's loads read page 0; what they bring is cleared
             return ((int64_t)max(blk, 0) * a.n_layer + a.layer) * kKvBlock * a.sb;
@@ -632,38 +649,40 @@ __global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) 
 }
 
 // ---------------------------------------------------------------- many rows
-// A block of 8 W keys in LDS, as f16 pieces (F16 slots: one).
+// Blocks of 8 W keys in LDS, as f16 pieces. Q8_0: two buffers of two pieces, decoded on the way. F16: a ring of
+// four, filled by direct loads two blocks ahead of the one in use, in rows without padding.
 template <int CT, int HD, int W>
 struct __align__(16) TreeBlock {
-    static constexpr int NPC = CT == kTypeQ8_0 ? 2 : 1;
-    // pitches: K rows are read 16 bytes per lane down a column of 32 rows (4 banks apart); V rows four
-    // at a time, 64 bytes each (16 banks apart)
-    static constexpr int KP = HD + 8, VP = HD + 32;
-    _Float16 k[2][NPC][8 * W][KP];  // [buffer][piece][key][dim]
-    _Float16 v[2][NPC][8 * W][VP];
+    static constexpr bool DMA = CT == kTypeF16;
+    static constexpr int NPC = DMA ? 1 : 2, NBUF = DMA ? 4 : 2;
+    // K rows are read 16 bytes per lane down a column of 32 rows, V rows four at a time, 64 bytes each. Padded
+    // rows lie 4 and 16 banks apart for that; in rows without padding the 16-byte pieces are permuted instead,
+    // piece c of row r at c ^ swizzle(r).
+    static constexpr int KP = DMA ? HD : HD + 8, VP = DMA ? HD : HD + 32;
+    _Float16 k[NBUF][NPC][8 * W][KP];  // [buffer][piece][key][dim]
+    _Float16 v[NBUF][NPC][8 * W][VP];
+    static __device__ __forceinline__ int k_swizzle(int r) { return DMA ? r & (HD / 8 - 1) & 15 : 0; }
+    static __device__ __forceinline__ int v_swizzle(int r) { return DMA ? (r & 3) << 1 : 0; }
 };
 
-// E elements of a slot's head piece from element e0, as loaded, and their way into LDS.
-template <int CT, int E>
-struct TreeRaw;
+// 16 bytes per lane from global memory (uniform base + per-lane byte offset) into LDS at lds_base + 16 lane.
+// Inline asm: the compiler's builtin form makes LDS reads of any buffer wait for it. Not counted by the compiler;
+// counted_wait below comes before the barrier that publishes the block.
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, const void* lds_base) {
+    typedef __attribute__((address_space(3))) const void* LdsPtr;
+    const uint32_t m0 = (uint32_t)(uintptr_t)(LdsPtr)lds_base;
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
+}
+// All loads but the N issued last have landed.
+template <int N>
+__device__ __forceinline__ void counted_wait() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0F70);  // vmcnt(N) alone
+    asm volatile(";dcq counted wait" ::: "memory");
+}
+
+// E elements of a Q8_0 slot's head piece from element e0, as loaded, and their way into LDS.
 template <int E>
-struct TreeRaw<kTypeF16, E> {
-    uint4 w[E / 8];
-    __device__ __forceinline__ void load(const uint8_t* head, int e0) {
-#pragma unroll
-        for (int j = 0; j < E / 8; ++j) w[j] = ld16(head + 2 * e0 + 16 * j);
-    }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int j = 0; j < E / 8; ++j) w[j] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    __device__ __forceinline__ void store(_Float16* h, _Float16*) const {
-#pragma unroll
-        for (int j = 0; j < E / 8; ++j) *reinterpret_cast<uint4*>(h + 8 * j) = w[j];
-    }
-};
-template <int E>
-struct TreeRaw<kTypeQ8_0, E> {
+struct TreeRaw {
     uint32_t w[E / 4], d;
     __device__ __forceinline__ void load(const uint8_t* head, int e0) {
         const uint8_t* b = head + e0 / 32 * 34;
@@ -686,11 +705,11 @@ struct TreeRaw<kTypeQ8_0, E> {
 };
 
 // 32 W rows of a KV head over a share of its cached keys (slots 1 ..), or 16 rows over the drafted keys (slot 0:
-// the first draft_wgs workgroups).
+// the workgroups from hist_wgs on, which fill the end of the launch).
 template <int CT, int HD, int W>
 __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(TreeArgs a) {
     using Block = TreeBlock<CT, HD, W>;
-    constexpr int E = HD / 8;    // elements per staging thread: key tid / 8 of the block
+    constexpr int E = HD / 8;    // elements per staging thread of Q8_0: key tid / 8 of the block
     constexpr int KS = HD / 16;  // k-steps of the score product
     constexpr int NT = HD / 32;  // 32-dim tiles of the output
     constexpr int NPC = Block::NPC;
@@ -700,8 +719,8 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
     } sm;
     __shared__ uint32_t again[W];
     TreeJob w;
-    int id = blockIdx.x;
-    if (id < a.draft_wgs) {
+    int id = (int)blockIdx.x - a.hist_wgs;
+    if (id >= 0) {
         const int per_seq = a.n_head_kv * a.tiles16;
         tree_job(a, w, id / per_seq);
         w.h_kv = id % per_seq / a.tiles16;
@@ -712,7 +731,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         if (w.row0 < w.n_rows) tree_tile<kTypeF32, HD, W, false>(a, w, sm.t);
         return;
     }
-    id -= a.draft_wgs;
+    id = blockIdx.x;
     const int turn = id / (8 * a.tiles), rest = id % (8 * a.tiles), unit = turn * 8 + rest % 8;
     if (unit >= a.units) return;
     w.h_kv = unit % a.n_head_kv;
@@ -760,14 +779,17 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         }
     }
 
-    // ---- staging: a block's loads are issued before the products of the block before, and stored after them
     constexpr int BK = 8 * W;  // keys of a block
-    const int skey = tid >> 3, se0 = E * (tid & 7);
+    constexpr bool DMA = Block::DMA;
+    constexpr int NBUF = Block::NBUF;
     const int64_t head = a.sb / a.n_head_kv * w.h_kv;
-    TreeRaw<CT, E> rk, rv;
-    auto page_at = [&](int kb) { return kb + skey < w.k_end ? page_of(a, w.seq, (kb + skey) / kKvBlock) : -1; };
+    // ---- staging, Q8_0: a block's loads are issued before the products of the block before, and stored after them
+    const int skey = tid >> 3, se0 = E * (tid & 7);
+    TreeRaw<E> rk, rv;
+    // the page of the wave's rows 8 w .. + 7
+    auto wave_page = [&](int kb) { return kb < w.k_end ? page_of(a, w.seq, (kb + 8 * wave) / kKvBlock) : -1; };
     auto load_block = [&](int kb, int blk) {  // zeros for missing pages and past the last key
-        if (blk >= 0) {
+        if (blk >= 0 && kb + skey < w.k_end) {
             const int64_t off = (((int64_t)blk * a.n_layer + a.layer) * kKvBlock + (kb + skey) % kKvBlock) * a.sb + head;
             rk.load(a.k_arena + off, se0);
             rv.load(a.v_arena + off, se0);
@@ -780,6 +802,45 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         rk.store(&sm.b.k[buf][0][skey][se0], &sm.b.k[buf][NPC - 1][skey][se0]);
         rv.store(&sm.b.v[buf][0][skey][se0], &sm.b.v[buf][NPC - 1][skey][se0]);
     };
+    // ---- staging, F16: NI loads of RI rows each for K and for V
+    constexpr int RI = 512 / HD, NI = 8 / RI;
+    uint32_t k_off[NI], v_off[NI];
+    uint32_t partial = 0;  // (uniform) bit i: of the block issued i turns ago this wave has rows to clear
+    int page_next = 0;
+    if constexpr (DMA) {
+        const int c = lane % (HD / 8);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int r = 8 * wave + i * RI + lane / (HD / 8);
+            const uint32_t at = (uint32_t)(r % kKvBlock) * (uint32_t)a.sb + (uint32_t)head;
+            k_off[i] = at + 16 * (c ^ Block::k_swizzle(r));
+            v_off[i] = at + 16 * (c ^ Block::v_swizzle(r));
+        }
+    }
+    auto issue = [&](int kb, int blk, int buf) {  // a missing page's loads read page 0; their rows are cleared
+        const int64_t page = ((int64_t)max(blk, 0) * a.n_layer + a.layer) * kKvBlock * a.sb;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            dma16(a.k_arena + page, k_off[i], &sm.b.k[buf][0][8 * wave + i * RI][0]);
+            dma16(a.v_arena + page, v_off[i], &sm.b.v[buf][0][8 * wave + i * RI][0]);
+        }
+        partial = partial << 1 | (blk < 0 || kb + 8 * wave + 8 > w.k_end ? 1u : 0u);
+    };
+    auto clear_rows = [&](int kb, int buf) {  // rows of a missing page, and past the last key
+        const int from = wave_page(kb) < 0 ? 0 : max(w.k_end - kb - 8 * wave, 0);
+        for (int i = from * (HD / 8) + lane; i < HD; i += 64) {  // 8 rows of HD / 8 pieces
+            *reinterpret_cast<uint4*>(&sm.b.k[buf][0][8 * wave][8 * i]) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(&sm.b.v[buf][0][8 * wave][8 * i]) = make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+    // the wave's rows of block kb have landed, in buffer buf; `after` blocks were issued since (-1: there is no
+    // block kb, and nothing in flight)
+    auto landed = [&](int kb, int buf, int after) {
+        const bool wait_all = after != 2 || (partial >> 2 & 1);
+        if (wait_all) counted_wait<0>();
+        counted_wait<2 * 2 * NI>();
+        if (wait_all && after >= 0 && (partial >> after & 1)) clear_rows(kb, buf);
+    };
 
     f32x16 o[NT];
 #pragma unroll
@@ -788,16 +849,29 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         for (int v = 0; v < 16; ++v) o[t][v] = 0.0f;
     float m = -INFINITY, l = 0.0f;  // l: this lane's keys only, until the end
 
-    load_block(w.k_begin, page_at(w.k_begin));
-    int blk_next = page_at(w.k_begin + BK);
-    store_block(0);
+    int blk_next = -1, issued = 0;  // issued: blocks, of this wave
+    if constexpr (DMA) {
+        for (; issued < 3 && w.k_begin + issued * BK < w.k_end; ++issued)
+            issue(w.k_begin + issued * BK, wave_page(w.k_begin + issued * BK), issued);
+        page_next = wave_page(w.k_begin + 3 * BK);
+        landed(w.k_begin, 0, issued - 1);
+    } else {
+        load_block(w.k_begin, wave_page(w.k_begin));
+        blk_next = wave_page(w.k_begin + BK);
+        store_block(0);
+    }
     __syncthreads();
     int buf = 0;
-    for (int kb = w.k_begin; kb < w.k_end; kb += BK, buf ^= 1) {
+    for (int kb = w.k_begin; kb < w.k_end; kb += BK, buf = (buf + 1) % NBUF) {
         const bool more = kb + BK < w.k_end;
-        if (more) {
+        if constexpr (DMA) {
+            if (kb + 3 * BK < w.k_end) {
+                issue(kb + 3 * BK, page_next, (buf + 3) % NBUF);
+                page_next = wave_page(kb + 4 * BK);
+            }
+        } else if (more) {
             load_block(kb + BK, blk_next);
-            blk_next = page_at(kb + 2 * BK);
+            blk_next = wave_page(kb + 2 * BK);
         }
         if (r0 < w.n_rows) {
 #pragma unroll 1
@@ -806,13 +880,14 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
                 f32x16 sc, hi;
 #pragma unroll
                 for (int v = 0; v < 16; ++v) sc[v] = 0.0f, hi[v] = 0.0f;
-                const _Float16* kh = &sm.b.k[buf][0][sub + c32][8 * p];
-                const _Float16* kl = &sm.b.k[buf][NPC - 1][sub + c32][8 * p];
+                const _Float16* kh = &sm.b.k[buf][0][sub + c32][0];
+                const _Float16* kl = &sm.b.k[buf][NPC - 1][sub + c32][0];
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    const f16x8 fh = *reinterpret_cast<const f16x8*>(kh + 16 * s);
+                    const int at = 8 * ((2 * s + p) ^ Block::k_swizzle(c32));
+                    const f16x8 fh = *reinterpret_cast<const f16x8*>(kh + at);
                     if constexpr (NPC == 2) {
-                        const f16x8 fl = *reinterpret_cast<const f16x8*>(kl + 16 * s);
+                        const f16x8 fl = *reinterpret_cast<const f16x8*>(kl + at);
                         sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl, qh[s], sc, 0, 0, 0);
                     }
                     sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fh, ql[s], sc, 0, 0, 0);
@@ -850,7 +925,9 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
 
                 // ---- O^T += V^T P^T: step s takes the lane's weights i = 8s .. 8s + 7, keys 16s + 4p + 0..3
                 // and 16s + 8 + 4p + 0..3
-                const int vrow = sub + 4 * p + ((lane & 15) >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                const int vrow = sub + 4 * p + ((lane & 15) >> 2);
+                // of tile t the 16-byte piece 4 t + vc of the row, its half lane % 2
+                const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vx = Block::v_swizzle(lane >> 2);
                 f16x8 ph[2], pl[2];
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
@@ -869,8 +946,9 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
                         f16x8 f[NPC];
 #pragma unroll
                         for (int u = 0; u < NPC; ++u) {
-                            const f16x4 a0 = lds_transposed(&sm.b.v[buf][u][16 * s + vrow][32 * t + vcol]);
-                            const f16x4 a1 = lds_transposed(&sm.b.v[buf][u][16 * s + 8 + vrow][32 * t + vcol]);
+                            const int at = 8 * ((4 * t + vc) ^ vx) + 4 * (lane & 1);
+                            const f16x4 a0 = lds_transposed(&sm.b.v[buf][u][16 * s + vrow][at]);
+                            const f16x4 a1 = lds_transposed(&sm.b.v[buf][u][16 * s + 8 + vrow][at]);
                             f[u] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
                         }
                         if constexpr (NPC == 2)
@@ -880,7 +958,10 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
                     }
             }
         }
-        if (more) store_block(buf ^ 1);
+        if constexpr (DMA)
+            landed(kb + BK, (buf + 1) % NBUF, min((w.k_end - kb - 1) / BK, 3) - 1);
+        else if (more)
+            store_block(buf ^ 1);
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
@@ -910,17 +991,14 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
 
 // The merge of a sequence's splits: M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L, zeros for a row
 // that saw no key or has no drafted token. P lanes share 4 outputs, lane p the splits p, p + P, ...
-template <int P>
-__global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, int hd) {
-    constexpr int NS = 4;  // splits of a lane whose loads are issued together
-    const int q4 = hd / 4;
-    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / P;
-    const int p = threadIdx.x & (P - 1);
-    const bool in = unit < a.rows * q4;
-    const int64_t row = in ? unit / q4 : 0;
-    const int d = in ? (int)(unit % q4) * 4 : 0;
-    const int64_t trow = row / a.n_head;
-    const int h = (int)(row % a.n_head), seq = (int)(trow / a.n_tokens), tok = (int)(trow % a.n_tokens);
+template <int HD, int P>
+__global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
+    constexpr int NS = 8;  // splits of a lane whose loads are issued together
+    constexpr int QP = HD / 4 * P;  // threads of a row
+    const int p = threadIdx.x % P, d = threadIdx.x / P % (HD / 4) * 4;
+    const int row = (int)blockIdx.x * (256 / QP) + threadIdx.x / QP;  // below 2^27
+    if (row >= a.rows) return;
+    const int trow = row / a.n_head, h = row % a.n_head, seq = trow / a.n_tokens, tok = trow % a.n_tokens;
     const int past = min(max(a.past[seq], 0), a.max_past);
     const int n_draft = a.n_draft ? min(max(a.n_draft[seq], 0), a.n_tokens) : a.n_tokens;
     const int n_hist = (past + a.kps - 1) / a.kps;
@@ -935,7 +1013,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, int hd) {
             const int s = s0 + P * k;
             const int64_t r = (int64_t)s * a.rows + row;
             ml[k] = s < n_split ? *reinterpret_cast<const float2*>(a.ws_ml + 2 * r) : make_float2(-INFINITY, 0.0f);
-            ov[k] = s < n_split ? *reinterpret_cast<const f32x4*>(a.ws_o + r * hd + d) : (f32x4){0.f, 0.f, 0.f, 0.f};
+            ov[k] = s < n_split ? *reinterpret_cast<const f32x4*>(a.ws_o + r * HD + d) : (f32x4){0.f, 0.f, 0.f, 0.f};
         }
         float mn = m;
 #pragma unroll
@@ -955,10 +1033,11 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a, int hd) {
     l = lanes_sum<P>(l * f);
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = lanes_sum<P>(acc[e] * f);
-    if (!in || p != 0) return;
-    float* out = a.out + trow * a.out_stride + (int64_t)h * hd + d;
+    if (p != 0) return;
+    float* out = a.out + (int64_t)trow * a.out_stride + (int64_t)h * HD + d;
+    const float inv = 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = l != 0.0f ? acc[e] / l : 0.0f;
+    for (int e = 0; e < 4; ++e) out[e] = l != 0.0f ? acc[e] * inv : 0.0f;
 }
 
 // ---------------------------------------------------------------- host side
@@ -1001,10 +1080,21 @@ size_t tree_workspace_bytes(int hd, int n_head, int n_head_kv, int n_seqs, int n
                     tree_partial_bytes(tree_plan(kTypeF16, hd, n_head, n_head_kv, n_seqs, n_tokens, max_past), hd, rows));
 }
 
-template <int P>
-static void launch_tree_merge(const TreeArgs& a, int hd, hipStream_t st) {
-    const int64_t threads = a.rows * (hd / 4) * P;
-    hipLaunchKernelGGL((tree_merge_kernel<P>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a, hd);
+template <int HD, int P>
+static void launch_tree_merge_t(const TreeArgs& a, hipStream_t st) {
+    constexpr int rows = 256 / (HD / 4 * P);
+    hipLaunchKernelGGL((tree_merge_kernel<HD, P>), dim3((unsigned)((a.rows + rows - 1) / rows)), dim3(256), 0, st, a);
+}
+
+// Lanes that share an output: one where a lane takes all splits in one step or there are outputs for half the
+// CUs' waves (2048 rows x 128, 33 splits: 9.2 us, four lanes 11.8; 6144 rows, 9 splits 6.0 and 9.4), else a
+// workgroup a row.
+template <int HD>
+static void launch_tree_merge(const TreeArgs& a, hipStream_t st) {
+    if (a.splits <= 8 || a.rows * (HD / 4) >= 32768)
+        launch_tree_merge_t<HD, 1>(a, st);
+    else
+        launch_tree_merge_t<HD, 1024 / HD>(a, st);
 }
 
 template <int CT, int HD>
@@ -1033,8 +1123,8 @@ hipError_t launch_tree_attention(int ct, int hd, TreeArgs a, void* ws, hipStream
     const int64_t drafts = p.block_waves ? (int64_t)a.n_seqs * a.n_head_kv * a.tiles16 : 0;
     const int64_t units = (int64_t)a.n_seqs * (p.block_waves ? p.splits - 1 : p.splits) * a.n_head_kv;
     const int64_t wgs = drafts + (units + 7) / 8 * 8 * p.tiles;
-    if (wgs > INT32_MAX || a.rows * (hd / 4) * 32 > (int64_t)INT32_MAX * 256) return hipErrorInvalidValue;
-    a.units = (int)units, a.draft_wgs = (int)drafts;
+    if (wgs > INT32_MAX) return hipErrorInvalidValue;
+    a.units = (int)units, a.draft_wgs = (int)drafts, a.hist_wgs = (int)(wgs - drafts);
     if (p.splits > 1) {
         a.ws_o = static_cast<float*>(ws);
         a.ws_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round_up(p.splits * a.rows * hd * 4, 256));
@@ -1056,12 +1146,12 @@ hipError_t launch_tree_attention(int ct, int hd, TreeArgs a, void* ws, hipStream
 #undef DCQ_TREE_CASE
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
-    if (p.splits <= 4)
-        launch_tree_merge<1>(a, hd, st);
-    else if (p.splits <= 32)
-        launch_tree_merge<8>(a, hd, st);
+    if (hd == 64)
+        launch_tree_merge<64>(a, st);
+    else if (hd == 128)
+        launch_tree_merge<128>(a, st);
     else
-        launch_tree_merge<32>(a, hd, st);
+        launch_tree_merge<256>(a, st);
     return hipGetLastError();
 }
 
