@@ -832,8 +832,8 @@ static int validate_pages(int cache_type, const void* k_arena, const void* v_are
 }
 
 size_t dcq_kv_fork_workspace_size(int64_t n_blocks, int64_t n_seqs, int64_t n_children) {
-    if (n_blocks <= 0 || n_seqs <= 0 || n_children <= 0 || n_children > 4096) return 0;
-    return fork_workspace_bytes(n_children);
+    if (n_blocks <= 0 || n_blocks > ((int64_t)1 << 24) || n_seqs <= 0 || n_children <= 0 || n_children > 4096) return 0;
+    return fork_workspace_bytes(n_blocks, n_children);
 }
 
 int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer, int64_t row_elems,
@@ -858,7 +858,7 @@ int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, 
     for (const auto& o : out)
         for (const auto& i : in)
             if (overlap(o.p, o.n, i.p, i.n)) return DCQ_ERR_INVALID_ARG;
-    if ((rc = validate_workspace(workspace, workspace_bytes, fork_workspace_bytes(n_children)))) return rc;
+    if ((rc = validate_workspace(workspace, workspace_bytes, fork_workspace_bytes(n_blocks, n_children)))) return rc;
     if ((rc = check_device())) return rc;
     ForkArgs a{};
     a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table, a.lengths = lengths, a.n_seqs = (int)n_seqs;

@@ -10,8 +10,7 @@
 //   fork_count_kernel    the children's tables, and the counts without the parents' and with the children's
 //   fork_plan_kernel     who keeps a partial last page, who gets a copy and where; one workgroup
 //   compact_plan_kernel  the holes among the first n_live pages and the pages that move there; one workgroup
-//   compact_map_kernel   the tables and counts after the move
-//   copy_pages_kernel    whole pages (from, to) of both arenas
+//   copy_pages_kernel    whole pages (from, to) of both arenas, and the tables and counts after a compaction
 #include <algorithm>
 
 #include "dcq_common.h"
@@ -55,14 +54,44 @@ hipError_t launch_path_write(const PathArgs& a, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------- whole pages
+// A compaction's tables and counts after the move, by the first map_wgs workgroups of a launch.
+__device__ __forceinline__ void compact_map(const CompactArgs& a, int map_wgs) {
+    const int live = a.plan[1];
+    const int64_t entries = (int64_t)a.n_seqs * a.n_table;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries + a.n_blocks; i += (int64_t)map_wgs * 256) {
+        if (i < entries) {
+            const int row = (int)(i / a.n_table), at = (int)(i % a.n_table);
+            int page = a.tables[(int64_t)row * a.table_stride + at];
+            if (at < pages_of_length(a.lengths[row], a.n_table) && page >= live && page < a.n_blocks && a.refs[page] > 0)
+                page = a.plan[3 + 2 * a.rank[page]];
+            a.tables_out[(int64_t)row * a.tables_out_stride + at] = page;
+        } else {
+            const int page = (int)(i - entries), n = a.refs[page];
+            if (page < live ? n > 0 : n <= 0) {
+                a.refs_out[page] = n;
+            } else if (page >= live) {  // moves: the pair's counts; a hole's comes from its pair
+                a.refs_out[a.plan[3 + 2 * a.rank[page]]] = n;
+                a.refs_out[page] = 0;
+            }
+        }
+    }
+}
+
 // plan[0] pairs (from, to) at plan[2 + 2 i]: pieces of 16 KB, dealt to the workgroups in turn.
 constexpr int kPiece = 16384;
+template <bool MAP>
 __global__ void __launch_bounds__(256) copy_pages_kernel(uint8_t* k_arena, uint8_t* v_arena, const int32_t* plan,
-                                                         int64_t page_bytes) {
-    const int64_t per_page = (page_bytes + kPiece - 1) / kPiece;
-    const int64_t pieces = 2 * per_page * plan[0];
-    for (int64_t i = blockIdx.x; i < pieces; i += gridDim.x) {
-        const int64_t unit = i / per_page, at = (i % per_page) * kPiece;
+                                                         int64_t page_bytes, int map_wgs, CompactArgs c) {
+    if (MAP && (int)blockIdx.x < map_wgs) {
+        compact_map(c, map_wgs);
+        return;
+    }
+    const int wg = blockIdx.x - (MAP ? map_wgs : 0), wgs = gridDim.x - (MAP ? map_wgs : 0);
+    const uint32_t per_page = (uint32_t)((page_bytes + kPiece - 1) / kPiece);
+    const uint32_t pieces = 2 * per_page * plan[0];
+    for (uint32_t i = wg; i < pieces; i += wgs) {
+        const uint32_t unit = i / per_page;
+        const int64_t at = (int64_t)(i - unit * per_page) * kPiece;
         const int64_t from = plan[2 + 2 * (unit / 2)], to = plan[3 + 2 * (unit / 2)];
         uint8_t* arena = unit % 2 ? v_arena : k_arena;
         const uint8_t* src = arena + from * page_bytes + at;
@@ -82,12 +111,22 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(uint8_t* k_arena, uint8
     }
 }
 
+// map: a compaction's tables and counts, in workgroups before the copying ones.
 static hipError_t launch_copy_pages(void* k_arena, void* v_arena, const int32_t* plan, int64_t max_pages,
-                                    int64_t page_bytes, hipStream_t st) {
+                                    int64_t page_bytes, const CompactArgs* map, hipStream_t st) {
     const int64_t pieces = 2 * max_pages * ((page_bytes + kPiece - 1) / kPiece);
-    const unsigned grid = (unsigned)std::min<int64_t>(pieces, 8 * (int64_t)cu_count());
-    hipLaunchKernelGGL(copy_pages_kernel, dim3(grid), dim3(256), 0, st, static_cast<uint8_t*>(k_arena),
-                       static_cast<uint8_t*>(v_arena), plan, page_bytes);
+    if (pieces > INT32_MAX) return hipErrorInvalidValue;
+    const int wgs = (int)std::min<int64_t>(std::max<int64_t>(pieces, 1), 8 * (int64_t)cu_count());
+    uint8_t *k = static_cast<uint8_t*>(k_arena), *v = static_cast<uint8_t*>(v_arena);
+    if (map) {
+        const int64_t items = (int64_t)map->n_seqs * map->n_table + map->n_blocks;
+        const int map_wgs = (int)std::min<int64_t>((items + 255) / 256, 2 * (int64_t)cu_count());
+        hipLaunchKernelGGL((copy_pages_kernel<true>), dim3((unsigned)(map_wgs + wgs)), dim3(256), 0, st, k, v, plan,
+                           page_bytes, map_wgs, *map);
+    } else {
+        hipLaunchKernelGGL((copy_pages_kernel<false>), dim3((unsigned)wgs), dim3(256), 0, st, k, v, plan, page_bytes, 0,
+                           CompactArgs{});
+    }
     return hipGetLastError();
 }
 
@@ -114,64 +153,87 @@ __device__ __forceinline__ Scan block_scan(bool flag, int* counts /* kPlanWaves 
 
 // ---------------------------------------------------------------- forks
 // The counts: refs_out = refs - one for each page a sequence holds + one for each page a child takes over, and
-// the children's tables and lengths. The part of one (sequence or child, table entry).
-template <class Add>
-__device__ __forceinline__ void fork_count_entry(const ForkArgs& a, int row, int at, Add add) {
-    if (row < a.n_seqs) {
-        const int page = a.tables[(int64_t)row * a.table_stride + at];
-        if (at < pages_of_length(a.lengths[row], a.n_table) && page >= 0 && page < a.n_blocks) add(page, -1);
-        return;
-    }
-    const int child = row - a.n_seqs, parent = a.parents[child];
-    const bool known = parent >= 0 && parent < a.n_seqs;
-    const int length = known ? min(max(a.lengths[parent], 0), a.n_table * kKvBlock) : 0;
+// the children's tables and lengths. The part of one (sequence or child, table entry). length_of(i): sequence i's,
+// 0 .. 16 n_table; parent_of(i): child i's, or -1; tail(i, page): the partial last page of child i.
+template <class Length, class Parent, class Add, class Tail>
+__device__ __forceinline__ void fork_count_entry(const ForkArgs& a, int row, int at, Length length_of, Parent parent_of,
+                                                 Add add, Tail tail) {
+    const bool child = row >= a.n_seqs;
+    const int i = child ? row - a.n_seqs : row, from = child ? parent_of(i) : i;
+    const int length = from >= 0 ? length_of(from) : 0;
     int page = -1;
     if (at < pages_of_length(length, a.n_table)) {
-        page = a.tables[(int64_t)parent * a.table_stride + at];
-        if (page >= 0 && page < a.n_blocks) add(page, 1);
+        page = a.tables[(int64_t)from * a.table_stride + at];
+        const bool real = page >= 0 && page < a.n_blocks;
+        if (real) add(page, child ? 1 : -1);
+        if (child && real && at == length / kKvBlock) tail(i, page);
     }
-    a.tables_out[(int64_t)child * a.tables_out_stride + at] = page;
-    if (at == 0) a.lengths_out[child] = length;
+    if (!child) return;
+    a.tables_out[(int64_t)i * a.tables_out_stride + at] = page;
+    if (at == 0) a.lengths_out[i] = length;
+}
+__device__ __forceinline__ int fork_length(const ForkArgs& a, int i) {
+    return min(max(a.lengths[i], 0), a.n_table * kKvBlock);
+}
+__device__ __forceinline__ int fork_parent(const ForkArgs& a, int i) {
+    const int p = a.parents[i];
+    return p >= 0 && p < a.n_seqs ? p : -1;
 }
 
-__global__ void __launch_bounds__(256) fork_refs_kernel(const int32_t* refs, int32_t* refs_out, int n_blocks) {
+// Of a partial last page: the children that would write into it, and the first of them.
+__device__ __forceinline__ void fork_count_tail(int32_t* users, int32_t* first, int child, int page) {
+    atomicAdd(users + page, 1);
+    atomicMin(first + page, child);
+}
+
+__global__ void __launch_bounds__(256) fork_refs_kernel(ForkArgs a) {
     const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < n_blocks) refs_out[i] = refs[i];
+    if (i < a.n_blocks) a.refs_out[i] = a.refs[i], a.users[i] = 0, a.first[i] = INT32_MAX;
 }
 
 __global__ void __launch_bounds__(256) fork_count_kernel(ForkArgs a) {
     const int64_t entries = (int64_t)(a.n_seqs + a.n_children) * a.n_table;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256)
-        fork_count_entry(a, (int)(i / a.n_table), (int)(i % a.n_table),
-                         [&](int page, int by) { atomicAdd(a.refs_out + page, by); });
+        fork_count_entry(
+            a, (int)(i / a.n_table), (int)(i % a.n_table), [&](int k) { return fork_length(a, k); },
+            [&](int k) { return fork_parent(a, k); }, [&](int page, int by) { atomicAdd(a.refs_out + page, by); },
+            [&](int k, int page) { fork_count_tail(a.users, a.first, k, page); });
 }
 
 // LDS: the counts are in LDS, and this workgroup does the counting too (few pages and entries). Otherwise
-// refs_out holds the counts already.
+// refs_out, users and first hold them already.
 template <bool LDS>
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
     extern __shared__ int32_t lds[];
     __shared__ int counts[kPlanWaves];
     const int tid = threadIdx.x;
     int32_t* tails = lds;                                        // [n_children]: partial last page, or -1
-    int32_t* fresh = lds + a.n_children;                         // [n_children]: the copy's page, by its rank
-    int32_t* refs = LDS ? lds + 2 * a.n_children : a.refs_out;  // [n_blocks]
+    int32_t* fresh = tails + a.n_children;                       // [n_children]: the copy's page, by its rank
+    int32_t* refs = LDS ? fresh + a.n_children : a.refs_out;     // [n_blocks]
+    int32_t* users = LDS ? refs + a.n_blocks : a.users;          // [n_blocks]
+    int32_t* first = LDS ? users + a.n_blocks : a.first;         // [n_blocks]
     if (LDS) {
-        for (int i = tid; i < a.n_blocks; i += kPlanThreads) refs[i] = a.refs[i];
+        int32_t* parents = first + a.n_blocks;       // [n_children]
+        int32_t* lengths = parents + a.n_children;  // [n_seqs]
+        for (int i = tid; i < a.n_blocks; i += kPlanThreads) refs[i] = a.refs[i], users[i] = 0, first[i] = INT32_MAX;
+        for (int i = tid; i < a.n_seqs; i += kPlanThreads) lengths[i] = fork_length(a, i);
+        for (int i = tid; i < a.n_children; i += kPlanThreads) parents[i] = fork_parent(a, i), tails[i] = -1;
         __syncthreads();
         const int entries = (a.n_seqs + a.n_children) * a.n_table;
         for (int i = tid; i < entries; i += kPlanThreads)
-            fork_count_entry(a, i / a.n_table, i % a.n_table, [&](int page, int by) { atomicAdd(refs + page, by); });
-    }
-    for (int i = tid; i < a.n_children; i += kPlanThreads) {
-        const int parent = a.parents[i];
-        int tail = -1;
-        if (parent >= 0 && parent < a.n_seqs) {
-            const int length = min(max(a.lengths[parent], 0), a.n_table * kKvBlock);
-            if (length % kKvBlock) tail = a.tables[(int64_t)parent * a.table_stride + length / kKvBlock];
-            if (tail >= a.n_blocks) tail = -1;
+            fork_count_entry(
+                a, i / a.n_table, i % a.n_table, [&](int k) { return lengths[k]; }, [&](int k) { return parents[k]; },
+                [&](int page, int by) { atomicAdd(refs + page, by); },
+                [&](int k, int page) {
+                    tails[k] = page;
+                    fork_count_tail(users, first, k, page);
+                });
+    } else {
+        for (int i = tid; i < a.n_children; i += kPlanThreads) {
+            const int parent = fork_parent(a, i), length = parent >= 0 ? fork_length(a, parent) : 0;
+            const int tail = length % kKvBlock ? a.tables[(int64_t)parent * a.table_stride + length / kKvBlock] : -1;
+            tails[i] = tail < a.n_blocks ? tail : -1;
         }
-        tails[i] = tail;
     }
     __syncthreads();
     // ---- a child keeps its partial page if all who hold it are children that would write into it, and it is
@@ -179,17 +241,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
     int copies = 0;
     for (int i0 = 0; i0 < a.n_children; i0 += kPlanThreads) {
         const int i = i0 + tid, tail = i < a.n_children ? tails[i] : -1;
-        bool copy = false;
-        if (tail >= 0) {
-            int users = 0;
-            bool first = true;
-            for (int k = 0; k < a.n_children; ++k) {
-                const bool same = tails[k] == tail;
-                users += same;
-                first &= !(same && k < i);
-            }
-            copy = !(first && refs[tail] == users);
-        }
+        const bool copy = tail >= 0 && !(first[tail] == i && refs[tail] == users[tail]);
         const Scan s = block_scan(copy, counts);
         if (i < a.n_children) a.rank[i] = copy ? copies + s.before : -1;
         copies += s.total;
@@ -228,30 +280,32 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
     }
 }
 
-// Workspace: rank [n_children], then the plan (its length, a spare word, the pairs).
-size_t fork_workspace_bytes(int64_t n_children) {
-    return (size_t)round_up(n_children * 4, 256) + (size_t)round_up((2 + 2 * n_children) * 4, 256);
+// Workspace: rank [n_children], the plan (its length, a spare word, the pairs), users and first [n_blocks].
+size_t fork_workspace_bytes(int64_t n_blocks, int64_t n_children) {
+    return (size_t)(round_up(n_children * 4, 256) + round_up((2 + 2 * n_children) * 4, 256) + 2 * round_up(n_blocks * 4, 256));
 }
 
 hipError_t launch_fork(ForkArgs a, void* k_arena, void* v_arena, int64_t page_bytes, void* ws, hipStream_t st) {
-    a.rank = static_cast<int32_t*>(ws);
-    a.plan = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(ws) + round_up((int64_t)a.n_children * 4, 256));
+    uint8_t* w = static_cast<uint8_t*>(ws);
+    a.rank = reinterpret_cast<int32_t*>(w), w += round_up((int64_t)a.n_children * 4, 256);
+    a.plan = reinterpret_cast<int32_t*>(w), w += round_up((2 + 2 * (int64_t)a.n_children) * 4, 256);
+    a.users = reinterpret_cast<int32_t*>(w), w += round_up((int64_t)a.n_blocks * 4, 256);
+    a.first = reinterpret_cast<int32_t*>(w);
     const int64_t entries = (int64_t)(a.n_seqs + a.n_children) * a.n_table;
-    const size_t lds = 2 * (size_t)a.n_children * 4;
-    // one workgroup does it all while the counts fit in LDS and its threads have few entries to see; beyond, the
-    // counting alone takes longer than the two launches it then gets
-    if (2 * a.n_children + a.n_blocks <= 12288 && entries <= 32768) {
-        hipLaunchKernelGGL((fork_plan_kernel<true>), dim3(1), dim3(kPlanThreads), lds + (size_t)a.n_blocks * 4, st, a);
+    // one workgroup does it all while the counts fit in LDS (64 KB with the scans') and its threads have few
+    // entries to see; beyond, the counting alone takes longer than the two launches it then gets
+    const int64_t words = 3 * ((int64_t)a.n_children + a.n_blocks) + a.n_seqs;
+    if (words <= 16000 && entries <= 32768) {
+        hipLaunchKernelGGL((fork_plan_kernel<true>), dim3(1), dim3(kPlanThreads), (size_t)words * 4, st, a);
     } else {
-        hipLaunchKernelGGL(fork_refs_kernel, dim3((unsigned)((a.n_blocks + 255) / 256)), dim3(256), 0, st, a.refs,
-                           a.refs_out, a.n_blocks);
+        hipLaunchKernelGGL(fork_refs_kernel, dim3((unsigned)((a.n_blocks + 255) / 256)), dim3(256), 0, st, a);
         const int64_t wgs = std::min<int64_t>((entries + 255) / 256, 4 * (int64_t)cu_count());
         hipLaunchKernelGGL(fork_count_kernel, dim3((unsigned)wgs), dim3(256), 0, st, a);
-        hipLaunchKernelGGL((fork_plan_kernel<false>), dim3(1), dim3(kPlanThreads), lds, st, a);
+        hipLaunchKernelGGL((fork_plan_kernel<false>), dim3(1), dim3(kPlanThreads), 2 * (size_t)a.n_children * 4, st, a);
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    return launch_copy_pages(k_arena, v_arena, a.plan, a.n_children, page_bytes, st);
+    return launch_copy_pages(k_arena, v_arena, a.plan, a.n_children, page_bytes, nullptr, st);
 }
 
 // ---------------------------------------------------------------- compaction
@@ -290,28 +344,6 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs 
     if (tid == 0) a.plan[0] = movers, a.plan[1] = live, a.n_live[0] = live;
 }
 
-__global__ void __launch_bounds__(256) compact_map_kernel(CompactArgs a) {
-    const int live = a.plan[1];
-    const int64_t entries = (int64_t)a.n_seqs * a.n_table;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries + a.n_blocks; i += (int64_t)gridDim.x * 256) {
-        if (i < entries) {
-            const int row = (int)(i / a.n_table), at = (int)(i % a.n_table);
-            int page = a.tables[(int64_t)row * a.table_stride + at];
-            if (at < pages_of_length(a.lengths[row], a.n_table) && page >= live && page < a.n_blocks && a.refs[page] > 0)
-                page = a.plan[3 + 2 * a.rank[page]];
-            a.tables_out[(int64_t)row * a.tables_out_stride + at] = page;
-        } else {
-            const int page = (int)(i - entries), n = a.refs[page];
-            if (page < live ? n > 0 : n <= 0) {
-                a.refs_out[page] = n;
-            } else if (page >= live) {  // moves: the pair's counts; a hole's comes from its pair
-                a.refs_out[a.plan[3 + 2 * a.rank[page]]] = n;
-                a.refs_out[page] = 0;
-            }
-        }
-    }
-}
-
 size_t compact_workspace_bytes(int64_t n_blocks) {
     return (size_t)round_up(n_blocks * 4, 256) + (size_t)round_up((2 + n_blocks) * 4, 256);
 }
@@ -320,12 +352,9 @@ hipError_t launch_compact(CompactArgs a, void* k_arena, void* v_arena, int64_t p
     a.rank = static_cast<int32_t*>(ws);
     a.plan = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(ws) + round_up((int64_t)a.n_blocks * 4, 256));
     hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
-    const int64_t items = (int64_t)a.n_seqs * a.n_table + a.n_blocks;
-    const int64_t wgs = std::min<int64_t>((items + 255) / 256, 4 * (int64_t)cu_count());
-    hipLaunchKernelGGL(compact_map_kernel, dim3((unsigned)wgs), dim3(256), 0, st, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.n_blocks < 2) return e;
-    return launch_copy_pages(k_arena, v_arena, a.plan, a.n_blocks / 2, page_bytes, st);
+    if (e != hipSuccess) return e;
+    return launch_copy_pages(k_arena, v_arena, a.plan, a.n_blocks / 2, page_bytes, &a, st);
 }
 
 }  // namespace dcq

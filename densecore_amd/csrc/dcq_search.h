@@ -76,10 +76,12 @@ struct ForkArgs {
     int32_t* lengths_out;
     int32_t* refs_out;
     int32_t* missing;
-    int32_t* rank;  // these two: the launcher's, in the workspace
+    int32_t* rank;  // from here on the launcher's, in the workspace
     int32_t* plan;
+    int32_t* users;
+    int32_t* first;
 };
-size_t fork_workspace_bytes(int64_t n_children);
+size_t fork_workspace_bytes(int64_t n_blocks, int64_t n_children);
 hipError_t launch_fork(ForkArgs a, void* k_arena, void* v_arena, int64_t page_bytes, void* ws, hipStream_t st);
 
 struct CompactArgs {

@@ -70,6 +70,7 @@ __device__ __forceinline__ f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, ui
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     return __builtin_bit_cast(f16x8, (u32x4){a, b, c, d});
 }
+__device__ __forceinline__ f16x8 as_f16x8(const uint4& w) { return as_f16x8(w.x, w.y, w.z, w.w); }
 __device__ __forceinline__ uint32_t ldu32(const uint8_t* p) {  // 2-byte aligned
     uint32_t w;
     __builtin_memcpy(&w, p, 4);
@@ -104,15 +105,23 @@ struct TreeKeys<kTypeF16, HD> {
 #pragma unroll
         for (int u = 0; u < U; ++u) v[j][i][u] = make_uint2(0u, 0u);
     }
-    __device__ __forceinline__ f32x4 scores(int j, const f16x8 (&qh)[S], const f16x8 (&ql)[S]) const {
-        f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+    // q: the lane's operand of k-step 0; k-steps and pieces lie 64 apart
+    __device__ __forceinline__ void scores(const uint4* q, f32x4 (&r)[2]) const {
+        f32x4 lo[2], hi[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) lo[j] = hi[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const f16x8 f = as_f16x8(k[j][s].x, k[j][s].y, k[j][s].z, k[j][s].w);
-            lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ql[s], lo, 0, 0, 0);
-            hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qh[s], hi, 0, 0, 0);
+            const f16x8 qh = as_f16x8(q[128 * s]), ql = as_f16x8(q[128 * s + 64]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const f16x8 f = as_f16x8(k[j][s]);
+                lo[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ql, lo[j], 0, 0, 0);
+                hi[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qh, hi[j], 0, 0, 0);
+            }
         }
-        return hi + lo;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) r[j] = hi[j] + lo[j];
     }
     __device__ __forceinline__ void weigh(const f16x8 ph, const f16x8 pl, f32x4 (&o)[U][4]) const {
 #pragma unroll
@@ -165,23 +174,30 @@ struct TreeKeys<kTypeQ8_0, HD> {
 #pragma unroll
         for (int u = 0; u < U; ++u) vd[j][i][u] = 0u;
     }
-    __device__ __forceinline__ f32x4 scores(int j, const f16x8 (&qh)[S], const f16x8 (&ql)[S]) const {
-        f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+    __device__ __forceinline__ void scores(const uint4* q, f32x4 (&r)[2]) const {
+        f32x4 lo[2], hi[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) lo[j] = hi[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const f16x2 d = as_f16x2(kd[j][s] | kd[j][s] << 16);
-            const uint32_t w[2] = {k[j][s].x, k[j][s].y};
-            Pieces p[4];
+            const f16x8 qh = as_f16x8(q[128 * s]), ql = as_f16x8(q[128 * s + 64]);
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-                p[t] = q8_pieces(int8_pair(__builtin_amdgcn_perm(0u, w[t / 2], t % 2 ? 0x0c030c02u : 0x0c010c00u)), d);
-            const f16x8 fh = as_f16x8(as_u32(p[0].h), as_u32(p[1].h), as_u32(p[2].h), as_u32(p[3].h));
-            const f16x8 fl = as_f16x8(as_u32(p[0].l), as_u32(p[1].l), as_u32(p[2].l), as_u32(p[3].l));
-            lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl, qh[s], lo, 0, 0, 0);
-            lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, ql[s], lo, 0, 0, 0);
-            hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, qh[s], hi, 0, 0, 0);
+            for (int j = 0; j < 2; ++j) {
+                const f16x2 d = as_f16x2(kd[j][s] | kd[j][s] << 16);
+                const uint32_t w[2] = {k[j][s].x, k[j][s].y};
+                Pieces p[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    p[t] = q8_pieces(int8_pair(__builtin_amdgcn_perm(0u, w[t / 2], t % 2 ? 0x0c030c02u : 0x0c010c00u)), d);
+                const f16x8 fh = as_f16x8(as_u32(p[0].h), as_u32(p[1].h), as_u32(p[2].h), as_u32(p[3].h));
+                const f16x8 fl = as_f16x8(as_u32(p[0].l), as_u32(p[1].l), as_u32(p[2].l), as_u32(p[3].l));
+                lo[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl, qh, lo[j], 0, 0, 0);
+                lo[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, ql, lo[j], 0, 0, 0);
+                hi[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, qh, hi[j], 0, 0, 0);
+            }
         }
-        return hi + lo;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) r[j] = hi[j] + lo[j];
     }
     __device__ __forceinline__ void weigh(const f16x8 ph, const f16x8 pl, f32x4 (&o)[U][4]) const {
 #pragma unroll
@@ -234,18 +250,21 @@ struct TreeKeys<kTypeF32, HD> {
 #pragma unroll
         for (int u = 0; u < U; ++u) v[i][u] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    __device__ __forceinline__ f32x4 scores(const f32x4 (&q)[S]) const {
+    __device__ __forceinline__ void scores(const uint4* qs, f32x4 (&r)[1]) const {
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;  // two sums: half the roundings in a row
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][0], q[s][0], a, 0, 0, 0);
-            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][1], q[s][1], b, 0, 0, 0);
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][2], q[s][2], a, 0, 0, 0);
-            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][3], q[s][3], b, 0, 0, 0);
+            const f32x4 q = __builtin_bit_cast(f32x4, qs[64 * s]);
+            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][0], q[0], a, 0, 0, 0);
+            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][1], q[1], b, 0, 0, 0);
+            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][2], q[2], a, 0, 0, 0);
+            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][3], q[3], b, 0, 0, 0);
+            keep(q);
+            if (HD == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // no more of q at once
         }
 #pragma unroll
-        for (int s = 0; s < S; ++s) keep(k[s]), keep(q[s]);
-        return a + b;
+        for (int s = 0; s < S; ++s) keep(k[s]);
+        r[0] = a + b;
     }
     __device__ __forceinline__ void weigh(const float (&p)[4], f32x4 (&o)[U][4]) const {
         const f32x4 w = (f32x4){p[0], p[1], p[2], p[3]} * kPieces;
@@ -310,8 +329,11 @@ __device__ __forceinline__ float slot_value(const uint8_t* head, int e) {
 }
 
 template <int W>
-struct TreeSmem {
-    float o[W][kTile][68];  // 64 dims of the waves' sums; pitch: 16-byte aligned, 4 banks apart
+struct __align__(16) TreeSmem {
+    union {
+        float o[W][kTile][68];  // 64 dims of the waves' sums; pitch: 16-byte aligned, 4 banks apart
+        uint4 q[16][64];        // before: the tile's queries as operands, [k-step][lane] (f16: [k-step * 2 + piece])
+    };
     float m[W][kTile], l[W][kTile];
     uint32_t again;  // rows to compute again
 };
@@ -412,6 +434,11 @@ __device__ __forceinline__ void tree_row_again(const TreeArgs& a, const TreeJob&
 template <int CT, int HD, int W, bool HIST>
 __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, TreeSmem<W>& sm) {
     constexpr int U = HD / 64, CK = tree_chunk<CT>(), NP = CK / kKvBlock;
+    // When a step's V is loaded and the next one's K: with K and after the scores, so that both have a step's time
+    // to come, or (head_dim 256) after the scores and after the products, for fewer registers and two waves
+    // on a SIMD in place of one: 37 beams over 301..1501 F32 keys 39.8 -> 26.1 us, 16 over 1000..4096 59 -> 44
+    // (F16 39 -> 34, Q8_0 46 -> 33)
+    constexpr bool LATE = HD == 256;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, n = lane & 15;
 
@@ -424,64 +451,74 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
         f32x4 t = *reinterpret_cast<const f32x4*>(qp + d);
         return q_ok ? t * a.scale_log2e : (f32x4){0.f, 0.f, 0.f, 0.f};
     };
+    // ---- cached keys: the waves take steps of CK keys in turn. The first step's loads come before all else
+    const uint32_t head = (uint32_t)(a.sb / a.n_head_kv) * w.h_kv;
+    const uint32_t sb = (uint32_t)a.sb, off_k = n * sb + head, off_v = 4 * g * sb + head;
+    const int c0 = w.k_begin / CK + wave, c1 = HIST ? (w.k_end + CK - 1) / CK : 0;
+    TreeKeys<CT, HD> t;
+    int pages[NP], next[NP];
+    auto pages_of = [&](int c, int (&p)[NP]) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) p[j] = page_of(a, w.seq, c * NP + j);
+    };
+    auto page_bytes = [&](int blk) {  // a missing page's loads read page 0; what they bring is cleared
+        return ((int64_t)max(blk, 0) * a.n_layer + a.layer) * kKvBlock * a.sb;
+    };
+    if (c0 < c1) {
+        pages_of(c0, pages);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) t.load_k(j, a.k_arena + page_bytes(pages[j]), off_k, g);
+        if constexpr (!LATE)
+#pragma unroll
+            for (int j = 0; j < NP; ++j) t.load_v(j, a.v_arena + page_bytes(pages[j]), off_v, sb, n);
+    }
+
+    // ---- the queries as operands, in LDS: a wave makes every W-th k-step's
+    float qsc = 1.0f;
+    if constexpr (CT == kTypeF32) {
+        for (int s = wave; s < HD / 16; s += W) sm.q[s][lane] = __builtin_bit_cast(uint4, load_q(16 * s + 4 * g));
+    } else {
+        constexpr int S = HD / 32;
+        f32x4 x[S][2];
+        float mx = 0.0f;  // of the whole row
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                x[s][k] = load_q(32 * s + 8 * g + 4 * k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[s][k][e]));
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const int ex = norm_exp(__float_as_uint(mx));
+        const float f = pow2_bits(268 - ex);
+        qsc = pow2_bits(ex - 14);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            if (s % W != wave) continue;
+            f16x4 h0, l0, h1, l1;
+            split4(x[s][0][0] * f, x[s][0][1] * f, x[s][0][2] * f, x[s][0][3] * f, h0, l0);
+            split4(x[s][1][0] * f, x[s][1][1] * f, x[s][1][2] * f, x[s][1][3] * f, h1, l1);
+            sm.q[2 * s][lane] = __builtin_bit_cast(uint4, __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7));
+            sm.q[2 * s + 1][lane] = __builtin_bit_cast(uint4, __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
     f32x4 o[U][4];
     float m = -INFINITY, l = 0.0f;  // l: of this lane's keys
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[u][e] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+    // read again in every step: kept over the loop they would take as many registers as the keys
+    auto operands = [&] {
+        int at = lane;
+        asm volatile("" : "+v"(at));
+        return &sm.q[0][at];
+    };
 
-    // ---- cached keys: the waves take steps of CK keys in turn
-    const uint32_t head = (uint32_t)(a.sb / a.n_head_kv) * w.h_kv;
-    const uint32_t sb = (uint32_t)a.sb, off_k = n * sb + head, off_v = 4 * g * sb + head;
-    const int c0 = w.k_begin / CK + wave, c1 = (w.k_end + CK - 1) / CK;
-    if (HIST && c0 < c1) {
-        constexpr int S = CT == kTypeF32 ? HD / 16 : HD / 32;
-        f16x8 qh[CT == kTypeF32 ? 1 : S], ql[CT == kTypeF32 ? 1 : S];
-        f32x4 qf[CT == kTypeF32 ? S : 1];
-        float qsc = 1.0f;
-        if constexpr (CT == kTypeF32) {
-#pragma unroll
-            for (int s = 0; s < S; ++s) qf[s] = load_q(16 * s + 4 * g);
-        } else {
-            f32x4 t[S][2];
-            float mx = 0.0f;
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    t[s][k] = load_q(32 * s + 8 * g + 4 * k);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(t[s][k][e]));
-                }
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const int ex = norm_exp(__float_as_uint(mx));
-            const float f = pow2_bits(268 - ex);
-            qsc = pow2_bits(ex - 14);
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-                f16x4 h0, l0, h1, l1;
-                split4(t[s][0][0] * f, t[s][0][1] * f, t[s][0][2] * f, t[s][0][3] * f, h0, l0);
-                split4(t[s][1][0] * f, t[s][1][1] * f, t[s][1][2] * f, t[s][1][3] * f, h1, l1);
-                qh[s] = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
-                ql[s] = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
-        }
-        TreeKeys<CT, HD> t;
-        int pages[NP], next[NP];
-        auto pages_of = [&](int c, int (&p)[NP]) {
-#pragma unroll
-            for (int j = 0; j < NP; ++j) p[j] = page_of(a, w.seq, c * NP + j);
-        };
-        auto page_bytes = [&](int blk) {  // a missing page's loads read page 0; what they bring is cleared
-            return ((int64_t)max(blk, 0) * a.n_layer + a.layer) * kKvBlock * a.sb;
-        };
-        pages_of(c0, pages);
-#pragma unroll
-        for (int j = 0; j < NP; ++j) t.load_k(j, a.k_arena + page_bytes(pages[j]), off_k, g);
-#pragma unroll
-        for (int j = 0; j < NP; ++j) t.load_v(j, a.v_arena + page_bytes(pages[j]), off_v, sb, n);
+    if (c0 < c1) {
         for (int c = c0; c < c1; c += W) {
             const bool more = c + W < c1;
             if (more) pages_of(c + W, next);
@@ -489,30 +526,32 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
             bool whole = left >= CK;
 #pragma unroll
             for (int j = 0; j < NP; ++j) whole &= pages[j] >= 0;
-            if (!whole) {  // zero rows for missing pages; no rows past the last key
+            if (!whole)  // zero rows for missing pages
 #pragma unroll
-                for (int j = 0; j < NP; ++j) {
+                for (int j = 0; j < NP; ++j)
                     if (pages[j] < 0) t.zero_k(j);
+            f32x4 r[NP];
+            t.scores(operands(), r);
+            if constexpr (LATE) {
+                __builtin_amdgcn_sched_barrier(0);  // not over the scores' registers
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (pages[j] < 0 || 16 * j + 4 * g + i >= left) t.zero_v(j, i);
-                }
-            }
-            float s[4 * NP];
-#pragma unroll
-            for (int j = 0; j < NP; ++j) {
-                f32x4 r;
-                if constexpr (CT == kTypeF32)
-                    r = t.scores(qf);
-                else
-                    r = t.scores(j, qh, ql) * qsc;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[4 * j + i] = left >= CK || 16 * j + 4 * g + i < left ? r[i] : -INFINITY;
-            }
-            if (more) {
+                for (int j = 0; j < NP; ++j) t.load_v(j, a.v_arena + page_bytes(pages[j]), off_v, sb, n);
+            } else if (more) {
 #pragma unroll
                 for (int j = 0; j < NP; ++j) t.load_k(j, a.k_arena + page_bytes(next[j]), off_k, g);
             }
+            float s[4 * NP];
+#pragma unroll
+            for (int j = 0; j < NP; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[4 * j + i] = left >= CK || 16 * j + 4 * g + i < left ? r[j][i] * qsc : -INFINITY;
+            if (!whole)  // no rows past the last key
+#pragma unroll
+                for (int j = 0; j < NP; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (pages[j] < 0 || 16 * j + 4 * g + i >= left) t.zero_v(j, i);
             softmax_step<4 * NP, U>(s, m, l, o);
             if constexpr (CT == kTypeF32) {
                 t.weigh(s, o);
@@ -526,21 +565,27 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
             if (more) {
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
-                    t.load_v(j, a.v_arena + page_bytes(next[j]), off_v, sb, n);
+                    if constexpr (LATE)
+                        t.load_k(j, a.k_arena + page_bytes(next[j]), off_k, g);
+                    else
+                        t.load_v(j, a.v_arena + page_bytes(next[j]), off_v, sb, n);
                     pages[j] = next[j];
                 }
             }
         }
     }
 
-    // ---- drafted keys, 16 at a time
-    if (w.drafts && 16 * wave < w.n_draft) {
-        constexpr int S = HD / 16;
-        f32x4 qf[S];
-#pragma unroll
-        for (int s = 0; s < S; ++s) qf[s] = load_q(16 * s + 4 * g);
+    // ---- drafted keys, 16 at a time, from the last wave on, which has the fewest cached ones
+    if constexpr (CT != kTypeF32) {
+        if (w.drafts) {
+            __syncthreads();  // the f16 operands are read
+            for (int s = wave; s < HD / 16; s += W) sm.q[s][lane] = __builtin_bit_cast(uint4, load_q(16 * s + 4 * g));
+            __syncthreads();
+        }
+    }
+    if (w.drafts) {
         const uint32_t rs = (uint32_t)(a.kv_stride * 4);
-        for (int k0 = 16 * wave; k0 < w.n_draft; k0 += 16 * W) {
+        for (int k0 = 16 * (W - 1 - wave); k0 < w.n_draft; k0 += 16 * W) {
             const int left = w.n_draft - k0;
             const int64_t base = ((int64_t)w.seq * a.n_tokens + k0) * a.kv_stride + (int64_t)w.h_kv * HD;
             TreeKeys<kTypeF32, HD> t;
@@ -553,12 +598,13 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
                 seen = (uint32_t)(a.mask[((int64_t)w.seq * a.n_tokens + tok) * a.words + k0 / 64] >> (k0 % 64 + 4 * g));
             else
                 seen = (1u << min(max(tok + 1 - k0 - 4 * g, 0), 4)) - 1u;
-            const f32x4 r = t.scores(qf);
+            f32x4 r[1];
+            t.scores(operands(), r);
             float s[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool in = 4 * g + i < left;
-                s[i] = in && (seen >> i & 1) ? r[i] : -INFINITY;
+                s[i] = in && (seen >> i & 1) ? r[0][i] : -INFINITY;
                 if (!in) t.zero_v(0, i);
             }
             softmax_step<4, U>(s, m, l, o);
@@ -631,7 +677,7 @@ __device__ __forceinline__ void tree_job(const TreeArgs& a, TreeJob& w, int seq)
 // Grid: (unit, tile) pairs with the tiles of a unit on one XCD (workgroup id % 8) one after another, as they
 // read the same keys; unit = (sequence, split, KV head).
 template <int CT, int HD>
-__global__ void __launch_bounds__(64 * kTreeWaves) tree_attn_kernel(TreeArgs a) {
+__global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_kernel(TreeArgs a) {
     __shared__ TreeSmem<kTreeWaves> sm;
     TreeJob w;
     const int id = blockIdx.x, turn = id / (8 * a.tiles), rest = id % (8 * a.tiles), unit = turn * 8 + rest % 8;
@@ -1051,7 +1097,7 @@ static TreePlan tree_plan16(int n_head, int n_head_kv, int n_seqs, int n_tokens,
     TreePlan p{};
     p.tiles = (n_tokens * (n_head / n_head_kv) + kTile - 1) / kTile;
     const int64_t base = (int64_t)p.tiles * n_head_kv * n_seqs, want = std::max<int64_t>(1, (3 * cu_count() + base - 1) / base);
-    p.kps = (int)std::max<int64_t>(128, round_up((max_past + want - 1) / want, 128));
+    p.kps = (int)std::max<int64_t>(128, round_up((max_past + want - 1) / want, 64));
     p.splits = std::max(1, (max_past + p.kps - 1) / p.kps);
     return p;
 }
