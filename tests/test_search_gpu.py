@@ -603,3 +603,61 @@ def test_beam_select_in_graphs(dev):
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert torch.equal(o, w)
+
+
+# ---------------------------------------------------------------- the operators together
+def _example():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "search_decode.py")
+    spec = importlib.util.spec_from_file_location("search_decode", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+def _whole(ex, model, cache_type, tokens):
+    """Logits of a sequence run at once, without a cache."""
+    import torch
+    s = ex.Search(model, cache_type)
+    logits, _, _ = model.forward(torch.tensor([tokens], device="cuda"), s.cache, s.tables, s.lengths, 0)
+    return logits.double().cpu().numpy()
+
+
+def test_search_example_beams_and_speculation(dev):
+    """The example's beams, from forked pages, score what their sequences score when run at once without a cache,
+    and its speculative steps take the tokens that one-by-one greedy decoding takes. The model's products are
+    made in 64 bits here (the library's round the activations to 8 bits, where a last bit can decide a step of
+    2^-7), and an F32 cache holds the rows unrounded, so that fp32 roundings alone tell the two apart."""
+    import torch
+    ex = _example()
+
+    class Smooth(ex.Model):
+        @staticmethod
+        def _product(w, x):
+            return (x.double() @ dc.dequantize_rows(dc.TYPE_Q8_0, w[0], w[1], w[2]).double().T.contiguous()).float()
+
+        @staticmethod
+        def _residual(w, x, r):
+            return Smooth._product(w, x) + r
+    model = Smooth(layers=2, vocab=500, seed=3)
+    prompt = (torch.arange(21, device="cuda") * 13 % 500)[None]
+    search = ex.Search(model, dc.TYPE_F32)
+    out, scores, missing = search.beams(prompt, beams=5, steps=30)
+    assert int(missing) == 0 and search.length == 21 + 29
+    out, scores = to_host(out), to_host(scores)[0]
+    assert (np.diff(scores) <= 0).all() and len({tuple(o) for o in out.tolist()}) == 5
+    for o, s in zip(out.tolist(), scores):
+        x = _whole(ex, model, dc.TYPE_F32, prompt[0].tolist() + o)[20:-1]
+        lp = x - np.log(np.exp(x - x.max(1, keepdims=True)).sum(1, keepdims=True)) - x.max(1, keepdims=True)
+        assert abs(lp[np.arange(30), o].sum() - s) < 2e-2, "a beam's pages are not its sequence's"
+    held = to_host(search.refs)
+    n_live = int(search.keep(2))
+    assert n_live == 4 and (to_host(search.refs) == ([1] * 4 + [0] * 60)).all() and held.sum() >= 20
+    text = prompt[0].tolist() + out[2].tolist()
+    x = _whole(ex, model, dc.TYPE_F32, text)[-1]
+    first = int(x.argmax())
+    taken = search.speculate(text[-1], [first, (first + 1) % 500, 7], [0, 0, 1])
+    assert taken[0] == first and len(taken) >= 2  # the drafted first token was right
+    x = _whole(ex, model, dc.TYPE_F32, text + [first])[-1]
+    assert taken[1] == int(x.argmax()) and search.length == 50 + len(taken)
