@@ -31,10 +31,11 @@ struct TreeArgs {
     int64_t out_stride;
     int n_seqs, n_tokens, n_head, n_head_kv;
     float scale_log2e;
-    int rep, tiles, tiles16, splits, kps, units, hist_wgs, draft_wgs;
+    int rep, tiles, tiles16, splits, kps, units, share, hist_wgs, draft_wgs;
     int64_t rows;  // n_seqs * n_tokens * n_head
     float* ws_o;   // [splits][rows][HD]
     float* ws_ml;  // [splits][rows][2]
+    int* ws_kps;   // keys per split, where the device chooses them
 };
 size_t tree_workspace_bytes(int hd, int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past);
 hipError_t launch_tree_attention(int ct, int hd, TreeArgs a, void* ws, hipStream_t st);

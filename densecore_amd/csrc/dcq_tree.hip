@@ -332,7 +332,10 @@ template <int W>
 struct __align__(16) TreeSmem {
     union {
         float o[W][kTile][68];  // 64 dims of the waves' sums; pitch: 16-byte aligned, 4 banks apart
-        uint4 q[16][64];        // before: the tile's queries as operands, [k-step][lane] (f16: [k-step * 2 + piece])
+        struct {                // before: the tile's queries as operands, [k-step][lane]
+            uint4 qf[16][64];   // fp32
+            uint4 q[16][64];    // f16 pieces, [k-step * 2 + piece]
+        };
     };
     float m[W][kTile], l[W][kTile];
     uint32_t again;  // rows to compute again
@@ -344,6 +347,7 @@ struct TreeJob {
     int k_begin, k_end;  // cached keys
     bool drafts;         // and the drafted ones
     int slot;            // of the partial results
+    int first[2];        // the pages of this wave's first step
 };
 
 // The page of a sequence's logical block (uniform), negative where there is none. A scalar load: its wait is
@@ -430,8 +434,12 @@ __device__ __forceinline__ void tree_row_again(const TreeArgs& a, const TreeJob&
     __syncthreads();
 }
 
-// A tile of 16 rows over a share of the keys, by a workgroup of W waves (HIST: cached keys too).
-template <int CT, int HD, int W, bool HIST>
+// A tile of 16 rows over a share of the keys, by a workgroup of W waves (HIST: cached keys too). EARLY: the first
+// drafted keys are loaded before all else and taken before the cached ones, whose loads are in flight meanwhile:
+// for calls without key splits, where a workgroup is a chain of latencies (7 tokens over 100 keys 11.1 -> 10.3 us,
+// one over one 9.5 -> 7.6). In larger calls their registers cost a wave per SIMD (16 sequences of 1000..4096 keys,
+// 16/4 heads x 128, F16 22.4 -> 26.0 us), at head_dim 256 they do not fit.
+template <int CT, int HD, int W, bool HIST, bool EARLY>
 __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, TreeSmem<W>& sm) {
     constexpr int U = HD / 64, CK = tree_chunk<CT>(), NP = CK / kKvBlock;
     // When a step's V is loaded and the next one's K: with K and after the scores, so that both have a step's time
@@ -451,7 +459,26 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
         f32x4 t = *reinterpret_cast<const f32x4*>(qp + d);
         return q_ok ? t * a.scale_log2e : (f32x4){0.f, 0.f, 0.f, 0.f};
     };
-    // ---- cached keys: the waves take steps of CK keys in turn. The first step's loads come before all else
+    // ---- drafted keys, 16 at a time: the waves from the last on, which have the fewest cached keys
+    const uint32_t rs = (uint32_t)(a.kv_stride * 4);
+    uint64_t seen = 0;  // the row's mask word of the drafted keys in td, from the lane's first one
+    auto load_drafts = [&](TreeKeys<kTypeF32, HD>& t, int k0) {
+        const int left = w.n_draft - k0;
+        const int64_t base = ((int64_t)w.seq * a.n_tokens + k0) * a.kv_stride + (int64_t)w.h_kv * HD;
+        t.load_k(0, reinterpret_cast<const uint8_t*>(a.k_cur + base), min(n, left - 1) * rs, g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            t.load_v_key(i, reinterpret_cast<const uint8_t*>(a.v_cur + base), min(4 * g + i, left - 1) * rs, n);
+        if (a.mask)
+            seen = a.mask[((int64_t)w.seq * a.n_tokens + tok) * a.words + k0 / 64] >> (k0 % 64 + 4 * g);
+        else
+            seen = (1u << min(max(tok + 1 - k0 - 4 * g, 0), 4)) - 1u;
+    };
+    const int d0 = w.drafts ? 16 * (W - 1 - wave) : w.n_draft;
+    TreeKeys<kTypeF32, HD> early;
+    if (EARLY && d0 < w.n_draft) load_drafts(early, d0);
+
+    // ---- cached keys: the waves take steps of CK keys in turn. The first step's loads come before the queries
     const uint32_t head = (uint32_t)(a.sb / a.n_head_kv) * w.h_kv;
     const uint32_t sb = (uint32_t)a.sb, off_k = n * sb + head, off_v = 4 * g * sb + head;
     const int c0 = w.k_begin / CK + wave, c1 = HIST ? (w.k_end + CK - 1) / CK : 0;
@@ -465,7 +492,8 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
         return ((int64_t)max(blk, 0) * a.n_layer + a.layer) * kKvBlock * a.sb;
     };
     if (c0 < c1) {
-        pages_of(c0, pages);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) pages[j] = w.first[j];
 #pragma unroll
         for (int j = 0; j < NP; ++j) t.load_k(j, a.k_arena + page_bytes(pages[j]), off_k, g);
         if constexpr (!LATE)
@@ -475,9 +503,9 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
 
     // ---- the queries as operands, in LDS: a wave makes every W-th k-step's
     float qsc = 1.0f;
-    if constexpr (CT == kTypeF32) {
-        for (int s = wave; s < HD / 16; s += W) sm.q[s][lane] = __builtin_bit_cast(uint4, load_q(16 * s + 4 * g));
-    } else {
+    if (CT == kTypeF32 || w.drafts)
+        for (int s = wave; s < HD / 16; s += W) sm.qf[s][lane] = __builtin_bit_cast(uint4, load_q(16 * s + 4 * g));
+    if constexpr (CT != kTypeF32) {
         constexpr int S = HD / 32;
         f32x4 x[S][2];
         float mx = 0.0f;  // of the whole row
@@ -512,11 +540,26 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
         for (int e = 0; e < 4; ++e) o[u][e] = (f32x4){0.f, 0.f, 0.f, 0.f};
     __syncthreads();
     // read again in every step: kept over the loop they would take as many registers as the keys
-    auto operands = [&] {
+    auto operands = [&](const uint4(&q)[16][64]) {
         int at = lane;
         asm volatile("" : "+v"(at));
-        return &sm.q[0][at];
+        return &q[0][at];
     };
+
+    auto add_drafts = [&](TreeKeys<kTypeF32, HD>& t, int k0) {
+        f32x4 r[1];
+        t.scores(operands(sm.qf), r);
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in = 4 * g + i < w.n_draft - k0;
+            s[i] = in && (seen >> i & 1) ? r[0][i] : -INFINITY;
+            if (!in) t.zero_v(0, i);
+        }
+        softmax_step<4, U>(s, m, l, o);
+        t.weigh(s, o);
+    };
+    if (EARLY && d0 < w.n_draft) add_drafts(early, d0);
 
     if (c0 < c1) {
         for (int c = c0; c < c1; c += W) {
@@ -531,7 +574,10 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
                 for (int j = 0; j < NP; ++j)
                     if (pages[j] < 0) t.zero_k(j);
             f32x4 r[NP];
-            t.scores(operands(), r);
+            if constexpr (CT == kTypeF32)
+                t.scores(operands(sm.qf), r);
+            else
+                t.scores(operands(sm.q), r);
             if constexpr (LATE) {
                 __builtin_amdgcn_sched_barrier(0);  // not over the scores' registers
 #pragma unroll
@@ -575,41 +621,10 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
         }
     }
 
-    // ---- drafted keys, 16 at a time, from the last wave on, which has the fewest cached ones
-    if constexpr (CT != kTypeF32) {
-        if (w.drafts) {
-            __syncthreads();  // the f16 operands are read
-            for (int s = wave; s < HD / 16; s += W) sm.q[s][lane] = __builtin_bit_cast(uint4, load_q(16 * s + 4 * g));
-            __syncthreads();
-        }
-    }
-    if (w.drafts) {
-        const uint32_t rs = (uint32_t)(a.kv_stride * 4);
-        for (int k0 = 16 * (W - 1 - wave); k0 < w.n_draft; k0 += 16 * W) {
-            const int left = w.n_draft - k0;
-            const int64_t base = ((int64_t)w.seq * a.n_tokens + k0) * a.kv_stride + (int64_t)w.h_kv * HD;
-            TreeKeys<kTypeF32, HD> t;
-            t.load_k(0, reinterpret_cast<const uint8_t*>(a.k_cur + base), min(n, left - 1) * rs, g);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                t.load_v_key(i, reinterpret_cast<const uint8_t*>(a.v_cur + base), min(4 * g + i, left - 1) * rs, n);
-            uint32_t seen;  // bit i: key 4 g + i
-            if (a.mask)
-                seen = (uint32_t)(a.mask[((int64_t)w.seq * a.n_tokens + tok) * a.words + k0 / 64] >> (k0 % 64 + 4 * g));
-            else
-                seen = (1u << min(max(tok + 1 - k0 - 4 * g, 0), 4)) - 1u;
-            f32x4 r[1];
-            t.scores(operands(), r);
-            float s[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool in = 4 * g + i < left;
-                s[i] = in && (seen >> i & 1) ? r[0][i] : -INFINITY;
-                if (!in) t.zero_v(0, i);
-            }
-            softmax_step<4, U>(s, m, l, o);
-            t.weigh(s, o);
-        }
+    for (int k0 = EARLY ? d0 + 16 * W : d0; k0 < w.n_draft; k0 += 16 * W) {
+        TreeKeys<kTypeF32, HD> t;
+        load_drafts(t, k0);
+        add_drafts(t, k0);
     }
 
     // ---- the waves' sums together, 64 dims at a time: thread (of the first 256) -> row tid / 16, 4 dims
@@ -676,7 +691,7 @@ __device__ __forceinline__ void tree_job(const TreeArgs& a, TreeJob& w, int seq)
 
 // Grid: (unit, tile) pairs with the tiles of a unit on one XCD (workgroup id % 8) one after another, as they
 // read the same keys; unit = (sequence, split, KV head).
-template <int CT, int HD>
+template <int CT, int HD, bool EARLY>
 __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_kernel(TreeArgs a) {
     __shared__ TreeSmem<kTreeWaves> sm;
     TreeJob w;
@@ -684,14 +699,19 @@ __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_
     if (unit >= a.units) return;
     w.h_kv = unit % a.n_head_kv;
     w.slot = unit / a.n_head_kv % a.splits;
-    tree_job(a, w, unit / a.n_head_kv / a.splits);
+    w.k_begin = w.slot * a.kps;
     w.row0 = rest / 8 * kTile;
+    const int seq = unit / a.n_head_kv / a.splits, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int CK = tree_chunk<CT>();
+#pragma unroll
+    for (int j = 0; j < CK / kKvBlock; ++j)  // beside the loads of the lengths, not after them
+        w.first[j] = page_of(a, seq, (w.k_begin / CK + wave) * (CK / kKvBlock) + j);
+    tree_job(a, w, seq);
     const int n_split = max((w.past + a.kps - 1) / a.kps, 1);
     if (w.slot >= n_split || (w.row0 >= w.n_rows && a.splits > 1)) return;  // the merge writes such rows' zeros
-    w.k_begin = w.slot * a.kps;
     w.k_end = w.row0 < w.n_rows ? min(w.past, w.k_begin + a.kps) : 0;
     w.drafts = w.slot == n_split - 1 && w.row0 < w.n_rows;
-    tree_tile<CT, HD, kTreeWaves, true>(a, w, sm);
+    tree_tile<CT, HD, kTreeWaves, true, EARLY>(a, w, sm);
 }
 
 // ---------------------------------------------------------------- many rows
@@ -750,6 +770,39 @@ struct TreeRaw {
     }
 };
 
+// What the unit-th workgroups (of every KV head and tile) work on: split `split` of kps keys of a sequence.
+struct TreeShare {
+    int seq, split, kps;  // seq -1: nothing
+};
+// Up to 64 sequences share the units by their lengths, which the host does not know: the fewest keys per unit
+// (a.kps or more, in steps of an eighth) that a.share units suffice for. 8 sequences of 1500..4096 keys on 64
+// units: 384 keys, where their longest alone would ask for 512 and leave a quarter of the units without work;
+// 24 tokens of 32/8 heads x 128, F16: 40 -> 32 us. More sequences even out by themselves.
+__device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, int unit) {
+    const int per_seq = a.splits - 1;
+    if (!a.share) return {unit / per_seq, unit % per_seq, a.kps};
+    const int lane = threadIdx.x & 63;
+    const int past = lane < a.n_seqs ? min(max(a.past[lane], 0), a.max_past) : 0;
+    int sum = past;  // below 2^30
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k, 64);
+    int kps = max(a.kps, (int)(((uint32_t)sum + a.share - 1) / a.share + 31) & ~31), n, upto;
+    for (;; kps += max(kps / 8 & ~31, 32)) {
+        n = ((uint32_t)past + kps - 1) / (uint32_t)kps;
+        upto = n;  // units up to this lane's sequence
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) {
+            const int o = __shfl_up(upto, k, 64);
+            upto += lane >= k ? o : 0;
+        }
+        if (__builtin_amdgcn_readlane(upto, 63) <= a.share || kps >= a.max_past) break;
+    }
+    const uint64_t after = __ballot(upto > unit);
+    if (!after) return {-1, 0, kps};
+    const int seq = __ffsll((unsigned long long)after) - 1;
+    return {seq, unit - __builtin_amdgcn_readlane(upto - n, seq), kps};
+}
+
 // 32 W rows of a KV head over a share of its cached keys (slots 1 ..), or 16 rows over the drafted keys (slot 0:
 // the workgroups from hist_wgs on, which fill the end of the launch).
 template <int CT, int HD, int W>
@@ -774,18 +827,24 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         w.k_begin = w.k_end = 0;
         w.drafts = true;
         w.slot = 0;
-        if (w.row0 < w.n_rows) tree_tile<kTypeF32, HD, W, false>(a, w, sm.t);
+        if (w.row0 < w.n_rows) tree_tile<kTypeF32, HD, W, false, HD < 256>(a, w, sm.t);
         return;
     }
     id = blockIdx.x;
     const int turn = id / (8 * a.tiles), rest = id % (8 * a.tiles), unit = turn * 8 + rest % 8;
     if (unit >= a.units) return;
     w.h_kv = unit % a.n_head_kv;
-    w.slot = unit / a.n_head_kv % (a.splits - 1) + 1;
-    tree_job(a, w, unit / a.n_head_kv / (a.splits - 1));
     w.row0 = rest / 8 * (kRowsPerWave * W);
-    w.k_begin = (w.slot - 1) * a.kps;
-    w.k_end = min(w.past, w.k_begin + a.kps);
+    TreeShare share = tree_share(a, unit / a.n_head_kv);
+    share.seq = __builtin_amdgcn_readfirstlane(share.seq);
+    share.split = __builtin_amdgcn_readfirstlane(share.split);
+    share.kps = __builtin_amdgcn_readfirstlane(share.kps);
+    if (id == 0 && threadIdx.x == 0 && a.ws_kps) *a.ws_kps = share.kps;
+    if (share.seq < 0) return;
+    tree_job(a, w, share.seq);
+    w.slot = share.split + 1;
+    w.k_begin = share.split * share.kps;
+    w.k_end = min(w.past, w.k_begin + share.kps);
     w.drafts = false;
     if (w.k_begin >= w.k_end || w.row0 >= w.n_rows) return;
 
@@ -1047,7 +1106,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
     const int trow = row / a.n_head, h = row % a.n_head, seq = trow / a.n_tokens, tok = trow % a.n_tokens;
     const int past = min(max(a.past[seq], 0), a.max_past);
     const int n_draft = a.n_draft ? min(max(a.n_draft[seq], 0), a.n_tokens) : a.n_tokens;
-    const int n_hist = (past + a.kps - 1) / a.kps;
+    const int kps = a.ws_kps ? *a.ws_kps : a.kps, n_hist = (past + kps - 1) / kps;
     const int n_split = tok < n_draft ? (a.draft_wgs ? n_hist + 1 : max(n_hist, 1)) : 0;
     float m = -INFINITY, l = 0.0f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -1090,6 +1149,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
 struct TreePlan {
     int block_waves;  // 0: the 16-row kernel
     int tiles, splits, kps;
+    int share, units;  // of the block kernel: see tree_share; units: of all KV heads
 };
 
 // Key splits: workgroups until about three per CU have work, 128 keys (a step of each wave) at the least.
@@ -1108,15 +1168,20 @@ static TreePlan tree_plan(int ct, int hd, int n_head, int n_head_kv, int n_seqs,
     TreePlan p{};
     p.block_waves = rows > 128 && hd <= 128 ? 8 : 4;
     p.tiles = (rows + kRowsPerWave * p.block_waves - 1) / (kRowsPerWave * p.block_waves);
-    const int64_t base = (int64_t)p.tiles * n_head_kv * n_seqs, wgs = p.block_waves == 8 ? cu_count() : 2 * cu_count();
-    const int64_t want = std::max<int64_t>(1, (wgs + base - 1) / base);
-    p.kps = (int)std::max<int64_t>(256, round_up((max_past + want - 1) / want, 64));
+    const int64_t base = (int64_t)p.tiles * n_head_kv, wgs = p.block_waves == 8 ? cu_count() : 2 * cu_count();
+    const int share = (int)std::max<int64_t>((wgs + base - 1) / base, n_seqs), bk = 8 * p.block_waves;
+    // keys of a split were all sequences as long as the longest; up to 64 sequences share out by their lengths,
+    // of no fewer than half as many keys (which bounds the partial results)
+    const int64_t kps = std::max<int64_t>(256, round_up(((int64_t)max_past * n_seqs + share - 1) / share, bk));
+    p.share = n_seqs > 1 && n_seqs <= 64 ? share : 0;
+    p.kps = (int)(p.share ? std::max<int64_t>(256, round_up(kps / 2, bk)) : kps);
     p.splits = 1 + (max_past + p.kps - 1) / p.kps;
+    p.units = (p.share ? p.share : n_seqs * (p.splits - 1)) * n_head_kv;
     return p;
 }
 
 static size_t tree_partial_bytes(const TreePlan& p, int hd, int64_t rows) {
-    return p.splits <= 1 ? 0 : (size_t)(round_up(p.splits * rows * hd * 4, 256) + round_up(p.splits * rows * 2 * 4, 256));
+    return p.splits <= 1 ? 0 : (size_t)(round_up(p.splits * rows * hd * 4, 256) + round_up(p.splits * rows * 2 * 4, 256) + 256);
 }
 
 // Of the larger plan: the query does not know the cache type.
@@ -1157,7 +1222,13 @@ static void launch_tree_t(const TreeArgs& a, int block_waves, int wgs, hipStream
             return;
         }
     }
-    hipLaunchKernelGGL((tree_attn_kernel<CT, HD>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
+    if constexpr (HD < 256) {
+        if (a.splits == 1) {
+            hipLaunchKernelGGL((tree_attn_kernel<CT, HD, true>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((tree_attn_kernel<CT, HD, false>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
 }
 
 hipError_t launch_tree_attention(int ct, int hd, TreeArgs a, void* ws, hipStream_t st) {
@@ -1167,13 +1238,16 @@ hipError_t launch_tree_attention(int ct, int hd, TreeArgs a, void* ws, hipStream
     a.rows = (int64_t)a.n_seqs * a.n_tokens * a.n_head;
     a.tiles16 = (a.n_tokens * a.rep + kTile - 1) / kTile;
     const int64_t drafts = p.block_waves ? (int64_t)a.n_seqs * a.n_head_kv * a.tiles16 : 0;
-    const int64_t units = (int64_t)a.n_seqs * (p.block_waves ? p.splits - 1 : p.splits) * a.n_head_kv;
+    const int64_t units = p.block_waves ? p.units : (int64_t)a.n_seqs * p.splits * a.n_head_kv;
     const int64_t wgs = drafts + (units + 7) / 8 * 8 * p.tiles;
     if (wgs > INT32_MAX) return hipErrorInvalidValue;
     a.units = (int)units, a.draft_wgs = (int)drafts, a.hist_wgs = (int)(wgs - drafts);
-    if (p.splits > 1) {
-        a.ws_o = static_cast<float*>(ws);
-        a.ws_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round_up(p.splits * a.rows * hd * 4, 256));
+    a.share = p.share;
+    if (p.splits > 1) {  // O, (m, l), and the keys per split where the device chooses them
+        uint8_t* w = static_cast<uint8_t*>(ws);
+        a.ws_o = reinterpret_cast<float*>(w), w += round_up(p.splits * a.rows * hd * 4, 256);
+        a.ws_ml = reinterpret_cast<float*>(w), w += round_up(p.splits * a.rows * 2 * 4, 256);
+        if (p.share) a.ws_kps = reinterpret_cast<int*>(w);
     }
 #define DCQ_TREE_CASE(C, H)                                         \
     if (ct == C && hd == H) {                                       \
