@@ -251,20 +251,20 @@ struct TreeKeys<kTypeF32, HD> {
         for (int u = 0; u < U; ++u) v[i][u] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
     __device__ __forceinline__ void scores(const uint4* qs, f32x4 (&r)[1]) const {
-        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;  // two sums: half the roundings in a row
+        f32x4 a[4];  // four sums: a quarter of the roundings in a row
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             const f32x4 q = __builtin_bit_cast(f32x4, qs[64 * s]);
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][0], q[0], a, 0, 0, 0);
-            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][1], q[1], b, 0, 0, 0);
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][2], q[2], a, 0, 0, 0);
-            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][3], q[3], b, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][e], q[e], a[e], 0, 0, 0);
             keep(q);
             if (HD == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // no more of q at once
         }
 #pragma unroll
         for (int s = 0; s < S; ++s) keep(k[s]);
-        r[0] = a + b;
+        r[0] = (a[0] + a[1]) + (a[2] + a[3]);
     }
     __device__ __forceinline__ void weigh(const float (&p)[4], f32x4 (&o)[U][4]) const {
         const f32x4 w = (f32x4){p[0], p[1], p[2], p[3]} * kPieces;
@@ -720,13 +720,13 @@ __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_
 template <int CT, int HD, int W>
 struct __align__(16) TreeBlock {
     static constexpr bool DMA = CT == kTypeF16;
-    static constexpr int NPC = DMA ? 1 : 2, NBUF = DMA ? 4 : 2;
+    static constexpr int NPC = DMA ? 1 : 2, NBUF = 2, BK = DMA ? 64 : 8 * W;
     // K rows are read 16 bytes per lane down a column of 32 rows, V rows four at a time, 64 bytes each. Padded
     // rows lie 4 and 16 banks apart for that; in rows without padding the 16-byte pieces are permuted instead,
     // piece c of row r at c ^ swizzle(r).
     static constexpr int KP = DMA ? HD : HD + 8, VP = DMA ? HD : HD + 32;
-    _Float16 k[NBUF][NPC][8 * W][KP];  // [buffer][piece][key][dim]
-    _Float16 v[NBUF][NPC][8 * W][VP];
+    _Float16 k[NBUF][NPC][BK][KP];  // [buffer][piece][key][dim]
+    _Float16 v[NBUF][NPC][BK][VP];
     static __device__ __forceinline__ int k_swizzle(int r) { return DMA ? r & (HD / 8 - 1) & 15 : 0; }
     static __device__ __forceinline__ int v_swizzle(int r) { return DMA ? (r & 3) << 1 : 0; }
 };
@@ -884,7 +884,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         }
     }
 
-    constexpr int BK = 8 * W;  // keys of a block
+    constexpr int BK = Block::BK, RW = BK / W;  // keys of a block, and of them a wave's
     constexpr bool DMA = Block::DMA;
     constexpr int NBUF = Block::NBUF;
     const int64_t head = a.sb / a.n_head_kv * w.h_kv;
@@ -892,7 +892,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
     const int skey = tid >> 3, se0 = E * (tid & 7);
     TreeRaw<E> rk, rv;
     // the page of the wave's rows 8 w .. + 7
-    auto wave_page = [&](int kb) { return kb < w.k_end ? page_of(a, w.seq, (kb + 8 * wave) / kKvBlock) : -1; };
+    auto wave_page = [&](int kb) { return kb < w.k_end ? page_of(a, w.seq, (kb + RW * wave) / kKvBlock) : -1; };
     auto load_block = [&](int kb, int blk) {  // zeros for missing pages and past the last key
         if (blk >= 0 && kb + skey < w.k_end) {
             const int64_t off = (((int64_t)blk * a.n_layer + a.layer) * kKvBlock + (kb + skey) % kKvBlock) * a.sb + head;
@@ -908,15 +908,15 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         rv.store(&sm.b.v[buf][0][skey][se0], &sm.b.v[buf][NPC - 1][skey][se0]);
     };
     // ---- staging, F16: NI loads of RI rows each for K and for V
-    constexpr int RI = 512 / HD, NI = 8 / RI;
+    constexpr int RI = 512 / HD, NI = RW / RI;
     uint32_t k_off[NI], v_off[NI];
-    uint32_t partial = 0;  // (uniform) bit i: of the block issued i turns ago this wave has rows to clear
+    bool partial = false;  // of the block issued last this wave has rows to clear
     int page_next = 0;
     if constexpr (DMA) {
         const int c = lane % (HD / 8);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int r = 8 * wave + i * RI + lane / (HD / 8);
+            const int r = RW * wave + i * RI + lane / (HD / 8);
             const uint32_t at = (uint32_t)(r % kKvBlock) * (uint32_t)a.sb + (uint32_t)head;
             k_off[i] = at + 16 * (c ^ Block::k_swizzle(r));
             v_off[i] = at + 16 * (c ^ Block::v_swizzle(r));
@@ -926,25 +926,21 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         const int64_t page = ((int64_t)max(blk, 0) * a.n_layer + a.layer) * kKvBlock * a.sb;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            dma16(a.k_arena + page, k_off[i], &sm.b.k[buf][0][8 * wave + i * RI][0]);
-            dma16(a.v_arena + page, v_off[i], &sm.b.v[buf][0][8 * wave + i * RI][0]);
+            dma16(a.k_arena + page, k_off[i], &sm.b.k[buf][0][RW * wave + i * RI][0]);
+            dma16(a.v_arena + page, v_off[i], &sm.b.v[buf][0][RW * wave + i * RI][0]);
         }
-        partial = partial << 1 | (blk < 0 || kb + 8 * wave + 8 > w.k_end ? 1u : 0u);
+        partial = blk < 0 || kb + RW * (wave + 1) > w.k_end;
     };
     auto clear_rows = [&](int kb, int buf) {  // rows of a missing page, and past the last key
-        const int from = wave_page(kb) < 0 ? 0 : max(w.k_end - kb - 8 * wave, 0);
-        for (int i = from * (HD / 8) + lane; i < HD; i += 64) {  // 8 rows of HD / 8 pieces
-            *reinterpret_cast<uint4*>(&sm.b.k[buf][0][8 * wave][8 * i]) = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(&sm.b.v[buf][0][8 * wave][8 * i]) = make_uint4(0u, 0u, 0u, 0u);
+        const int from = wave_page(kb) < 0 ? 0 : max(w.k_end - kb - RW * wave, 0);
+        for (int i = from * (HD / 8) + lane; i < RW * HD / 8; i += 64) {  // RW rows of HD / 8 pieces
+            *reinterpret_cast<uint4*>(&sm.b.k[buf][0][RW * wave][8 * i]) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(&sm.b.v[buf][0][RW * wave][8 * i]) = make_uint4(0u, 0u, 0u, 0u);
         }
     };
-    // the wave's rows of block kb have landed, in buffer buf; `after` blocks were issued since (-1: there is no
-    // block kb, and nothing in flight)
-    auto landed = [&](int kb, int buf, int after) {
-        const bool wait_all = after != 2 || (partial >> 2 & 1);
-        if (wait_all) counted_wait<0>();
-        counted_wait<2 * 2 * NI>();
-        if (wait_all && after >= 0 && (partial >> after & 1)) clear_rows(kb, buf);
+    auto landed = [&](int kb, int buf) {  // the wave's rows of block kb, the last one issued
+        counted_wait<0>();
+        if (partial && kb < w.k_end) clear_rows(kb, buf);
     };
 
     f32x16 o[NT];
@@ -954,12 +950,99 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         for (int v = 0; v < 16; ++v) o[t][v] = 0.0f;
     float m = -INFINITY, l = 0.0f;  // l: this lane's keys only, until the end
 
-    int blk_next = -1, issued = 0;  // issued: blocks, of this wave
+    // ---- S^T = K Q^T of the 32 keys from row `sub` of a block, the small products in a sum of their own
+    auto scores = [&](int buf, int sub, f32x16& sc) {
+        f32x16 hi;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sc[v] = 0.0f, hi[v] = 0.0f;
+        const _Float16* kh = &sm.b.k[buf][0][sub + c32][0];
+        const _Float16* kl = &sm.b.k[buf][NPC - 1][sub + c32][0];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int at = 8 * ((2 * s + p) ^ Block::k_swizzle(c32));
+            const f16x8 fh = *reinterpret_cast<const f16x8*>(kh + at);
+            if constexpr (NPC == 2) {
+                const f16x8 fl = *reinterpret_cast<const f16x8*>(kl + at);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl, qh[s], sc, 0, 0, 0);
+            }
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fh, ql[s], sc, 0, 0, 0);
+            hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(fh, qh[s], hi, 0, 0, 0);
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sc[v] += hi[v];
+    };
+    // the lane's keys are 8 (i / 4) + 4 p + i % 4
+    auto mask = [&](f32x16& sc, int left) {
+        if (left < 32) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (8 * (i >> 2) + 4 * p + (i & 3) >= left) sc[i] = -INFINITY;
+        }
+    };
+    // a new reference where the scores ask for one; the factor of what is in units of the old one
+    auto raise = [&](const f32x16& sc) {
+        float mx = sc[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * qsc;
+        const float m_new = mx > m + 8.0f ? __builtin_ceilf(mx) : m;
+        const float alpha = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+        m = m_new;
+        return alpha;
+    };
+    auto rescale = [&](float alpha) {
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[t][v] *= alpha;
+    };
+    // the weights, their sum, and their pieces as operands: step s takes i = 8 s .. + 7, keys 16 s + 4 p + 0..3 and
+    // 16 s + 8 + 4 p + 0..3
+    auto weights = [&](f32x16& sc, f16x8(&ph)[2], f16x8(&pl)[2]) {
+        const float ref = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qsc, ref));
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) l += (sc[i] + sc[i + 1]) + (sc[i + 2] + sc[i + 3]);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            f16x4 h0, l0, h1, l1;
+            split4(sc[8 * s] * kPieces, sc[8 * s + 1] * kPieces, sc[8 * s + 2] * kPieces, sc[8 * s + 3] * kPieces, h0, l0);
+            split4(sc[8 * s + 4] * kPieces, sc[8 * s + 5] * kPieces, sc[8 * s + 6] * kPieces, sc[8 * s + 7] * kPieces, h1,
+                   l1);
+            ph[s] = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+            pl[s] = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    };
+    // O^T += V^T P^T
+    auto values = [&](int buf, int sub, const f16x8(&ph)[2], const f16x8(&pl)[2]) {
+        const int vrow = sub + 4 * p + ((lane & 15) >> 2);
+        // of tile t the 16-byte piece 4 t + vc of the row, its half lane % 2
+        const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vx = Block::v_swizzle(lane >> 2);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                f16x8 f[NPC];
+#pragma unroll
+                for (int u = 0; u < NPC; ++u) {
+                    const int at = 8 * ((4 * t + vc) ^ vx) + 4 * (lane & 1);
+                    const f16x4 a0 = lds_transposed(&sm.b.v[buf][u][16 * s + vrow][at]);
+                    const f16x4 a1 = lds_transposed(&sm.b.v[buf][u][16 * s + 8 + vrow][at]);
+                    f[u] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+                if constexpr (NPC == 2) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[1], ph[s], o[t], 0, 0, 0);
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], pl[s], o[t], 0, 0, 0);
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], ph[s], o[t], 0, 0, 0);
+            }
+    };
+
+    int blk_next = -1;
     if constexpr (DMA) {
-        for (; issued < 3 && w.k_begin + issued * BK < w.k_end; ++issued)
-            issue(w.k_begin + issued * BK, wave_page(w.k_begin + issued * BK), issued);
-        page_next = wave_page(w.k_begin + 3 * BK);
-        landed(w.k_begin, 0, issued - 1);
+        issue(w.k_begin, wave_page(w.k_begin), 0);
+        page_next = wave_page(w.k_begin + BK);
+        landed(w.k_begin, 0);
     } else {
         load_block(w.k_begin, wave_page(w.k_begin));
         blk_next = wave_page(w.k_begin + BK);
@@ -967,104 +1050,52 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
     }
     __syncthreads();
     int buf = 0;
-    for (int kb = w.k_begin; kb < w.k_end; kb += BK, buf = (buf + 1) % NBUF) {
+    for (int kb = w.k_begin; kb < w.k_end; kb += BK, buf ^= 1) {
         const bool more = kb + BK < w.k_end;
         if constexpr (DMA) {
-            if (kb + 3 * BK < w.k_end) {
-                issue(kb + 3 * BK, page_next, (buf + 3) % NBUF);
-                page_next = wave_page(kb + 4 * BK);
+            if (more) {
+                issue(kb + BK, page_next, buf ^ 1);
+                page_next = wave_page(kb + 2 * BK);
             }
         } else if (more) {
             load_block(kb + BK, blk_next);
             blk_next = wave_page(kb + 2 * BK);
         }
         if (r0 < w.n_rows) {
-#pragma unroll 1
-            for (int sub = 0; sub < BK && kb + sub < w.k_end; sub += 32) {
-                // ---- S^T = K Q^T, the small products apart
-                f32x16 sc, hi;
+            if constexpr (BK == 64) {
+                // two halves, the weights of one made beside the products of the other
+                f32x16 s0, s1;
+                f16x8 h0[2], l0[2], h1[2], l1[2];
+                scores(buf, 0, s0);
+                mask(s0, w.k_end - kb);
+                const float a0 = raise(s0);
+                if (__any(a0 != 1.0f)) rescale(a0);
+                scores(buf, 32, s1);
+                weights(s0, h0, l0);
+                mask(s1, w.k_end - kb - 32);
+                const float a1 = raise(s1);
+                if (__any(a1 != 1.0f)) {
+                    rescale(a1);
+                    const _Float16 f = (_Float16)a1;  // a power of two
 #pragma unroll
-                for (int v = 0; v < 16; ++v) sc[v] = 0.0f, hi[v] = 0.0f;
-                const _Float16* kh = &sm.b.k[buf][0][sub + c32][0];
-                const _Float16* kl = &sm.b.k[buf][NPC - 1][sub + c32][0];
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const int at = 8 * ((2 * s + p) ^ Block::k_swizzle(c32));
-                    const f16x8 fh = *reinterpret_cast<const f16x8*>(kh + at);
-                    if constexpr (NPC == 2) {
-                        const f16x8 fl = *reinterpret_cast<const f16x8*>(kl + at);
-                        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl, qh[s], sc, 0, 0, 0);
-                    }
-                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fh, ql[s], sc, 0, 0, 0);
-                    hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(fh, qh[s], hi, 0, 0, 0);
+                    for (int s = 0; s < 2; ++s) h0[s] *= f, l0[s] *= f;
                 }
-#pragma unroll
-                for (int v = 0; v < 16; ++v) sc[v] += hi[v];
-
-                // ---- the online softmax of the lane's row over its 16 keys, 8 (i / 4) + 4 p + i % 4
-                const int left = w.k_end - kb - sub;
-                if (left < 32) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (8 * (i >> 2) + 4 * p + (i & 3) >= left) sc[i] = -INFINITY;
-                }
-                float mx = sc[0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * qsc;
-                if (__any(mx > m + 8.0f)) {
-                    const float m_new = mx > m + 8.0f ? __builtin_ceilf(mx) : m;
-                    const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-                    l *= alpha;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) o[t][v] *= alpha;
-                    m = m_new;
-                }
-                const float ref = m == -INFINITY ? 0.0f : -m;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qsc, ref));
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) l += (sc[i] + sc[i + 1]) + (sc[i + 2] + sc[i + 3]);
-
-                // ---- O^T += V^T P^T: step s takes the lane's weights i = 8s .. 8s + 7, keys 16s + 4p + 0..3
-                // and 16s + 8 + 4p + 0..3
-                const int vrow = sub + 4 * p + ((lane & 15) >> 2);
-                // of tile t the 16-byte piece 4 t + vc of the row, its half lane % 2
-                const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vx = Block::v_swizzle(lane >> 2);
-                f16x8 ph[2], pl[2];
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    f16x4 h0, l0, h1, l1;
-                    split4(sc[8 * s] * kPieces, sc[8 * s + 1] * kPieces, sc[8 * s + 2] * kPieces, sc[8 * s + 3] * kPieces,
-                           h0, l0);
-                    split4(sc[8 * s + 4] * kPieces, sc[8 * s + 5] * kPieces, sc[8 * s + 6] * kPieces,
-                           sc[8 * s + 7] * kPieces, h1, l1);
-                    ph[s] = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    pl[s] = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
-                }
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        f16x8 f[NPC];
-#pragma unroll
-                        for (int u = 0; u < NPC; ++u) {
-                            const int at = 8 * ((4 * t + vc) ^ vx) + 4 * (lane & 1);
-                            const f16x4 a0 = lds_transposed(&sm.b.v[buf][u][16 * s + vrow][at]);
-                            const f16x4 a1 = lds_transposed(&sm.b.v[buf][u][16 * s + 8 + vrow][at]);
-                            f[u] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-                        }
-                        if constexpr (NPC == 2)
-                            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[1], ph[s], o[t], 0, 0, 0);
-                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], pl[s], o[t], 0, 0, 0);
-                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], ph[s], o[t], 0, 0, 0);
-                    }
+                values(buf, 0, h0, l0);
+                weights(s1, h1, l1);
+                values(buf, 32, h1, l1);
+            } else {
+                f32x16 s0;
+                f16x8 h0[2], l0[2];
+                scores(buf, 0, s0);
+                mask(s0, w.k_end - kb);
+                const float a0 = raise(s0);
+                if (__any(a0 != 1.0f)) rescale(a0);
+                weights(s0, h0, l0);
+                values(buf, 0, h0, l0);
             }
         }
         if constexpr (DMA)
-            landed(kb + BK, (buf + 1) % NBUF, min((w.k_end - kb - 1) / BK, 3) - 1);
+            landed(kb + BK, buf ^ 1);
         else if (more)
             store_block(buf ^ 1);
         __syncthreads();
@@ -1169,10 +1200,10 @@ static TreePlan tree_plan(int ct, int hd, int n_head, int n_head_kv, int n_seqs,
     p.block_waves = rows > 128 && hd <= 128 ? 8 : 4;
     p.tiles = (rows + kRowsPerWave * p.block_waves - 1) / (kRowsPerWave * p.block_waves);
     const int64_t base = (int64_t)p.tiles * n_head_kv, wgs = p.block_waves == 8 ? cu_count() : 2 * cu_count();
-    const int share = (int)std::max<int64_t>((wgs + base - 1) / base, n_seqs), bk = 8 * p.block_waves;
+    const int share = (int)std::max<int64_t>((wgs + base - 1) / base, n_seqs), bk = 64;
     // keys of a split were all sequences as long as the longest; up to 64 sequences share out by their lengths,
     // of no fewer than half as many keys (which bounds the partial results)
-    const int64_t kps = std::max<int64_t>(256, round_up(((int64_t)max_past * n_seqs + share - 1) / share, bk));
+    const int64_t kps = std::max<int64_t>(256, round_up(((int64_t)max_past * n_seqs + share - 1) / share, 64));
     p.share = n_seqs > 1 && n_seqs <= 64 ? share : 0;
     p.kps = (int)(p.share ? std::max<int64_t>(256, round_up(kps / 2, bk)) : kps);
     p.splits = 1 + (max_past + p.kps - 1) / p.kps;
