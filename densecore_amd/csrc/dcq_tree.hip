@@ -43,10 +43,23 @@ constexpr int kTreeWaves = 4;      // waves of a workgroup, a share of the keys 
 constexpr int kRowsPerWave = 32;   // of the block kernel
 constexpr float kPieces = 128.0f;  // of the weights in O: 2^15 at most before the reference is raised
 
-// An empty use: the operand of a matrix instruction stays in its registers until here, so that no result is put
-// over it.
+// No sum of the 16 x 16 matrix instructions is to be put over an operand, or half over the sum before it. TIED: an
+// empty statement uses operands and sum once more when the new sum is there. That is free at head_dim 256; at 128 it
+// has sums moved between register files (fp32, 256 rows: 118 -> 160 us), and operands kept to the end of a chain of
+// instructions do.
+template <bool TIED>
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+    f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    if constexpr (TIED) asm volatile("" : "+v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+template <bool TIED>
+__device__ __forceinline__ f32x4 mfma16(float a, float b, f32x4 c) {
+    f32x4 d = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+    if constexpr (TIED) asm volatile("" : "+v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
 __device__ __forceinline__ void keep(f32x4 x) { asm volatile("" ::"v"(x)); }
-__device__ __forceinline__ void keep(f16x8 x) { asm volatile("" ::"v"(x)); }
 
 template <int CT>
 constexpr int tree_chunk() { return CT == kTypeF32 ? 16 : 32; }  // keys of a wave's step
@@ -116,8 +129,8 @@ struct TreeKeys<kTypeF16, HD> {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const f16x8 f = as_f16x8(k[j][s]);
-                lo[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ql, lo[j], 0, 0, 0);
-                hi[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qh, hi[j], 0, 0, 0);
+                lo[j] = mfma16<HD == 256>(f, ql, lo[j]);
+                hi[j] = mfma16<HD == 256>(f, qh, hi[j]);
             }
         }
 #pragma unroll
@@ -136,8 +149,8 @@ struct TreeKeys<kTypeF16, HD> {
                                                  e % 2 ? 0x07060302u : 0x05040100u);
                 }
                 const f16x8 f = as_f16x8(w[0], w[1], w[2], w[3]);
-                o[u][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, pl, o[u][e], 0, 0, 0);
-                o[u][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ph, o[u][e], 0, 0, 0);
+                o[u][e] = mfma16<HD == 256>(f, pl, o[u][e]);
+                o[u][e] = mfma16<HD == 256>(f, ph, o[u][e]);
             }
     }
 };
@@ -191,9 +204,9 @@ struct TreeKeys<kTypeQ8_0, HD> {
                     p[t] = q8_pieces(int8_pair(__builtin_amdgcn_perm(0u, w[t / 2], t % 2 ? 0x0c030c02u : 0x0c010c00u)), d);
                 const f16x8 fh = as_f16x8(as_u32(p[0].h), as_u32(p[1].h), as_u32(p[2].h), as_u32(p[3].h));
                 const f16x8 fl = as_f16x8(as_u32(p[0].l), as_u32(p[1].l), as_u32(p[2].l), as_u32(p[3].l));
-                lo[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl, qh, lo[j], 0, 0, 0);
-                lo[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, ql, lo[j], 0, 0, 0);
-                hi[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, qh, hi[j], 0, 0, 0);
+                lo[j] = mfma16<HD == 256>(fl, qh, lo[j]);
+                lo[j] = mfma16<HD == 256>(fh, ql, lo[j]);
+                hi[j] = mfma16<HD == 256>(fh, qh, hi[j]);
             }
         }
 #pragma unroll
@@ -216,9 +229,9 @@ struct TreeKeys<kTypeQ8_0, HD> {
                                                                      0x0c040c00u + 0x00010001u * e)), d[t]);
                 const f16x8 fh = as_f16x8(as_u32(p[0].h), as_u32(p[1].h), as_u32(p[2].h), as_u32(p[3].h));
                 const f16x8 fl = as_f16x8(as_u32(p[0].l), as_u32(p[1].l), as_u32(p[2].l), as_u32(p[3].l));
-                o[u][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl, ph, o[u][e], 0, 0, 0);
-                o[u][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, pl, o[u][e], 0, 0, 0);
-                o[u][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fh, ph, o[u][e], 0, 0, 0);
+                o[u][e] = mfma16<HD == 256>(fl, ph, o[u][e]);
+                o[u][e] = mfma16<HD == 256>(fh, pl, o[u][e]);
+                o[u][e] = mfma16<HD == 256>(fh, ph, o[u][e]);
             }
         }
     }
@@ -230,6 +243,7 @@ struct TreeKeys<kTypeF32, HD> {
     static constexpr int U = HD / 64, S = HD / 16;
     f32x4 k[S];
     f32x4 v[4][U];
+    f32x4 last_k, last_q;  // of the scores' last instructions
     __device__ __forceinline__ void load_k(int, const uint8_t* page, uint32_t off, int g) {
 #pragma unroll
         for (int s = 0; s < S; ++s) k[s] = *reinterpret_cast<const f32x4*>(page + (off + 16 * g + 64 * s));
@@ -250,21 +264,27 @@ struct TreeKeys<kTypeF32, HD> {
 #pragma unroll
         for (int u = 0; u < U; ++u) v[i][u] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    __device__ __forceinline__ void scores(const uint4* qs, f32x4 (&r)[1]) const {
+    __device__ __forceinline__ void scores(const uint4* qs, f32x4 (&r)[1]) {
         f32x4 a[4];  // four sums: a quarter of the roundings in a row
 #pragma unroll
         for (int e = 0; e < 4; ++e) a[e] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const f32x4 q = __builtin_bit_cast(f32x4, qs[64 * s]);
+            const f32x4 q = last_q = __builtin_bit_cast(f32x4, qs[64 * s]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][e], q[e], a[e], 0, 0, 0);
-            keep(q);
+            for (int e = 0; e < 4; ++e) a[e] = mfma16<HD == 256>(k[s][e], q[e], a[e]);
+            if (HD < 256) keep(q);
             if (HD == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // no more of q at once
         }
 #pragma unroll
-        for (int s = 0; s < S; ++s) keep(k[s]);
+        for (int s = 0; s < S; ++s)
+            if (HD < 256) keep(k[s]);
         r[0] = (a[0] + a[1]) + (a[2] + a[3]);
+        last_k = k[S - 1];
+    }
+    // keeps the last instructions' operands until the scores are there; after the loads that are issued meanwhile
+    __device__ __forceinline__ void scored(f32x4 (&r)[1]) const {
+        if constexpr (HD < 256) asm volatile("" : "+v"(r[0]) : "v"(last_k), "v"(last_q));
     }
     __device__ __forceinline__ void weigh(const float (&p)[4], f32x4 (&o)[U][4]) const {
         const f32x4 w = (f32x4){p[0], p[1], p[2], p[3]} * kPieces;
@@ -274,12 +294,13 @@ struct TreeKeys<kTypeF32, HD> {
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    o[u][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][u][e], w[i], o[u][e], 0, 0, 0);
+                    o[u][e] = mfma16<HD == 256>(v[i][u][e], w[i], o[u][e]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int u = 0; u < U; ++u) keep(v[i][u]);
-        keep(w);
+            for (int u = 0; u < U; ++u)
+                if (HD < 256) keep(v[i][u]);
+        if (HD < 256) keep(w);
     }
 };
 
@@ -549,6 +570,7 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
     auto add_drafts = [&](TreeKeys<kTypeF32, HD>& t, int k0) {
         f32x4 r[1];
         t.scores(operands(sm.qf), r);
+        t.scored(r);
         float s[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -586,6 +608,7 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
 #pragma unroll
                 for (int j = 0; j < NP; ++j) t.load_k(j, a.k_arena + page_bytes(next[j]), off_k, g);
             }
+            if constexpr (CT == kTypeF32) t.scored(r);
             float s[4 * NP];
 #pragma unroll
             for (int j = 0; j < NP; ++j)
@@ -827,7 +850,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         w.k_begin = w.k_end = 0;
         w.drafts = true;
         w.slot = 0;
-        if (w.row0 < w.n_rows) tree_tile<kTypeF32, HD, W, false, HD < 256>(a, w, sm.t);
+        if (w.row0 < w.n_rows) tree_tile<kTypeF32, HD, W, false, false>(a, w, sm.t);
         return;
     }
     id = blockIdx.x;
