@@ -9,7 +9,7 @@
 // Query rows of a KV head are the (token, head of its group) pairs, token-major, in tiles of 16: a column of
 // the matrix instructions, whatever the group size. S^T = K Q^T puts the keys 4 (lane / 16) + i of row
 // lane % 16 into lane registers i, and O^T += V^T P^T takes its weights from the same lanes, so P never
-// moves; K, V and Q go from memory to the matrix registers without LDS:
+// moves; K and V go from memory to the matrix registers without LDS (Q's operands wait there):
 //   K: a lane holds 8 consecutive dims of key lane % 16 (fp32: 4), the A operand as it is.
 //   V: a lane holds dims 64 u + 4 (lane % 16) + 0..3 of the keys whose weights it has; output tile (u, e) is
 //      made of the dims 64 u + 4 m + e, so that its A operand is in the lane, one byte permute per two keys.
@@ -738,8 +738,10 @@ __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_
 }
 
 // ---------------------------------------------------------------- many rows
-// Blocks of 8 W keys in LDS, as f16 pieces. Q8_0: two buffers of two pieces, decoded on the way. F16: a ring of
-// four, filled by direct loads two blocks ahead of the one in use, in rows without padding.
+// Blocks of keys in LDS, two buffers of them, as f16 pieces. Q8_0: 8 W keys, decoded on the way into two pieces.
+// F16: 64 keys, by direct loads, in rows without padding; two halves of 32 give a wave products to issue while the
+// other half's weights are made (8 sequences of 1500..4096 keys, 96 rows x 128: 51 -> 49 us a call, against a ring of
+// four blocks of 32).
 template <int CT, int HD, int W>
 struct __align__(16) TreeBlock {
     static constexpr bool DMA = CT == kTypeF16;
@@ -756,11 +758,13 @@ struct __align__(16) TreeBlock {
 
 // 16 bytes per lane from global memory (uniform base + per-lane byte offset) into LDS at lds_base + 16 lane.
 // Inline asm: the compiler's builtin form makes LDS reads of any buffer wait for it. Not counted by the compiler;
-// counted_wait below comes before the barrier that publishes the block.
+// counted_wait below comes before the barrier that publishes the block. M0 is read one instruction after its write
+// at the earliest.
 __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, const void* lds_base) {
     typedef __attribute__((address_space(3))) const void* LdsPtr;
     const uint32_t m0 = (uint32_t)(uintptr_t)(LdsPtr)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0)
+                 : "memory", "m0");
 }
 // All loads but the N issued last have landed.
 template <int N>
@@ -800,7 +804,7 @@ struct TreeShare {
 // Up to 64 sequences share the units by their lengths, which the host does not know: the fewest keys per unit
 // (a.kps or more, in steps of an eighth) that a.share units suffice for. 8 sequences of 1500..4096 keys on 64
 // units: 384 keys, where their longest alone would ask for 512 and leave a quarter of the units without work;
-// 24 tokens of 32/8 heads x 128, F16: 40 -> 32 us. More sequences even out by themselves.
+// 24 tokens of 32/8 heads x 128, F16: 40.7 -> 38.5 us. More sequences even out by themselves.
 __device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, int unit) {
     const int per_seq = a.splits - 1;
     if (!a.share) return {unit / per_seq, unit % per_seq, a.kps};
@@ -1216,17 +1220,45 @@ static TreePlan tree_plan16(int n_head, int n_head_kv, int n_seqs, int n_tokens,
     return p;
 }
 
+// The block kernel's rows share the keys that the 16-row kernel reads once per tile, but its workgroups need more of
+// both to be worth their start. From which number of rows on it is the faster (16-row kernel | block kernel, us;
+// 16/4 heads at head_dim 256, else 32/8):
+//   8 sequences of 1500..4096 keys, head_dim 128: 20 rows F16 40 | 27, Q8_0 55 | 33
+//   the same, head_dim 256: F16 20 rows 36 | 75, 64 rows 88 | 90, 80 rows 105 | 104, 128 rows 152 | 119;
+//                           Q8_0 32 rows 47 | 81, 48 rows 98 | 91, 128 rows 391 | 179
+//   one sequence of 4096 keys, where the block kernel's 256 keys per workgroup leave CUs without one: head_dim 128
+//   32 rows F16 14.4 | 14.8, Q8_0 20 rows 17.4 | 20.2, F16 64 rows 21.4 | 15.9; head_dim 256 F16 128 rows 43 | 48,
+//   Q8_0 64 rows 35 | 46
+//   fewer than 256 keys: never (8 sequences of 100..255 keys: 64 rows 19 | 22, 256 rows 37 | 43)
+static bool tree_in_blocks(int ct, int hd, int n_head_kv, int n_seqs, int rows, int max_past) {
+    if (ct == kTypeF32 || max_past < 256) return false;
+    const int from = hd < 256 ? 16 : ct == kTypeF16 ? 64 : 32;
+    const bool idle = (int64_t)n_head_kv * n_seqs * ((max_past + 255) / 256) < cu_count();
+    return rows > (idle ? 2 * from : from);
+}
+
 static TreePlan tree_plan(int ct, int hd, int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
-    const int rows = n_tokens * (n_head / n_head_kv);
-    if (ct == kTypeF32 || rows <= 16 || max_past < 256) return tree_plan16(n_head, n_head_kv, n_seqs, n_tokens, max_past);
+    const int rows = n_tokens * (n_head / n_head_kv), bk = 64;
+    if (!tree_in_blocks(ct, hd, n_head_kv, n_seqs, rows, max_past))
+        return tree_plan16(n_head, n_head_kv, n_seqs, n_tokens, max_past);
     TreePlan p{};
-    p.block_waves = rows > 128 && hd <= 128 ? 8 : 4;
-    p.tiles = (rows + kRowsPerWave * p.block_waves - 1) / (kRowsPerWave * p.block_waves);
-    const int64_t base = (int64_t)p.tiles * n_head_kv, wgs = p.block_waves == 8 ? cu_count() : 2 * cu_count();
-    const int share = (int)std::max<int64_t>((wgs + base - 1) / base, n_seqs), bk = 64;
-    // keys of a split were all sequences as long as the longest; up to 64 sequences share out by their lengths,
+    int share;
+    int64_t kps;
+    auto plan_of = [&](int waves) {  // as many workgroups as there is room for at once
+        p.block_waves = waves;
+        p.tiles = (rows + kRowsPerWave * waves - 1) / (kRowsPerWave * waves);
+        const int64_t base = (int64_t)p.tiles * n_head_kv, wgs = waves == 8 ? cu_count() : 2 * cu_count();
+        share = (int)std::max<int64_t>((wgs + base - 1) / base, n_seqs);
+        kps = std::max<int64_t>(256, round_up(((int64_t)max_past * n_seqs + share - 1) / share, bk));
+    };
+    // Eight waves decode a Q8_0 block for twice the rows, four start and end sooner: eight for long shares of long
+    // histories. 256 rows x 128, four | eight: one sequence of 4096 keys 28 | 34, of 16384 (512 keys a share) 66 | 67,
+    // of 32768 116 | 112, of 65536 213 | 200, 64 dims 133 | 116; four of 16384 219 | 212, 16 of 4096 255 | 268.
+    // F16, which is not decoded: 16 of 500..2048 89 | 114, one of 4096 22 | 28, of 65536 143 | 142.
+    if (ct == kTypeQ8_0 && rows > 128 && hd <= 128 && max_past >= 8192) plan_of(8);
+    if (p.block_waves == 0 || kps < 1024) plan_of(4);
+    // kps: keys of a split were all sequences as long as the longest; up to 64 sequences share out by their lengths,
     // of no fewer than half as many keys (which bounds the partial results)
-    const int64_t kps = std::max<int64_t>(256, round_up(((int64_t)max_past * n_seqs + share - 1) / share, 64));
     p.share = n_seqs > 1 && n_seqs <= 64 ? share : 0;
     p.kps = (int)(p.share ? std::max<int64_t>(256, round_up(kps / 2, bk)) : kps);
     p.splits = 1 + (max_past + p.kps - 1) / p.kps;
@@ -1238,11 +1270,13 @@ static size_t tree_partial_bytes(const TreePlan& p, int hd, int64_t rows) {
     return p.splits <= 1 ? 0 : (size_t)(round_up(p.splits * rows * hd * 4, 256) + round_up(p.splits * rows * 2 * 4, 256) + 256);
 }
 
-// Of the larger plan: the query does not know the cache type.
+// Of the largest plan: the query does not know the cache type.
 size_t tree_workspace_bytes(int hd, int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
     const int64_t rows = (int64_t)n_seqs * n_tokens * n_head;
-    return std::max(tree_partial_bytes(tree_plan(kTypeF32, hd, n_head, n_head_kv, n_seqs, n_tokens, max_past), hd, rows),
-                    tree_partial_bytes(tree_plan(kTypeF16, hd, n_head, n_head_kv, n_seqs, n_tokens, max_past), hd, rows));
+    size_t most = 0;
+    for (int ct : {kTypeF32, kTypeF16, kTypeQ8_0})
+        most = std::max(most, tree_partial_bytes(tree_plan(ct, hd, n_head, n_head_kv, n_seqs, n_tokens, max_past), hd, rows));
+    return most;
 }
 
 template <int HD, int P>
@@ -1264,13 +1298,13 @@ static void launch_tree_merge(const TreeArgs& a, hipStream_t st) {
 
 template <int CT, int HD>
 static void launch_tree_t(const TreeArgs& a, int block_waves, int wgs, hipStream_t st) {
-    if constexpr (CT != kTypeF32) {
-        if constexpr (HD <= 128) {
-            if (block_waves == 8) {
-                hipLaunchKernelGGL((tree_block_kernel<CT, HD, 8>), dim3(wgs), dim3(512), 0, st, a);
-                return;
-            }
+    if constexpr (CT == kTypeQ8_0 && HD <= 128) {
+        if (block_waves == 8) {
+            hipLaunchKernelGGL((tree_block_kernel<CT, HD, 8>), dim3(wgs), dim3(512), 0, st, a);
+            return;
         }
+    }
+    if constexpr (CT != kTypeF32) {
         if (block_waves == 4) {
             hipLaunchKernelGGL((tree_block_kernel<CT, HD, 4>), dim3(wgs), dim3(256), 0, st, a);
             return;

@@ -146,6 +146,24 @@ def test_tree_attention(KV, dev, ct, n, pasts, heads, kv, hd):
     t.check(t.run(dev))
 
 
+@pytest.mark.parametrize("ct", [F16, Q8_0])
+@pytest.mark.parametrize("n,pasts,heads,kv,hd", [
+    (40, [9001], 192, 6, 64),          # 1280 rows of a KV head, five tiles of eight waves
+    (17, [8200, 1, 515], 240, 15, 128),  # 272 rows: a second tile of 16, shares of three lengths
+])
+def test_tree_attention_long_shares(KV, dev, ct, n, pasts, heads, kv, hd):
+    """More than 128 rows over shares of 1024 keys and more."""
+    t = Tree(KV, ct, n, pasts, heads, kv, hd, seed=n + hd, holes=[(0, 70)], n_layer=1)
+    t.check(t.run(dev))
+
+
+@pytest.mark.parametrize("ct", CACHE_TYPES)
+@pytest.mark.parametrize("n,pasts,heads,kv,hd", [(11, [2001] * 9, 16, 4, 256), (12, [4000, 1200, 2800, 17], 32, 8, 256)])
+def test_tree_attention_wide_heads_in_blocks(KV, dev, ct, n, pasts, heads, kv, hd):
+    t = Tree(KV, ct, n, pasts, heads, kv, hd, seed=n, n_layer=1)
+    t.check(t.run(dev))
+
+
 @pytest.mark.parametrize("ct", CACHE_TYPES)
 @pytest.mark.parametrize("heads,kv,hd,n", [(8, 2, 128, 20), (4, 1, 64, 9), (16, 2, 256, 12)])
 def test_tree_attention_ragged_drafts_and_rows_that_see_nothing(KV, dev, ct, heads, kv, hd, n):
