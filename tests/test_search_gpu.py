@@ -148,12 +148,12 @@ def test_tree_attention(KV, dev, ct, n, pasts, heads, kv, hd):
 
 @pytest.mark.parametrize("ct", [F16, Q8_0])
 @pytest.mark.parametrize("n,pasts,heads,kv,hd", [
-    (40, [9001], 192, 6, 64),          # 1280 rows of a KV head, five tiles of eight waves
-    (17, [8200, 1, 515], 240, 15, 128),  # 272 rows: a second tile of 16, shares of three lengths
+    (17, [8200, 1, 515] + [0] * 29, 16, 1, 128),  # 272 rows: a second tile of 16, shares by the lengths
+    (36, [0, 3, 9001] + [20] * 63, 4, 1, 64),     # 144 rows, more sequences than share
 ])
 def test_tree_attention_long_shares(KV, dev, ct, n, pasts, heads, kv, hd):
     """More than 128 rows over shares of 1024 keys and more."""
-    t = Tree(KV, ct, n, pasts, heads, kv, hd, seed=n + hd, holes=[(0, 70)], n_layer=1)
+    t = Tree(KV, ct, n, pasts, heads, kv, hd, seed=n + hd, n_layer=1)
     t.check(t.run(dev))
 
 
