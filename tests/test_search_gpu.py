@@ -480,6 +480,12 @@ def test_compact(dev, ct, kv, hd, n_layer, n_blocks, live):
     assert_pages(cache, start, pairs)
 
 
+@pytest.mark.parametrize("n_blocks,live", [(2049, 1000), (2050, 1025), (16000, 8000), (40000, 21000), (33000, 40)])
+def test_compact_of_many_pages(dev, n_blocks, live):
+    """Beyond the copies that are made beside the plan."""
+    test_compact(dev, Q8_0, 1, 32, 1, n_blocks, live)
+
+
 def test_pages_in_graphs_and_on_streams(dev):
     """A fork and a compaction captured, replayed on changed inputs, on a stream of their own."""
     import torch
