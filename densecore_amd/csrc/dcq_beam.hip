@@ -7,7 +7,7 @@
 //                      2^ref sum 2^(x log2 e - ref), and its n_out largest logits (their order is the scores')
 //   beam_join_kernel   per request: lse of each row in 64 bits, and the n_out best of the chunks' candidates
 //                      by their 64-bit scores
-// A chunk's largest are found without sorting it: just below the n_out-th largest of the maxima of 64 groups of
+// A chunk's largest are found without sorting it: just below the n_out-th largest of the maxima of 64 or 256 groups of
 // threads lies a bound that n_out elements reach at least and few others do; those are ranked against each other.
 #include <algorithm>
 
@@ -36,25 +36,38 @@ __device__ __forceinline__ uint64_t beam_key(float x, uint32_t idx) {
 __device__ __forceinline__ float key_logit(uint64_t key) { return order_value((uint32_t)(key >> 32)); }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
 
-// A bound that n (<= 64) of the values in a wave's 64 lanes reach: the n-th largest to 20 bits (its sign,
+// A bound that n (<= 64) of the values in a wave's 64 lanes, G in each, reach: the n-th largest to 20 bits (its sign,
 // exponent and 11 bits, the rest as low as can be), found bit by bit with one comparison each. No more exact: a
 // bound a thousandth lower lets a few candidates more through.
-__device__ __forceinline__ float lanes_bound(float v, int n) {
-    const uint32_t o = order_bits(v);
-    uint32_t t = 0;
+template <int G>
+__device__ __forceinline__ float lanes_bound(const float (&v)[G], int n) {
+    uint32_t o[G], t = 0;
+#pragma unroll
+    for (int g = 0; g < G; ++g) o[g] = order_bits(v[g]);
 #pragma unroll
     for (int b = 31; b >= 12; --b) {
         const uint32_t with = t | 1u << b;
-        if ((int)__popcll(__ballot(o >= with)) >= n) t = with;
+        int reach = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) reach += (int)__popcll(__ballot(o[g] >= with));
+        if (reach >= n) t = with;
     }
     return t < 0x00800000u ? -INFINITY : order_value(t);  // below the finite ones
+}
+// The bound on the maxima of the workgroup's groups of threads: 64 of them up to 32 outputs, 256 beyond, where 64
+// groups' maxima would all have to be reached (4 beams over 151936 tokens, 64 outputs: hundreds of elements of a
+// chunk and more candidates than are ranked, 472 us).
+constexpr int kFewGroups = 32;
+__device__ __forceinline__ float groups_bound(const float* gmax, int lane, int n) {
+    if (n <= kFewGroups) return lanes_bound<1>({gmax[lane]}, n);
+    return lanes_bound<4>({gmax[lane], gmax[lane + 64], gmax[lane + 128], gmax[lane + 192]}, n);
 }
 
 template <class T, int EPT>
 __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
     constexpr int V = 16 / sizeof(T), NV = EPT / V;
     __shared__ uint64_t keys[kBeamCap];
-    __shared__ float wmax[4], gmax[64];
+    __shared__ float wmax[4], gmax[256];
     __shared__ double wsum[4];
     __shared__ int count;
     __shared__ unsigned long long best;
@@ -86,8 +99,12 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int k = 0; k < V; ++k) tmax = fmaxf(tmax, e[j][k]);
-    const float qmax = lanes_max<4>(tmax);
-    if (lane % 4 == 0) gmax[tid / 4] = qmax;
+    if (a.n_out <= kFewGroups) {
+        const float qmax = lanes_max<4>(tmax);
+        if (lane % 4 == 0) gmax[tid / 4] = qmax;
+    } else {
+        gmax[tid] = tmax;
+    }
     const float wm = lanes_max<64>(tmax);
     if (lane == 0) wmax[wave] = wm;
     if (tid == 0) count = 0;
@@ -118,7 +135,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
     if (lane == 0) wsum[wave] = sum;
 
     // ---- elements no smaller than the bound on the groups' maxima
-    const float bound = lanes_bound(gmax[lane], a.n_out);
+    const float bound = groups_bound(gmax, lane, a.n_out);
     const int64_t list = row * a.chunks + chunk;
     auto index_of = [&](int j, int k) { return beam | (uint32_t)((v0 + j * kBeamThreads) * V + k); };
     if (tmax >= bound && tmax > -INFINITY) {
@@ -179,20 +196,29 @@ struct BeamPick {
 };
 
 constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / 64;
+constexpr int kBeamBatch = 8;  // candidates of a thread that wait in registers
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
-    constexpr int NK = 4;  // candidates of a thread that wait in registers
+    constexpr int NK = kBeamBatch;
     __shared__ BeamPick picks[kBeamCap];
     __shared__ double lse[kBeamMaxBeams], base[kBeamMaxBeams];
-    __shared__ float gmax[64];
+    __shared__ float gmax[256];
     __shared__ BeamPick wbest[kJoinWaves];
     __shared__ int count;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t req = blockIdx.x, row0 = req * a.n_beams;
-    const int per_beam = a.chunks * a.n_out, total = a.n_beams * per_beam;
-    const uint64_t* cand = a.cand + row0 * per_beam;
+    const int lists = a.n_beams * a.chunks, total = lists * a.n_out;
+    const uint64_t* cand = a.cand + row0 * a.chunks * a.n_out;
+    // As they lie if all fit in registers and a list is no longer than a group of 16 threads; else the lists' first
+    // ones, then the second ones, ...: the best are spread over the groups, and held (8 beams over 151936 tokens, 16
+    // outputs, join 7.0 | 11.2 us; 4 beams, 64 outputs 45 | 21, 16 beams 416 | 18).
+    constexpr int held = NK * kJoinThreads;
+    const bool in_lists = total <= held && a.n_out <= 16;
+    auto candidate = [&](int i) {
+        return i >= total ? 0 : in_lists ? cand[i] : cand[(int64_t)(i % lists) * a.n_out + i / lists];
+    };
     uint64_t mine[NK];
 #pragma unroll
-    for (int k = 0; k < NK; ++k) mine[k] = tid + k * kJoinThreads < total ? cand[tid + k * kJoinThreads] : 0;
+    for (int k = 0; k < NK; ++k) mine[k] = candidate(tid + k * kJoinThreads);
     // ---- lse of each row; base is NaN for a beam without continuations
     for (int w = wave; w < a.n_beams; w += kJoinWaves) {
         const int64_t list = (row0 + w) * a.chunks;
@@ -221,26 +247,37 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
         const uint32_t at = key_index(key), w = at >> 24;
         return BeamPick{base[w] + ((double)key_logit(key) - lse[w]), at};
     };
-    // every candidate, those in registers first
-    auto each = [&](auto f) {
-#pragma unroll
-        for (int k = 0; k < NK; ++k)
-            if (mine[k]) f(pick_of(mine[k]));
-        for (int i = tid + NK * kJoinThreads; i < total; i += kJoinThreads)
-            if (const uint64_t key = cand[i]) f(pick_of(key));
-    };
-    // ---- a bound as in the chunks, on the largest score of 64 groups of threads (rounded down to fp32: no higher)
+    // ---- a bound as in the chunks, on the groups' largest scores among those in registers (rounded down to fp32: no
+    // higher)
     float tmax = -INFINITY;
-    each([&](const BeamPick& p) { tmax = fmaxf(tmax, __double2float_rd(p.score)); });
-    const float gm = lanes_max<16>(tmax);
-    if (lane % 16 == 0) gmax[tid / 16] = gm;
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+        if (mine[k]) tmax = fmaxf(tmax, __double2float_rd(pick_of(mine[k]).score));
+    if (a.n_out <= kFewGroups) {
+        const float gm = lanes_max<16>(tmax);
+        if (lane % 16 == 0) gmax[tid / 16] = gm;
+    } else {
+        const float gm = lanes_max<4>(tmax);
+        if (lane % 4 == 0) gmax[tid / 4] = gm;
+    }
     __syncthreads();
-    const double bound = lanes_bound(gmax[lane], a.n_out);
-    each([&](const BeamPick& p) {
-        if (!(p.score >= bound)) return;  // NaN: of a beam without continuations
+    const double bound = groups_bound(gmax, lane, a.n_out);
+    auto take = [&](uint64_t key) {
+        if (!key) return false;
+        const BeamPick p = pick_of(key);
+        if (!(p.score >= bound)) return false;  // NaN: of a beam without continuations
         const int at = atomicAdd(&count, 1);
         if (at < kBeamCap) picks[at] = p;
-    });
+        return true;
+    };
+#pragma unroll
+    for (int k = 0; k < NK; ++k) take(mine[k]);
+    // the lists' other candidates, which fall: up to the first below the bound
+    if (total > held)
+        for (int i = tid; i < lists; i += kJoinThreads) {
+            int r = i < held ? (held - i + lists - 1) / lists : 0;
+            while (r < a.n_out && take(cand[(int64_t)i * a.n_out + r])) ++r;
+        }
     __syncthreads();
     auto put = [&](int r, const BeamPick& p) {
         const int64_t o = req * a.n_out + r;
@@ -266,9 +303,11 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
     BeamPick last{INFINITY, 0};
     for (int r = 0; r < a.n_out; ++r) {
         BeamPick best{-INFINITY, 0xFFFFFFFFu};
-        each([&](const BeamPick& p) {
-            if (last.before(p) && p.before(best)) best = p;
-        });
+        for (int i = tid; i < total; i += kJoinThreads)
+            if (const uint64_t key = candidate(i)) {
+                const BeamPick p = pick_of(key);
+                if (last.before(p) && p.before(best)) best = p;
+            }
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) {
             const BeamPick o{__shfl_xor(best.score, k, 64), (uint32_t)__shfl_xor((int)best.at, k, 64)};
@@ -285,24 +324,29 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
 }
 
 // ---------------------------------------------------------------- host side
-// Elements of a thread: 32 where that makes two workgroups per CU or more, else 8.
+// Elements of a thread: 32 where that makes two workgroups per CU or more, or where 8 make more candidates of a request
+// than wait in the join's registers. Chunks + join, 8 | 32, us: 1 x 4 beams over 151936 F32 tokens, 8 outputs, 4.9 + 6.2 |
+// 6.3 + 5.3; 8 x 4 over 32000 5.0 + 6.6 | 6.4 + 12.6; 32 x 8 over 151936, 16 outputs, 48 + 13 | 34 + 9; one request of 8
+// beams over 151936, 16 outputs (9600 candidates | 2432), 5.7 + 11.1 | 7.0 + 6.9.
 struct BeamPlan {
     int ept, chunks;
 };
-static BeamPlan beam_plan(int64_t rows, int vocab) {
+static BeamPlan beam_plan(int64_t n_batch, int n_beams, int vocab, int n_out) {
     const auto chunks = [&](int ept) { return (vocab + kBeamThreads * ept - 1) / (kBeamThreads * ept); };
-    const int ept = rows * chunks(32) >= 2 * (int64_t)cu_count() ? 32 : 8;
+    const bool fill = n_batch * n_beams * chunks(32) >= 2 * (int64_t)cu_count();
+    const bool many = (int64_t)n_beams * chunks(8) * n_out > 4096;
+    const int ept = fill || many ? 32 : 8;
     return {ept, chunks(ept)};
 }
 
 size_t beam_workspace_bytes(int64_t n_batch, int n_beams, int vocab, int n_out) {
-    const int64_t lists = n_batch * n_beams * beam_plan(n_batch * n_beams, vocab).chunks;
+    const int64_t lists = n_batch * n_beams * beam_plan(n_batch, n_beams, vocab, n_out).chunks;
     return (size_t)(round_up(lists * 8, 256) + round_up(lists * 4, 256) + round_up(lists * n_out * 8, 256));
 }
 
 hipError_t launch_beam_select(int type, BeamArgs a, int64_t n_batch, void* ws, hipStream_t st) {
     const int64_t rows = n_batch * a.n_beams;
-    const BeamPlan p = beam_plan(rows, a.vocab);
+    const BeamPlan p = beam_plan(n_batch, a.n_beams, a.vocab, a.n_out);
     a.chunks = p.chunks;
     const int64_t lists = rows * p.chunks;
     uint8_t* w = static_cast<uint8_t*>(ws);

@@ -559,6 +559,13 @@ def test_beam_select(dev, dtype, b, w, v, n):
     check_beams(x, (-3 * rng.random((b, w))).astype(np.float32), n, dev)
 
 
+@pytest.mark.parametrize("b,w,v,n", [(1, 4, 151936, 64), (2, 16, 40000, 33), (1, 16, 60000, 64), (3, 9, 50000, 32),
+                                     (1, 200, 12000, 64), (1, 256, 270000, 3)])
+def test_beam_select_of_many_candidates(dev, b, w, v, n):
+    """More outputs than a quarter of the groups, more candidates than the join's registers hold, and more lists."""
+    test_beam_select(dev, np.float16 if v > 200000 else np.float32, b, w, v, n)
+
+
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
 def test_beam_select_ties_go_to_the_lowest(dev, dtype):
     """Equal logits (all of a row, all of a chunk and more than are ranked at once, negative and positive zeros),
