@@ -63,6 +63,8 @@ __device__ __forceinline__ float groups_bound(const float* gmax, int lane, int n
     return lanes_bound<4>({gmax[lane], gmax[lane + 64], gmax[lane + 128], gmax[lane + 192]}, n);
 }
 
+// All of a thread's logits are loaded at once and stay in registers. 256 rows of 151936 F32: 34 us for 156 MB, 4.6 TB/s,
+// 93 % of a copy's rate; VALU (the exponentials, and their sums in 64 bits) busy 73 % of it. 4 rows: 4.9 us, latency.
 template <class T, int EPT>
 __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
     constexpr int V = 16 / sizeof(T), NV = EPT / V;
@@ -197,6 +199,8 @@ struct BeamPick {
 
 constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / 64;
 constexpr int kBeamBatch = 8;  // candidates of a thread that wait in registers
+// A workgroup per request, bound by its latency: loads, the rows' sums, two barriers of bounds and ranks (4 rows of 75
+// chunks, 8 outputs: 6.4 us; 8 rows of 19, 16 outputs: 9).
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
     constexpr int NK = kBeamBatch;
     __shared__ BeamPick picks[kBeamCap];

@@ -714,6 +714,11 @@ __device__ __forceinline__ void tree_job(const TreeArgs& a, TreeJob& w, int seq)
 
 // Grid: (unit, tile) pairs with the tiles of a unit on one XCD (workgroup id % 8) one after another, as they
 // read the same keys; unit = (sequence, split, KV head).
+// Few keys: a chain of latencies, lengths and page numbers, K and V, the queries, then scores, softmax and products
+// once or twice, the waves' sums (7 tokens over 100 keys, 16/8 heads x 128 F16: 10 us, of which the memory is 0.4 MB).
+// Many: the keys' loads, one step ahead (37 beams over 301..1501 F32 keys, 8/1 x 256: 24.8 us, 69 MB, 2.8 TB/s; matrix
+// instructions busy 27 %), and from a few tiles on their repetition per tile (256 rows over 4096 F32 keys, two
+// sequences: 116 us, 58 of 157 TFLOP/s).
 template <int CT, int HD, bool EARLY>
 __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_kernel(TreeArgs a) {
     __shared__ TreeSmem<kTreeWaves> sm;
@@ -832,6 +837,13 @@ __device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, int unit) {
 
 // 32 W rows of a KV head over a share of its cached keys (slots 1 ..), or 16 rows over the drafted keys (slot 0:
 // the workgroups from hist_wgs on, which fill the end of the launch).
+// A wave's block is a chain: 32 to 48 matrix instructions of scores, the softmax, as many of values; two waves a SIMD
+// cover each other's. 24 tokens of 8 sequences of 1500..4096 keys, 32/8 heads x 128, F16: 37 us; by a timeline 2 for
+// the share, 3 for the queries, 2 for the first block, 19 for 384 keys (3.1 a block of 64, 2.2 alone on a SIMD), 2 for
+// the results, and 5 of drafted keys at the end, in part beside the others. 64 tokens over 32768 keys, Q8_0: 112 us
+// for 34.4 GFLOP, three products each: 0.92 PFLOP/s of f16 where a large library product reaches 1.42; matrix
+// instructions busy 49 % of the cycles, VALU 28 %, the clock near 1.9 GHz. In it 90 us of the shares' loops, 8 before
+// and 10 for drafted keys after them.
 template <int CT, int HD, int W>
 __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(TreeArgs a) {
     using Block = TreeBlock<CT, HD, W>;
@@ -1152,7 +1164,8 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
             tree_row_again<CT, HD, W>(a, w, sm.t, w.row0 + kRowsPerWave * k + __builtin_ctz(x));
 }
 
-// The merge of a sequence's splits: M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L, zeros for a row
+// The merge of a sequence's splits (6144 rows x 128 of up to 12 splits: 7.8 us, 2048 of 33: 9.1; the partial results
+// come from L2 at 4 to 5 TB/s): M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L, zeros for a row
 // that saw no key or has no drafted token. P lanes share 4 outputs, lane p the splits p, p + P, ...
 template <int HD, int P>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeArgs a) {
@@ -1210,7 +1223,9 @@ struct TreePlan {
     int share, units;  // of the block kernel: see tree_share; units: of all KV heads
 };
 
-// Key splits: workgroups until about three per CU have work, 128 keys (a step of each wave) at the least.
+// Key splits: workgroups until about three per CU have work, 128 keys (a step of each wave) at the least. Two, three,
+// five, six per CU, 16 sequences of 1000..4096 keys: F16, 16/4 heads x 128, 20.3, 19.9, 24.7, 24.0 us; F32, 8/2 x 256,
+// 42.9, 38.6, 49, 49.
 static TreePlan tree_plan16(int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
     TreePlan p{};
     p.tiles = (n_tokens * (n_head / n_head_kv) + kTile - 1) / kTile;
