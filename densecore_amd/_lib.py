@@ -272,10 +272,20 @@ def _table_shape(name, t):
     return a, b
 
 
-def _made(name, t, dtype, shape, device, rows=False):
+def _new(shape, dtype, device, stream):
+    """New memory for a call on `stream` (None: the current one). It comes from that stream's own: torch gives a
+    freed block to the stream's next tensor at once, which another stream's kernel may still be using."""
+    if stream is None or stream == _raw_stream():
+        return _torch.empty(shape, dtype=dtype, device=device)
+    cuda = _torch.cuda
+    with cuda.stream(cuda.ExternalStream(stream, device=device) if stream else cuda.default_stream(device)):
+        return _torch.empty(shape, dtype=dtype, device=device)
+
+
+def _made(name, t, dtype, shape, device, stream, rows=False):
     """An output of this type and shape: the caller's, checked, or a new one."""
     if t is None:
-        return _torch.empty(shape, dtype=dtype, device=device)
+        return _new(shape, dtype, device, stream)
     if not _plain(t, dtype, shape):
         _checked(name, t, dtype, shape, rows)
     return t
@@ -647,12 +657,12 @@ class PagedKVCache:
         if n_draft is not None and not _plain(n_draft, _I32, (s,)):
             _checked("n_draft", n_draft, _I32, (s,))
         if out is None:
-            out = torch.empty(q_shape, dtype=_F32, device=q.device)
+            out = _new(q_shape, _F32, q.device, stream)
         out_stride = _rows_of("out", out, _F32, q_shape)
         if workspace is None:
             need = kv_tree_attention_workspace_size(n_head, self.n_head_kv, self.head_dim, s, n, max_past)
             if need:
-                workspace = torch.empty(need, dtype=_U8, device=q.device)
+                workspace = _new(need, _U8, q.device, stream)
         k, v = self._arenas()
         status = lib().dcq_kv_tree_attention(
             self.cache_type, k, v, self.n_blocks, self.n_layer, layer, tables.data_ptr(), table_stride, width,
@@ -713,12 +723,12 @@ class PagedKVCache:
             if not _plain(t, _I32, shape):
                 _checked(name, t, _I32, shape)
         device = refs.device
-        tables_out = _made("tables_out", tables_out, _I32, (c, width), device, rows=True)
-        lengths_out = _made("lengths_out", lengths_out, _I32, (c,), device)
-        refs_out = _made("refs_out", refs_out, _I32, blocks, device)
-        missing = _made("missing", missing, _I32, (1,), device)
+        tables_out = _made("tables_out", tables_out, _I32, (c, width), device, stream, rows=True)
+        lengths_out = _made("lengths_out", lengths_out, _I32, (c,), device, stream)
+        refs_out = _made("refs_out", refs_out, _I32, blocks, device, stream)
+        missing = _made("missing", missing, _I32, (1,), device, stream)
         if workspace is None:
-            workspace = torch.empty(max(kv_fork_workspace_size(self.n_blocks, s, c), 256), dtype=_U8, device=device)
+            workspace = _new(max(kv_fork_workspace_size(self.n_blocks, s, c), 256), _U8, device, stream)
         k, v = self._arenas()
         status = lib().dcq_kv_fork(
             self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, tables.data_ptr(), table_stride, width,
@@ -740,11 +750,11 @@ class PagedKVCache:
             if not _plain(t, _I32, shape):
                 _checked(name, t, _I32, shape)
         device = refs.device
-        tables_out = _made("tables_out", tables_out, _I32, (s, width), device, rows=True)
-        refs_out = _made("refs_out", refs_out, _I32, blocks, device)
-        n_live = _made("n_live", n_live, _I32, (1,), device)
+        tables_out = _made("tables_out", tables_out, _I32, (s, width), device, stream, rows=True)
+        refs_out = _made("refs_out", refs_out, _I32, blocks, device, stream)
+        n_live = _made("n_live", n_live, _I32, (1,), device, stream)
         if workspace is None:
-            workspace = torch.empty(max(kv_compact_workspace_size(self.n_blocks), 256), dtype=_U8, device=device)
+            workspace = _new(max(kv_compact_workspace_size(self.n_blocks), 256), _U8, device, stream)
         k, v = self._arenas()
         status = lib().dcq_kv_compact(
             self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, tables.data_ptr(), table_stride, width,
@@ -790,11 +800,11 @@ def beam_select(logits, beam_scores, n_out, scores=None, parents=None, tokens=No
     if not _plain(beam_scores, _F32, (b, w)):
         _checked("beam_scores", beam_scores, _F32, (b, w))
     device, out = logits.device, (b, n_out)
-    scores = _made("scores", scores, _F32, out, device)
-    parents = _made("parents", parents, _I32, out, device)
-    tokens = _made("tokens", tokens, _I32, out, device)
+    scores = _made("scores", scores, _F32, out, device, stream)
+    parents = _made("parents", parents, _I32, out, device, stream)
+    tokens = _made("tokens", tokens, _I32, out, device, stream)
     if workspace is None:
-        workspace = torch.empty(max(beam_select_workspace_size(b, w, vocab, n_out), 256), dtype=_U8, device=device)
+        workspace = _new(max(beam_select_workspace_size(b, w, vocab, n_out), 256), _U8, device, stream)
     status = lib().dcq_beam_select(
         1 if half else 0, logits.data_ptr(), stride * (2 if half else 4), b, w, vocab, beam_scores.data_ptr(), n_out,
         scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), _nbytes(workspace),

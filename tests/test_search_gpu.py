@@ -189,6 +189,14 @@ def test_tree_attention_missing_pages_are_zero_rows(KV, dev, ct, n, hd, past, wi
     t.check(t.run(dev))
 
 
+@pytest.mark.parametrize("n,hd", [(3, 64), (40, 128), (24, 256)])
+def test_tree_attention_of_q8_0_values_past_the_f16_range(KV, dev, n, hd):
+    """Slots of magnitudes that no f16 piece holds, with queries as much smaller."""
+    t = Tree(KV, Q8_0, n, [300, 20], 8, 2, hd, seed=hd, spread=2.0 ** 18, n_layer=1)
+    t.q *= 2.0 ** -18
+    t.check(t.run(dev))
+
+
 def test_tree_attention_without_mask_is_a_chain(KV, dev):
     t = Tree(KV, F16, 70, [77, 0], 4, 2, 64, seed=5)
     t.seen[:] = np.tril(np.ones((70, 70), bool))
@@ -484,6 +492,36 @@ def test_compact(dev, ct, kv, hd, n_layer, n_blocks, live):
 def test_compact_of_many_pages(dev, n_blocks, live):
     """Beyond the copies that are made beside the plan."""
     test_compact(dev, Q8_0, 1, 32, 1, n_blocks, live)
+
+
+def test_memory_of_a_call_is_its_streams(KV, dev, monkeypatch):
+    """Outputs and workspaces that a call on another stream makes come from that stream's memory."""
+    import torch
+    t = Tree(KV, F16, 3, [900, 40], 4, 2, 64, seed=9)
+    cache, args = t.cache(dev), t.args(dev)
+    refs = torch.zeros(t.n_blocks, dtype=torch.int32, device=dev)
+    x, beam = torch.randn((2, 500), device=dev), torch.zeros((1, 2), device=dev)
+    parents = i32([0, 1, 1], dev)
+    kwargs = t.kwargs(dev)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    made, empty = [], torch.empty
+
+    def spy(*a, **kw):
+        made.append(torch.cuda.current_stream().cuda_stream)
+        return empty(*a, **kw)
+    monkeypatch.setattr(torch, "empty", spy)
+    out = cache.tree_attention(*args, **kwargs, stream=s.cuda_stream)
+    forked = cache.fork(args[1], args[2], parents, refs, stream=s.cuda_stream)
+    cache.compact(args[1], args[2], refs, stream=s.cuda_stream)
+    dc.beam_select(x, beam, 2, stream=s.cuda_stream)
+    assert len(made) == 15 and set(made) == {s.cuda_stream}
+    assert torch.cuda.current_stream().cuda_stream != s.cuda_stream
+    made.clear()
+    dc.beam_select(x, beam, 2)
+    assert set(made) == {torch.cuda.current_stream().cuda_stream}
+    t.check(to_host(out).reshape(2, 3, 4, 64))
+    assert forked[0].shape[0] == 3
 
 
 def test_pages_in_graphs_and_on_streams(dev):
