@@ -717,8 +717,9 @@ __device__ __forceinline__ void tree_job(const TreeArgs& a, TreeJob& w, int seq)
 // Few keys: a chain of latencies, lengths and page numbers, K and V, the queries, then scores, softmax and products
 // once or twice, the waves' sums (7 tokens over 100 keys, 16/8 heads x 128 F16: 10 us, of which the memory is 0.4 MB).
 // Many: the keys' loads, one step ahead (37 beams over 301..1501 F32 keys, 8/1 x 256: 24.8 us, 69 MB, 2.8 TB/s; matrix
-// instructions busy 27 %), and from a few tiles on their repetition per tile (256 rows over 4096 F32 keys, two
-// sequences: 116 us, 58 of 157 TFLOP/s).
+// instructions busy 27 %), and under many rows of F32 the fp32 matrix instructions and what a wave does between
+// them (256 rows over 4096 F32 keys, two sequences: 116 us, 58 of the 150 TFLOP/s of a large product; half the reads of
+// a key, by two tiles to a wave, 121).
 template <int CT, int HD, bool EARLY>
 __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_kernel(TreeArgs a) {
     __shared__ TreeSmem<kTreeWaves> sm;
