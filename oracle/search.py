@@ -1,7 +1,7 @@
 """Plain restatement, in numpy with 64-bit arithmetic, of the search operators over the paged KV cache:
 attention of drafted trees, accepted paths, forks, compaction and the selection of beams.
 
-TEST INFRASTRUCTURE ONLY: imported by tests/ as the checker. One row, sequence or page at a time, from the
+TEST INFRASTRUCTURE ONLY: imported by tests/ alone. One row, sequence or page at a time, from the
 definitions; slot bytes come from oracle/kv.py.
 """
 import numpy as np
