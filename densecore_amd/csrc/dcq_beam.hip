@@ -4,7 +4,7 @@
 // lse(w) = log sum_t exp x[w][t]; the n_out best of a request, ties to the lower w, then the lower t.
 //
 //   beam_chunk_kernel  one pass over the logits, a chunk of a row per workgroup: the chunk's sum of exp x, as
-//                      2^ref sum 2^(x log2 e - ref), and its n_out largest logits (their order is the scores')
+//                      e^ref sum e^(x - ref), and its n_out largest logits (their order is the scores')
 //   beam_join_kernel   per request: lse of each row in 64 bits, and the n_out best of the chunks' candidates
 //                      by their 64-bit scores
 // A chunk's largest are found without sorting it: just below the n_out-th largest of the maxima of 64 or 256 groups of
@@ -112,11 +112,12 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
     if (tid == 0) count = 0;
     __syncthreads();
     const float top = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-    // exp x = 2^ref 2^(x log2 e - ref) (1 + ln 2 low): the product rounded, and what that left, to first order.
-    // ref is 0 for all logits but far ones, and then a multiple of 64, so that a term is the same number in
-    // whatever chunk it is
-    const float far = top * kLog2e;
-    const float ref = fabsf(far) < 64.0f || top == -INFINITY ? 0.0f : 64.0f * rintf(far * (1.0f / 64.0f));
+    // exp x = e^ref e^d, d = x - ref: the difference first, so that nothing overflows or rounds by the size of x
+    // (finite logits go up to 3.4e38, and 2.4e38 times log2 e is infinite). e^d = 2^hi (1 + ln 2 low), the product
+    // d log2 e rounded and what that left; of a term that counts |d| is below 200, and low below 2^-16. ref is 0 for
+    // all logits but far ones, so that a term is the same number in whatever chunk it is, and then the multiple of 64
+    // (of 2^30 on: the logit) next to the chunk's largest
+    const float ref = fabsf(top) < 44.0f || top == -INFINITY ? 0.0f : 64.0f * rintf(top * (1.0f / 64.0f));
     double part[2] = {0.0, 0.0};
     {
 #pragma clang fp contract(off)
@@ -124,10 +125,10 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(BeamArgs a) {
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const float y = e[j][k], hi = y * kLog2e;
-                // in bounds where the first order says nothing, and a number beside -infinity
-                const float lo = __builtin_amdgcn_fmed3f(fmaf(y, kLog2eLow, fmaf(y, kLog2e, -hi)), -0.5f, 0.5f);
-                const float t = __builtin_amdgcn_exp2f(hi - ref);
+                const float d = e[j][k] - ref, hi = d * kLog2e;
+                // in bounds, and a number beside -infinity
+                const float lo = __builtin_amdgcn_fmed3f(fmaf(d, kLog2eLow, fmaf(d, kLog2e, -hi)), -0.5f, 0.5f);
+                const float t = __builtin_amdgcn_exp2f(hi);
                 part[k % 2] += (double)fmaf(t * lo, 0.693147181f, t);
             }
     }
@@ -204,7 +205,7 @@ constexpr int kBeamBatch = 8;  // candidates of a thread that wait in registers
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
     constexpr int NK = kBeamBatch;
     __shared__ BeamPick picks[kBeamCap];
-    __shared__ double lse[kBeamMaxBeams], base[kBeamMaxBeams];
+    __shared__ double lse[kBeamMaxBeams], base[kBeamMaxBeams], from[kBeamMaxBeams];
     __shared__ float gmax[256];
     __shared__ BeamPick wbest[kJoinWaves];
     __shared__ int count;
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
     uint64_t mine[NK];
 #pragma unroll
     for (int k = 0; k < NK; ++k) mine[k] = candidate(tid + k * kJoinThreads);
-    // ---- lse of each row; base is NaN for a beam without continuations
+    // ---- lse of each row, from its largest chunk's reference; base is NaN for a beam without continuations
     for (int w = wave; w < a.n_beams; w += kJoinWaves) {
         const int64_t list = (row0 + w) * a.chunks;
         double m = -(double)INFINITY;
@@ -233,15 +234,16 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
         for (int k = 1; k < 64; k <<= 1) m = fmax(m, __shfl_xor(m, k, 64));
         double s = 0.0;
         for (int c = lane; c < a.chunks; c += 64) {
-            const double sc = a.stat_sum[list + c];
-            s += sc == 0.0 ? 0.0 : ldexp(sc, (int)fmax((double)a.stat_ref[list + c] - m, -4096.0));
+            const double sc = a.stat_sum[list + c], r = a.stat_ref[list + c];
+            s += sc == 0.0 ? 0.0 : r == m ? sc : sc * exp(r - m);
         }
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k, 64);
         if (lane == 0) {
             const float b = a.beam[row0 + w];
+            from[w] = m;
             // to a multiple of 2^-32, less than its error: the same logits in another order have the same lse
-            lse[w] = rint((m + log2(s)) * (0.6931471805599453 * 0x1p32)) * 0x1p-32;
+            lse[w] = rint(log(s) * 0x1p32) * 0x1p-32;
             base[w] = s > 0.0 && s < INFINITY && fabsf(b) < INFINITY ? (double)b : (double)NAN;
         }
     }
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(BeamArgs a) {
     __syncthreads();
     auto pick_of = [&](uint64_t key) {
         const uint32_t at = key_index(key), w = at >> 24;
-        return BeamPick{base[w] + ((double)key_logit(key) - lse[w]), at};
+        return BeamPick{base[w] + (((double)key_logit(key) - from[w]) - lse[w]), at};
     };
     // ---- a bound as in the chunks, on the groups' largest scores among those in registers (rounded down to fp32: no
     // higher)

@@ -134,7 +134,7 @@ def beam_select(x, beam, n_out):
             if np.isnan(row).any() or (row == np.inf).any() or (row == -np.inf).all() or not np.isfinite(beam[i, j]):
                 continue
             top = row.max()
-            lp = float(beam[i, j]) + (row - (top + np.log(np.exp(row - top).sum())))
+            lp = float(beam[i, j]) + ((row - top) - np.log(np.exp(row - top).sum()))
             best = np.argsort(-lp, kind="stable")[:n_out]
             found += [(-lp[t], j, int(t)) for t in best if lp[t] > -np.inf]
         for r, (s, j, t) in enumerate(sorted(found)[:n_out]):

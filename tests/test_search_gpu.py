@@ -648,6 +648,37 @@ def test_beam_select_strides_alignment_and_large_scores(dev):
     check_beams(x, np.array([[-1e4, 1e4]] * 2, np.float32), 6, dev)
 
 
+@pytest.mark.parametrize("low", [np.finfo(np.float32).min, np.float32(-3e38)])
+def test_beam_select_masked_by_the_lowest_value(dev, low):
+    """Tokens ruled out by the type's lowest value, as constrained decoding masks them: whole chunks of them beside
+    ordinary ones, all but one token, and few enough others that the outputs reach them."""
+    rng = np.random.default_rng(43)
+    x = rng.normal(size=(6, 40000)).astype(np.float32)
+    x[0, :9000] = low
+    x[1, 8192:] = low
+    x[2] = low
+    x[2, 39999] = 1.5
+    x[3] = low
+    x[3, [5, 20000]] = 0.0
+    x[4, 100:] = low
+    check_beams(x, np.zeros((2, 3), np.float32), 8, dev)
+    check_beams(x[[2]], np.zeros((1, 1), np.float32), 4, dev)
+    check_beams(x[[3, 0], :700], np.array([[0, -2.0]], np.float32), 12, dev)
+
+
+@pytest.mark.parametrize("v", [1, 700, 9000, 40000])
+@pytest.mark.parametrize("value", [np.finfo(np.float32).min, np.finfo(np.float32).max, -3e38, 2.5e38, 1e12, -1e12])
+def test_beam_select_rows_of_one_far_value(dev, v, value):
+    """All of a row at a value from which its lse differs by less than a last bit, in 64 bits too: every score is the
+    beam's less log v. Bound as in check_beams."""
+    x = np.full((2, v), value, np.float32)
+    s, p, t = (to_host(y) for y in dc.beam_select(to_dev(x, dev), to_dev(np.array([[-1.0, 2.0]], np.float32), dev), 5))
+    n = min(v, 5)
+    want = 2.0 - np.log(v)
+    assert (p[0, :n] == 1).all() and t[0, :n].tolist() == list(range(n))
+    assert (np.abs(s[0, :n] - want) <= 2.0 ** -23 * abs(want) + 2.0 ** -20).all()
+
+
 def test_beam_select_in_graphs(dev):
     import torch
     x = torch.randn((8, 30001), device=dev)
