@@ -421,7 +421,8 @@ int dcq_kv_compact(int cache_type, void* k_arena, void* v_arena, int64_t n_block
 
 /* Beam search's selection. logits: F32 or F16, rows b * n_beams + w of vocab elements, stride_bytes apart (a
  * multiple of the element's size). Candidate (w, t) of request b scores beam_scores[b][w] + log softmax of the
- * row at t, with the row's sum in 64 bits and scores compared in 64; scores / parents / tokens [n_batch][n_out]
+ * row at t, with the row's sum in 64 bits (of terms to 2^-22 each, whatever the logits' size) and scores compared
+ * in 64; scores / parents / tokens [n_batch][n_out]
  * receive the best of each request in falling order, ties by the lower w, then the lower t: the score rounded to
  * fp32, the row b * n_beams + w, and t. A logit of -infinity rules a token out; a row whose logits hold a NaN
  * or +infinity, or are all -infinity, and a beam whose score is not finite have no continuations; where fewer

@@ -679,6 +679,17 @@ def test_beam_select_rows_of_one_far_value(dev, v, value):
     assert (np.abs(s[0, :n] - want) <= 2.0 ** -23 * abs(want) + 2.0 ** -20).all()
 
 
+@pytest.mark.parametrize("at", [5e4, 65504.0, -6e4, 1e5, -1e6, 8e6])
+def test_beam_select_of_logits_far_from_zero(dev, at):
+    """Rows around one far value each, F16 as far as it goes: the same bound, whatever the logits' size."""
+    rng = np.random.default_rng(44)
+    beam = -rng.random((2, 3)).astype(np.float32)
+    x = (at + rng.normal(size=(6, 9001)) * 8).astype(np.float32)
+    check_beams(x, beam, 8, dev)
+    if abs(at) <= 65504:
+        check_beams(np.clip(x * (1 - 1e-3 * np.arange(6)[:, None]), -65504, 65504).astype(np.float16), beam, 8, dev)
+
+
 def test_beam_select_in_graphs(dev):
     import torch
     x = torch.randn((8, 30001), device=dev)
