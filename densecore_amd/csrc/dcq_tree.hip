@@ -1019,12 +1019,14 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
                 if (8 * (i >> 2) + 4 * p + (i & 3) >= left) sc[i] = -INFINITY;
         }
     };
-    // a new reference where the scores ask for one; the factor of what is in units of the old one
-    auto raise = [&](const f32x16& sc) {
+    auto top = [&](const f32x16& sc) {
         float mx = sc[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * qsc;
+        return fmaxf(mx, __shfl_xor(mx, 32, 64)) * qsc;
+    };
+    // a new reference where the largest of a block's scores asks for one; the factor of what is in units of the old one
+    auto raise = [&](float mx) {
         const float m_new = mx > m + 8.0f ? __builtin_ceilf(mx) : m;
         const float alpha = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
         m = m_new;
@@ -1103,23 +1105,16 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
         }
         if (r0 < w.n_rows) {
             if constexpr (BK == 64) {
-                // two halves, the weights of one made beside the products of the other
+                // two halves of one reference, the weights of one made beside the products of the other
                 f32x16 s0, s1;
                 f16x8 h0[2], l0[2], h1[2], l1[2];
                 scores(buf, 0, s0);
                 mask(s0, w.k_end - kb);
-                const float a0 = raise(s0);
-                if (__any(a0 != 1.0f)) rescale(a0);
                 scores(buf, 32, s1);
-                weights(s0, h0, l0);
                 mask(s1, w.k_end - kb - 32);
-                const float a1 = raise(s1);
-                if (__any(a1 != 1.0f)) {
-                    rescale(a1);
-                    const _Float16 f = (_Float16)a1;  // a power of two
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) h0[s] *= f, l0[s] *= f;
-                }
+                const float a0 = raise(fmaxf(top(s0), top(s1)));
+                if (__any(a0 != 1.0f)) rescale(a0);
+                weights(s0, h0, l0);
                 values(buf, 0, h0, l0);
                 weights(s1, h1, l1);
                 values(buf, 32, h1, l1);
@@ -1128,7 +1123,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
                 f16x8 h0[2], l0[2];
                 scores(buf, 0, s0);
                 mask(s0, w.k_end - kb);
-                const float a0 = raise(s0);
+                const float a0 = raise(top(s0));
                 if (__any(a0 != 1.0f)) rescale(a0);
                 weights(s0, h0, l0);
                 values(buf, 0, h0, l0);

@@ -96,6 +96,9 @@ class Tree:
         out = self.cache(dev).tree_attention(*self.args(dev), **self.kwargs(dev))
         return to_host(out).reshape(self.s, self.n, self.heads, self.hd)
 
+    def run_and_check(self, dev):
+        self.check(self.run(dev))
+
     def check(self, out):
         """Every row of every head: |out - ref| <= (2e-6 + 2^-21 B) |A| in the 2-norm. A score of magnitude up to B
         is off by the dropped parts of its operands' pieces (2^-22 of B for both), its sums' roundings (about as
@@ -274,6 +277,37 @@ def test_tree_attention_wide_values(KV, dev, ct, n, hd):
     empty = np.zeros((0, row), np.float32)
     t.hist = [[KV.gather(ct, a, 1, 0, t.tables[0], 400, empty).reshape(400, 2, hd) for a in t.arena]]
     t.check(t.run(dev))
+
+
+def planted(KV, ct, n, hd, scores, zero, seed, heads=8, kv=2):
+    """A call whose cached keys have the given scores (in base 2, one sequence each) for every row, and values of
+    zero at the positions `zero`; no row sees a drafted key."""
+    t = Tree(KV, ct, n, [len(s) for s in scores], heads, kv, hd, seed=seed, n_layer=1)
+    t.q[:] = 0
+    t.q[..., 0] = 8 / (t.scale * np.log2(np.e))
+    t.seen[:] = False
+    empty = np.zeros((0, kv * hd), np.float32)
+    for b, s in enumerate(scores):
+        k = np.zeros((len(s), kv, hd), np.float32)
+        k[:, :, 0] = np.asarray(s)[:, None] / 8
+        v = t.rng.normal(size=k.shape).astype(np.float32) + 1
+        v[zero] = 0
+        for x, rows in enumerate((k, v)):
+            KV.write(ct, t.arena[x], 1, 0, t.tables[b], 0, rows.reshape(len(s), -1))
+    t.hist = [[KV.gather(ct, a, 1, 0, t.tables[b], p, empty).reshape(p, kv, hd) for a in t.arena]
+              for b, p in enumerate(t.pasts)]
+    return t
+
+
+@pytest.mark.parametrize("ct", CACHE_TYPES)
+@pytest.mark.parametrize("n,hd", [(40, 64), (40, 128), (40, 256), (3, 128)])
+@pytest.mark.parametrize("jump", [12, 17, 24])
+def test_tree_attention_a_key_far_above_those_beside_it(KV, dev, ct, n, hd, jump):
+    """Scores that rise by less than what raises a row's reference, then a key far above them a few places on, of
+    value zero: what the keys before it give must not be lost when the reference follows it."""
+    s = np.full(320, -40.0)
+    s[:64], s[64:96], s[100] = -8, 0, jump
+    planted(KV, ct, n, hd, [s], [100], seed=hd + jump).run_and_check(dev)
 
 
 def test_tree_attention_strided_rows_and_another_stream(KV, dev):
