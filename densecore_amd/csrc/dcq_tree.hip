@@ -3,7 +3,7 @@
 // Sequence b has n_past(b) cached keys (pages tables[b]) and n_draft(b) drafted tokens with fp32 K / V rows of
 // their own. Row (token j, query head h) attends every cached key, and drafted key i where bit i of mask[b][j]
 // is set:  out = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q . k_t).  The online softmax keeps a reference m
-// (an integer in base 2, raised when a score passes it by 8), the sum l of p' = 2^(s - m), s = scale log2(e)
+// (an integer in base 2, raised when a score passes it by 3), the sum l of p' = 2^(s - m), s = scale log2(e)
 // q . k, and O = sum p' v.
 //
 // Query rows of a KV head are the (token, head of its group) pairs, token-major, in tiles of 16: a column of
@@ -19,13 +19,23 @@
 // LDS reads. Drafted keys, a small part, are the other kernel's work, in workgroups of the same launch.
 //
 // Arithmetic. F16 and Q8_0 slots are multiplied on the f16 matrix instructions (16 x the fp32 ones' rate):
-// q and p', fp32, are split into two f16 pieces of 22 bits (q under an exponent per row, p' times 2^7), an
-// F16 slot is one exact piece, and a Q8_0 value d * q, a product of 11 and 7 bits, is exactly the two pieces
-// f16(d q) and d q - f16(d q). F32 slots and the drafted rows use the fp32 matrix instructions. Sums are fp32.
+// q and p', fp32, are split into two f16 pieces of 22 bits (q under an exponent per row, fewer bits below
+// 2^-16 of its largest), an F16 slot is one exact piece, and a Q8_0 value d * q, a product of 11 and 7 bits, is
+// exactly the two pieces f16(d q) and d q - f16(d q). F32 slots and the drafted rows use the fp32 matrix
+// instructions. Sums are fp32.
+// All weights keep 22 bits, however far below the row's largest one they are: a first key far above the others
+// whose value is next to zero, as models make them, leaves the output to weights of 2^-20 and less. So the
+// second piece is 2^11 times what the first one left, in a sum of its own, and scores more than 26 below the
+// reference take another pass over the step's values, in units of 2^-26 (piece_weights). With both pieces in one
+// unit and one sum, weights had 22 bits from 2^-10 on and none from 2^-32; that took, us a call, 24 tokens of 8
+// sequences of 1500..4096 keys, 32/8 heads x 128, F16 44 where it now takes 48, 64 tokens over 32768 keys Q8_0
+// 124 | 128, F16 91 | 101, 8 sequences x 64 dims 29 | 35. A unit of each step's own for one sum needs a second pass in
+// every seventh step of such scores: 68, 185, 152, 49.
 // Infinities and NaN: what a 16-row tile shares can reach a row that does not see it, and an infinity in one
 // piece has no second piece. A row whose m, l or O is not finite is therefore computed again one key at a
 // time in fp32, of the keys it sees alone.
 #include <algorithm>
+#include <type_traits>
 
 #include "dcq_attn.h"
 #include "dcq_common.h"
@@ -41,7 +51,10 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kTile = 16;          // query rows of a tile
 constexpr int kTreeWaves = 4;      // waves of a workgroup, a share of the keys each
 constexpr int kRowsPerWave = 32;   // of the block kernel
-constexpr float kPieces = 128.0f;  // of the weights in O: 2^15 at most before the reference is raised
+// A row's reference is raised when a score passes it by kSlack; a weight counts kPieces in O, 2^15 at most. Its first
+// f16 piece is a normal number, and both have their 11 bits, from 2^-kBandBits on.
+constexpr float kSlack = 3.0f, kBandBits = 26.0f;
+constexpr float kPieces = 0x1p12f, kLow = 0x1p11f;  // kLow: of the second piece
 
 // No sum of the 16 x 16 matrix instructions is to be put over an operand, or half over the sum before it. TIED: an
 // empty statement uses operands and sum once more when the new sum is there. That is free at head_dim 256; at 128 it
@@ -54,12 +67,39 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
     return d;
 }
 template <bool TIED>
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b) {
+    f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+    if constexpr (TIED) asm volatile("" : "+v"(d) : "v"(a), "v"(b));
+    return d;
+}
+template <bool TIED>
 __device__ __forceinline__ f32x4 mfma16(float a, float b, f32x4 c) {
     f32x4 d = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
     if constexpr (TIED) asm volatile("" : "+v"(d) : "v"(a), "v"(b), "v"(c));
     return d;
 }
 __device__ __forceinline__ void keep(f32x4 x) { asm volatile("" ::"v"(x)); }
+
+// Eight weights as f16 pieces.
+__device__ __forceinline__ void split_weights(const float* p, f16x8& h, f16x8& l) {
+    f16x2 hh[4], ll[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const f32x2 w = {p[2 * t] * kPieces, p[2 * t + 1] * kPieces};
+        hh[t] = __builtin_convertvector(w, f16x2);
+        ll[t] = __builtin_convertvector((f32x2){(w[0] - (float)hh[t][0]) * kLow, (w[1] - (float)hh[t][1]) * kLow}, f16x2);
+    }
+    h = __builtin_shufflevector(__builtin_shufflevector(hh[0], hh[1], 0, 1, 2, 3),
+                                __builtin_shufflevector(hh[2], hh[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+    l = __builtin_shufflevector(__builtin_shufflevector(ll[0], ll[1], 0, 1, 2, 3),
+                                __builtin_shufflevector(ll[2], ll[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// a + b f
+__device__ __forceinline__ f32x4 plus_low(f32x4 a, f32x4 b, float f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = __builtin_fmaf(b[i], f, a[i]);
+    return a;
+}
 
 template <int CT>
 constexpr int tree_chunk() { return CT == kTypeF32 ? 16 : 32; }  // keys of a wave's step
@@ -118,6 +158,15 @@ struct TreeKeys<kTypeF16, HD> {
 #pragma unroll
         for (int u = 0; u < U; ++u) v[j][i][u] = make_uint2(0u, 0u);
     }
+    // V's operands are made again in the next pass over a step's weights, not kept
+    __device__ __forceinline__ void again() {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int u = 0; u < U; ++u) asm volatile("" : "+v"(v[j][i][u].x), "+v"(v[j][i][u].y));
+    }
     // q: the lane's operand of k-step 0; k-steps and pieces lie 64 apart
     __device__ __forceinline__ void scores(const uint4* q, f32x4 (&r)[2]) const {
         f32x4 lo[2], hi[2];
@@ -136,7 +185,9 @@ struct TreeKeys<kTypeF16, HD> {
 #pragma unroll
         for (int j = 0; j < 2; ++j) r[j] = hi[j] + lo[j];
     }
-    __device__ __forceinline__ void weigh(const f16x8 ph, const f16x8 pl, f32x4 (&o)[U][4]) const {
+    // V^T P^T in units of `unit` into O. FIRST: the unit is 1, and the first piece's products go on from O
+    template <bool FIRST>
+    __device__ __forceinline__ void weigh(const f16x8 ph, const f16x8 pl, float unit, f32x4 (&o)[U][4]) const {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -149,8 +200,11 @@ struct TreeKeys<kTypeF16, HD> {
                                                  e % 2 ? 0x07060302u : 0x05040100u);
                 }
                 const f16x8 f = as_f16x8(w[0], w[1], w[2], w[3]);
-                o[u][e] = mfma16<HD == 256>(f, pl, o[u][e]);
-                o[u][e] = mfma16<HD == 256>(f, ph, o[u][e]);
+                const f32x4 low = mfma16<HD == 256>(f, pl);
+                if constexpr (FIRST)
+                    o[u][e] = plus_low(mfma16<HD == 256>(f, ph, o[u][e]), low, 1.0f / kLow);
+                else
+                    o[u][e] = plus_low(o[u][e], plus_low(mfma16<HD == 256>(f, ph), low, 1.0f / kLow), unit);
             }
     }
 };
@@ -187,6 +241,14 @@ struct TreeKeys<kTypeQ8_0, HD> {
 #pragma unroll
         for (int u = 0; u < U; ++u) vd[j][i][u] = 0u;
     }
+    __device__ __forceinline__ void again() {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int u = 0; u < U; ++u) asm volatile("" : "+v"(v[j][i][u]), "+v"(vd[j][i][u]));
+    }
     __device__ __forceinline__ void scores(const uint4* q, f32x4 (&r)[2]) const {
         f32x4 lo[2], hi[2];
 #pragma unroll
@@ -212,7 +274,8 @@ struct TreeKeys<kTypeQ8_0, HD> {
 #pragma unroll
         for (int j = 0; j < 2; ++j) r[j] = hi[j] + lo[j];
     }
-    __device__ __forceinline__ void weigh(const f16x8 ph, const f16x8 pl, f32x4 (&o)[U][4]) const {
+    template <bool FIRST>
+    __device__ __forceinline__ void weigh(const f16x8 ph, const f16x8 pl, float unit, f32x4 (&o)[U][4]) const {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             f16x2 d[4];
@@ -229,9 +292,12 @@ struct TreeKeys<kTypeQ8_0, HD> {
                                                                      0x0c040c00u + 0x00010001u * e)), d[t]);
                 const f16x8 fh = as_f16x8(as_u32(p[0].h), as_u32(p[1].h), as_u32(p[2].h), as_u32(p[3].h));
                 const f16x8 fl = as_f16x8(as_u32(p[0].l), as_u32(p[1].l), as_u32(p[2].l), as_u32(p[3].l));
-                o[u][e] = mfma16<HD == 256>(fl, ph, o[u][e]);
-                o[u][e] = mfma16<HD == 256>(fh, pl, o[u][e]);
-                o[u][e] = mfma16<HD == 256>(fh, ph, o[u][e]);
+                const f32x4 low = mfma16<HD == 256>(fh, pl);
+                if constexpr (FIRST)
+                    o[u][e] = plus_low(mfma16<HD == 256>(fh, ph, mfma16<HD == 256>(fl, ph, o[u][e])), low, 1.0f / kLow);
+                else
+                    o[u][e] = plus_low(o[u][e], plus_low(mfma16<HD == 256>(fh, ph, mfma16<HD == 256>(fl, ph)), low, 1.0f / kLow),
+                                       unit);
             }
         }
     }
@@ -304,16 +370,16 @@ struct TreeKeys<kTypeF32, HD> {
     }
 };
 
-// One step of the online softmax: scores of the lane's N keys of its row (-inf: not seen) to weights.
+// The row's reference raised where the largest score of a step asks for it (the lane has N keys of it; -inf: not seen).
 template <int N, int U>
-__device__ __forceinline__ void softmax_step(float (&s)[N], float& m, float& l, f32x4 (&o)[U][4]) {
+__device__ __forceinline__ void raise_reference(const float (&s)[N], float& m, float& l, f32x4 (&o)[U][4]) {
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__any(mx > m + 8.0f)) {
-        const float m_new = mx > m + 8.0f ? __builtin_ceilf(mx) : m;
+    if (__any(mx > m + kSlack)) {
+        const float m_new = mx > m + kSlack ? __builtin_ceilf(mx) : m;
         const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
         l *= alpha;
 #pragma unroll
@@ -322,12 +388,50 @@ __device__ __forceinline__ void softmax_step(float (&s)[N], float& m, float& l, 
             for (int e = 0; e < 4; ++e) o[u][e] *= alpha;
         m = m_new;
     }
+}
+
+// One step of the online softmax: scores to weights.
+template <int N, int U>
+__device__ __forceinline__ void softmax_step(float (&s)[N], float& m, float& l, f32x4 (&o)[U][4]) {
+    raise_reference<N, U>(s, m, l, o);
     const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
         l += s[i];
     }
+}
+
+// The same for weights that go into f16 pieces, of scores s qsc: the weights of a pass, those below 2^(-kBandBits pass)
+// and not below 2^(-kBandBits (pass + 1)), in units of the former (all from there up in pass 0). `again`, in the
+// whole wave, if keys are left whose weight is above 2^-126: five passes at the most.
+__device__ __forceinline__ float band_unit(int pass) { return __builtin_amdgcn_exp2f(-kBandBits * (float)pass); }
+template <int N>
+__device__ __forceinline__ void piece_weights(float (&s)[N], float qsc, float m, float& l, int pass, bool& again) {
+    const float ref = m == -INFINITY ? 0.0f : m - kBandBits * (float)pass;
+    if (pass)
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = s[i] * qsc < ref ? s[i] : -INFINITY;
+    float low = s[0], sum = 0.0f;
+#pragma unroll
+    for (int i = 1; i < N; ++i) low = fminf(low, s[i]);
+    again = false;
+    if (__any(low * qsc < ref - kBandBits)) {  // such keys, or some that are not seen
+        const float cut = ref < INFINITY ? ref - kBandBits : -INFINITY;  // an infinite reference: NaN, not keys left out
+        bool left = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool below = s[i] * qsc < cut;  // not a NaN
+            left |= below && s[i] * qsc > m - 126.0f;
+            s[i] = below ? -INFINITY : s[i];
+        }
+        again = pass < 4 && __any(left);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], qsc, -ref));
+#pragma unroll
+    for (int i = 0; i < N; i += 4) sum += (s[i] + s[i + 1]) + (s[i + 2] + s[i + 3]);
+    l = pass ? __builtin_fmaf(sum, band_unit(pass), l) : l + sum;
 }
 
 // The factor that takes sums in units of 2^m to units of 2^mx: 0 for sums of no key (l == 0, m = -inf), 1
@@ -464,9 +568,10 @@ template <int CT, int HD, int W, bool HIST, bool EARLY>
 __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, TreeSmem<W>& sm) {
     constexpr int U = HD / 64, CK = tree_chunk<CT>(), NP = CK / kKvBlock;
     // When a step's V is loaded and the next one's K: with K and after the scores, so that both have a step's time
-    // to come, or (head_dim 256) after the scores and after the products, for fewer registers and two waves
+    // to come, or (head_dim 256) after the scores and at the next step's start, for fewer registers and two waves
     // on a SIMD in place of one: 37 beams over 301..1501 F32 keys 39.8 -> 26.1 us, 16 over 1000..4096 59 -> 44
-    // (F16 39 -> 34, Q8_0 46 -> 33)
+    // (F16 39 -> 34, Q8_0 46 -> 33); the next K after the products, where their registers meet, spills: a call 31.7 where
+    // it now takes 27.3 (F16), 33.2 | 30.5 (Q8_0), the beams 28.2 | 27.2
     constexpr bool LATE = HD == 256;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int g = lane >> 4, n = lane & 15;
@@ -515,11 +620,12 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
     if (c0 < c1) {
 #pragma unroll
         for (int j = 0; j < NP; ++j) pages[j] = w.first[j];
+        if constexpr (!LATE) {
 #pragma unroll
-        for (int j = 0; j < NP; ++j) t.load_k(j, a.k_arena + page_bytes(pages[j]), off_k, g);
-        if constexpr (!LATE)
+            for (int j = 0; j < NP; ++j) t.load_k(j, a.k_arena + page_bytes(pages[j]), off_k, g);
 #pragma unroll
             for (int j = 0; j < NP; ++j) t.load_v(j, a.v_arena + page_bytes(pages[j]), off_v, sb, n);
+        }
     }
 
     // ---- the queries as operands, in LDS: a wave makes every W-th k-step's
@@ -584,9 +690,14 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
     if (EARLY && d0 < w.n_draft) add_drafts(early, d0);
 
     if (c0 < c1) {
-        for (int c = c0; c < c1; c += W) {
+        int pass = 0;
+        bool again = false;
+        for (int c = c0; c < c1;) {
             const bool more = c + W < c1;
             if (more) pages_of(c + W, next);
+            if constexpr (LATE)
+#pragma unroll
+                for (int j = 0; j < NP; ++j) t.load_k(j, a.k_arena + page_bytes(pages[j]), off_k, g);
             const int left = w.k_end - c * CK;  // keys of the step, if fewer than CK
             bool whole = left >= CK;
 #pragma unroll
@@ -621,23 +732,44 @@ __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, T
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (pages[j] < 0 || 16 * j + 4 * g + i >= left) t.zero_v(j, i);
-            softmax_step<4 * NP, U>(s, m, l, o);
             if constexpr (CT == kTypeF32) {
+                softmax_step<4 * NP, U>(s, m, l, o);
                 t.weigh(s, o);
             } else {
-                f16x4 h0, l0, h1, l1;
-                split4(s[0] * kPieces, s[1] * kPieces, s[2] * kPieces, s[3] * kPieces, h0, l0);
-                split4(s[4] * kPieces, s[5] * kPieces, s[6] * kPieces, s[7] * kPieces, h1, l1);
-                t.weigh(__builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7),
-                        __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7), o);
+                if constexpr (LATE) {
+                    f16x8 ph, pl;
+                    if (!again) raise_reference<4 * NP, U>(s, m, l, o);
+                    pass = again ? pass + 1 : 0;
+                    piece_weights<4 * NP>(s, 1.0f, m, l, pass, again);
+                    split_weights(s, ph, pl);
+                    t.template weigh<false>(ph, pl, band_unit(pass), o);
+                    __builtin_amdgcn_sched_barrier(0);  // the next keys' loads no earlier than that
+                } else {
+                    float p[4 * NP];
+                    f16x8 ph, pl;
+#pragma unroll
+                    for (int i = 0; i < 4 * NP; ++i) p[i] = s[i];
+                    raise_reference<4 * NP, U>(p, m, l, o);
+                    piece_weights<4 * NP>(p, 1.0f, m, l, 0, again);
+                    split_weights(p, ph, pl);
+                    t.template weigh<true>(ph, pl, 1.0f, o);
+#pragma unroll 1
+                    for (pass = 1; again; ++pass) {
+#pragma unroll
+                        for (int i = 0; i < 4 * NP; ++i) p[i] = s[i];
+                        piece_weights<4 * NP>(p, 1.0f, m, l, pass, again);
+                        split_weights(p, ph, pl);
+                        t.again();
+                        t.template weigh<false>(ph, pl, band_unit(pass), o);
+                    }
+                }
             }
+            if (LATE && again) continue;  // the step once more: there is no room to keep its scores
+            c += W;
             if (more) {
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
-                    if constexpr (LATE)
-                        t.load_k(j, a.k_arena + page_bytes(next[j]), off_k, g);
-                    else
-                        t.load_v(j, a.v_arena + page_bytes(next[j]), off_v, sb, n);
+                    if constexpr (!LATE) t.load_v(j, a.v_arena + page_bytes(next[j]), off_v, sb, n);
                     pages[j] = next[j];
                 }
             }
@@ -925,6 +1057,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
     }
 
     constexpr int BK = Block::BK, RW = BK / W;  // keys of a block, and of them a wave's
+    constexpr int NH = BK / 32;                 // 32-key parts of a block
     constexpr bool DMA = Block::DMA;
     constexpr int NBUF = Block::NBUF;
     const int64_t head = a.sb / a.n_head_kv * w.h_kv;
@@ -1019,53 +1152,43 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
                 if (8 * (i >> 2) + 4 * p + (i & 3) >= left) sc[i] = -INFINITY;
         }
     };
-    auto top = [&](const f32x16& sc) {
-        float mx = sc[0];
+    // a new reference where the largest of a block's scores asks for one
+    auto raise = [&](const float (&s)[16 * NH]) {
+        float mx = s[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-        return fmaxf(mx, __shfl_xor(mx, 32, 64)) * qsc;
-    };
-    // a new reference where the largest of a block's scores asks for one; the factor of what is in units of the old one
-    auto raise = [&](float mx) {
-        const float m_new = mx > m + 8.0f ? __builtin_ceilf(mx) : m;
+        for (int i = 1; i < 16 * NH; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * qsc;
+        if (!__any(mx > m + kSlack)) return;
+        const float m_new = mx > m + kSlack ? __builtin_ceilf(mx) : m;
         const float alpha = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
         m = m_new;
-        return alpha;
-    };
-    auto rescale = [&](float alpha) {
         l *= alpha;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int v = 0; v < 16; ++v) o[t][v] *= alpha;
     };
-    // the weights, their sum, and their pieces as operands: step s takes i = 8 s .. + 7, keys 16 s + 4 p + 0..3 and
-    // 16 s + 8 + 4 p + 0..3
-    auto weights = [&](f32x16& sc, f16x8(&ph)[2], f16x8(&pl)[2]) {
-        const float ref = m == -INFINITY ? 0.0f : -m;
+    // O^T += V^T P^T of a block, the weights in units of `unit`: as pieces, operand s takes i = 8 s .. + 7, keys
+    // 16 s + 4 p + 0..3 and 16 s + 8 + 4 p + 0..3. first: the unit is 1, and the first pieces' products go on from O
+    auto values = [&](auto first, int buf, const float (&pw)[16 * NH], float unit) {
+        f16x8 ph[2 * NH], pl[2 * NH];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qsc, ref));
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) l += (sc[i] + sc[i + 1]) + (sc[i + 2] + sc[i + 3]);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            f16x4 h0, l0, h1, l1;
-            split4(sc[8 * s] * kPieces, sc[8 * s + 1] * kPieces, sc[8 * s + 2] * kPieces, sc[8 * s + 3] * kPieces, h0, l0);
-            split4(sc[8 * s + 4] * kPieces, sc[8 * s + 5] * kPieces, sc[8 * s + 6] * kPieces, sc[8 * s + 7] * kPieces, h1,
-                   l1);
-            ph[s] = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
-            pl[s] = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-    };
-    // O^T += V^T P^T
-    auto values = [&](int buf, int sub, const f16x8(&ph)[2], const f16x8(&pl)[2]) {
-        const int vrow = sub + 4 * p + ((lane & 15) >> 2);
+        for (int s = 0; s < 2 * NH; ++s) split_weights(pw + 8 * s, ph[s], pl[s]);
+        const int vrow = 4 * p + ((lane & 15) >> 2);
         // of tile t the 16-byte piece 4 t + vc of the row, its half lane % 2
         const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vx = Block::v_swizzle(lane >> 2);
+        f32x16 low[2];
+        auto add_low = [&](int t) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+            for (int v = 0; v < 16; ++v) o[t][v] = __builtin_fmaf(low[t % 2][v], 1.0f / kLow, o[t][v]);
+        };
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
+        for (int t = 0; t < NT; ++t) {
+            f32x16 &lo = low[t % 2], high;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) lo[v] = 0.0f, high[v] = first ? o[t][v] : 0.0f;
+#pragma unroll
+            for (int s = 0; s < 2 * NH; ++s) {
                 f16x8 f[NPC];
 #pragma unroll
                 for (int u = 0; u < NPC; ++u) {
@@ -1074,10 +1197,23 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
                     const f16x4 a1 = lds_transposed(&sm.b.v[buf][u][16 * s + 8 + vrow][at]);
                     f[u] = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
                 }
-                if constexpr (NPC == 2) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[1], ph[s], o[t], 0, 0, 0);
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], pl[s], o[t], 0, 0, 0);
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], ph[s], o[t], 0, 0, 0);
+                lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], pl[s], lo, 0, 0, 0);
+                if constexpr (NPC == 2) high = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[1], ph[s], high, 0, 0, 0);
+                high = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[0], ph[s], high, 0, 0, 0);
             }
+            if constexpr (first) {
+                o[t] = high;
+                if (t) add_low(t - 1);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    o[t][v] = __builtin_fmaf(__builtin_fmaf(lo[v], 1.0f / kLow, high[v]), unit, o[t][v]);
+                // O where the VALU takes it, the queries (below) in the other half of the registers: Q8_0, 32 tokens of 8
+                // sequences of 1500..4096 keys, 16/4 heads, 132 -> 124 us a call
+                if constexpr (HD == 256) asm volatile("" : "+v"(o[t]));
+            }
+        }
+        if constexpr (first) add_low(NT - 1);
     };
 
     int blk_next = -1;
@@ -1104,29 +1240,37 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
             blk_next = wave_page(kb + 2 * BK);
         }
         if (r0 < w.n_rows) {
-            if constexpr (BK == 64) {
-                // two halves of one reference, the weights of one made beside the products of the other
-                f32x16 s0, s1;
-                f16x8 h0[2], l0[2], h1[2], l1[2];
-                scores(buf, 0, s0);
-                mask(s0, w.k_end - kb);
-                scores(buf, 32, s1);
-                mask(s1, w.k_end - kb - 32);
-                const float a0 = raise(fmaxf(top(s0), top(s1)));
-                if (__any(a0 != 1.0f)) rescale(a0);
-                weights(s0, h0, l0);
-                values(buf, 0, h0, l0);
-                weights(s1, h1, l1);
-                values(buf, 32, h1, l1);
-            } else {
-                f32x16 s0;
-                f16x8 h0[2], l0[2];
-                scores(buf, 0, s0);
-                mask(s0, w.k_end - kb);
-                const float a0 = raise(top(s0));
-                if (__any(a0 != 1.0f)) rescale(a0);
-                weights(s0, h0, l0);
-                values(buf, 0, h0, l0);
+            if constexpr (HD == 256) {
+#pragma unroll
+                for (int k = 0; k < KS; ++k) asm volatile("" : "+a"(qh[k]), "+a"(ql[k]));
+            }
+            float s[16 * NH];
+            auto all_scores = [&](int b) {
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    f32x16 sc;
+                    scores(b, 32 * h, sc);
+                    mask(sc, w.k_end - kb - 32 * h);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[16 * h + i] = sc[i];
+                }
+            };
+            // head_dim 256 has one form of the products for all passes: two spill (F16 139 us where this takes 97)
+            bool again = true;
+            if constexpr (HD < 256) {
+                all_scores(buf);
+                raise(s);
+                piece_weights<16 * NH>(s, qsc, m, l, 0, again);
+                values(std::true_type{}, buf, s, 1.0f);
+            }
+#pragma unroll 1
+            for (int pass = HD < 256; again; ++pass) {
+                int b = buf;
+                asm volatile("" : "+s"(b));  // read anew, not kept from pass to pass
+                all_scores(b);
+                if (HD == 256 && pass == 0) raise(s);
+                piece_weights<16 * NH>(s, qsc, m, l, pass, again);
+                values(std::false_type{}, b, s, band_unit(pass));
             }
         }
         if constexpr (DMA)

@@ -367,7 +367,9 @@ int dcq_kv_attention(int cache_type, const void* k_arena, const void* v_arena, i
  * zeros that is attended, as in dcq_kv_attention. A token that sees nothing, all of whose scores are
  * -infinity, or that is not drafted (j >= n_draft[b]) gets zeros. What a token does not see has no influence
  * on it, infinities and NaN included. head_dim 64, 128 or 256; n_tokens <= 1024; max_past <= 2^24.
- * Precision: as dcq_kv_attention (fp32 sums and weights; products of at least 22 bits of each operand).
+ * Precision: sums in fp32. F32 caches and drafted rows are multiplied in fp32. For F16 and Q8_0 caches the slots
+ * are exact, the softmax weights have 22 bits or more, however small they are beside the row's largest, and q has
+ * 22 bits or more of an element down to 2^-16 of the largest of its row, fewer below.
  * The workspace (256-byte aligned) holds the partial results of key splits; 0 needs none. */
 size_t dcq_kv_tree_attention_workspace_size(int n_head, int n_head_kv, int head_dim, int64_t n_seqs,
                                             int64_t n_tokens, int64_t max_past);

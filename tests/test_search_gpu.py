@@ -310,6 +310,17 @@ def test_tree_attention_a_key_far_above_those_beside_it(KV, dev, ct, n, hd, jump
     planted(KV, ct, n, hd, [s], [100], seed=hd + jump).run_and_check(dev)
 
 
+@pytest.mark.parametrize("ct", CACHE_TYPES)
+@pytest.mark.parametrize("n,hd", [(1, 64), (1, 128), (1, 256), (40, 64), (40, 128), (40, 256)])
+@pytest.mark.parametrize("sink", [15, 24, 36, 60, 100])
+def test_tree_attention_sinks(KV, dev, ct, n, hd, sink):
+    """A first key far above the others whose value is zero: the output is the others', each of a weight far below
+    the row's largest, in all of fp32's digits. In the second sequence the others' scores lie apart as well."""
+    s = [np.zeros(600), np.random.default_rng(sink).uniform(-30, 0, 290)]
+    s[0][0], s[1][0] = sink, sink
+    planted(KV, ct, n, hd, s, [0], seed=hd + sink).run_and_check(dev)
+
+
 def test_tree_attention_strided_rows_and_another_stream(KV, dev):
     """Rows of q, K / V, out and the tables inside wider tensors, on a stream other than the current one."""
     import torch
