@@ -724,10 +724,10 @@ static int validate_tree_shape(int n_head, int n_head_kv, int head_dim, int64_t 
                                int64_t max_past) {
     const int rc = validate_attention_shape(n_head, n_head_kv, head_dim, n_tokens, max_past);
     if (rc) return rc;
-    // rows whose merge fits a grid
-    if (n_tokens > 1024 || n_seqs <= 0 || n_seqs > 65535 || n_seqs * n_tokens * n_head > ((int64_t)1 << 27))
-        return DCQ_ERR_BAD_SHAPE;
-    return DCQ_OK;
+    if (n_tokens > 1024 || n_seqs <= 0 || n_seqs > 65535) return DCQ_ERR_BAD_SHAPE;
+    // rows that the kernels count in 32 bits and whose merge, a thread for 4 elements, is below 2^32 threads
+    const int64_t rows = n_seqs * n_tokens * n_head;
+    return rows <= ((int64_t)1 << 27) && rows * head_dim < ((int64_t)1 << 34) ? DCQ_OK : DCQ_ERR_BAD_SHAPE;
 }
 
 size_t dcq_kv_tree_attention_workspace_size(int n_head, int n_head_kv, int head_dim, int64_t n_seqs,
@@ -749,6 +749,7 @@ int dcq_kv_tree_attention(int cache_type, const void* k_arena, const void* v_are
     if ((rc = validate_arena(cache_type, k_arena, n_blocks, n_layer, layer, row_elems))) return rc;
     if ((rc = validate_arena(cache_type, v_arena, n_blocks, n_layer, layer, row_elems))) return rc;
     if ((rc = validate_tables(tables, table_stride, n_table, n_seqs))) return rc;
+    if (!tree_fits(cache_type, head_dim, n_head, n_head_kv, (int)n_seqs, (int)n_tokens, (int)max_past)) return DCQ_ERR_BAD_SHAPE;
     if (!past || !q || !k_cur || !v_cur || !out) return DCQ_ERR_INVALID_ARG;
     if (!(scale == scale) || scale == INFINITY || scale == -INFINITY) return DCQ_ERR_INVALID_ARG;
     const size_t q_row = (size_t)n_head * head_dim * 4, kv_row = (size_t)row_elems * 4;
@@ -793,7 +794,7 @@ int dcq_kv_write_path(int cache_type, void* k_arena, void* v_arena, int64_t n_bl
     if ((rc = validate_arena(cache_type, v_arena, n_blocks, n_layer, 0, row_elems))) return rc;
     if ((rc = validate_tables(tables, table_stride, n_table, n_seqs))) return rc;
     if (n_layer > 65535 || n_tokens <= 0 || n_tokens > 65535 || max_path < 0 || max_path > 65535 ||
-        n_seqs * max_path > INT32_MAX)
+        n_seqs * max_path >= 1 << 24)  // a workgroup of 256 each, below 2^32 threads
         return DCQ_ERR_BAD_SHAPE;
     if (max_path == 0) return DCQ_OK;
     if (!past || !path || !k_cur || !v_cur) return DCQ_ERR_INVALID_ARG;
@@ -844,7 +845,8 @@ int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, 
     int rc = validate_pages(cache_type, k_arena, v_arena, n_blocks, n_layer, row_elems, tables, table_stride, n_table,
                             lengths, n_seqs, refs);
     if (rc) return rc;
-    if (n_children <= 0 || n_children > 4096) return DCQ_ERR_BAD_SHAPE;
+    const int64_t page = (int64_t)dcq_kv_slot_bytes(cache_type, row_elems) * DCQ_KV_BLOCK_SIZE * n_layer;
+    if (n_children <= 0 || n_children > 4096 || !copies_fit(n_children, page)) return DCQ_ERR_BAD_SHAPE;
     if (!parents || !tables_out || !lengths_out || !refs_out || !missing) return DCQ_ERR_INVALID_ARG;
     if (n_children > 1 && (tables_out_stride < n_table || tables_out_stride > INT32_MAX)) return DCQ_ERR_INVALID_ARG;
     if (!aligned(parents, 4) || !aligned(tables_out, 4) || !aligned(lengths_out, 4) || !aligned(refs_out, 4) ||
@@ -865,7 +867,6 @@ int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, 
     a.parents = parents, a.n_children = (int)n_children, a.refs = refs, a.n_blocks = (int)n_blocks;
     a.tables_out = tables_out, a.tables_out_stride = tables_out_stride, a.lengths_out = lengths_out;
     a.refs_out = refs_out, a.missing = missing;
-    const int64_t page = (int64_t)dcq_kv_slot_bytes(cache_type, row_elems) * DCQ_KV_BLOCK_SIZE * n_layer;
     return hip_status(launch_fork(a, k_arena, v_arena, page, workspace, (hipStream_t)stream));
 }
 
@@ -880,6 +881,8 @@ int dcq_kv_compact(int cache_type, void* k_arena, void* v_arena, int64_t n_block
     int rc = validate_pages(cache_type, k_arena, v_arena, n_blocks, n_layer, row_elems, tables, table_stride, n_table,
                             lengths, n_seqs, refs);
     if (rc) return rc;
+    const int64_t page = (int64_t)dcq_kv_slot_bytes(cache_type, row_elems) * DCQ_KV_BLOCK_SIZE * n_layer;
+    if (!copies_fit(n_blocks / 2, page)) return DCQ_ERR_BAD_SHAPE;
     if (!tables_out || !refs_out || !n_live) return DCQ_ERR_INVALID_ARG;
     if (n_seqs > 1 && (tables_out_stride < n_table || tables_out_stride > INT32_MAX)) return DCQ_ERR_INVALID_ARG;
     if (!aligned(tables_out, 4) || !aligned(refs_out, 4) || !aligned(n_live, 4)) return DCQ_ERR_MISALIGNED;
@@ -895,7 +898,6 @@ int dcq_kv_compact(int cache_type, void* k_arena, void* v_arena, int64_t n_block
     a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table, a.lengths = lengths, a.n_seqs = (int)n_seqs;
     a.refs = refs, a.n_blocks = (int)n_blocks, a.tables_out = tables_out, a.tables_out_stride = tables_out_stride;
     a.refs_out = refs_out, a.n_live = n_live;
-    const int64_t page = (int64_t)dcq_kv_slot_bytes(cache_type, row_elems) * DCQ_KV_BLOCK_SIZE * n_layer;
     return hip_status(launch_compact(a, k_arena, v_arena, page, workspace, (hipStream_t)stream));
 }
 

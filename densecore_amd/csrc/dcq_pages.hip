@@ -50,9 +50,7 @@ __global__ void __launch_bounds__(256) path_write_kernel(PathArgs a) {
 }
 
 hipError_t launch_path_write(const PathArgs& a, hipStream_t st) {
-    const int64_t wgs = (int64_t)a.n_seqs * a.max_path;
-    if (wgs > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(path_write_kernel, dim3((unsigned)wgs, (unsigned)a.n_layer, 2), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(path_write_kernel, dim3((unsigned)(a.n_seqs * a.max_path), (unsigned)a.n_layer, 2), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -124,22 +122,25 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(uint8_t* k_arena, uint8
                [&](int i) { return make_int2(plan[2 + 2 * i], plan[3 + 2 * i]); });
 }
 
+static int64_t copy_pieces(int64_t max_pages, int64_t page_bytes) {
+    return 2 * max_pages * ((page_bytes + kPiece - 1) / kPiece);
+}
+bool copies_fit(int64_t max_pages, int64_t page_bytes) { return copy_pieces(max_pages, page_bytes) <= INT32_MAX; }
+
 // Groups of 256 threads that copy up to max_pages pages while they make the plan themselves, one launch for all: as
 // many as pieces, at most eight per CU; 0 where there are more pieces and the plan has a launch before the copies'.
 // One launch | two, us a call: 4 beams of 28 layers x 1024 F16 12.2 | 15.3, 120 pages of 16 layers x 512 F16 11.1 |
 // 14.5; 128 beams of 36 layers x 1024 F16 52 | 50.5, 501 pages of 36 layers x 512 F32 114.4 | 113.7: 512 workgroups
 // then wait for their own plans with nothing in flight, and longer than one does.
 static int copies_beside_plan(int64_t max_pages, int64_t page_bytes) {
-    const int64_t pieces = 2 * max_pages * ((page_bytes + kPiece - 1) / kPiece);
+    const int64_t pieces = copy_pieces(max_pages, page_bytes);
     return pieces > 8 * (int64_t)cu_count() ? 0 : (int)std::max<int64_t>(pieces, 1);
 }
 
 // map: a compaction's tables and counts, in workgroups before the copying ones.
 static hipError_t launch_copy_pages(void* k_arena, void* v_arena, const int32_t* plan, int64_t max_pages,
                                     int64_t page_bytes, const CompactArgs* map, hipStream_t st) {
-    const int64_t pieces = 2 * max_pages * ((page_bytes + kPiece - 1) / kPiece);
-    if (pieces > INT32_MAX) return hipErrorInvalidValue;
-    const int wgs = (int)std::min<int64_t>(std::max<int64_t>(pieces, 1), 8 * (int64_t)cu_count());
+    const int wgs = (int)std::min<int64_t>(std::max<int64_t>(copy_pieces(max_pages, page_bytes), 1), 8 * (int64_t)cu_count());
     uint8_t *k = static_cast<uint8_t*>(k_arena), *v = static_cast<uint8_t*>(v_arena);
     if (map) {
         const int64_t items = (int64_t)map->n_seqs * map->n_table + map->n_blocks;

@@ -38,6 +38,8 @@ struct TreeArgs {
     int* ws_kps;   // keys per split, where the device chooses them
 };
 size_t tree_workspace_bytes(int hd, int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past);
+// Whether a launch holds the call's workgroups.
+bool tree_fits(int ct, int hd, int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past);
 hipError_t launch_tree_attention(int ct, int hd, TreeArgs a, void* ws, hipStream_t st);
 
 // dcq_pages.hip
@@ -61,6 +63,9 @@ struct PathArgs {
     int n_seqs, n_tokens;
 };
 hipError_t launch_path_write(const PathArgs& a, hipStream_t st);
+
+// Whether a launch counts the pieces of that many pages' copies.
+bool copies_fit(int64_t max_pages, int64_t page_bytes);
 
 struct ForkArgs {
     const int32_t* tables;

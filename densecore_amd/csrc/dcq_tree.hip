@@ -1474,17 +1474,34 @@ static void launch_tree_t(const TreeArgs& a, int block_waves, int wgs, hipStream
     hipLaunchKernelGGL((tree_attn_kernel<CT, HD, false>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
 }
 
+// A call's workgroups: of the shares of the cached keys, and of drafted keys alone.
+struct TreeGrid {
+    int64_t units, drafts, wgs;
+};
+static TreeGrid tree_grid(const TreePlan& p, int n_head, int n_head_kv, int n_seqs, int n_tokens) {
+    const int tiles16 = (n_tokens * (n_head / n_head_kv) + kTile - 1) / kTile;
+    TreeGrid g;
+    g.drafts = p.block_waves ? (int64_t)n_seqs * n_head_kv * tiles16 : 0;
+    g.units = p.block_waves ? p.units : (int64_t)n_seqs * p.splits * n_head_kv;
+    g.wgs = g.drafts + (g.units + 7) / 8 * 8 * p.tiles;
+    return g;
+}
+
+bool tree_fits(int ct, int hd, int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
+    const TreePlan p = tree_plan(ct, hd, n_head, n_head_kv, n_seqs, n_tokens, max_past);
+    const int threads = 64 * (p.block_waves ? p.block_waves : kTreeWaves);
+    return tree_grid(p, n_head, n_head_kv, n_seqs, n_tokens).wgs * threads <= UINT32_MAX;
+}
+
 hipError_t launch_tree_attention(int ct, int hd, TreeArgs a, void* ws, hipStream_t st) {
     const TreePlan p = tree_plan(ct, hd, a.n_head, a.n_head_kv, a.n_seqs, a.n_tokens, a.max_past);
     a.rep = a.n_head / a.n_head_kv;
     a.tiles = p.tiles, a.splits = p.splits, a.kps = p.kps;
     a.rows = (int64_t)a.n_seqs * a.n_tokens * a.n_head;
     a.tiles16 = (a.n_tokens * a.rep + kTile - 1) / kTile;
-    const int64_t drafts = p.block_waves ? (int64_t)a.n_seqs * a.n_head_kv * a.tiles16 : 0;
-    const int64_t units = p.block_waves ? p.units : (int64_t)a.n_seqs * p.splits * a.n_head_kv;
-    const int64_t wgs = drafts + (units + 7) / 8 * 8 * p.tiles;
-    if (wgs > INT32_MAX) return hipErrorInvalidValue;
-    a.units = (int)units, a.draft_wgs = (int)drafts, a.hist_wgs = (int)(wgs - drafts);
+    const TreeGrid g = tree_grid(p, a.n_head, a.n_head_kv, a.n_seqs, a.n_tokens);
+    const int wgs = (int)g.wgs;
+    a.units = (int)g.units, a.draft_wgs = (int)g.drafts, a.hist_wgs = (int)(g.wgs - g.drafts);
     a.share = p.share;
     if (p.splits > 1) {  // O, (m, l), and the keys per split where the device chooses them
         uint8_t* w = static_cast<uint8_t*>(ws);
@@ -1494,7 +1511,7 @@ hipError_t launch_tree_attention(int ct, int hd, TreeArgs a, void* ws, hipStream
     }
 #define DCQ_TREE_CASE(C, H)                                         \
     if (ct == C && hd == H) {                                       \
-        launch_tree_t<C, H>(a, p.block_waves, (int)wgs, st);        \
+        launch_tree_t<C, H>(a, p.block_waves, wgs, st);             \
     } else
     DCQ_TREE_CASE(kTypeQ8_0, 128)
     DCQ_TREE_CASE(kTypeQ8_0, 64)

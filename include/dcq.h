@@ -366,7 +366,10 @@ int dcq_kv_attention(int cache_type, const void* k_arena, const void* v_arena, i
  * count as 0. A cached position whose page is missing from the table, or outside [0, n_blocks), is a row of
  * zeros that is attended, as in dcq_kv_attention. A token that sees nothing, all of whose scores are
  * -infinity, or that is not drafted (j >= n_draft[b]) gets zeros. What a token does not see has no influence
- * on it, infinities and NaN included. head_dim 64, 128 or 256; n_tokens <= 1024; max_past <= 2^24.
+ * on it, infinities and NaN included. head_dim 64, 128 or 256; n_tokens <= 1024; n_seqs <= 65535;
+ * max_past <= 2^24; n_seqs * n_tokens * n_head <= 2^27 and times head_dim below 2^34; and no more (sequence, KV
+ * head, 16 rows of its tokens and query heads) than a launch has workgroups (2^24 - 1 of 256 threads;
+ * DCQ_ERR_BAD_SHAPE for all of these).
  * Precision: sums in fp32. F32 caches and drafted rows are multiplied in fp32. For F16 and Q8_0 caches the slots
  * are exact, the softmax weights have 22 bits or more, however small they are beside the row's largest, and q has
  * 22 bits or more of an element down to 2^-16 of the largest of its row, fewer below.
@@ -386,7 +389,7 @@ int dcq_kv_tree_attention(int cache_type, const void* k_arena, const void* v_are
  * position past[b] + j in the bytes of dcq_kv_write. Layers lie layer_stride_bytes apart, rows
  * kv_stride_bytes. A place whose token is outside 0 .. n_tokens - 1, or whose position is negative, past
  * the table or on a page outside [0, n_blocks), is skipped. Two places must not have one position (two
- * sequences share pages only before past[b]). */
+ * sequences share pages only before past[b]). n_seqs * max_path below 2^24. */
 int dcq_kv_write_path(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer,
                       int64_t row_elems, const int32_t* tables, int64_t table_stride, int64_t n_table,
                       const int32_t* past, const int32_t* path, int64_t path_stride, int64_t max_path,
@@ -402,7 +405,7 @@ int dcq_kv_write_path(int cache_type, void* k_arena, void* v_arena, int64_t n_bl
  * (refs_out <= 0; the lowest pages, in the order of the children). Where the free pages do not suffice, the
  * children that are left have -1 there, and *missing is their number (0 otherwise). tables_out
  * [n_children][n_table] has -1 past each child's pages. A child whose parent is outside 0 .. n_seqs - 1 is
- * empty; lengths count as 0 .. 16 * n_table. n_children <= 4096. */
+ * empty; lengths count as 0 .. 16 * n_table. n_children <= 4096, n_blocks <= 2^24. */
 size_t dcq_kv_fork_workspace_size(int64_t n_blocks, int64_t n_seqs, int64_t n_children);
 int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer, int64_t row_elems,
                 const int32_t* tables, int64_t table_stride, int64_t n_table, const int32_t* lengths, int64_t n_seqs,
@@ -414,7 +417,7 @@ int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, 
  * goes to the lowest free page below n_live, the next to the next, K and V of every layer; pages below
  * n_live stay. tables_out: the tables with the pages that the sequences hold renamed, other entries as they
  * are; refs_out: the counts in their new places, 0 where a page left. Every sequence that holds a page must
- * be in the tables. */
+ * be in the tables. n_blocks <= 2^24. */
 size_t dcq_kv_compact_workspace_size(int64_t n_blocks);
 int dcq_kv_compact(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer, int64_t row_elems,
                    const int32_t* tables, int64_t table_stride, int64_t n_table, const int32_t* lengths,

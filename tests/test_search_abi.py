@@ -126,6 +126,43 @@ def test_beam_select_refusals(kw, want):
     assert beam(**kw) == want
 
 
+GRIDS = [
+    # one workgroup of 256 threads per (sequence, KV head): 2^24 workgroups are 2^32 threads, one more than a launch has
+    (dict(seqs=65535, tokens=1, heads=257, kv=257), BAD_SHAPE), (dict(seqs=65535, tokens=1, heads=256, kv=256), None),
+    (dict(seqs=4096, tokens=1, heads=4096, kv=4096), BAD_SHAPE),
+    (dict(seqs=4096, tokens=1, heads=4096, kv=4096, max_past=100000, ct=F32), BAD_SHAPE),
+    (dict(seqs=65535, tokens=2, heads=512, kv=128), None), (dict(seqs=65535, tokens=9, heads=192, kv=48), None),
+    # blocks of rows: the workgroups of the drafted keys come on top
+    (dict(seqs=65535, tokens=17, heads=120, kv=120, max_past=1000), BAD_SHAPE),
+    (dict(seqs=20000, tokens=17, heads=120, kv=120, max_past=1000), None),
+    # the merge: a thread for four elements
+    (dict(seqs=16384, tokens=1024, heads=4, kv=1, hd=256, max_past=0), BAD_SHAPE),
+    (dict(seqs=16383, tokens=1024, heads=4, kv=1, hd=256, max_past=0), None),
+    (dict(seqs=16384, tokens=1024, heads=8, kv=1, hd=128, max_past=0), BAD_SHAPE),
+    (dict(seqs=16384, tokens=1024, heads=8, kv=1, hd=64, max_past=0), None),
+    (dict(seqs=16385, tokens=1024, heads=8, kv=1, hd=64, max_past=0), BAD_SHAPE),
+]
+
+
+@pytest.mark.parametrize("kw,want", GRIDS)
+def test_tree_attention_shapes_past_a_launch(kw, want):
+    """What no launch holds is refused as a shape, what one just holds goes on to the next check (addresses of 0)."""
+    assert tree(out=None, **kw) == (INVALID if want is None else want)
+
+
+@pytest.mark.parametrize("seqs,n,want", [(65535, 257, BAD_SHAPE), (16384, 1024, BAD_SHAPE), (65535, 256, None), (16383, 1024, None)])
+def test_write_path_shapes_past_a_launch(seqs, n, want):
+    assert path(seqs=seqs, n=n, ps=n, past=None) == (INVALID if want is None else want)
+
+
+def test_pages_past_a_launch():
+    """Copies in more pieces than a launch counts (arenas of many terabytes)."""
+    assert fork(blocks=8, layers=60000, elems=1 << 20, children=4096, ws=None) == BAD_SHAPE
+    assert fork(layers=36, elems=1024, children=4096, to=0x100000, lo=0x200000, parents=0x300000, ws=None) == WORKSPACE
+    assert compact(blocks=1 << 24, layers=36, elems=1 << 16, ws=None) == BAD_SHAPE
+    assert compact(blocks=1 << 24, layers=36, elems=1024, ws=None, refs=0x80000000, ro=0x90000000) == WORKSPACE
+
+
 def test_well_formed_calls_without_gpu_fail_loudly():
     if not no_gpu():
         pytest.skip("a GPU is present")
