@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <array>
+#include <initializer_list>
 #include <mutex>
 #include <stdlib.h>
 #include <string.h>
@@ -179,14 +180,38 @@ int validate_arena(int ct, const void* arena, int64_t n_blocks, int n_layer, int
     return DCQ_OK;
 }
 
-// Whether the byte ranges [a, a + an) and [b, b + bn) meet.
-bool overlap(const void* a, int64_t an, const void* b, int64_t bn) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return an > 0 && bn > 0 && x < y + (uintptr_t)bn && y < x + (uintptr_t)an;
+// An argument's bytes: rows of `width`, `stride` apart.
+struct Span {
+    uintptr_t at;
+    int64_t rows, stride, width;
+    Span(const void* p, int64_t bytes) : at((uintptr_t)p), rows(1), stride(bytes), width(bytes) {}
+    Span(const void* p, int64_t n, int64_t row_stride, int64_t row_width)
+        : at((uintptr_t)p), rows(n > 1 && row_stride > row_width ? n : 1), stride(row_stride),
+          width(rows > 1 ? row_width : (n - 1) * row_stride + row_width) {}
+    uintptr_t end() const { return at + (uintptr_t)((rows - 1) * stride + width); }
+};
+// Whether two spans share a byte. Rows of one stride may lie between each other's, as parts of wider rows; other
+// strides count as one range.
+bool overlap(const Span& a, const Span& b) {
+    if (a.width <= 0 || b.width <= 0 || a.at >= b.end() || b.at >= a.end()) return false;
+    if (a.rows == 1 || b.rows == 1 || a.stride != b.stride) return true;
+    const int64_t ahead = a.at <= b.at ? (int64_t)(b.at - a.at) % a.stride
+                                       : (a.stride - (int64_t)(a.at - b.at) % a.stride) % a.stride;
+    return ahead < a.width || ahead + b.width > a.stride;
+}
+// Whether one of `out` shares a byte with one of `in`.
+bool overlap(std::initializer_list<Span> out, std::initializer_list<Span> in) {
+    for (const Span* o = out.begin(); o != out.end(); ++o) {
+        for (const Span& i : in)
+            if (overlap(*o, i)) return true;
+    }
+    return false;
 }
 
-// int32 rows [n][width], `stride` entries apart: their extent in bytes.
-int64_t rows_bytes(int64_t n, int64_t stride, int64_t width) { return n > 0 ? ((n - 1) * stride + width) * 4 : 0; }
+// int32 rows [n][width], `stride` entries apart.
+Span int_rows(const void* p, int64_t n, int64_t stride, int64_t width) {
+    return width > 0 ? Span(p, n, n > 1 ? stride * 4 : 0, width * 4) : Span(p, 0);
+}
 
 // Block tables of several sequences.
 int validate_tables(const int32_t* tables, int64_t table_stride, int64_t n_table, int64_t n_seqs) {
@@ -761,12 +786,10 @@ int dcq_kv_tree_attention(int cache_type, const void* k_arena, const void* v_are
         return DCQ_ERR_MISALIGNED;
     if (q_stride_bytes % 16 || kv_stride_bytes % 16 || out_stride_bytes % 4) return DCQ_ERR_MISALIGNED;
     const int64_t rows = n_seqs * n_tokens;
-    const int64_t out_bytes = (rows - 1) * (int64_t)out_stride_bytes + (int64_t)q_row;
-    const int64_t kv_bytes = (rows - 1) * (int64_t)kv_stride_bytes + (int64_t)kv_row;
-    if (overlap(out, out_bytes, q, (rows - 1) * (int64_t)q_stride_bytes + (int64_t)q_row) ||
-        overlap(out, out_bytes, k_cur, kv_bytes) || overlap(out, out_bytes, v_cur, kv_bytes))
-        return DCQ_ERR_INVALID_ARG;
     const size_t need = tree_workspace_bytes(head_dim, n_head, n_head_kv, (int)n_seqs, (int)n_tokens, (int)max_past);
+    const Span out_rows(out, rows, (int64_t)out_stride_bytes, (int64_t)q_row), qs(q, rows, (int64_t)q_stride_bytes, (int64_t)q_row),
+        ks(k_cur, rows, (int64_t)kv_stride_bytes, (int64_t)kv_row), vs(v_cur, rows, (int64_t)kv_stride_bytes, (int64_t)kv_row);
+    if (overlap({out_rows}, {qs, ks, vs})) return DCQ_ERR_INVALID_ARG;
     if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
     if ((rc = check_device())) return rc;
     TreeArgs a{};
@@ -852,15 +875,12 @@ int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, 
     if (!aligned(parents, 4) || !aligned(tables_out, 4) || !aligned(lengths_out, 4) || !aligned(refs_out, 4) ||
         !aligned(missing, 4))
         return DCQ_ERR_MISALIGNED;
-    const struct { const void* p; int64_t n; } in[] = {{tables, rows_bytes(n_seqs, table_stride, n_table)},
-                                                       {lengths, n_seqs * 4}, {parents, n_children * 4},
-                                                       {refs, n_blocks * 4}},
-        out[] = {{tables_out, rows_bytes(n_children, tables_out_stride, n_table)}, {lengths_out, n_children * 4},
-                 {refs_out, n_blocks * 4}, {missing, 4}};
-    for (const auto& o : out)
-        for (const auto& i : in)
-            if (overlap(o.p, o.n, i.p, i.n)) return DCQ_ERR_INVALID_ARG;
-    if ((rc = validate_workspace(workspace, workspace_bytes, fork_workspace_bytes(n_blocks, n_children)))) return rc;
+    const Span ts = int_rows(tables, n_seqs, table_stride, n_table), ls(lengths, n_seqs * 4), ps(parents, n_children * 4),
+        rs(refs, n_blocks * 4), to = int_rows(tables_out, n_children, tables_out_stride, n_table),
+        lo(lengths_out, n_children * 4), ro(refs_out, n_blocks * 4), mo(missing, 4);
+    if (overlap({to, lo, ro, mo}, {ts, ls, ps, rs})) return DCQ_ERR_INVALID_ARG;
+    const size_t need = fork_workspace_bytes(n_blocks, n_children);
+    if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
     if ((rc = check_device())) return rc;
     ForkArgs a{};
     a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table, a.lengths = lengths, a.n_seqs = (int)n_seqs;
@@ -886,13 +906,11 @@ int dcq_kv_compact(int cache_type, void* k_arena, void* v_arena, int64_t n_block
     if (!tables_out || !refs_out || !n_live) return DCQ_ERR_INVALID_ARG;
     if (n_seqs > 1 && (tables_out_stride < n_table || tables_out_stride > INT32_MAX)) return DCQ_ERR_INVALID_ARG;
     if (!aligned(tables_out, 4) || !aligned(refs_out, 4) || !aligned(n_live, 4)) return DCQ_ERR_MISALIGNED;
-    const struct { const void* p; int64_t n; } in[] = {{tables, rows_bytes(n_seqs, table_stride, n_table)},
-                                                       {lengths, n_seqs * 4}, {refs, n_blocks * 4}},
-        out[] = {{tables_out, rows_bytes(n_seqs, tables_out_stride, n_table)}, {refs_out, n_blocks * 4}, {n_live, 4}};
-    for (const auto& o : out)
-        for (const auto& i : in)
-            if (overlap(o.p, o.n, i.p, i.n)) return DCQ_ERR_INVALID_ARG;
-    if ((rc = validate_workspace(workspace, workspace_bytes, compact_workspace_bytes(n_blocks)))) return rc;
+    const Span ts = int_rows(tables, n_seqs, table_stride, n_table), ls(lengths, n_seqs * 4), rs(refs, n_blocks * 4),
+        to = int_rows(tables_out, n_seqs, tables_out_stride, n_table), ro(refs_out, n_blocks * 4), no(n_live, 4);
+    if (overlap({to, ro, no}, {ts, ls, rs})) return DCQ_ERR_INVALID_ARG;
+    const size_t need = compact_workspace_bytes(n_blocks);
+    if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
     if ((rc = check_device())) return rc;
     CompactArgs a{};
     a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table, a.lengths = lengths, a.n_seqs = (int)n_seqs;
@@ -925,10 +943,10 @@ int dcq_beam_select(int type, const void* logits, size_t stride_bytes, int64_t n
     if (!aligned(logits, size) || stride_bytes % size || !aligned(beam_scores, 4) || !aligned(scores, 4) ||
         !aligned(parents, 4) || !aligned(tokens, 4))
         return DCQ_ERR_MISALIGNED;
-    const int64_t rows = n_batch * n_beams, x_bytes = (rows - 1) * (int64_t)stride_bytes + vocab * (int64_t)size;
-    for (const void* o : {(const void*)scores, (const void*)parents, (const void*)tokens})
-        if (overlap(o, n_batch * n_out * 4, logits, x_bytes) || overlap(o, n_batch * n_out * 4, beam_scores, rows * 4))
-            return DCQ_ERR_INVALID_ARG;
+    const int64_t rows = n_batch * n_beams, outs = n_batch * n_out * 4;
+    const Span xs(logits, rows, (int64_t)stride_bytes, vocab * (int64_t)size), bs(beam_scores, rows * 4), so(scores, outs),
+        po(parents, outs), to(tokens, outs);
+    if (overlap({so, po, to}, {xs, bs})) return DCQ_ERR_INVALID_ARG;
     const size_t need = beam_workspace_bytes(n_batch, n_beams, (int)vocab, n_out);
     if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
     if ((rc = check_device())) return rc;

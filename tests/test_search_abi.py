@@ -126,6 +126,32 @@ def test_beam_select_refusals(kw, want):
     assert beam(**kw) == want
 
 
+W = dict(max_past=100000, ws=None)  # a call that goes as far as the workspace's check
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(q=0x100000, qs=8192, out=0x100800, outs=8192, **W), WORKSPACE),   # outputs beside the queries in wider rows
+    (dict(q=0x100800, qs=8192, out=0x100000, outs=8192, **W), WORKSPACE),
+    (dict(q=0x100000, qs=8192, out=0x101800, outs=8192, **W), WORKSPACE),
+    (dict(q=0x100000, qs=8192, out=0x100000 + 6 * 8192, outs=8192, **W), WORKSPACE),
+    (dict(q=0x100000, qs=8192, out=0x1007fc, outs=8192, **W), INVALID),     # a row's last element
+    (dict(q=0x100000, qs=8192, out=0x101804, outs=8192, **W), INVALID),     # the next row's first one
+    (dict(q=0x101000, qs=8192, out=0x1007fc, outs=8192, **W), WORKSPACE),
+    (dict(q=0x101000, qs=8192, out=0x100804, outs=8192, **W), INVALID),
+    (dict(q=0x100000, qs=8192, out=0x100800, outs=4096, **W), INVALID),     # other strides
+])
+def test_tree_attention_overlaps(kw, want):
+    assert tree(**kw) == want
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(stride=8, to=0x3010, tos=8, ws=None), WORKSPACE),   # two tables in turn, in wider rows
+    (dict(stride=8, to=0x300c, tos=8, ws=None), INVALID), (dict(stride=8, to=0x3014, tos=8, ws=None), INVALID),
+])
+def test_fork_and_compact_tables_in_wider_rows(kw, want):
+    assert fork(**kw) == want and compact(**kw) == want
+
+
 GRIDS = [
     # one workgroup of 256 threads per (sequence, KV head): 2^24 workgroups are 2^32 threads, one more than a launch has
     (dict(seqs=65535, tokens=1, heads=257, kv=257), BAD_SHAPE), (dict(seqs=65535, tokens=1, heads=256, kv=256), None),
