@@ -199,11 +199,13 @@ bool overlap(const Span& a, const Span& b) {
                                        : (a.stride - (int64_t)(a.at - b.at) % a.stride) % a.stride;
     return ahead < a.width || ahead + b.width > a.stride;
 }
-// Whether one of `out` shares a byte with one of `in`.
+// Whether one of `out` shares a byte with one of `in` or another of `out`.
 bool overlap(std::initializer_list<Span> out, std::initializer_list<Span> in) {
     for (const Span* o = out.begin(); o != out.end(); ++o) {
         for (const Span& i : in)
             if (overlap(*o, i)) return true;
+        for (const Span* p = out.begin(); p != o; ++p)
+            if (overlap(*o, *p)) return true;
     }
     return false;
 }
@@ -788,9 +790,12 @@ int dcq_kv_tree_attention(int cache_type, const void* k_arena, const void* v_are
     const int64_t rows = n_seqs * n_tokens;
     const size_t need = tree_workspace_bytes(head_dim, n_head, n_head_kv, (int)n_seqs, (int)n_tokens, (int)max_past);
     const Span out_rows(out, rows, (int64_t)out_stride_bytes, (int64_t)q_row), qs(q, rows, (int64_t)q_stride_bytes, (int64_t)q_row),
-        ks(k_cur, rows, (int64_t)kv_stride_bytes, (int64_t)kv_row), vs(v_cur, rows, (int64_t)kv_stride_bytes, (int64_t)kv_row);
-    if (overlap({out_rows}, {qs, ks, vs})) return DCQ_ERR_INVALID_ARG;
+        ks(k_cur, rows, (int64_t)kv_stride_bytes, (int64_t)kv_row), vs(v_cur, rows, (int64_t)kv_stride_bytes, (int64_t)kv_row),
+        ts = int_rows(tables, n_seqs, table_stride, n_table), ps(past, n_seqs * 4), ds(n_draft, n_draft ? n_seqs * 4 : 0),
+        ms(mask, mask ? rows * ((n_tokens + 63) / 64) * 8 : 0);
+    if (overlap({out_rows}, {qs, ks, vs, ts, ps, ds, ms})) return DCQ_ERR_INVALID_ARG;
     if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
+    if (need && overlap({Span(workspace, (int64_t)need)}, {out_rows, qs, ks, vs, ts, ps, ds, ms})) return DCQ_ERR_INVALID_ARG;
     if ((rc = check_device())) return rc;
     TreeArgs a{};
     a.k_arena = static_cast<const uint8_t*>(k_arena), a.v_arena = static_cast<const uint8_t*>(v_arena);
@@ -881,6 +886,7 @@ int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, 
     if (overlap({to, lo, ro, mo}, {ts, ls, ps, rs})) return DCQ_ERR_INVALID_ARG;
     const size_t need = fork_workspace_bytes(n_blocks, n_children);
     if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
+    if (overlap({Span(workspace, (int64_t)need)}, {ts, ls, ps, rs, to, lo, ro, mo})) return DCQ_ERR_INVALID_ARG;
     if ((rc = check_device())) return rc;
     ForkArgs a{};
     a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table, a.lengths = lengths, a.n_seqs = (int)n_seqs;
@@ -911,6 +917,7 @@ int dcq_kv_compact(int cache_type, void* k_arena, void* v_arena, int64_t n_block
     if (overlap({to, ro, no}, {ts, ls, rs})) return DCQ_ERR_INVALID_ARG;
     const size_t need = compact_workspace_bytes(n_blocks);
     if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
+    if (overlap({Span(workspace, (int64_t)need)}, {ts, ls, rs, to, ro, no})) return DCQ_ERR_INVALID_ARG;
     if ((rc = check_device())) return rc;
     CompactArgs a{};
     a.tables = tables, a.table_stride = table_stride, a.n_table = (int)n_table, a.lengths = lengths, a.n_seqs = (int)n_seqs;
@@ -949,6 +956,7 @@ int dcq_beam_select(int type, const void* logits, size_t stride_bytes, int64_t n
     if (overlap({so, po, to}, {xs, bs})) return DCQ_ERR_INVALID_ARG;
     const size_t need = beam_workspace_bytes(n_batch, n_beams, (int)vocab, n_out);
     if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
+    if (overlap({Span(workspace, (int64_t)need)}, {xs, bs, so, po, to})) return DCQ_ERR_INVALID_ARG;
     if ((rc = check_device())) return rc;
     BeamArgs a{};
     a.x = logits, a.stride = (int64_t)(stride_bytes / size), a.n_beams = n_beams, a.vocab = (int)vocab;

@@ -355,7 +355,8 @@ int dcq_kv_attention(int cache_type, const void* k_arena, const void* v_arena, i
  * refs and the like are int32 device arrays, so that a step needs nothing back on the host. What a device
  * array holds out of its range is not an error (the host cannot see it): it is clamped or skipped as each
  * call says, and no access leaves the arrays. All results are the same from run to run. Layers, arenas,
- * types and alignment as above; no output may overlap an input. */
+ * types and alignment as above. No output or workspace may share a byte with an input or with another of them
+ * (DCQ_ERR_INVALID_ARG; rows of one stride may lie between each other's), nor with the arenas (not checked). */
 
 /* Attention of one layer for the drafted tokens of n_seqs sequences. Sequence b has past[b] cached positions
  * (below 0 counts as 0, above max_past as max_past) and n_draft[b] drafted tokens (clamped to 0 .. n_tokens;

@@ -152,6 +152,39 @@ def test_fork_and_compact_tables_in_wider_rows(kw, want):
     assert fork(**kw) == want and compact(**kw) == want
 
 
+@pytest.mark.parametrize("kw,want", [
+    (dict(out=0x3000, **W), INVALID), (dict(out=0x4004, **W), INVALID), (dict(out=0x6000, **W), INVALID),
+    (dict(max_past=100000, ws=0x400000), INVALID), (dict(max_past=100000, ws=0x100000), INVALID),
+    (dict(max_past=100000, ws=0x4000, wsb=1 << 26), INVALID),
+])
+def test_tree_attention_output_and_workspace_overlaps(kw, want):
+    assert tree(**kw) == want
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(lo=0x7000), INVALID), (dict(ro=0x8008), INVALID), (dict(missing=0x901c), INVALID), (dict(missing=0x7000), INVALID),
+    (dict(ws=0x7000), INVALID), (dict(ws=0x2f00), INVALID), (dict(ws=0x6000), INVALID), (dict(ws=0x8f00), INVALID),
+])
+def test_fork_overlaps(kw, want):
+    assert fork(**kw) == want
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(ro=0x7010), INVALID), (dict(live=0x9004), INVALID), (dict(live=0x7000), INVALID),
+    (dict(ws=0x7000), INVALID), (dict(ws=0x4000), INVALID), (dict(ws=0x8f00), INVALID),
+])
+def test_compact_overlaps(kw, want):
+    assert compact(**kw) == want
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(pa=0x20001c), INVALID), (dict(to=0x300000), INVALID), (dict(to=0x200000), INVALID), (dict(ws=0x200000), INVALID),
+    (dict(ws=0x1000), INVALID), (dict(ws=0x100000), INVALID), (dict(pa=0x200020, ws=None), WORKSPACE),
+])
+def test_beam_select_overlaps(kw, want):
+    assert beam(**kw) == want
+
+
 GRIDS = [
     # one workgroup of 256 threads per (sequence, KV head): 2^24 workgroups are 2^32 threads, one more than a launch has
     (dict(seqs=65535, tokens=1, heads=257, kv=257), BAD_SHAPE), (dict(seqs=65535, tokens=1, heads=256, kv=256), None),
