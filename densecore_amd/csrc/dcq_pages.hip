@@ -2,7 +2,8 @@
 // into their slots, forks of sequences, and compaction. All of it moves bytes; the plans are whole numbers.
 //
 // A page is block b of both arenas: n_layer * 16 slots in a row, a multiple of 16 bytes. refs[b] counts the
-// sequences (of this call or not) that hold page b; a page is free where refs[b] <= 0. Sequence i holds the
+// sequences (of this call or not) that hold page b; a page is free where refs[b] <= 0 and, in a fork, no child
+// holds it (counts that are too low must not make it the source and the target of copies). Sequence i holds the
 // first ceil(length / 16) entries of its table row; entries outside [0, n_blocks) hold nothing.
 //
 // Kernels:
@@ -178,11 +179,12 @@ __device__ __forceinline__ Scan block_scan(bool flag, int* counts /* kPlanWaves 
 // ---------------------------------------------------------------- forks
 // The counts: refs_out = refs - one for each page a sequence holds + one for each page a child takes over, and
 // the children's tables and lengths. The part of one (sequence or child, table entry). length_of(i): sequence i's,
-// 0 .. 16 n_table; parent_of(i): child i's, or -1; tail(i, page): the partial last page of child i. write: tables and
-// lengths.
-template <class Length, class Parent, class Add, class Tail>
-__device__ __forceinline__ void fork_count_entry(const ForkArgs& a, int row, int at, bool write, Length length_of,
-                                                 Parent parent_of, Add add, Tail tail) {
+// 0 .. 16 n_table; parent_of(i): child i's, or -1; tail(i, page): the partial last page of child i; users: see
+// fork_count_tail. write: tables and lengths.
+constexpr int kHeld = 1 << 30;
+template <class Length, class Parent, class Tail>
+__device__ __forceinline__ void fork_count_entry(const ForkArgs& a, int row, int at, bool write, int32_t* refs, int32_t* users,
+                                                 Length length_of, Parent parent_of, Tail tail) {
     const bool child = row >= a.n_seqs;
     const int i = child ? row - a.n_seqs : row, from = child ? parent_of(i) : i;
     const int length = from >= 0 ? length_of(from) : 0;
@@ -190,7 +192,8 @@ __device__ __forceinline__ void fork_count_entry(const ForkArgs& a, int row, int
     if (at < pages_of_length(length, a.n_table)) {
         page = a.tables[(int64_t)from * a.table_stride + at];
         const bool real = page >= 0 && page < a.n_blocks;
-        if (real) add(page, child ? 1 : -1);
+        if (real) atomicAdd(refs + page, child ? 1 : -1);
+        if (real && child) atomicOr(users + page, kHeld);
         if (child && real && at == length / kKvBlock) tail(i, page);
     }
     if (!child || !write) return;
@@ -205,7 +208,8 @@ __device__ __forceinline__ int fork_parent(const ForkArgs& a, int i) {
     return p >= 0 && p < a.n_seqs ? p : -1;
 }
 
-// Of a partial last page: the children that would write into it, and the first of them.
+// Of a partial last page: the children that would write into it (beside kHeld, of all pages that a child holds), and
+// the first of them.
 __device__ __forceinline__ void fork_count_tail(int32_t* users, int32_t* first, int child, int page) {
     atomicAdd(users + page, 1);
     atomicMin(first + page, child);
@@ -220,8 +224,8 @@ __global__ void __launch_bounds__(256) fork_count_kernel(ForkArgs a) {
     const int64_t entries = (int64_t)(a.n_seqs + a.n_children) * a.n_table;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256)
         fork_count_entry(
-            a, (int)(i / a.n_table), (int)(i % a.n_table), true, [&](int k) { return fork_length(a, k); },
-            [&](int k) { return fork_parent(a, k); }, [&](int page, int by) { atomicAdd(a.refs_out + page, by); },
+            a, (int)(i / a.n_table), (int)(i % a.n_table), true, a.refs_out, a.users,
+            [&](int k) { return fork_length(a, k); }, [&](int k) { return fork_parent(a, k); },
             [&](int k, int page) { fork_count_tail(a.users, a.first, k, page); });
 }
 
@@ -252,8 +256,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a, uin
         const int entries = (a.n_seqs + a.n_children) * a.n_table;
         for (int i = tid; i < entries; i += kPlanThreads)
             fork_count_entry(
-                a, i / a.n_table, i % a.n_table, lead, [&](int k) { return lengths[k]; },
-                [&](int k) { return parents[k]; }, [&](int page, int by) { atomicAdd(refs + page, by); },
+                a, i / a.n_table, i % a.n_table, lead, refs, users, [&](int k) { return lengths[k]; },
+                [&](int k) { return parents[k]; },
                 [&](int k, int page) {
                     tails[k] = page;
                     fork_count_tail(users, first, k, page);
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a, uin
     int copies = 0;
     for (int i0 = 0; i0 < a.n_children; i0 += kPlanThreads) {
         const int i = i0 + tid, tail = i < a.n_children ? tails[i] : -1;
-        const bool copy = tail >= 0 && !(first[tail] == i && refs[tail] == users[tail]);
+        const bool copy = tail >= 0 && !(first[tail] == i && refs[tail] == (users[tail] & ~kHeld));
         const Scan s = block_scan(copy, counts);
         if (i < a.n_children) ranks[i] = copy ? copies + s.before : -1;
         copies += s.total;
@@ -280,7 +284,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a, uin
     int found = 0;
     for (int i0 = 0; i0 < a.n_blocks && found < copies; i0 += kPlanThreads) {
         const int i = i0 + tid;
-        const bool free = i < a.n_blocks && refs[i] <= 0;
+        const bool free = i < a.n_blocks && refs[i] <= 0 && users[i] == 0;
         const Scan s = block_scan(free, counts);
         if (free && found + s.before < copies) fresh[found + s.before] = i;
         found += s.total;

@@ -403,10 +403,10 @@ int dcq_kv_write_path(int cache_type, void* k_arena, void* v_arena, int64_t n_bl
  * n_seqs sequences and with the n_children children. A last page that is not full would be written by all
  * who hold it, so it stays with the first child that has it, if no full page of a child and no sequence
  * beyond this call holds it; each other child gets a copy of it (every layer, K and V) on a free page
- * (refs_out <= 0; the lowest pages, in the order of the children). Where the free pages do not suffice, the
- * children that are left have -1 there, and *missing is their number (0 otherwise). tables_out
- * [n_children][n_table] has -1 past each child's pages. A child whose parent is outside 0 .. n_seqs - 1 is
- * empty; lengths count as 0 .. 16 * n_table. n_children <= 4096, n_blocks <= 2^24. */
+ * (refs_out <= 0 and held by no child; the lowest pages, in the order of the children). Where the free pages
+ * do not suffice, the children that are left have -1 there, and *missing is their number (0 otherwise).
+ * tables_out [n_children][n_table] has -1 past each child's pages. A child whose parent is outside
+ * 0 .. n_seqs - 1 is empty; lengths count as 0 .. 16 * n_table. n_children <= 4096, n_blocks <= 2^24. */
 size_t dcq_kv_fork_workspace_size(int64_t n_blocks, int64_t n_seqs, int64_t n_children);
 int dcq_kv_fork(int cache_type, void* k_arena, void* v_arena, int64_t n_blocks, int n_layer, int64_t row_elems,
                 const int32_t* tables, int64_t table_stride, int64_t n_table, const int32_t* lengths, int64_t n_seqs,

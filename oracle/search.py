@@ -88,7 +88,8 @@ def fork(tables, lengths, parents, refs):
     full = set()
     for t, n in zip(new, lens):
         full |= {p for p in t[:n // BLOCK] if 0 <= p < n_blocks}
-    free, kept, pairs, missing = [p for p in range(n_blocks) if refs[p] <= 0], set(), [], 0
+    held = {p for t, n in zip(new, lens) for p in _held(t, n, n_blocks)}
+    free, kept, pairs, missing = [p for p in range(n_blocks) if refs[p] <= 0 and p not in held], set(), [], 0
     for t, n in zip(new, lens):
         if n % BLOCK == 0 or not 0 <= t[-1] < n_blocks:
             continue

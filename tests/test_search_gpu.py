@@ -496,6 +496,21 @@ def test_fork_parents_lengths_and_holders_out_of_the_ordinary(dev):
     check_fork(cache, start, tables, [0, -5, 1 << 30, 64, 0, 0, 0], [0, 1, 2, 2, 3, 3], refs, dev)
 
 
+@pytest.mark.parametrize("n_blocks", [40, 20000])
+def test_fork_counts_that_are_too_low(dev, n_blocks):
+    """Pages that children hold though the counts say that nobody does are not taken as free: no page is the source
+    and the target of copies, and the counts are the same from run to run."""
+    tables = [[3, 0, 1, -1], [3, 0, 1, -1], [3, 5, 2, -1], [4, 6, 7, 8]]
+    lengths = [40, 40, 37, 60]
+    for low in (0, -1):
+        refs = np.full(n_blocks, 1, np.int64)
+        refs[[0, 1, 2, 3, 4, 5, 6, 7, 8, 11, 30, 31]] = low
+        for parents in ([0], [0, 0], [0, 2, 2, 3, 3], [3, 3, 3, 0, 2, 0], [2, 2, 2, 2]):
+            for _ in range(2):
+                cache, start = filled_cache(F16, n_blocks, 1, 1, 64, dev, 37)
+                check_fork(cache, start, tables, lengths, parents, refs, dev)
+
+
 def test_fork_then_fork_again_leaves_no_page_behind(dev):
     """A beam search's forks one after another, each with the last one's tables and counts."""
     rng = np.random.default_rng(33)
