@@ -282,6 +282,15 @@ def _new(shape, dtype, device, stream):
         return _torch.empty(shape, dtype=dtype, device=device)
 
 
+def _scratch(workspace):
+    """Address and size of a workspace (None: none). The library writes all of it, so it must be packed GPU memory."""
+    if workspace is None:
+        return None, 0
+    if not (getattr(workspace, "is_cuda", False) and workspace.is_contiguous()):
+        raise ValueError("workspace: must be a contiguous GPU tensor")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 def _made(name, t, dtype, shape, device, stream, rows=False):
     """An output of this type and shape: the caller's, checked, or a new one."""
     if t is None:
@@ -622,9 +631,10 @@ class PagedKVCache:
     # ---- search: several sequences per call, their block tables int32 [S, T] (rows may be strided)
     def _arenas(self):
         k, v, nbytes = self.k, self.v, self.n_blocks * self.n_layer * KV_BLOCK_SIZE * self.slot_bytes
-        if k.numel() < nbytes or v.numel() < nbytes:
-            raise ValueError(f"arenas of {k.numel()} and {v.numel()} bytes, {self.n_blocks} blocks need {nbytes}")
-        return k.data_ptr(), v.data_ptr()
+        (pk, nk), (pv, nv) = _scratch(k), _scratch(v)
+        if nk < nbytes or nv < nbytes:
+            raise ValueError(f"arenas of {nk} and {nv} bytes, {self.n_blocks} blocks need {nbytes}")
+        return pk, pv
 
     def tree_attention(self, layer, tables, past, max_past, q, k_cur, v_cur, scale, mask=None, n_draft=None, out=None,
                        workspace=None, stream=None):
@@ -668,7 +678,7 @@ class PagedKVCache:
             self.cache_type, k, v, self.n_blocks, self.n_layer, layer, tables.data_ptr(), table_stride, width,
             past.data_ptr(), max_past, _ptr(n_draft), _ptr(mask), n_head, self.n_head_kv, self.head_dim, q.data_ptr(),
             q_stride * 4, k_cur.data_ptr(), v_cur.data_ptr(), kv_stride * 4, s, n, scale, out.data_ptr(), out_stride * 4,
-            _ptr(workspace), _nbytes(workspace), _stream(stream))
+            *_scratch(workspace), _stream(stream))
         if status:
             raise DcqError("dcq_kv_tree_attention", status)
         return out
@@ -734,7 +744,7 @@ class PagedKVCache:
             self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, tables.data_ptr(), table_stride, width,
             lengths.data_ptr(), s, parents.data_ptr(), c, refs.data_ptr(), tables_out.data_ptr(),
             tables_out.stride(0) if c > 1 else width, lengths_out.data_ptr(), refs_out.data_ptr(), missing.data_ptr(),
-            workspace.data_ptr(), _nbytes(workspace), _stream(stream))
+            *_scratch(workspace), _stream(stream))
         if status:
             raise DcqError("dcq_kv_fork", status)
         return tables_out, lengths_out, refs_out, missing
@@ -759,7 +769,7 @@ class PagedKVCache:
         status = lib().dcq_kv_compact(
             self.cache_type, k, v, self.n_blocks, self.n_layer, self.row_elems, tables.data_ptr(), table_stride, width,
             lengths.data_ptr(), s, refs.data_ptr(), tables_out.data_ptr(), tables_out.stride(0) if s > 1 else width,
-            refs_out.data_ptr(), n_live.data_ptr(), workspace.data_ptr(), _nbytes(workspace), _stream(stream))
+            refs_out.data_ptr(), n_live.data_ptr(), *_scratch(workspace), _stream(stream))
         if status:
             raise DcqError("dcq_kv_compact", status)
         return tables_out, refs_out, n_live
@@ -807,8 +817,7 @@ def beam_select(logits, beam_scores, n_out, scores=None, parents=None, tokens=No
         workspace = _new(max(beam_select_workspace_size(b, w, vocab, n_out), 256), _U8, device, stream)
     status = lib().dcq_beam_select(
         1 if half else 0, logits.data_ptr(), stride * (2 if half else 4), b, w, vocab, beam_scores.data_ptr(), n_out,
-        scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), _nbytes(workspace),
-        _stream(stream))
+        scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), *_scratch(workspace), _stream(stream))
     if status:
         raise DcqError("dcq_beam_select", status)
     return scores, parents, tokens

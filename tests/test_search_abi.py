@@ -245,6 +245,34 @@ def test_binding_refuses_host_tensors_and_wrong_dtypes():
                       torch.zeros(4, dtype=torch.int32))
 
 
+def test_binding_refuses_memory_that_is_not_packed_on_the_gpu():
+    """A workspace or an arena in host memory, or one that has fewer bytes than elements."""
+    import torch
+    from densecore_amd import _lib
+    assert _lib._scratch(None) == (None, 0)
+    for ws in (torch.empty(4096, dtype=torch.uint8), 4096, [0] * 4096):
+        with pytest.raises(ValueError, match="contiguous GPU tensor"):
+            _lib._scratch(ws)
+
+    class Fake:  # what a GPU tensor answers, without a GPU
+        is_cuda = True
+
+        def __init__(self, t):
+            self.t = t
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+    with pytest.raises(ValueError, match="contiguous GPU tensor"):
+        _lib._scratch(Fake(torch.empty(1, dtype=torch.uint8).expand(1 << 20)))
+    assert _lib._scratch(Fake(torch.empty(100, dtype=torch.int32)))[1] == 400
+    cache = dc.PagedKVCache(F16, 4, 1, 2, 64, device="cpu")
+    with pytest.raises(ValueError, match="contiguous GPU tensor"):
+        cache._arenas()
+    cache.k, cache.v = Fake(cache.k), Fake(cache.v[:100])
+    with pytest.raises(ValueError, match="4 blocks need"):
+        cache._arenas()
+
+
 # ---------------------------------------------------------------- the oracle
 def test_oracle_tree_of_a_chain_is_causal_attention(O):
     from oracle import kv as KV
