@@ -242,7 +242,10 @@ def _u8(name, t, ndim=(1, 2)):
 def _plain(t, dtype, shape):
     """Whether t is a packed GPU tensor of this type and shape: the one test of a usual argument, where _checked
     takes the unusual ones (a call of the search functions has six to twelve tensors)."""
-    return t.dtype is dtype and t.is_cuda and t.shape == shape and t.is_contiguous()
+    try:
+        return t.dtype is dtype and t.is_cuda and t.shape == shape and t.is_contiguous()
+    except AttributeError:
+        return False
 
 
 def _checked(name, t, dtype, shape, rows=False):

@@ -245,6 +245,17 @@ def test_binding_refuses_host_tensors_and_wrong_dtypes():
                       torch.zeros(4, dtype=torch.int32))
 
 
+def test_binding_names_arguments_that_are_no_tensors():
+    from densecore_amd import _lib
+    _lib._t()
+    for value in ([3, 4], 7, None):
+        with pytest.raises(ValueError, match="past: expected a torch tensor"):
+            if not _lib._plain(value, _lib._I32, (2,)):
+                _lib._checked("past", value, _lib._I32, (2,))
+        with pytest.raises(ValueError, match="tables_out: expected a torch tensor" if value is not None else "tables"):
+            _lib._rows_of("tables_out" if value is not None else "tables", value, _lib._I32, (2, 2))
+
+
 def test_binding_refuses_memory_that_is_not_packed_on_the_gpu():
     """A workspace or an arena in host memory, or one that has fewer bytes than elements."""
     import torch
