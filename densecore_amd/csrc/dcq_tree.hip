@@ -560,10 +560,9 @@ __device__ __forceinline__ void tree_row_again(const TreeArgs& a, const TreeJob&
 }
 
 // A tile of 16 rows over a share of the keys, by a workgroup of W waves (HIST: cached keys too). EARLY: the first
-// drafted keys are loaded before all else and taken before the cached ones, whose loads are in flight meanwhile:
-// for calls without key splits, where a workgroup is a chain of latencies (7 tokens over 100 keys 11.1 -> 10.3 us,
-// one over one 9.5 -> 7.6). In larger calls their registers cost a wave per SIMD (16 sequences of 1000..4096 keys,
-// 16/4 heads x 128, F16 22.4 -> 26.0 us), at head_dim 256 they do not fit.
+// drafted keys are loaded before all else and taken before the cached ones, whose loads are in flight meanwhile
+// (on the device, 7 tokens over 100 keys 9.8 -> 9.4 us, one over one 8.0 -> 7.7, 16 sequences of 1000..4096 keys, 16/4
+// heads x 128, F16 20.8 -> 21.0). At head_dim 256 their registers do not fit.
 template <int CT, int HD, int W, bool HIST, bool EARLY>
 __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, TreeSmem<W>& sm) {
     constexpr int U = HD / 64, CK = tree_chunk<CT>(), NP = CK / kKvBlock;
@@ -852,7 +851,7 @@ __device__ __forceinline__ void tree_job(const TreeArgs& a, TreeJob& w, int seq)
 // instructions busy 27 %), and under many rows of F32 the fp32 matrix instructions and what a wave does between
 // them (256 rows over 4096 F32 keys, two sequences: 116 us, 58 of the 150 TFLOP/s of a large product; half the reads of
 // a key, by two tiles to a wave, 121).
-template <int CT, int HD, bool EARLY>
+template <int CT, int HD>
 __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_kernel(TreeArgs a) {
     __shared__ TreeSmem<kTreeWaves> sm;
     TreeJob w;
@@ -872,7 +871,7 @@ __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_
     if (w.slot >= n_split || (w.row0 >= w.n_rows && a.splits > 1)) return;  // the merge writes such rows' zeros
     w.k_end = w.row0 < w.n_rows ? min(w.past, w.k_begin + a.kps) : 0;
     w.drafts = w.slot == n_split - 1 && w.row0 < w.n_rows;
-    tree_tile<CT, HD, kTreeWaves, true, EARLY>(a, w, sm);
+    tree_tile<CT, HD, kTreeWaves, true, HD < 256>(a, w, sm);
 }
 
 // ---------------------------------------------------------------- many rows
@@ -1376,20 +1375,22 @@ static TreePlan tree_plan16(int n_head, int n_head_kv, int n_seqs, int n_tokens,
 }
 
 // The block kernel's rows share the keys that the 16-row kernel reads once per tile, but its workgroups need more of
-// both to be worth their start. From which number of rows on it is the faster (16-row kernel | block kernel, us;
+// both to be worth their start. From which number of rows on it is the faster (16-row kernel | block kernel, us a call;
 // 16/4 heads at head_dim 256, else 32/8):
-//   8 sequences of 1500..4096 keys, head_dim 128: 20 rows F16 40 | 27, Q8_0 55 | 33
-//   the same, head_dim 256: F16 20 rows 36 | 75, 64 rows 88 | 90, 80 rows 105 | 104, 128 rows 152 | 119;
-//                           Q8_0 32 rows 47 | 81, 48 rows 98 | 91, 128 rows 391 | 179
+//   8 sequences of 1500..4096 keys, head_dim 128: 16 rows F16 26 | 33, Q8_0 30 | 41; 20 rows 42 | 32, 61 | 44
+//   the same, head_dim 64: 64 rows F16 32 | 34, Q8_0 43 | 37; 80 rows 37 | 34, 50 | 39; 32 of 1000..2048 keys 64 rows
+//   59 | 61, 74 | 75; 80 rows 69 | 65, 91 | 81
+//   the same, head_dim 256: 80 rows F16 86 | 89, Q8_0 122 | 116; 96 rows 98 | 91, 144 | 119; 128 rows 110 | 97, 143 | 126;
+//   32 of 1000..2048 keys 96 rows 173 | 170, 241 | 222; one of 32768 96 rows 97 | 109, 135 | 137; 128 rows 119 | 115, 168 | 146
 //   one sequence of 4096 keys, where the block kernel's 256 keys per workgroup leave CUs without one: head_dim 128
-//   32 rows F16 14.4 | 14.8, Q8_0 20 rows 17.4 | 20.2, F16 64 rows 21.4 | 15.9; head_dim 256 F16 128 rows 43 | 48,
-//   Q8_0 64 rows 35 | 46
-//   fewer than 256 keys: never (8 sequences of 100..255 keys: 64 rows 19 | 22, 256 rows 37 | 43)
+//   32 rows F16 18 | 20, Q8_0 21 | 27; 40 rows 25 | 21, 29 | 28; head_dim 64 128 rows 19 | 23, 23 | 24; 256 rows 23 | 25,
+//   30 | 26; head_dim 256 192 rows 44 | 47, 55 | 64; 256 rows 48 | 50, 63 | 65
+//   fewer than 256 keys: never (8 sequences of 100..255 keys: 64 rows F16 18 | 24, Q8_0 22 | 30, 256 rows 37 | 36, 45 | 40)
 static bool tree_in_blocks(int ct, int hd, int n_head_kv, int n_seqs, int rows, int max_past) {
     if (ct == kTypeF32 || max_past < 256) return false;
-    const int from = hd < 256 ? 16 : ct == kTypeF16 ? 64 : 32;
+    const int from = hd == 128 ? 16 : hd == 64 ? 64 : ct == kTypeF16 ? 96 : 80;
     const bool idle = (int64_t)n_head_kv * n_seqs * ((max_past + 255) / 256) < cu_count();
-    return rows > (idle ? 2 * from : from);
+    return rows > (idle ? (hd == 128 ? 2 : 3) * from : from);
 }
 
 static TreePlan tree_plan(int ct, int hd, int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
@@ -1407,9 +1408,10 @@ static TreePlan tree_plan(int ct, int hd, int n_head, int n_head_kv, int n_seqs,
         kps = std::max<int64_t>(256, round_up(((int64_t)max_past * n_seqs + share - 1) / share, bk));
     };
     // Eight waves decode a Q8_0 block for twice the rows, four start and end sooner: eight for long shares of long
-    // histories. 256 rows x 128, four | eight: one sequence of 4096 keys 28 | 34, of 16384 (512 keys a share) 66 | 67,
-    // of 32768 116 | 112, of 65536 213 | 200, 64 dims 133 | 116; four of 16384 219 | 212, 16 of 4096 255 | 268.
-    // F16, which is not decoded: 16 of 500..2048 89 | 114, one of 4096 22 | 28, of 65536 143 | 142.
+    // histories. 256 rows x 128, four | eight, us a call: one sequence of 4096 keys 38 | 43, of 16384 (512 keys a share)
+    // 80 | 76, of 32768 131 | 121, of 65536 255 | 242, 64 dims 178 | 172; four of 16384 267 | 257, 16 of 4096 258 | 263.
+    // F16, which is not decoded, with one sum for both pieces of the weights: 16 of 500..2048 89 | 114, one of 4096
+    // 22 | 28, of 65536 143 | 142.
     if (ct == kTypeQ8_0 && rows > 128 && hd <= 128 && max_past >= 8192) plan_of(8);
     if (p.block_waves == 0 || kps < 1024) plan_of(4);
     // kps: keys of a split were all sequences as long as the longest; up to 64 sequences share out by their lengths,
@@ -1465,13 +1467,7 @@ static void launch_tree_t(const TreeArgs& a, int block_waves, int wgs, hipStream
             return;
         }
     }
-    if constexpr (HD < 256) {
-        if (a.splits == 1) {
-            hipLaunchKernelGGL((tree_attn_kernel<CT, HD, true>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
-            return;
-        }
-    }
-    hipLaunchKernelGGL((tree_attn_kernel<CT, HD, false>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
+    hipLaunchKernelGGL((tree_attn_kernel<CT, HD>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
 }
 
 // A call's workgroups: of the shares of the cached keys, and of drafted keys alone.

@@ -192,8 +192,8 @@ GRIDS = [
     (dict(seqs=4096, tokens=1, heads=4096, kv=4096, max_past=100000, ct=F32), BAD_SHAPE),
     (dict(seqs=65535, tokens=2, heads=512, kv=128), None), (dict(seqs=65535, tokens=9, heads=192, kv=48), None),
     # blocks of rows: the workgroups of the drafted keys come on top
-    (dict(seqs=65535, tokens=17, heads=120, kv=120, max_past=1000), BAD_SHAPE),
-    (dict(seqs=20000, tokens=17, heads=120, kv=120, max_past=1000), None),
+    (dict(seqs=65535, tokens=17, heads=120, kv=120, max_past=1000, hd=128), BAD_SHAPE),
+    (dict(seqs=20000, tokens=17, heads=120, kv=120, max_past=1000, hd=128), None),
     # the merge: a thread for four elements
     (dict(seqs=16384, tokens=1024, heads=4, kv=1, hd=256, max_past=0), BAD_SHAPE),
     (dict(seqs=16383, tokens=1024, heads=4, kv=1, hd=256, max_past=0), None),

@@ -321,6 +321,29 @@ def test_tree_attention_sinks(KV, dev, ct, n, hd, sink):
     planted(KV, ct, n, hd, s, [0], seed=hd + sink).run_and_check(dev)
 
 
+OTHER_WIDTHS = {
+    "random": lambda KV, dev, ct, hd: test_tree_attention(KV, dev, ct, 100, [700, 5, 333], 8, 2, hd),
+    "far above": lambda KV, dev, ct, hd: [
+        test_tree_attention_a_key_far_above_those_beside_it(KV, dev, ct, 100, hd, jump) for jump in (17, 24)],
+    "sinks": lambda KV, dev, ct, hd: [test_tree_attention_sinks(KV, dev, ct, 100, hd, sink) for sink in (24, 60)],
+    "hidden": lambda KV, dev, ct, hd: test_tree_attention_hidden_infinities_and_nan(KV, dev, ct, 100, 8, 2, hd, 777),
+    "cached": lambda KV, dev, ct, hd: ct != Q8_0 and test_tree_attention_infinities_in_the_cache(
+        KV, dev, ct, 100, 8, 2, hd, 600),
+    "wide": lambda KV, dev, ct, hd: test_tree_attention_wide_values(KV, dev, ct, 100, hd),
+    "missing pages": lambda KV, dev, ct, hd: test_tree_attention_missing_pages_are_zero_rows(KV, dev, ct, 100, hd, 900, 50),
+    "several": lambda KV, dev, ct, hd: test_tree_attention(KV, dev, ct, 40 if hd == 256 else 20, [2001, 1030] * 8, 8, 2, hd),
+}
+
+
+@pytest.mark.parametrize("ct", CACHE_TYPES)
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("what", OTHER_WIDTHS)
+def test_tree_attention_many_rows_at_other_widths(KV, dev, ct, hd, what):
+    """400 rows of a KV head, or 160 and 80 of several sequences: as many as share their keys through blocks at head_dim
+    64 and 256."""
+    OTHER_WIDTHS[what](KV, dev, ct, hd)
+
+
 def test_tree_attention_strided_rows_and_another_stream(KV, dev):
     """Rows of q, K / V, out and the tables inside wider tensors, on a stream other than the current one."""
     import torch
