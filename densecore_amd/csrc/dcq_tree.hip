@@ -560,9 +560,11 @@ __device__ __forceinline__ void tree_row_again(const TreeArgs& a, const TreeJob&
 }
 
 // A tile of 16 rows over a share of the keys, by a workgroup of W waves (HIST: cached keys too). EARLY: the first
-// drafted keys are loaded before all else and taken before the cached ones, whose loads are in flight meanwhile
-// (on the device, 7 tokens over 100 keys 9.8 -> 9.4 us, one over one 8.0 -> 7.7, 16 sequences of 1000..4096 keys, 16/4
-// heads x 128, F16 20.8 -> 21.0). At head_dim 256 their registers do not fit.
+// drafted keys are loaded before all else and taken before the cached ones, whose loads are in flight meanwhile:
+// for calls without key splits, where a workgroup is a chain of latencies (on the device, 7 tokens over 100 keys 9.8 ->
+// 9.4 us, one over one 8.0 -> 7.7). With splits few workgroups have drafted keys, and all pay for the registers (us a
+// call: 8 sequences of 1500..4096 keys, 16 rows x 128, F16 25.9 -> 26.6, 64 dims 19.6 -> 20.5; 256 rows over 4096 F32 keys of
+// two sequences 115 -> 139); at head_dim 256 they do not fit.
 template <int CT, int HD, int W, bool HIST, bool EARLY>
 __device__ __forceinline__ void tree_tile(const TreeArgs& a, const TreeJob& w, TreeSmem<W>& sm) {
     constexpr int U = HD / 64, CK = tree_chunk<CT>(), NP = CK / kKvBlock;
@@ -851,7 +853,7 @@ __device__ __forceinline__ void tree_job(const TreeArgs& a, TreeJob& w, int seq)
 // instructions busy 27 %), and under many rows of F32 the fp32 matrix instructions and what a wave does between
 // them (256 rows over 4096 F32 keys, two sequences: 116 us, 58 of the 150 TFLOP/s of a large product; half the reads of
 // a key, by two tiles to a wave, 121).
-template <int CT, int HD>
+template <int CT, int HD, bool EARLY>
 __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_kernel(TreeArgs a) {
     __shared__ TreeSmem<kTreeWaves> sm;
     TreeJob w;
@@ -871,7 +873,7 @@ __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_
     if (w.slot >= n_split || (w.row0 >= w.n_rows && a.splits > 1)) return;  // the merge writes such rows' zeros
     w.k_end = w.row0 < w.n_rows ? min(w.past, w.k_begin + a.kps) : 0;
     w.drafts = w.slot == n_split - 1 && w.row0 < w.n_rows;
-    tree_tile<CT, HD, kTreeWaves, true, HD < 256>(a, w, sm);
+    tree_tile<CT, HD, kTreeWaves, true, EARLY>(a, w, sm);
 }
 
 // ---------------------------------------------------------------- many rows
@@ -1467,7 +1469,13 @@ static void launch_tree_t(const TreeArgs& a, int block_waves, int wgs, hipStream
             return;
         }
     }
-    hipLaunchKernelGGL((tree_attn_kernel<CT, HD>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
+    if constexpr (HD < 256) {
+        if (a.splits == 1) {
+            hipLaunchKernelGGL((tree_attn_kernel<CT, HD, true>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((tree_attn_kernel<CT, HD, false>), dim3(wgs), dim3(64 * kTreeWaves), 0, st, a);
 }
 
 // A call's workgroups: of the shares of the cached keys, and of drafted keys alone.
