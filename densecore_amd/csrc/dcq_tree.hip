@@ -30,7 +30,7 @@
 // unit and one sum, weights had 22 bits from 2^-10 on and none from 2^-32; that took, us a call, 24 tokens of 8
 // sequences of 1500..4096 keys, 32/8 heads x 128, F16 44 where it now takes 48, 64 tokens over 32768 keys Q8_0
 // 124 | 128, F16 91 | 101, 8 sequences x 64 dims 29 | 35. A unit of each step's own for one sum needs a second pass in
-// every seventh step of such scores: 68, 185, 152, 49.
+// about every seventh step of such scores: 68, 185, 152, 49.
 // Infinities and NaN: what a 16-row tile shares can reach a row that does not see it, and an infinity in one
 // piece has no second piece. A row whose m, l or O is not finite is therefore computed again one key at a
 // time in fp32, of the keys it sees alone.
@@ -849,7 +849,7 @@ __device__ __forceinline__ void tree_job(const TreeArgs& a, TreeJob& w, int seq)
 // read the same keys; unit = (sequence, split, KV head).
 // Few keys: a chain of latencies, lengths and page numbers, K and V, the queries, then scores, softmax and products
 // once or twice, the waves' sums (7 tokens over 100 keys, 16/8 heads x 128 F16: 10 us, of which the memory is 0.4 MB).
-// Many: the keys' loads, one step ahead (37 beams over 301..1501 F32 keys, 8/1 x 256: 24.8 us, 69 MB, 2.8 TB/s; matrix
+// Many: the keys' loads, one step ahead (37 beams over 301..1501 F32 keys, 8/1 x 256: 24.6 us, 69 MB, 2.8 TB/s; matrix
 // instructions busy 27 %), and under many rows of F32 the fp32 matrix instructions and what a wave does between
 // them (256 rows over 4096 F32 keys, two sequences: 116 us, 58 of the 150 TFLOP/s of a large product; half the reads of
 // a key, by two tiles to a wave, 121).
@@ -878,9 +878,8 @@ __global__ void __launch_bounds__(64 * kTreeWaves, HD == 256 ? 2 : 1) tree_attn_
 
 // ---------------------------------------------------------------- many rows
 // Blocks of keys in LDS, two buffers of them, as f16 pieces. Q8_0: 8 W keys, decoded on the way into two pieces.
-// F16: 64 keys, by direct loads, in rows without padding; two halves of 32 give a wave products to issue while the
-// other half's weights are made (8 sequences of 1500..4096 keys, 96 rows x 128: 51 -> 49 us a call, against a ring of
-// four blocks of 32).
+// F16: 64 keys, by direct loads, in rows without padding (8 sequences of 1500..4096 keys, 96 rows x 128: 51 -> 49 us a
+// call, against a ring of four blocks of 32, when weights had one sum).
 template <int CT, int HD, int W>
 struct __align__(16) TreeBlock {
     static constexpr bool DMA = CT == kTypeF16;
@@ -943,7 +942,7 @@ struct TreeShare {
 // Up to 64 sequences share the units by their lengths, which the host does not know: the fewest keys per unit
 // (a.kps or more, in steps of an eighth) that a.share units suffice for. 8 sequences of 1500..4096 keys on 64
 // units: 384 keys, where their longest alone would ask for 512 and leave a quarter of the units without work;
-// 24 tokens of 32/8 heads x 128, F16: 40.7 -> 38.5 us. More sequences even out by themselves.
+// 24 tokens of 32/8 heads x 128, F16: 40.7 -> 38.5 us as it was taken. More sequences even out by themselves.
 __device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, int unit) {
     const int per_seq = a.splits - 1;
     if (!a.share) return {unit / per_seq, unit % per_seq, a.kps};
@@ -971,13 +970,13 @@ __device__ __forceinline__ TreeShare tree_share(const TreeArgs& a, int unit) {
 
 // 32 W rows of a KV head over a share of its cached keys (slots 1 ..), or 16 rows over the drafted keys (slot 0:
 // the workgroups from hist_wgs on, which fill the end of the launch).
-// A wave's block is a chain: 32 to 48 matrix instructions of scores, the softmax, as many of values; two waves a SIMD
-// cover each other's. 24 tokens of 8 sequences of 1500..4096 keys, 32/8 heads x 128, F16: 37 us; by a timeline 2 for
-// the share, 3 for the queries, 2 for the first block, 19 for 384 keys (3.1 a block of 64, 2.2 alone on a SIMD), 2 for
-// the results, and 5 of drafted keys at the end, in part beside the others. 64 tokens over 32768 keys, Q8_0: 112 us
-// for 34.4 GFLOP, three products each: 0.92 PFLOP/s of f16 where a large library product reaches 1.42; matrix
-// instructions busy 49 % of the cycles, VALU 28 %, the clock near 1.9 GHz. In it 90 us of the shares' loops, 8 before
-// and 10 for drafted keys after them.
+// A wave's block is a chain: 32 to 48 matrix instructions of scores, the softmax, as many of values and their sums into
+// O; two waves a SIMD cover each other's. 24 tokens of 8 sequences of 1500..4096 keys, 32/8 heads x 128, F16: 41 us; by
+// a timeline 2 for the share, 2.7 for the queries, 2 for the first block, 22 for 384 keys (3.7 a block of 64, 2.8 alone on
+// a SIMD), 2 for the results, and 6 of drafted keys at the end, in part beside the others. 64 tokens over 32768 keys,
+// Q8_0: 120 us for 34.4 GFLOP, three products each: 0.86 PFLOP/s of f16 where a large library product reaches 1.42; matrix
+// instructions busy 47 % of the cycles, VALU 36 %. In it 99 us of the shares' loops, 7 before and 6 for drafted keys after
+// them.
 template <int CT, int HD, int W>
 __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(TreeArgs a) {
     using Block = TreeBlock<CT, HD, W>;
@@ -1305,7 +1304,7 @@ __global__ void __launch_bounds__(64 * W, HD == 256 ? 1 : 2) tree_block_kernel(T
             tree_row_again<CT, HD, W>(a, w, sm.t, w.row0 + kRowsPerWave * k + __builtin_ctz(x));
 }
 
-// The merge of a sequence's splits (6144 rows x 128 of up to 12 splits: 7.8 us, 2048 of 33: 9.1; the partial results
+// The merge of a sequence's splits (6144 rows x 128 of up to 12 splits: 7.2 us, 2048 of 33: 9.3; the partial results
 // come from L2 at 4 to 5 TB/s): M = max m, L = sum l 2^(m - M), out = sum o 2^(m - M) / L, zeros for a row
 // that saw no key or has no drafted token. P lanes share 4 outputs, lane p the splits p, p + P, ...
 template <int HD, int P>
@@ -1365,8 +1364,9 @@ struct TreePlan {
 };
 
 // Key splits: workgroups until about three per CU have work, 128 keys (a step of each wave) at the least. Two, three,
-// five, six per CU, 16 sequences of 1000..4096 keys: F16, 16/4 heads x 128, 20.3, 19.9, 24.7, 24.0 us; F32, 8/2 x 256,
-// 42.9, 38.6, 49, 49.
+// four, five, six per CU, 16 sequences of 1000..4096 keys, us a call: F16, 16/4 heads x 128, 24.9, 23.8, 29.8, 29.8, 29.5;
+// x 64 17.4, 18.6, 20.8, 20.8, 21.6; 8/2 x 256 26.9, 27.1, 35.1, 35.2, 35.2; Q8_0 x 128 31, 27.2, 36.5, 36.6, 36.7; F32 x 256
+// 43.5, 39.4, 48.7, 48.6, 48.8.
 static TreePlan tree_plan16(int n_head, int n_head_kv, int n_seqs, int n_tokens, int max_past) {
     TreePlan p{};
     p.tiles = (n_tokens * (n_head / n_head_kv) + kTile - 1) / kTile;
