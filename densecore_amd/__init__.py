@@ -12,6 +12,8 @@ from .configs import (CONFIGS, TYPE_F16, TYPE_F32, TYPE_NAMES, TYPE_Q4_0, TYPE_Q
 from ._lib import (GGUF, KV_BLOCK_SIZE, PagedKVCache, kv_attention_workspace_size, kv_slot_bytes,  # noqa: F401
                    kv_compact_workspace_size, kv_fork_workspace_size, kv_tree_attention_workspace_size,
                    beam_select, beam_select_workspace_size,
+                   mul_mat_i8, mul_mat_i8_workspace_size, quantize_i8, rms_norm, rms_norm_i8,
+                   moe_down_i8, moe_down_i8_workspace_size, moe_gate_up_i8, moe_plan, moe_plan_size, moe_route,
                    DcqError, LIB_PATH, block_size, block_sums_per_row, build, dequantize_rows,  # noqa: F401
                    dot_rows, ffn_gate_up, ffn_gate_up_workspace_size, lib, mul_mat, mul_mat_add,
                    mul_mat_add_workspace_size, mul_mat_ex, mul_mat_noalloc, NOALLOC_SCRATCH_BYTES, probe_stream_read,
@@ -30,5 +32,6 @@ __all__ = [
     "TYPE_Q6_K", "TYPE_Q8_K", "TYPE_Q8_0_RS",
     "TYPE_NAMES", "KV_BLOCK_SIZE", "PagedKVCache", "kv_slot_bytes", "kv_attention_workspace_size",
     "kv_tree_attention_workspace_size", "kv_fork_workspace_size", "kv_compact_workspace_size", "beam_select",
-    "beam_select_workspace_size",
+    "beam_select_workspace_size", "quantize_i8", "rms_norm", "rms_norm_i8", "mul_mat_i8", "mul_mat_i8_workspace_size",
+    "moe_route", "moe_plan", "moe_plan_size", "moe_gate_up_i8", "moe_down_i8", "moe_down_i8_workspace_size",
 ]

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <array>
+#include <cmath>
 #include <initializer_list>
 #include <mutex>
 #include <stdlib.h>
@@ -13,6 +14,7 @@
 
 #include "../../include/dcq.h"
 #include "dcq_common.h"
+#include "dcq_i8.h"
 #include "dcq_kernels.h"
 #include "dcq_search.h"
 
@@ -98,7 +100,8 @@ int knob(Knob k) {
         "DCQ_Q4K_SHAPE",    "DCQ_Q4K_NW",  "DCQ_NO_FUSE",      "DCQ_Q6K_DECODE", "DCQ_Q6K_LDS_OFF",
         "DCQ_Q6K_NO_FUSE",  "DCQ_Q6K_FUSE_NW", "DCQ_Q8_SHAPE", "DCQ_GEMV_GENERIC", "DCQ_GEMV_LG",
         "DCQ_ATTN_NO_MFMA", "DCQ_Q6K_RPW", "DCQ_Q6K_MFMA",     "DCQ_SPLIT_K",    "DCQ_BATCH_MTI",
-        "DCQ_GEMM_MT",      "DCQ_GEMM_KQ",
+        "DCQ_GEMM_MT",      "DCQ_GEMM_KQ", "DCQ_I8_TILE",      "DCQ_I8_SPLIT",   "DCQ_I8_ROWS",
+        "DCQ_I8_EXPERTS",   "DCQ_I8_SHAPE",
     };
     static const std::array<int, (int)Knob::kCount> values = [] {
         std::array<int, (int)Knob::kCount> v{};
@@ -962,6 +965,234 @@ int dcq_beam_select(int type, const void* logits, size_t stride_bytes, int64_t n
     a.x = logits, a.stride = (int64_t)(stride_bytes / size), a.n_beams = n_beams, a.vocab = (int)vocab;
     a.beam = beam_scores, a.n_out = n_out, a.scores = scores, a.parents = parents, a.tokens = tokens;
     return hip_status(launch_beam_select(type, a, n_batch, workspace, (hipStream_t)stream));
+}
+
+// ---- layers in 8-bit integers
+static bool is_float_type(int t) { return t == DCQ_TYPE_F32 || t == DCQ_TYPE_F16; }
+static size_t float_size(int t) { return t == DCQ_TYPE_F32 ? 4 : 2; }
+// Rows of `width` bytes, `stride` apart: packed enough, and small enough for the kernels' 32-bit offsets.
+static int validate_rows(const void* p, size_t stride, int64_t width, size_t align) {
+    if (!p || stride < (size_t)width || stride > DCQ_I8_MAX_STRIDE) return DCQ_ERR_INVALID_ARG;
+    return aligned(p, align) && stride % align == 0 ? DCQ_OK : DCQ_ERR_MISALIGNED;
+}
+
+int dcq_rms_norm_i8(int type, const void* X, size_t x_stride_bytes, const float* R, size_t r_stride_bytes, float* H,
+                    size_t h_stride_bytes, const float* W, float eps, int64_t M, int64_t K, int8_t* Q,
+                    size_t q_stride_bytes, float* S, float* Y, size_t y_stride_bytes, void* stream) {
+    if (!is_float_type(type)) return DCQ_ERR_UNSUPPORTED;
+    if (M <= 0 || M >= DCQ_I8_MAX_NORM_ROWS || K <= 0 || K % 16 || K > DCQ_I8_MAX_K) return DCQ_ERR_BAD_SHAPE;
+    if (!W || (!Q && !Y) || !Q != !S || !R != !H) return DCQ_ERR_INVALID_ARG;
+    if (!(eps >= 0.0f) || eps == INFINITY) return DCQ_ERR_INVALID_ARG;
+    const int64_t size = (int64_t)float_size(type);
+    int rc = validate_rows(X, x_stride_bytes, K * size, 16);
+    if (rc) return rc;
+    if (R && ((rc = validate_rows(R, r_stride_bytes, K * 4, 16)) || (rc = validate_rows(H, h_stride_bytes, K * 4, 16)))) return rc;
+    if (Q && (rc = validate_rows(Q, q_stride_bytes, K, 16))) return rc;
+    if (Y && (rc = validate_rows(Y, y_stride_bytes, K * 4, 16))) return rc;
+    if (!aligned(W, 16) || !aligned(S, 4)) return DCQ_ERR_MISALIGNED;
+    const Span xs(X, M, (int64_t)x_stride_bytes, K * size), rs = R ? Span(R, M, (int64_t)r_stride_bytes, K * 4) : Span(R, 0),
+        hs = H ? Span(H, M, (int64_t)h_stride_bytes, K * 4) : Span(H, 0), ws(W, K * 4),
+        qs = Q ? Span(Q, M, (int64_t)q_stride_bytes, K) : Span(Q, 0), ss(S, S ? M * 4 : 0),
+        ys = Y ? Span(Y, M, (int64_t)y_stride_bytes, K * 4) : Span(Y, 0);
+    if (overlap({hs, qs, ss, ys}, {xs, ws})) return DCQ_ERR_INVALID_ARG;
+    const bool in_place = H == R && h_stride_bytes == r_stride_bytes;  // the residual stream updated where it is
+    if (overlap({qs, ss, ys}, {rs}) || (!in_place && overlap(hs, rs))) return DCQ_ERR_INVALID_ARG;
+    if ((rc = check_device())) return rc;
+    NormArgs a{};
+    a.x = X, a.x_stride = (int64_t)x_stride_bytes / size, a.r = R, a.r_stride = (int64_t)(r_stride_bytes / 4);
+    a.h = H, a.h_stride = (int64_t)(h_stride_bytes / 4), a.w = W, a.eps = eps, a.rows = M, a.width = (int)K;
+    a.q = Q, a.q_stride = (int64_t)q_stride_bytes, a.s = S, a.y = Y, a.y_stride = (int64_t)(y_stride_bytes / 4);
+    return hip_status(launch_norm_i8(type, a, (hipStream_t)stream));
+}
+
+int dcq_quantize_i8(int type, const void* X, int64_t M, int64_t K, size_t x_stride_bytes, int8_t* Q,
+                    size_t q_stride_bytes, float* S, void* stream) {
+    if (!is_float_type(type)) return DCQ_ERR_UNSUPPORTED;
+    if (M <= 0 || M >= DCQ_I8_MAX_NORM_ROWS || K <= 0 || K % 16 || K > DCQ_I8_MAX_K) return DCQ_ERR_BAD_SHAPE;
+    const int64_t size = (int64_t)float_size(type);
+    int rc = validate_rows(X, x_stride_bytes, K * size, 16);
+    if (rc) return rc;
+    if ((rc = validate_rows(Q, q_stride_bytes, K, 16))) return rc;
+    if (!S) return DCQ_ERR_INVALID_ARG;
+    if (!aligned(S, 4)) return DCQ_ERR_MISALIGNED;
+    if (overlap({Span(Q, M, (int64_t)q_stride_bytes, K), Span(S, M * 4)}, {Span(X, M, (int64_t)x_stride_bytes, K * size)}))
+        return DCQ_ERR_INVALID_ARG;
+    if ((rc = check_device())) return rc;
+    NormArgs a{};
+    a.x = X, a.x_stride = (int64_t)x_stride_bytes / size, a.rows = M, a.width = (int)K;
+    a.q = Q, a.q_stride = (int64_t)q_stride_bytes, a.s = S;
+    return hip_status(launch_norm_i8(type, a, (hipStream_t)stream));
+}
+
+static int validate_i8_shape(int64_t M, int64_t N, int64_t K) {
+    return M > 0 && N > 0 && K > 0 && K % 16 == 0 && K <= DCQ_I8_MAX_K && M <= DCQ_I8_MAX_ROWS && N <= DCQ_I8_MAX_ROWS
+               ? DCQ_OK
+               : DCQ_ERR_BAD_SHAPE;
+}
+
+size_t dcq_mul_mat_i8_workspace_size(int64_t M, int64_t N, int64_t K) {
+    return validate_i8_shape(M, N, K) ? 0 : i8_workspace_bytes(M, N, K);
+}
+
+int dcq_mul_mat_i8(const int8_t* W, const float* Ws, int64_t N, int64_t K, size_t w_stride_bytes, const int8_t* X,
+                   const float* Xs, int64_t M, size_t x_stride_bytes, const float* R, size_t r_stride_bytes, int ytype,
+                   void* Y, size_t y_stride_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!is_float_type(ytype)) return DCQ_ERR_UNSUPPORTED;
+    int rc = validate_i8_shape(M, N, K);
+    if (rc) return rc;
+    const int64_t size = (int64_t)float_size(ytype);
+    if ((rc = validate_rows(W, w_stride_bytes, K, 16)) || (rc = validate_rows(X, x_stride_bytes, K, 16)) ||
+        (rc = validate_rows(Y, y_stride_bytes, N * size, (size_t)size)))
+        return rc;
+    if (!Ws || !Xs) return DCQ_ERR_INVALID_ARG;
+    if (R && r_stride_bytes && (rc = validate_rows(R, r_stride_bytes, N * 4, 4))) return rc;
+    if (!aligned(Ws, 4) || !aligned(Xs, 4) || !aligned(R, 4)) return DCQ_ERR_MISALIGNED;
+    const Span w(W, N, (int64_t)w_stride_bytes, K), x(X, M, (int64_t)x_stride_bytes, K), wsp(Ws, N * 4), xsp(Xs, M * 4),
+        r = !R ? Span(R, 0) : r_stride_bytes ? Span(R, M, (int64_t)r_stride_bytes, N * 4) : Span(R, N * 4),
+        y(Y, M, (int64_t)y_stride_bytes, N * size);
+    const bool in_place = R == Y && ytype == DCQ_TYPE_F32 && r_stride_bytes == y_stride_bytes;
+    if (overlap({y}, {w, x, wsp, xsp}) || (!in_place && overlap(y, r))) return DCQ_ERR_INVALID_ARG;
+    const size_t need = i8_workspace_bytes(M, N, K);
+    if (workspace && need) {
+        if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
+        if (overlap({Span(workspace, (int64_t)need)}, {w, x, wsp, xsp, r, y})) return DCQ_ERR_INVALID_ARG;
+    }
+    if ((rc = check_device())) return rc;
+    I8Args a{};
+    a.x = X, a.xs = Xs, a.x_stride = (int64_t)x_stride_bytes, a.M = M;
+    a.w = W, a.ws = Ws, a.w_stride = (int64_t)w_stride_bytes, a.N = (int)N, a.K = (int)K;
+    a.R = R, a.r_stride = (int64_t)(r_stride_bytes / 4), a.y = Y, a.y_stride = (int64_t)y_stride_bytes / size;
+    return hip_status(launch_i8_product(ytype, a, workspace, workspace ? need : 0, (hipStream_t)stream));
+}
+
+int dcq_moe_route(int type, const void* logits, size_t stride_bytes, int64_t M, int n_expert, int scoring,
+                  const float* bias, int n_group, int topk_group, int group_best, int k, int renorm, float scale,
+                  int32_t* ids, float* weights, void* stream) {
+    if (!is_float_type(type) || (scoring != DCQ_MOE_SOFTMAX && scoring != DCQ_MOE_SIGMOID)) return DCQ_ERR_UNSUPPORTED;
+    if (M <= 0 || M > DCQ_I8_MAX_ROWS || n_expert <= 0 || n_expert > DCQ_MOE_MAX_EXPERTS || k <= 0 || k > 64 || k > n_expert)
+        return DCQ_ERR_BAD_SHAPE;
+    if (n_group <= 0 || n_group > 64 || n_expert % n_group || topk_group <= 0 || topk_group > n_group || group_best < 1 ||
+        group_best > 2)
+        return DCQ_ERR_BAD_SHAPE;
+    if (!(fabsf(scale) < INFINITY) || !ids || !weights) return DCQ_ERR_INVALID_ARG;
+    const int64_t size = (int64_t)float_size(type);
+    int rc = validate_rows(logits, stride_bytes, n_expert * size, (size_t)size);
+    if (rc) return rc;
+    if (!aligned(bias, 4) || !aligned(ids, 4) || !aligned(weights, 4)) return DCQ_ERR_MISALIGNED;
+    if (overlap({Span(ids, M * k * 4), Span(weights, M * k * 4)},
+                {Span(logits, M, (int64_t)stride_bytes, n_expert * size), Span(bias, bias ? n_expert * 4 : 0)}))
+        return DCQ_ERR_INVALID_ARG;
+    if ((rc = check_device())) return rc;
+    RouteArgs a{};
+    a.x = logits, a.stride = (int64_t)stride_bytes / size, a.rows = M, a.n_expert = n_expert, a.sigmoid = scoring == DCQ_MOE_SIGMOID;
+    a.bias = bias, a.n_group = n_group, a.topk_group = topk_group, a.group_best = group_best, a.k = k, a.renorm = renorm != 0;
+    a.scale = scale, a.ids = ids, a.weights = weights;
+    return hip_status(launch_moe_route(type, a, (hipStream_t)stream));
+}
+
+static int validate_plan(int64_t M, int k, int n_expert) {
+    return M > 0 && k > 0 && k <= DCQ_MOE_MAX_EXPERTS && n_expert > 0 && n_expert <= DCQ_MOE_MAX_EXPERTS && M <= DCQ_MOE_MAX_SLOTS / k
+               ? DCQ_OK
+               : DCQ_ERR_BAD_SHAPE;
+}
+static int64_t plan_bytes(int64_t M, int k, int n_expert) { return (plan_expert_at(n_expert, M * k) + M * k) * 4; }
+
+size_t dcq_moe_plan_size(int64_t M, int k, int n_expert) {
+    return validate_plan(M, k, n_expert) ? 0 : (size_t)plan_bytes(M, k, n_expert);
+}
+
+int dcq_moe_plan(const int32_t* ids, int64_t M, int k, int n_expert, void* plan, size_t plan_size, void* stream) {
+    int rc = validate_plan(M, k, n_expert);
+    if (rc) return rc;
+    if (!ids || !plan) return DCQ_ERR_INVALID_ARG;
+    if (plan_size < (size_t)plan_bytes(M, k, n_expert)) return DCQ_ERR_WORKSPACE;
+    if (!aligned(ids, 4) || !aligned(plan, 256)) return DCQ_ERR_MISALIGNED;
+    if (overlap(Span(plan, plan_bytes(M, k, n_expert)), Span(ids, M * k * 4))) return DCQ_ERR_INVALID_ARG;
+    if ((rc = check_device())) return rc;
+    return hip_status(launch_moe_plan(ids, M * k, n_expert, static_cast<int32_t*>(plan), (hipStream_t)stream));
+}
+
+// Arguments that the experts' products share. rows: of X, whose offsets the kernels count in 32 bits.
+static int validate_experts(const void* plan, size_t plan_size, int64_t M, int k, int n_expert, int64_t N, int64_t K,
+                            size_t w_stride, size_t expert_stride, const int8_t* X, const float* Xs, int64_t rows,
+                            size_t x_stride) {
+    int rc = validate_plan(M, k, n_expert);
+    if (rc) return rc;
+    if ((rc = validate_i8_shape(M * k, N, K))) return rc;
+    if (!plan || !Xs) return DCQ_ERR_INVALID_ARG;
+    if (plan_size < (size_t)plan_bytes(M, k, n_expert)) return DCQ_ERR_WORKSPACE;
+    if (expert_stride < w_stride * (size_t)(N - 1) + (size_t)K || expert_stride > ((size_t)1 << 40)) return DCQ_ERR_INVALID_ARG;
+    if (!aligned(plan, 256) || expert_stride % 16 || !aligned(Xs, 4)) return DCQ_ERR_MISALIGNED;
+    if ((rc = validate_rows(X, x_stride, K, 16))) return rc;
+    return (uint64_t)rows * x_stride < (1ull << 32) ? DCQ_OK : DCQ_ERR_BAD_SHAPE;
+}
+
+int dcq_moe_gate_up_i8(const void* plan, size_t plan_size, int64_t M, int k, int n_expert, const int8_t* Wg,
+                       const float* Wgs, const int8_t* Wu, const float* Wus, int64_t N, int64_t K, size_t w_stride_bytes,
+                       size_t expert_stride_bytes, const int8_t* X, const float* Xs, size_t x_stride_bytes, int htype, void* H,
+                       size_t h_stride_bytes, void* stream) {
+    if (!is_float_type(htype)) return DCQ_ERR_UNSUPPORTED;
+    int rc = validate_experts(plan, plan_size, M, k, n_expert, N, K, w_stride_bytes, expert_stride_bytes, X, Xs, M,
+                              x_stride_bytes);
+    if (rc) return rc;
+    const int64_t size = (int64_t)float_size(htype);
+    if ((rc = validate_rows(Wg, w_stride_bytes, K, 16)) || (rc = validate_rows(Wu, w_stride_bytes, K, 16)) ||
+        (rc = validate_rows(H, h_stride_bytes, N * size, (size_t)size)))
+        return rc;
+    if (!Wgs || !Wus) return DCQ_ERR_INVALID_ARG;
+    if (!aligned(Wgs, 4) || !aligned(Wus, 4)) return DCQ_ERR_MISALIGNED;
+    const int64_t w_bytes = (int64_t)expert_stride_bytes * (n_expert - 1) + (int64_t)w_stride_bytes * (N - 1) + K;
+    if (overlap({Span(H, M * k, (int64_t)h_stride_bytes, N * size)},
+                {Span(plan, plan_bytes(M, k, n_expert)), Span(Wg, w_bytes), Span(Wu, w_bytes), Span(Wgs, n_expert * N * 4),
+                 Span(Wus, n_expert * N * 4), Span(X, M, (int64_t)x_stride_bytes, K), Span(Xs, M * 4)}))
+        return DCQ_ERR_INVALID_ARG;
+    if ((rc = check_device())) return rc;
+    I8Args a{};
+    a.x = X, a.xs = Xs, a.x_stride = (int64_t)x_stride_bytes, a.M = M * k, a.w = Wg, a.ws = Wgs, a.w2 = Wu, a.ws2 = Wus;
+    a.w_stride = (int64_t)w_stride_bytes, a.w_expert = (int64_t)expert_stride_bytes, a.N = (int)N, a.K = (int)K;
+    a.y = H, a.y_stride = (int64_t)h_stride_bytes / size, a.plan = static_cast<const int32_t*>(plan), a.n_expert = n_expert, a.top = k;
+    return hip_status(launch_i8_experts(kI8Up, htype, a, (hipStream_t)stream));
+}
+
+size_t dcq_moe_down_i8_workspace_size(int64_t M, int k, int64_t N) {
+    if (validate_plan(M, k, 1) || N <= 0 || N > DCQ_I8_MAX_ROWS) return 0;
+    return (size_t)round_up(M * k * N * 4, 256);
+}
+
+int dcq_moe_down_i8(const void* plan, size_t plan_size, int64_t M, int k, int n_expert, const int8_t* W, const float* Ws,
+                    int64_t N, int64_t K, size_t w_stride_bytes, size_t expert_stride_bytes, const int8_t* Hq, const float* Hs,
+                    size_t h_stride_bytes, const float* weights, const float* R, size_t r_stride_bytes, int ytype, void* Y,
+                    size_t y_stride_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!is_float_type(ytype)) return DCQ_ERR_UNSUPPORTED;
+    int rc = validate_experts(plan, plan_size, M, k, n_expert, N, K, w_stride_bytes, expert_stride_bytes, Hq, Hs, M * k,
+                              h_stride_bytes);
+    if (rc) return rc;
+    const int64_t size = (int64_t)float_size(ytype);
+    if ((rc = validate_rows(W, w_stride_bytes, K, 16)) || (rc = validate_rows(Y, y_stride_bytes, N * size, (size_t)size))) return rc;
+    if (!Ws || !weights) return DCQ_ERR_INVALID_ARG;
+    if (R && (rc = validate_rows(R, r_stride_bytes, N * 4, 4))) return rc;
+    if (!aligned(Ws, 4) || !aligned(weights, 4)) return DCQ_ERR_MISALIGNED;
+    const int64_t w_bytes = (int64_t)expert_stride_bytes * (n_expert - 1) + (int64_t)w_stride_bytes * (N - 1) + K;
+    const Span ps(plan, plan_bytes(M, k, n_expert)), w(W, w_bytes), wsp(Ws, n_expert * N * 4),
+        h(Hq, M * k, (int64_t)h_stride_bytes, K), hsp(Hs, M * k * 4), g(weights, M * k * 4),
+        r = R ? Span(R, M, (int64_t)r_stride_bytes, N * 4) : Span(R, 0), y(Y, M, (int64_t)y_stride_bytes, N * size);
+    const bool in_place = R == Y && ytype == DCQ_TYPE_F32 && r_stride_bytes == y_stride_bytes;
+    if (overlap({y}, {ps, w, wsp, h, hsp, g}) || (!in_place && overlap(y, r))) return DCQ_ERR_INVALID_ARG;
+    const size_t need = dcq_moe_down_i8_workspace_size(M, k, N);
+    if ((rc = validate_workspace(workspace, workspace_bytes, need))) return rc;
+    if (overlap({Span(workspace, (int64_t)need)}, {ps, w, wsp, h, hsp, g, r, y})) return DCQ_ERR_INVALID_ARG;
+    if ((rc = check_device())) return rc;
+    I8Args a{};
+    a.x = Hq, a.xs = Hs, a.x_stride = (int64_t)h_stride_bytes, a.M = M * k, a.w = W, a.ws = Ws;
+    a.w_stride = (int64_t)w_stride_bytes, a.w_expert = (int64_t)expert_stride_bytes, a.N = (int)N, a.K = (int)K;
+    a.y = workspace, a.y_stride = N, a.plan = static_cast<const int32_t*>(plan), a.n_expert = n_expert, a.top = k;
+    const hipError_t e = launch_i8_experts(kI8Down, DCQ_TYPE_F32, a, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_status(e);
+    CombineArgs c{};
+    c.p = static_cast<const float*>(workspace), c.expert = a.plan + plan_expert_at(n_expert, M * k), c.weights = weights;
+    c.top = k, c.N = (int)N, c.rows = M, c.R = R, c.r_stride = (int64_t)(r_stride_bytes / 4);
+    c.y = Y, c.y_stride = (int64_t)y_stride_bytes / size;
+    return hip_status(launch_moe_combine(ytype, c, (hipStream_t)stream));
 }
 
 }  // extern "C"

@@ -439,6 +439,83 @@ int dcq_beam_select(int type, const void* logits, size_t stride_bytes, int64_t n
                     const float* beam_scores, int n_out, float* scores, int32_t* parents, int32_t* tokens,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Layers in 8-bit integers, dense and of experts ----
+ * No counterpart in the reference, whose quantized weights all have a scale for every 32 to 256 elements. Here a
+ * row of int8 has one fp32 scale: element k of row r stands for q[r][k] * s[r], for weights (a row per output) and
+ * for activations (a row per token). Sums over K are exact 32-bit integers, so that results do not depend on
+ * how a product is split, nor from run to run. Rows of int8 are 16-byte aligned, K a multiple of 16 up to DCQ_I8_MAX_K,
+ * strides up to DCQ_I8_MAX_STRIDE bytes. No output, plan or workspace may share a byte with an input or another of them
+ * (DCQ_ERR_INVALID_ARG; rows of one stride may lie between each other's), but where a call says so. Workspaces and plans are
+ * 256-byte aligned. A call whose tiles no launch holds (2^32 threads) is DCQ_ERR_BAD_SHAPE. */
+#define DCQ_I8_MAX_K 131056 /* 128 * 128 * K below 2^31 */
+#define DCQ_I8_MAX_STRIDE ((size_t)1 << 24)
+#define DCQ_I8_MAX_ROWS ((int64_t)1 << 22)
+#define DCQ_I8_MAX_NORM_ROWS ((int64_t)1 << 22)
+
+/* Rows to int8: s = max |x| / 127 rounded to fp32, q = x * (127 / max |x|) in 64 bits, each step rounded, then to the
+ * nearest integer, halves to even: -127 .. 127. An all-zero row has s = 0; a row that holds a NaN or an infinity has q = 0 and
+ * s = NaN, so that what is made of it is NaN. type: F32 or F16 rows, 16-byte aligned. For weights (N rows) and for
+ * activations that no norm precedes. */
+int dcq_quantize_i8(int type, const void* X, int64_t M, int64_t K, size_t x_stride_bytes, int8_t* Q,
+                    size_t q_stride_bytes, float* S, void* stream);
+
+/* The residual's addition, the RMS norm and the quantization of M rows: H = X + R (fp32; H may be R; without R, H is X and not
+ * written: both NULL), y = H * W / sqrt(mean H^2 + eps), and y as int8 rows Q with scales S (as dcq_quantize_i8, of the
+ * products H * W in 64 bits, which the norm's factor leaves in proportion: bytes do not depend on the order of a sum)
+ * and / or as fp32 rows Y for the products that take those (Q and S, or Y, may be NULL). Sums are in 64 bits. type: of X, F32 or
+ * F16; W fp32 [K]; all rows 16-byte aligned. A row that holds a NaN or an infinity has q = 0 and s = NaN. */
+int dcq_rms_norm_i8(int type, const void* X, size_t x_stride_bytes, const float* R, size_t r_stride_bytes, float* H,
+                    size_t h_stride_bytes, const float* W, float eps, int64_t M, int64_t K, int8_t* Q,
+                    size_t q_stride_bytes, float* S, float* Y, size_t y_stride_bytes, void* stream);
+
+/* Y[m][n] = (sum_k W[n][k] X[m][k]) * Ws[n] * Xs[m] (+ R[m][n]), rounded to fp32 after each operation and, with ytype F16,
+ * once more at the end. R fp32: rows r_stride_bytes apart (a residual; may be Y itself where Y is F32 with the
+ * same stride), or r_stride_bytes 0: one row for all (a bias); NULL: none. Without a workspace (NULL) few large rows run on
+ * fewer workgroups; the result is the same. */
+size_t dcq_mul_mat_i8_workspace_size(int64_t M, int64_t N, int64_t K);
+int dcq_mul_mat_i8(const int8_t* W, const float* Ws, int64_t N, int64_t K, size_t w_stride_bytes, const int8_t* X,
+                   const float* Xs, int64_t M, size_t x_stride_bytes, const float* R, size_t r_stride_bytes, int ytype,
+                   void* Y, size_t y_stride_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The k experts of each token, best first, and their weights. A token's scores are the softmax of its logits (F32 or F16,
+ * rows stride_bytes apart) or their sigmoid, in 64 bits. The choice goes by score + bias[e] (fp32, or NULL), ties to the
+ * lower expert. With n_group > 1 the experts are n_group runs of equal length, a group is worth its best choice
+ * (group_best 1) or the sum of its best two (2), and only the experts of the topk_group best groups (ties to the lower) are
+ * chosen from. weights are scale * score, without the bias; with renorm, divided by the sum of the k scores (all 0
+ * where that sum is). A logit of -infinity, or a bias that is not finite, rules an expert out; where fewer than k are
+ * left, or the token's logits hold a NaN or +infinity, the rest is -1 with weight 0. n_expert <= DCQ_MOE_MAX_EXPERTS,
+ * n_group <= 64, k <= 64. ids, weights [M][k]. */
+#define DCQ_MOE_SOFTMAX 0
+#define DCQ_MOE_SIGMOID 1
+#define DCQ_MOE_MAX_EXPERTS 512
+#define DCQ_MOE_MAX_SLOTS ((int64_t)1 << 22)
+int dcq_moe_route(int type, const void* logits, size_t stride_bytes, int64_t M, int n_expert, int scoring,
+                  const float* bias, int n_group, int topk_group, int group_best, int k, int renorm, float scale,
+                  int32_t* ids, float* weights, void* stream);
+
+/* The tokens' slots (slot = token * k + place, its expert ids[slot]) sorted by expert, for the two products below, which
+ * take the plan of the same M, k and n_expert. A slot whose id is outside 0 .. n_expert - 1 (padding) has no expert. One
+ * expert may have several of a token's slots. M * k <= DCQ_MOE_MAX_SLOTS. */
+size_t dcq_moe_plan_size(int64_t M, int k, int n_expert);
+int dcq_moe_plan(const int32_t* ids, int64_t M, int k, int n_expert, void* plan, size_t plan_size, void* stream);
+
+/* H[slot] = silu(Wg[e] x) * (Wu[e] x), silu(g) = g / (1 + e^-g), of each slot's expert e and its token's row x of X; zeros for
+ * slots of no expert. Wg, Wu: rows of K, w_stride_bytes apart, experts expert_stride_bytes apart; Wgs, Wus [n_expert][N].
+ * H: F32 or F16 (htype), M * k rows. M * x_stride_bytes below 4 GiB. */
+int dcq_moe_gate_up_i8(const void* plan, size_t plan_size, int64_t M, int k, int n_expert, const int8_t* Wg,
+                       const float* Wgs, const int8_t* Wu, const float* Wus, int64_t N, int64_t K, size_t w_stride_bytes,
+                       size_t expert_stride_bytes, const int8_t* X, const float* Xs, size_t x_stride_bytes, int htype, void* H,
+                       size_t h_stride_bytes, void* stream);
+
+/* Y[m] = R[m] + sum_j weights[m][j] * (W[e] h), over the token's slots in their order, h = row m * k + j of Hq (int8, scales
+ * Hs) and e its expert; slots of no expert add nothing, whatever their weight. R fp32 rows, or NULL; may be Y itself where Y is F32
+ * with the same stride. M * k * h_stride_bytes below 4 GiB. */
+size_t dcq_moe_down_i8_workspace_size(int64_t M, int k, int64_t N);
+int dcq_moe_down_i8(const void* plan, size_t plan_size, int64_t M, int k, int n_expert, const int8_t* W, const float* Ws,
+                    int64_t N, int64_t K, size_t w_stride_bytes, size_t expert_stride_bytes, const int8_t* Hq, const float* Hs,
+                    size_t h_stride_bytes, const float* weights, const float* R, size_t r_stride_bytes, int ytype, void* Y,
+                    size_t y_stride_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,350 @@
+"""Layers in 8-bit integers on the GPU against the 64-bit restatement (oracle/i8.py).
+
+Bounds, u = 2^-24 (half a step of fp32): an exact sum becomes a product by three roundings (the sum's, two scales'),
+so 3 u relative; a residual or bias adds one of the result. F16 outputs add half a step, 2^-11 relative or 2^-25.
+silu(g) u: g has 3 u, e^-g what |g| 3 u makes of it and 2 u of its own, the sum one and the quotient two more, so silu has
+(8 + 3 |g|) u, and with the other product (12 + 3 |g|) u. Below g = -88 e^-g is infinite in fp32 and the result -0, off by
+less than 1e-36 |u|. Weighted sums: 3 u of each term and one of each of the k + 1 additions, of the terms' magnitudes."""
+import math
+import zlib
+
+import numpy as np
+import pytest
+import torch
+
+import densecore_amd as dc
+from oracle import i8 as I
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def rng(*key):
+    return np.random.default_rng([zlib.crc32(k.encode()) if isinstance(k, str) else int(k) for k in key])
+
+
+def gpu(a, dev):
+    return torch.from_numpy(np.ascontiguousarray(a)).to(dev)
+
+
+def strided(a, dev, extra):
+    """The array on the GPU as the first columns of wider rows."""
+    wide = torch.zeros((*a.shape[:-1], a.shape[-1] + extra), dtype=torch.from_numpy(a).dtype, device=dev)
+    wide[..., :a.shape[-1]] = torch.from_numpy(a).to(dev)
+    return wide[..., :a.shape[-1]]
+
+
+def i8_rows(r, *shape):
+    q = r.integers(-127, 128, shape, dtype=np.int8)
+    return q, r.uniform(0.2, 1.5, shape[:-1]).astype(np.float32) * np.float32(0.01)
+
+
+def hidden(r, m, k, half):
+    x = r.standard_normal((m, k)).astype(np.float32)
+    x[:, r.integers(0, k, max(k // 50, 1))] *= 30
+    return x.astype(np.float16) if half else x
+
+
+# ---------------------------------------------------------------- rows to int8, norms
+WIDTHS = [16, 48, 512, 528, 1024, 2048, 2560, 4096, 4112, 8192, 9728, 16384, 16400, 40000]
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("k", WIDTHS)
+def test_quantize(dev, k, half):
+    r = rng("quantize", k, half)
+    x = hidden(r, 7, k, half)
+    q, s = dc.quantize_i8(gpu(x, dev))
+    qr, sr = I.quantize(x)
+    assert (q.cpu().numpy() == qr).all()
+    assert (s.cpu().numpy() == sr).all()
+
+
+def test_quantize_steps_halves_and_extremes(dev):
+    """Halves go to even, the largest is +-127, rows of tiny and huge values keep their steps."""
+    x = np.zeros((6, 32), np.float32)
+    x[0, :] = np.arange(32) - 16 + 0.5
+    x[0, 0] = 127.0
+    x[1, :] = 3.0e38
+    x[1, 1] = -1.5e38
+    x[2, :] = 1e-42  # below the normal range
+    x[2, 3] = -3e-42
+    x[3, 5] = -2.0
+    x[5, :] = np.float32(1.0) / 3
+    q, s = dc.quantize_i8(gpu(x, dev))
+    qr, sr = I.quantize(x)
+    assert (q.cpu().numpy() == qr).all() and (s.cpu().numpy() == sr).all()
+    assert q[0, 1].item() == -14 and q[0, 2].item() == -14 and s[4].item() == 0 and (q[4] == 0).all()
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("half", [False, True])
+def test_rows_that_are_not_finite_show_it(dev, value, half):
+    x = hidden(rng("bad", half), 5, 2560, half)
+    x[2, 1777] = value
+    q, s = dc.quantize_i8(gpu(x, dev))
+    assert math.isnan(s[2].item()) and (q[2] == 0).all()
+    qr, sr = I.quantize(x)
+    ok = [0, 1, 3, 4]
+    assert (q.cpu().numpy()[ok] == qr[ok]).all() and (s.cpu().numpy()[ok] == sr[ok]).all()
+    w = np.ones(2560, np.float32)
+    h, q, s = dc.rms_norm_i8(gpu(x, dev), gpu(w, dev), 1e-6, r=gpu(np.zeros((5, 2560), np.float32), dev))
+    assert math.isnan(s[2].item()) and (q[2] == 0).all() and not math.isfinite(h[2, 1777].item())
+    assert torch.isfinite(s[ok]).all()
+    y = dc.mul_mat_i8(q[:4].contiguous(), s[:4].nan_to_num(1.0), q, s)
+    assert torch.isnan(y[2]).all() and torch.isfinite(y[ok]).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("residual", ["none", "new", "in_place"])
+@pytest.mark.parametrize("m,k", [(1, 2560), (3, 16), (5, 528), (130, 4096), (2, 4112), (9, 8192), (3, 16400), (2, 40000)])
+def test_rms_norm(dev, m, k, residual, half):
+    r = rng("norm", m, k, residual, half)
+    x, w = hidden(r, m, k, half), (1 + 0.3 * r.standard_normal(k)).astype(np.float32)
+    res = None if residual == "none" else 3 * hidden(r, m, k, False)
+    rt = None if res is None else strided(res, dev, 16)
+    y = torch.empty((m, k), device=dev)
+    h, q, s = dc.rms_norm_i8(strided(x, dev, 8), gpu(w, dev), 1e-5, r=rt, h=rt if residual == "in_place" else None, y=y)
+    hr, qr, sr, yr = I.rms_norm(x, w, 1e-5, res)
+    if res is None:
+        assert h is None
+    else:
+        assert (h.cpu().numpy() == hr).all()
+        assert residual != "in_place" or h.data_ptr() == rt.data_ptr()
+    assert (q.cpu().numpy() == qr).all()
+    assert (np.abs(s.cpu().numpy() - sr) <= 1.001 * U * sr).all()
+    assert (np.abs(y.cpu().numpy() - yr) <= 1.001 * U * np.abs(yr) + 2.0 ** -149).all()
+    # the fp32 rows alone, and the int8 rows alone
+    _, y2 = dc.rms_norm(strided(x, dev, 8), gpu(w, dev), 1e-5, r=None if res is None else gpu(res, dev))
+    assert torch.equal(y, y2)
+
+
+def test_rms_norm_of_zeros_and_of_values_whose_squares_overflow(dev):
+    x = np.zeros((3, 2560), np.float32)
+    x[1] = 1e30 * rng("huge").standard_normal(2560)
+    x[2] = 1e-30 * rng("small").standard_normal(2560)
+    w = np.ones(2560, np.float32)
+    _, q, s = dc.rms_norm_i8(gpu(x, dev), gpu(w, dev), 1e-6)
+    _, qr, sr, _ = I.rms_norm(x, w, 1e-6)
+    assert (q.cpu().numpy() == qr).all() and (np.abs(s.cpu().numpy() - sr) <= 1.001 * U * sr).all()
+    assert s[0].item() == 0
+
+
+# ---------------------------------------------------------------- products
+SHAPES = [(1, 1, 16), (1, 9728, 2560), (1, 33, 131056), (3, 65, 272), (5, 1000, 768), (16, 17, 4096), (17, 300, 528), (31, 2560, 1024),
+          (33, 64, 2048), (48, 513, 1040), (61, 2560, 9728), (64, 129, 112), (65, 100, 256), (100, 2560, 1040), (128, 128, 128),
+          (129, 257, 400), (200, 1111, 3088), (256, 2048, 2048), (300, 5000, 656), (513, 770, 144), (700, 9728, 2560),
+          (1025, 4096, 2064), (2048, 8192, 2048), (4099, 1500, 272)]
+
+
+def check_product(y, w, ws, x, xs, r=None, half=False):
+    ref = I.mul_mat(w, ws, x, xs)
+    bound = 3.01 * U * np.abs(ref)
+    if r is not None:
+        ref = ref + r
+        bound += 1.01 * U * np.abs(ref)
+    if half:
+        bound += 2.0 ** -11 * np.abs(ref) * 1.01 + 2.0 ** -25
+    err = np.abs(y.double().cpu().numpy() - ref)
+    assert (err <= bound).all(), f"worst {np.max(err / np.maximum(bound, 1e-300))} of its bound"
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_mul_mat(dev, m, n, k):
+    r = rng("product", m, n, k)
+    w, ws = i8_rows(r, n, k)
+    x, xs = i8_rows(r, m, k)
+    y = dc.mul_mat_i8(gpu(w, dev), gpu(ws, dev), gpu(x, dev), gpu(xs, dev))
+    check_product(y, w, ws, x, xs)
+    # the same bits without a workspace, and again
+    none = torch.full((m, n), 7.0, device=dev)
+    t = [gpu(a, dev) for a in (w, ws, x, xs)]
+    status = dc.lib().dcq_mul_mat_i8(t[0].data_ptr(), t[1].data_ptr(), n, k, k, t[2].data_ptr(), t[3].data_ptr(), m, k, None, 0,
+                                     0, none.data_ptr(), 4 * n, None, 0, None)
+    torch.cuda.synchronize()
+    assert status == 0 and torch.equal(y, none)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("add", ["none", "residual", "bias", "in_place"])
+@pytest.mark.parametrize("m,n,k", [(1, 100, 2560), (13, 257, 272), (61, 512, 4096), (70, 130, 2064), (600, 1029, 656)])
+def test_mul_mat_of_strided_rows_with_an_addend(dev, m, n, k, add, half):
+    if add == "in_place" and half:
+        pytest.skip("R is fp32")
+    r = rng("added", m, n, k, add, half)
+    w, ws = i8_rows(r, n, k)
+    x, xs = i8_rows(r, m, k)
+    res = None if add == "none" else r.standard_normal(n if add == "bias" else (m, n)).astype(np.float32)
+    y = torch.full((m, n + 5), 7.0, dtype=torch.float16 if half else torch.float32, device=dev)
+    if add == "in_place":
+        y[:, :n] = gpu(res, dev)
+    rt = None if add == "none" else y[:, :n] if add == "in_place" else gpu(res, dev) if add == "bias" else strided(res, dev, 3)
+    out = dc.mul_mat_i8(strided(w, dev, 32), gpu(ws, dev), strided(x, dev, 16), gpu(xs, dev), r=rt, y=y[:, :n])
+    assert out.data_ptr() == y.data_ptr()
+    check_product(out, w, ws, x, xs, res, half)
+    assert (y[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_mul_mat_sums_of_the_largest_values_are_exact(dev, m):
+    k, n = 131056, 40
+    w, x = np.full((n, k), -128, np.int8), np.full((m, k), -128, np.int8)
+    w[1] = 127
+    one = np.ones(max(m, n), np.float32)
+    y = dc.mul_mat_i8(gpu(w, dev), gpu(one[:n], dev), gpu(x, dev), gpu(one[:m], dev))
+    assert (y[:, 0] == 128.0 * 128 * k).all() and (y[:, 1] == float(np.float32(-128.0 * 127 * k))).all()
+
+
+# ---------------------------------------------------------------- the router
+def check_route(dev, logits, k, **kw):
+    bias = kw.get("bias")
+    got = dc.moe_route(gpu(logits, dev), k, **{**kw, **({} if bias is None else {"bias": gpu(bias, dev)})})
+    ids, weights = (t.cpu().numpy() for t in got)
+    ri, rw = I.route(logits, k, **kw)
+    assert (ids == ri).all(), f"{(ids != ri).sum()} of {ids.size} differ"
+    assert (np.abs(weights - rw) <= 1.001 * U * np.abs(rw) + 2.0 ** -149).all()
+    return ids, weights
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("m,e,k,groups,kept,best", [(1, 1, 1, 1, 1, 1), (5, 128, 8, 1, 1, 1), (33, 60, 4, 1, 1, 1), (70, 256, 8, 8, 4, 2),
+                                                    (9, 160, 6, 8, 3, 1), (17, 512, 10, 1, 1, 1), (4, 64, 64, 64, 64, 2),
+                                                    (40, 384, 6, 4, 2, 2), (3, 300, 33, 2, 1, 1)])
+def test_route(dev, m, e, k, groups, kept, best, scoring, half):
+    r = rng("route", m, e, k, scoring, half)
+    x = (2 * r.standard_normal((m, e))).astype(np.float16 if half else np.float32)
+    for bias in (None, (0.2 * r.standard_normal(e)).astype(np.float32)):
+        for renorm in (True, False):
+            check_route(dev, x, k, scoring=scoring, bias=bias, n_group=groups, topk_group=kept, group_best=best, renorm=renorm,
+                        scale=2.5 if renorm else 1.0)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_ties_go_to_the_lower_expert(dev, scoring):
+    x = np.zeros((4, 200), np.float32)
+    x[1, 1::2] = 1
+    x[2] = rng("ties").integers(0, 3, 200)
+    x[3] = np.repeat(rng("ties", 1).integers(0, 4, 8), 25)
+    for groups in (1, 8):
+        check_route(dev, x, 9, scoring=scoring, n_group=groups, topk_group=max(groups // 2, 1), group_best=2)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_without_enough_experts(dev, scoring):
+    """-infinity and biases that are not finite rule experts out; NaN and +infinity leave a token without any."""
+    r = rng("few")
+    x = r.standard_normal((9, 96)).astype(np.float32)
+    x[0, 5:] = -np.inf
+    x[1, :] = -np.inf
+    x[2, 17] = np.nan
+    x[3, 80] = np.inf
+    x[4, :48] = -np.inf
+    x[5, :] = np.finfo(np.float32).min
+    x[6, :] = -3e4
+    x[7, 3] = 3e38
+    bias = r.standard_normal(96).astype(np.float32)
+    check_route(dev, x, 8, scoring=scoring)
+    check_route(dev, x, 8, scoring=scoring, n_group=6, topk_group=2, group_best=2)
+    bias[[2, 3]] = np.inf, np.nan
+    bias[10:16] = -np.inf
+    ids, w = check_route(dev, x, 8, scoring=scoring, bias=bias, n_group=6, topk_group=2, group_best=2)
+    assert not np.isin(ids, [2, 3, 10, 11, 12, 13, 14, 15]).any() and (ids[1:4] == -1).all() and (w[1:4] == 0).all()
+
+
+def test_route_of_strided_rows(dev):
+    x = rng("strided").standard_normal((21, 100)).astype(np.float32)
+    ids, weights = dc.moe_route(strided(x, dev, 7), 5)
+    ri, rw = I.route(x, 5)
+    assert (ids.cpu().numpy() == ri).all() and np.allclose(weights.cpu().numpy(), rw, rtol=2 * U, atol=0)
+
+
+# ---------------------------------------------------------------- experts
+def experts(r, e, n, k):
+    return i8_rows(r, e, n, k)
+
+
+def some_ids(r, m, e, k, kind):
+    if kind == "one":  # all tokens to the same experts
+        return np.tile(r.permutation(e)[:k].astype(np.int32), (m, 1))
+    if kind == "twice":  # one expert several times in a token
+        return np.repeat(r.integers(0, e, (m, 1)), k, 1).astype(np.int32)
+    ids = np.stack([r.permutation(e)[:k] for _ in range(m)]).astype(np.int32)
+    if kind == "padded":
+        ids[m // 2:] = -1
+        ids[0, 0] = e
+        ids[m // 4, -1] = -7
+        ids[m // 3, 0] = 2 ** 31 - 1
+    if kind == "none":
+        ids[:] = -1
+    return ids
+
+
+EXPERTS = [(1, 8, 2, 64, 64, "mixed"), (5, 128, 8, 768, 2048, "mixed"), (1, 1, 1, 17, 16, "mixed"), (7, 16, 3, 100, 272, "padded"),
+           (40, 4, 2, 130, 528, "padded"), (33, 8, 4, 65, 144, "one"), (20, 512, 6, 40, 80, "mixed"), (16, 3, 3, 48, 1040, "twice"),
+           (9, 8, 2, 33, 64, "none"), (64, 16, 4, 96, 256, "mixed"), (150, 4, 2, 200, 400, "padded"), (300, 2, 2, 257, 144, "mixed"),
+           (513, 8, 1, 64, 128, "mixed"), (700, 60, 4, 80, 160, "padded"), (1000, 3, 2, 300, 272, "mixed"), (260, 2, 2, 128, 2064, "one")]
+
+
+@pytest.mark.parametrize("m,e,k,n,width,kind", EXPERTS)
+def test_gate_up(dev, m, e, k, n, width, kind):
+    r = rng("up", m, e, k, n, width)
+    wg, wgs = experts(r, e, n, width)
+    wu, wus = experts(r, e, n, width)
+    x, xs = i8_rows(r, m, width)
+    ids = some_ids(r, m, e, k, kind)
+    h = torch.full((m * k, n + 3), 7.0, device=dev)
+    plan = dc.moe_plan(gpu(ids, dev), e)
+    args = (plan, gpu(wg, dev), gpu(wgs, dev), gpu(wu, dev), gpu(wus, dev), gpu(x, dev), gpu(xs, dev), k)
+    dc.moe_gate_up_i8(*args, h=h[:, :n])
+    ref, gate, up = I.gate_up(ids, e, wg, wgs, wu, wus, x, xs)
+    bound = (12.1 + 3.01 * np.abs(gate)) * U * np.abs(ref) + 1e-36 * np.abs(up)
+    got = h[:, :n].double().cpu().numpy()
+    assert (np.abs(got - ref) <= bound).all()
+    assert (h[:, n:] == 7).all()
+    half = dc.moe_gate_up_i8(*args, dtype=torch.float16).double().cpu().numpy()
+    lim = np.abs(ref) < 65000
+    assert (np.abs(half - ref) <= bound + 2.0 ** -11 * 1.01 * np.abs(ref) + 2.0 ** -25)[lim].all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("residual", ["none", "new", "in_place"])
+@pytest.mark.parametrize("m,e,k,n,width,kind", EXPERTS)
+def test_down(dev, m, e, k, n, width, kind, residual, half):
+    if residual == "in_place" and half:
+        pytest.skip("R is fp32")
+    r = rng("down", m, e, k, n, width, residual)
+    w, ws = experts(r, e, n, width)
+    h, hs = i8_rows(r, m * k, width)
+    ids = some_ids(r, m, e, k, kind)
+    weights = r.uniform(0, 1, (m, k)).astype(np.float32)
+    weights[ids < 0] = np.nan  # what is there for padding does not count
+    hs[ids.reshape(-1) < 0] = np.nan
+    res = None if residual == "none" else r.standard_normal((m, n)).astype(np.float32)
+    y = torch.full((m, n + 3), 7.0, dtype=torch.float16 if half else torch.float32, device=dev)
+    rt = None if res is None else gpu(res, dev)
+    if residual == "in_place":
+        y[:, :n] = rt
+        rt = y[:, :n]
+    plan = dc.moe_plan(gpu(ids, dev), e)
+    dc.moe_down_i8(plan, gpu(w, dev), gpu(ws, dev), gpu(h, dev), gpu(hs, dev), gpu(weights, dev), r=rt, y=y[:, :n])
+    ref, size = I.down(ids, e, w, ws, h, hs, weights, res)
+    bound = (k + 4.1) * U * size
+    if half:
+        bound = bound + 2.0 ** -11 * 1.01 * np.abs(ref) + 2.0 ** -25
+    assert (np.abs(y[:, :n].double().cpu().numpy() - ref) <= bound).all()
+    assert (y[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("m,e,k", [(1, 1, 1), (5, 128, 8), (1000, 512, 7), (4097, 60, 4), (3, 7, 2)])
+def test_plan(dev, m, e, k):
+    r = rng("plan", m, e, k)
+    ids = r.integers(-2, e + 2, (m, k)).astype(np.int32)
+    plan = dc.moe_plan(gpu(ids, dev), e).view(torch.int32).cpu().numpy()
+    slots = m * k
+    flat = np.where((ids < 0) | (ids >= e), e, ids).reshape(-1)
+    order_at = -(-(e + 2) // 64) * 64
+    assert (plan[:e + 2] == np.concatenate([[0], np.cumsum(np.bincount(flat, minlength=e + 1))])).all()
+    assert (plan[order_at:order_at + slots] == np.argsort(flat, kind="stable")).all()
+    at = order_at + -(-slots // 64) * 64
+    assert (plan[at:at + slots] == np.where(flat < e, flat, -1)).all()
