@@ -51,6 +51,7 @@ struct I8Args {
     const int32_t* plan;
     int n_expert, top;
     int tiles_n, tiles_m, splits, stps;  // from here on the launcher's
+    bool y_wide;  // rows of y are of whole dwords
 };
 size_t i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 hipError_t launch_i8_product(int ytype, I8Args a, void* ws, size_t ws_bytes, hipStream_t st);

@@ -127,16 +127,19 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     const int s_begin = split * a.stps, s_end = min(stages, s_begin + a.stps);
     const int tail_pieces = (a.K % kRowB) / 16;  // 0: the last stage is whole
 
-    auto issue = [&](int s, Stage& S) {
+    // loads from .. to of the wave's LA + LB
+    auto issue = [&](int s, Stage& S, int from, int to) {
         const bool tail = tail_pieces && s == stages - 1;
         const int64_t k0 = (int64_t)s * kRowB;
 #pragma unroll
         for (int i = 0; i < LA; ++i) {
+            if (i < from || i >= to) continue;
             const uint32_t piece = (lane & 7) ^ piece_key(8 * (LA * wave + i) + l_row);
             dma16(xb + k0, tail && (int)piece >= tail_pieces ? a_off[i] - 16 * piece : a_off[i], S.a + 1024 * (LA * wave + i));
         }
 #pragma unroll
         for (int i = 0; i < LB; ++i) {
+            if (i + LA < from || i + LA >= to) continue;
             const uint32_t piece = (lane & 7) ^ piece_key(8 * (LB * wave + i) + l_row);
             dma16(wbase[i] + k0, tail && (int)piece >= tail_pieces ? b_off[i] - 16 * piece : b_off[i],
                   S.b + 1024 * (LB * wave + i));
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
 
-    issue(s_begin, st[0]);
+    issue(s_begin, st[0], 0, LA + LB);
     __builtin_amdgcn_s_waitcnt(0);
     clear_tail(s_begin, st[0]);
     __syncthreads();
@@ -170,7 +173,6 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
         const Stage& S = st[(s - s_begin) & 1];
         Stage& next = st[(s - s_begin + 1) & 1];
         const bool more = s + 1 < s_end;
-        if (more) issue(s + 1, next);
         v4i fa[2][MI], fb[2][NJ];
         auto read = [&](int kb, int into) {
             const int fo = col * kRowB + 16 * ((2 * kb + hl) ^ piece_key(col));
@@ -183,11 +185,12 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
             if (kb < 3) read(kb + 1, (kb + 1) & 1);
+            if (kb < 2 && more) issue(s + 1, next, kb * (LA + LB) / 2, (kb + 1) * (LA + LB) / 2);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[kb & 1][i], fb[kb & 1][j], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[kb & 1][j], fa[kb & 1][i], acc[i][j], 0, 0, 0);
         }
         if (more) {
             __builtin_amdgcn_s_waitcnt(0);
@@ -196,53 +199,88 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
         }
     }
 
-    // ---- out: a lane holds column n of rows 32 i + 8 (v / 4) + 4 hl + v % 4 ----
-    if constexpr (UP) {
+    // ---- out, 32 rows of a wave at a time: a lane holds row col, columns 32 j + 8 q + 4 hl .. + 3 in sums 4 q .. + 3. Through
+    // LDS (the stages' room), so that a row's columns go out in wide stores ----
+    constexpr bool SUMS = sizeof(T) == 4 && T(0.5f) == T(0);  // int32_t: a plane of sums
+    constexpr int OUT = UP ? TN / 2 : TN, PITCH = OUT + 4, PER = 16 / sizeof(T);  // PER: elements of a store
+    __syncthreads();
+    float* mine = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
+    const int nw = n0 + wn / (UP ? 2 : 1);  // the wave's first output
+    float ws[NJ][16];
+    if constexpr (!SUMS) {
 #pragma unroll
-        for (int j = 0; j < NJ / 2; ++j) {
-            const int n = n0 + wn / 2 + 32 * j + col;
-            const bool in = n < a.N;
-            const int64_t ns = (int64_t)expert * a.N + min(n, a.N - 1);
-            const float gs = a.ws[ns], us = a.ws2[ns];
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int v = 0; v < 16; ++v) {
+                const int n = nw + 32 * (UP ? j % (NJ / 2) : j) + 8 * (v >> 2) + 4 * hl + (v & 3);
+                ws[j][v] = (UP && j >= NJ / 2 ? a.ws2 : a.ws)[(int64_t)expert * a.N + min(n, a.N - 1)];
+            }
+    }
+    const bool wide = a.y_wide;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int r = wm + 32 * i + 8 * (v >> 2) + 4 * hl + (v & 3);
-                    const float xs = row_scale[r];
-                    const float g = i8_value(acc[i][j][v], gs, xs), u = i8_value(acc[i][j + NJ / 2][v], us, xs);
-                    if (in && r < rows_here) put<T>(a.y, (int64_t)row_out[r] * a.y_stride + n, silu(g) * u);
+    for (int i = 0; i < MI; ++i) {
+        if (wm + 32 * i >= rows_here) break;
+        const float xs = row_scale[wm + 32 * i + col];
+#pragma unroll
+        for (int j = 0; j < OUT / 32; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at = 4 * q + e;
+                    if constexpr (SUMS) v[e] = __int_as_float(acc[i][j][at]);
+                    else if constexpr (UP)
+                        v[e] = silu(i8_value(acc[i][j][at], ws[j][at], xs)) *
+                               i8_value(acc[i][j + NJ / 2][at], ws[j + NJ / 2][at], xs);
+                    else v[e] = i8_value(acc[i][j][at], ws[j][at], xs);
                 }
-        }
-    } else {
+                *reinterpret_cast<float4*>(mine + col * PITCH + 32 * j + 8 * q + 4 * hl) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        constexpr int LANES = OUT / PER;  // of a row
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int n = n0 + wn + 32 * j + col;
-            if (n >= a.N) continue;
-            if constexpr (sizeof(T) == 4 && T(0.5f) == T(0)) {  // int32_t: a plane of sums
-                int32_t* p = static_cast<int32_t*>(a.y) + (int64_t)split * a.M * a.N + (int64_t)tile_m * BM * a.N + n;
+        for (int t = 0; t < 32 * LANES / 64; ++t) {
+            const int r = t * (64 / LANES) + lane / LANES, c = lane % LANES * PER, n = nw + c;
+            if (wm + 32 * i + r >= rows_here || n >= a.N) continue;
+            const int64_t row = SUMS ? (int64_t)tile_m * BM + wm + 32 * i + r
+                                : GROUPED ? (int64_t)row_out[wm + 32 * i + r] : (int64_t)tile_m * BM + wm + 32 * i + r;
+            float v[PER];
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+            for (int e = 0; e < PER; e += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(mine + r * PITCH + c + e);
+                v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+            }
+            const int left = min(PER, a.N - n);
+            if (MODE == kI8Dense && !SUMS && a.R) {
+                const float* add = a.R + row * a.r_stride + n;
+                if (left == PER) {
+                    float u[PER];
+                    __builtin_memcpy(u, __builtin_assume_aligned(add, 4), 4 * PER);
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) {
-                        const int r = wm + 32 * i + 8 * (v >> 2) + 4 * hl + (v & 3);
-                        if (r < rows_here) p[(int64_t)r * a.N] = acc[i][j][v];
-                    }
+                    for (int e = 0; e < PER; ++e) v[e] += u[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < PER; ++e)
+                        if (e < left) v[e] += add[e];
+                }
+            }
+            T o[PER];
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                if constexpr (SUMS) o[e] = __float_as_int(v[e]);
+                else o[e] = (T)v[e];
+            }
+            T* y = static_cast<T*>(a.y) + (SUMS ? (int64_t)split * a.M * a.N : 0) + row * a.y_stride + n;
+            if (left == PER && wide) {
+                __builtin_memcpy(__builtin_assume_aligned(y, 4), o, 16);
             } else {
-                const float ws = a.ws[(int64_t)expert * a.N + n];
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) {
-                        const int r = wm + 32 * i + 8 * (v >> 2) + 4 * hl + (v & 3);
-                        if (r >= rows_here) continue;
-                        float y = i8_value(acc[i][j][v], ws, row_scale[r]);
-                        const int64_t row = GROUPED ? (int64_t)row_out[r] : (int64_t)tile_m * BM + r;
-                        if (!GROUPED && a.R) y += a.R[row * a.r_stride + n];
-                        put<T>(a.y, row * a.y_stride + n, y);
-                    }
+                for (int e = 0; e < PER; ++e)
+                    if (e < left) y[e] = o[e];
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
@@ -288,6 +326,8 @@ hipError_t launch_shape(I8Args a, int shape, hipStream_t st) {
 hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, size_t ws_bytes, hipStream_t st) {
     const int stages = (a.K + kRowB - 1) / kRowB;
     a.splits = 1, a.stps = stages;
+    // wide stores need whole dwords
+    a.y_wide = ytype == kTypeF32 || (a.y_stride % 2 == 0 && (uintptr_t)a.y % 4 == 0);
     const int forced = knob(Knob::I8Tile);
     if (mode != kI8Dense) {
         const int64_t mean = a.M / a.n_expert;
@@ -311,7 +351,7 @@ hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, size_t ws_
     a.stps = (stages + splits - 1) / splits;
     a.splits = (stages + a.stps - 1) / a.stps;
     I8Args p = a;
-    p.y = ws;
+    p.y = ws, p.y_stride = a.N, p.y_wide = true;
     hipError_t e = launch_shape<kI8Dense, int32_t>(p, shape, st);
     if (e != hipSuccess) return e;
     const unsigned blocks = (unsigned)std::min<int64_t>((a.M * a.N + 255) / 256, 2048);
