@@ -1095,7 +1095,7 @@ static int validate_plan(int64_t M, int k, int n_expert) {
                ? DCQ_OK
                : DCQ_ERR_BAD_SHAPE;
 }
-static int64_t plan_bytes(int64_t M, int k, int n_expert) { return (plan_expert_at(n_expert, M * k) + M * k) * 4; }
+static int64_t plan_bytes(int64_t M, int k, int n_expert) { return plan_ints(n_expert, M * k) * 4; }
 
 size_t dcq_moe_plan_size(int64_t M, int k, int n_expert) {
     return validate_plan(M, k, n_expert) ? 0 : (size_t)plan_bytes(M, k, n_expert);
@@ -1151,7 +1151,7 @@ int dcq_moe_gate_up_i8(const void* plan, size_t plan_size, int64_t M, int k, int
     a.x = X, a.xs = Xs, a.x_stride = (int64_t)x_stride_bytes, a.M = M * k, a.w = Wg, a.ws = Wgs, a.w2 = Wu, a.ws2 = Wus;
     a.w_stride = (int64_t)w_stride_bytes, a.w_expert = (int64_t)expert_stride_bytes, a.N = (int)N, a.K = (int)K;
     a.y = H, a.y_stride = (int64_t)h_stride_bytes / size, a.plan = static_cast<const int32_t*>(plan), a.n_expert = n_expert, a.top = k;
-    return hip_status(launch_i8_experts(kI8Up, htype, a, (hipStream_t)stream));
+    return hip_status(launch_moe_gate_up(htype, a, (hipStream_t)stream));
 }
 
 size_t dcq_moe_down_i8_workspace_size(int64_t M, int k, int64_t N) {
@@ -1186,13 +1186,11 @@ int dcq_moe_down_i8(const void* plan, size_t plan_size, int64_t M, int k, int n_
     a.x = Hq, a.xs = Hs, a.x_stride = (int64_t)h_stride_bytes, a.M = M * k, a.w = W, a.ws = Ws;
     a.w_stride = (int64_t)w_stride_bytes, a.w_expert = (int64_t)expert_stride_bytes, a.N = (int)N, a.K = (int)K;
     a.y = workspace, a.y_stride = N, a.plan = static_cast<const int32_t*>(plan), a.n_expert = n_expert, a.top = k;
-    const hipError_t e = launch_i8_experts(kI8Down, DCQ_TYPE_F32, a, (hipStream_t)stream);
-    if (e != hipSuccess) return hip_status(e);
     CombineArgs c{};
     c.p = static_cast<const float*>(workspace), c.expert = a.plan + plan_expert_at(n_expert, M * k), c.weights = weights;
     c.top = k, c.N = (int)N, c.rows = M, c.R = R, c.r_stride = (int64_t)(r_stride_bytes / 4);
     c.y = Y, c.y_stride = (int64_t)y_stride_bytes / size;
-    return hip_status(launch_moe_combine(ytype, c, (hipStream_t)stream));
+    return hip_status(launch_moe_down(ytype, a, c, (hipStream_t)stream));
 }
 
 }  // extern "C"

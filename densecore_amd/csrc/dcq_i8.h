@@ -54,17 +54,39 @@ struct I8Args {
     bool y_wide;  // rows of y are of whole dwords
 };
 size_t i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
-hipError_t launch_i8_product(int ytype, I8Args a, void* ws, size_t ws_bytes, hipStream_t st);
-hipError_t launch_i8_experts(I8Mode mode, int ytype, I8Args a, hipStream_t st);
+hipError_t launch_i8_product(int ytype, const I8Args& a, void* ws, size_t ws_bytes, hipStream_t st);
+hipError_t launch_moe_gate_up(int htype, const I8Args& a, hipStream_t st);
+struct CombineArgs;
+hipError_t launch_moe_down(int ytype, I8Args a, const CombineArgs& c, hipStream_t st);
 // dcq_i8_rows.hip: few rows (of an expert); dcq_i8_gemm.hip: many
-hipError_t launch_i8_rows(I8Mode mode, int ytype, I8Args a, hipStream_t st);
+hipError_t launch_i8_rows(I8Mode mode, int ytype, const I8Args& a, hipStream_t st);
 hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, size_t ws_bytes, hipStream_t st);
 
-// dcq_moe.hip. A plan: int32 offsets[n_expert + 2] (expert e's slots are places offsets[e] .. offsets[e + 1] - 1 of the
-// order, those of no expert offsets[n_expert] ..), then the order: slots sorted by expert; then each slot's expert, or -1.
+// dcq_moe.hip. A plan, in int32: offsets[n_expert + 2] (expert e's slots are places offsets[e] .. offsets[e + 1] - 1 of the
+// order, those of no expert offsets[n_expert] ..); the order: slots sorted by expert; each slot's expert, or -1; and tiles of
+// the order, `plan_height` places each: {expert, first place, places, 0}, -1 for a tile that is not used. Tiles do not cross
+// experts: group g's begin at (its first place + g (height - 1)) / height, which leaves every group room for its last,
+// partial one whatever the others' sizes, so that each group's place is known without the others' tiles.
+struct PlanTile {
+    int expert, begin, count, unused;
+};
+// Rows of a tile: what the products' kernels take at a time, by the rows that an expert has on average.
+__host__ __device__ inline int plan_height(int64_t slots, int n_expert) {
+    const int64_t mean = slots / n_expert;
+    return mean <= 12 ? 16 : mean <= 24 ? 32 : mean <= 40 ? 64 : mean <= 384 ? 128 : 256;
+}
+__host__ __device__ inline int64_t plan_tiles(int64_t slots, int n_expert, int height) {
+    return (slots + (int64_t)(n_expert + 1) * (height - 1)) / height;
+}
 __host__ __device__ inline int64_t plan_order_at(int n_expert) { return (n_expert + 2 + 63) / 64 * 64; }
 __host__ __device__ inline int64_t plan_expert_at(int n_expert, int64_t slots) {
     return plan_order_at(n_expert) + (slots + 63) / 64 * 64;
+}
+__host__ __device__ inline int64_t plan_tiles_at(int n_expert, int64_t slots) {
+    return plan_expert_at(n_expert, slots) + (slots + 63) / 64 * 64;
+}
+__host__ __device__ inline int64_t plan_ints(int n_expert, int64_t slots) {
+    return plan_tiles_at(n_expert, slots) + 4 * plan_tiles(slots, n_expert, plan_height(slots, n_expert));
 }
 struct RouteArgs {
     const void* x;

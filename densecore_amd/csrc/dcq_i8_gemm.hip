@@ -6,25 +6,11 @@
 #include "dcq_i8_tile.h"
 #include "dcq_kernels.h"
 
-#pragma clang diagnostic ignored "-Winline-asm"  // M0 in the clobber list (see dma16)
-
 namespace dcq {
 
 namespace {
 
-constexpr int kRowB = 128;  // k per stage = bytes of an LDS row: 8 pieces of 16, piece p of row r at p ^ key(r)
 constexpr int kXcds = 8;
-
-__device__ __forceinline__ int piece_key(int row) { return (row & 7) ^ ((row >> 3) & 1); }
-
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-
-// 16 bytes per lane from a uniform base + per-lane offset to LDS at lds_base + 16 * lane (lds_base uniform, in M0). The
-// compiler does not count these loads: an explicit wait comes before the barrier that publishes them.
-__device__ __forceinline__ void dma16(const void* g, uint32_t off, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "s"(m0) : "memory", "m0");
-}
 
 template <class T>
 __device__ __forceinline__ void put(void* y, int64_t at, float v) {
@@ -36,46 +22,46 @@ __device__ __forceinline__ void put(void* y, int64_t at, float v) {
 // A tile of BM rows x BN weight rows per workgroup of WM x WN waves. kI8Up: half of a wave's columns are gate rows and
 // half the same rows of the up matrix, so that a lane holds both products of an output.
 // T: the output's type; int32_t: the sums themselves, to a plane of `splits`.
-template <I8Mode MODE, int BM, int BN, int WM, int WN, class T>
+template <I8Mode MODE, int BM, int BN, int WM, int WN, int KB, int ST, class T>
 __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     constexpr int W = WM * WN, TM = BM / WM, TN = BN / WN, MI = TM / 32, NJ = TN / 32;
-    constexpr int LA = BM / 8 / W, LB = BN / 8 / W;  // 1 KB loads of a wave and stage
+    constexpr int P = KB / 16, LR = 64 / P;  // 16-byte pieces of an LDS row; rows of a 1 KB load
+    constexpr int LA = BM / LR / W, LB = BN / LR / W;  // loads of a wave and stage
+    constexpr int Q = KB / 32;  // products' steps of a stage
     constexpr bool UP = MODE == kI8Up, GROUPED = MODE != kI8Dense;
     constexpr int TILE_N = UP ? BN / 2 : BN;  // outputs
     struct __align__(16) Stage {
-        int8_t a[BM * kRowB];
-        int8_t b[BN * kRowB];
+        int8_t a[BM * KB];
+        int8_t b[BN * KB];
     };
     extern __shared__ __align__(16) uint8_t smem[];
     Stage* st = reinterpret_cast<Stage*>(smem);
-    __shared__ float row_scale[BM];
+    __shared__ __align__(16) float row_scale[BM], col_scale[BN];
     __shared__ int row_out[BM];  // grouped: the slot
-    __shared__ PlanTile found;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    // ---- which tile: an XCD (workgroup id % 8) takes a run of tiles, the row tiles of one band of weights ----
+    // ---- which tile: an XCD (workgroup id % 8) takes a run of tiles ----
     const int tiles = a.tiles_n * a.tiles_m;
     const int split = GROUPED ? 0 : (int)blockIdx.x / tiles;
     const int id = (int)blockIdx.x - split * tiles;
-    int at = id;
-    if (tiles % kXcds == 0) at = id % kXcds * (tiles / kXcds) + id / kXcds;
+    const int xcd = id % kXcds;
+    const int at = xcd * (tiles / kXcds) + min(xcd, tiles % kXcds) + id / kXcds;
     int tile_m, tile_n;
-    if constexpr (GROUPED) tile_m = at / a.tiles_n, tile_n = at % a.tiles_n;
-    else tile_n = at / a.tiles_m, tile_m = at % a.tiles_m;
-    const int n0 = tile_n * TILE_N;
-    int rows_here, expert = 0, begin = 0;
     if constexpr (GROUPED) {
-        if (wave == 0) {
-            const PlanTile t = find_tile(a.plan, a.n_expert, BM, tile_m);
-            if (lane == 0) found = t;
-        }
-        __syncthreads();
-        expert = __builtin_amdgcn_readfirstlane(found.expert);
-        begin = __builtin_amdgcn_readfirstlane(found.begin);
-        rows_here = __builtin_amdgcn_readfirstlane(found.count);
-        if (expert < 0) return;
-        const int32_t* order = a.plan + plan_order_at(a.n_expert) + begin;
+        tile_m = at / a.tiles_n, tile_n = at % a.tiles_n;
+    } else {  // bands of 8 row tiles, so that what an XCD's CUs hold at a time is 8 x 4 tiles
+        const int band = at / (8 * a.tiles_n), high = min(8, a.tiles_m - 8 * band), in = at - band * 8 * a.tiles_n;
+        tile_m = 8 * band + in % high, tile_n = in / high;
+    }
+    const int n0 = tile_n * TILE_N;
+    int rows_here, expert = 0;
+    const int32_t* order = nullptr;
+    if constexpr (GROUPED) {
+        const PlanTile t = reinterpret_cast<const PlanTile*>(a.plan + plan_tiles_at(a.n_expert, a.M))[tile_m];
+        if (t.expert < 0) return;
+        expert = t.expert, rows_here = t.count;
+        order = a.plan + plan_order_at(a.n_expert) + t.begin;
         if (expert == a.n_expert) {  // slots of no expert
             if constexpr (UP) {
                 for (int i = tid; i < rows_here * TILE_N; i += 64 * W)
@@ -83,15 +69,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
             }
             return;
         }
-        for (int i = tid; i < BM; i += 64 * W) {
-            const int slot = order[min(i, rows_here - 1)];
-            row_out[i] = slot;
-            row_scale[i] = a.xs[UP ? slot / a.top : slot];
-        }
-        __syncthreads();
     } else {
         rows_here = (int)min((int64_t)BM, a.M - (int64_t)tile_m * BM);
-        for (int i = tid; i < BM; i += 64 * W) row_scale[i] = a.xs[(int64_t)tile_m * BM + min(i, rows_here - 1)];
     }
 
     // ---- loads of a stage: instruction i of a wave fills 8 tile rows, lane l piece l % 8 of row l / 8 ----
@@ -99,17 +78,11 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     const int8_t* wb = a.w + (int64_t)expert * a.w_expert;
     const int8_t* wb2 = UP ? a.w2 + (int64_t)expert * a.w_expert : nullptr;
     uint32_t a_off[LA], b_off[LB];
-    const int l_row = lane >> 3;
-#pragma unroll
-    for (int i = 0; i < LA; ++i) {
-        const int r = 8 * (LA * wave + i) + l_row;
-        const int src = GROUPED ? (UP ? row_out[r] / a.top : row_out[r]) : min(r, rows_here - 1);
-        a_off[i] = (uint32_t)src * (uint32_t)a.x_stride + 16u * (uint32_t)((lane & 7) ^ piece_key(r));
-    }
+    const int l_row = lane / P;
     const int8_t* wbase[LB];
 #pragma unroll
     for (int i = 0; i < LB; ++i) {
-        const int r0 = 8 * (LB * wave + i), r = r0 + l_row;
+        const int r0 = LR * (LB * wave + i), r = r0 + l_row;
         int n;
         if constexpr (UP) {  // 8 rows of one instruction are of one matrix (TN / 2 is a multiple of 8)
             const int in = r0 % TN;
@@ -120,27 +93,34 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
             n = r;
         }
         // within the tile's rows: offsets of 32 bits from the tile's first row
-        wbase[i] += (int64_t)n0 * a.w_stride;
-        b_off[i] = (uint32_t)min(n, a.N - 1 - n0) * (uint32_t)a.w_stride + 16u * (uint32_t)((lane & 7) ^ piece_key(r));
+        wbase[i] = uniform(wbase[i] + (int64_t)n0 * a.w_stride);
+        b_off[i] = (uint32_t)min(n, a.N - 1 - n0) * (uint32_t)a.w_stride + 16u * (uint32_t)((lane % P) ^ piece_key<KB>(r));
     }
-    const int stages = (a.K + kRowB - 1) / kRowB;
-    const int s_begin = split * a.stps, s_end = min(stages, s_begin + a.stps);
-    const int tail_pieces = (a.K % kRowB) / 16;  // 0: the last stage is whole
+#pragma unroll
+    for (int i = 0; i < LA; ++i) {
+        const int r = LR * (LA * wave + i) + l_row;
+        int src = min(r, rows_here - 1);
+        if constexpr (GROUPED) src = UP ? order[src] / a.top : order[src];
+        a_off[i] = (uint32_t)src * (uint32_t)a.x_stride + 16u * (uint32_t)((lane % P) ^ piece_key<KB>(r));
+    }
+    const int stages = (a.K + KB - 1) / KB;
+    const int stps = a.stps * (128 / KB), s_begin = split * stps, s_end = min(stages, s_begin + stps);
+    const int tail_pieces = (a.K % KB) / 16;  // 0: the last stage is whole
 
     // loads from .. to of the wave's LA + LB
     auto issue = [&](int s, Stage& S, int from, int to) {
         const bool tail = tail_pieces && s == stages - 1;
-        const int64_t k0 = (int64_t)s * kRowB;
+        const int64_t k0 = (int64_t)s * KB;
 #pragma unroll
         for (int i = 0; i < LA; ++i) {
             if (i < from || i >= to) continue;
-            const uint32_t piece = (lane & 7) ^ piece_key(8 * (LA * wave + i) + l_row);
+            const uint32_t piece = (lane % P) ^ piece_key<KB>(LR * (LA * wave + i) + l_row);
             dma16(xb + k0, tail && (int)piece >= tail_pieces ? a_off[i] - 16 * piece : a_off[i], S.a + 1024 * (LA * wave + i));
         }
 #pragma unroll
         for (int i = 0; i < LB; ++i) {
             if (i + LA < from || i + LA >= to) continue;
-            const uint32_t piece = (lane & 7) ^ piece_key(8 * (LB * wave + i) + l_row);
+            const uint32_t piece = (lane % P) ^ piece_key<KB>(LR * (LB * wave + i) + l_row);
             dma16(wbase[i] + k0, tail && (int)piece >= tail_pieces ? b_off[i] - 16 * piece : b_off[i],
                   S.b + 1024 * (LB * wave + i));
         }
@@ -150,7 +130,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
         if (!(tail_pieces && s == stages - 1)) return;
 #pragma unroll
         for (int i = 0; i < LA; ++i) {
-            const int piece = (lane & 7) ^ piece_key(8 * (LA * wave + i) + l_row);
+            const int piece = (lane % P) ^ piece_key<KB>(LR * (LA * wave + i) + l_row);
             if (piece >= tail_pieces) *reinterpret_cast<uint4*>(S.a + 1024 * (LA * wave + i) + 16 * lane) = make_uint4(0, 0, 0, 0);
         }
     };
@@ -165,45 +145,96 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
 
-    issue(s_begin, st[0], 0, LA + LB);
-    __builtin_amdgcn_s_waitcnt(0);
+    // The products run a quarter stage behind the operands' reads, over the stages' borders too: in front of a stage's last
+    // quarter, whose operands are in registers, every wave waits for its part of the next stage; behind the barrier that
+    // stage is whole and this one's room free for the stage after it.
+    v4i fa[2][MI], fb[2][NJ];
+    auto read = [&](const Stage& S, int kb, int into) {
+        const int fo = col * KB + 16 * ((2 * kb + hl) ^ piece_key<KB>(col));
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fb[into][j] = *reinterpret_cast<const v4i*>(S.b + fo + (wn + 32 * j) * KB);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[into][i] = *reinterpret_cast<const v4i*>(S.a + fo + (wm + 32 * i) * KB);
+    };
+    auto multiply = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[from][j], fa[from][i], acc[i][j], 0, 0, 0);
+    };
+    // ---- a ring of ST stages; a wave's loads retire in order, so all but the last n stages' have landed when no more than
+    // n (LA + LB) are on their way ----
+    auto landed = [&](int behind) {
+        if (ST > 3 && behind >= 3) counted_wait<3 * (LA + LB)>();
+        else if (ST > 2 && behind >= 2) counted_wait<2 * (LA + LB)>();
+        else if (behind >= 1) counted_wait<LA + LB>();
+        else __builtin_amdgcn_s_waitcnt(0);
+    };
+    // the tile's scales, on their way before the stages, and to LDS after the products
+    constexpr int RT = (BM + 64 * W - 1) / (64 * W), CT = (BN + 64 * W - 1) / (64 * W);
+    float rs[RT], cs[CT];
+    int slot[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int r = min(tid + 64 * W * t, rows_here - 1);
+        if constexpr (GROUPED) {
+            slot[t] = order[r];
+            rs[t] = a.xs[UP ? slot[t] / a.top : slot[t]];
+        } else {
+            rs[t] = a.xs[(int64_t)tile_m * BM + r];
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+        const int i = min(tid + 64 * W * t, BN - 1);
+        int n = i;
+        if constexpr (UP) n = i / TN * (TN / 2) + i % (TN / 2);
+        cs[t] = (UP && i % TN >= TN / 2 ? a.ws2 : a.ws)[(int64_t)expert * a.N + min(n0 + n, a.N - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < ST; ++i)
+        if (s_begin + i < s_end) issue(s_begin + i, st[i], 0, LA + LB);
+    landed(min(ST, s_end - s_begin) - 1);
     clear_tail(s_begin, st[0]);
     __syncthreads();
+    read(st[0], 0, 0);
+    int now = 0;
     for (int s = s_begin; s < s_end; ++s) {
-        const Stage& S = st[(s - s_begin) & 1];
-        Stage& next = st[(s - s_begin + 1) & 1];
-        const bool more = s + 1 < s_end;
-        v4i fa[2][MI], fb[2][NJ];
-        auto read = [&](int kb, int into) {
-            const int fo = col * kRowB + 16 * ((2 * kb + hl) ^ piece_key(col));
+        Stage& S = st[now];
+        now = now + 1 == ST ? 0 : now + 1;
+        Stage& next = st[now];
 #pragma unroll
-            for (int i = 0; i < MI; ++i) fa[into][i] = *reinterpret_cast<const v4i*>(S.a + fo + (wm + 32 * i) * kRowB);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) fb[into][j] = *reinterpret_cast<const v4i*>(S.b + fo + (wn + 32 * j) * kRowB);
-        };
-        read(0, 0);
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-            if (kb < 3) read(kb + 1, (kb + 1) & 1);
-            if (kb < 2 && more) issue(s + 1, next, kb * (LA + LB) / 2, (kb + 1) * (LA + LB) / 2);
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[kb & 1][j], fa[kb & 1][i], acc[i][j], 0, 0, 0);
+        for (int q = 1; q < Q; ++q) {
+            read(S, q, q & 1);
+            multiply((q - 1) & 1);
         }
-        if (more) {
-            __builtin_amdgcn_s_waitcnt(0);
+        if (s + 1 < s_end) {
+            landed(min(ST - 2, s_end - 2 - s));
             clear_tail(s + 1, next);
             __syncthreads();
+            read(next, 0, 0);
+            if (s + ST < s_end) issue(s + ST, S, 0, LA + LB);
         }
+        multiply(1);
     }
 
     // ---- out, 32 rows of a wave at a time: a lane holds row col, columns 32 j + 8 q + 4 hl .. + 3 in sums 4 q .. + 3. Through
     // LDS (the stages' room), so that a row's columns go out in wide stores ----
     constexpr bool SUMS = sizeof(T) == 4 && T(0.5f) == T(0);  // int32_t: a plane of sums
     constexpr int OUT = UP ? TN / 2 : TN, PITCH = OUT + 4, PER = 16 / sizeof(T);  // PER: elements of a store
-    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int i = tid + 64 * W * t;
+        if (i < BM) {
+            row_scale[i] = rs[t];
+            if constexpr (GROUPED) row_out[i] = slot[t];
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+        if (tid + 64 * W * t < BN) col_scale[tid + 64 * W * t] = cs[t];
+    __syncthreads();  // and the stages' room is free
     float* mine = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
     const int nw = n0 + wn / (UP ? 2 : 1);  // the wave's first output
     float ws[NJ][16];
@@ -211,9 +242,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int n = nw + 32 * (UP ? j % (NJ / 2) : j) + 8 * (v >> 2) + 4 * hl + (v & 3);
-                ws[j][v] = (UP && j >= NJ / 2 ? a.ws2 : a.ws)[(int64_t)expert * a.N + min(n, a.N - 1)];
+            for (int q = 0; q < 4; ++q) {
+                const float4 f = *reinterpret_cast<const float4*>(col_scale + wn + 32 * j + 8 * q + 4 * hl);
+                ws[j][4 * q] = f.x, ws[j][4 * q + 1] = f.y, ws[j][4 * q + 2] = f.z, ws[j][4 * q + 3] = f.w;
             }
     }
     const bool wide = a.y_wide;
@@ -284,30 +315,53 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     }
 }
 
-// y = the sum of the planes' int32 sums (exact, so that any split gives the same bits), scaled, plus R.
-template <class T>
+// y = the sum of the planes' int32 sums (exact, so that any split gives the same bits), scaled, plus R. A thread for V
+// columns of a row.
+template <class T, int V>
 __global__ void __launch_bounds__(256) i8_join_kernel(I8Args a, const int32_t* planes) {
-    const int64_t n = a.N, plane = a.M * n;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / n, c = i - row * n;
-        int sum = 0;
-        for (int s = 0; s < a.splits; ++s) sum += planes[s * plane + i];
-        float y = i8_value(sum, a.ws[c], a.xs[row]);
-        if (a.R) y += a.R[row * a.r_stride + c];
-        put<T>(a.y, row * a.y_stride + c, y);
+    const int blocks = (a.N + 256 * V - 1) / (256 * V);
+    const int64_t row = blockIdx.x / blocks;
+    const int n = ((int)blockIdx.x % blocks * 256 + (int)threadIdx.x) * V;
+    if (n >= a.N) return;
+    const int32_t* p = planes + row * a.N + n;
+    int sum[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[e] = 0;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        int v[V];
+        __builtin_memcpy(v, __builtin_assume_aligned(p + s * (a.M * a.N), 4 * V), 4 * V);
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] += v[e];
+    }
+    const float xs = a.xs[row];
+    T o[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        float y = i8_value(sum[e], a.ws[n + e], xs);
+        if (a.R) y += a.R[row * a.r_stride + n + e];
+        o[e] = (T)y;
+    }
+    T* y = static_cast<T*>(a.y) + row * a.y_stride + n;
+    if (V > 1 && a.y_wide) {
+        __builtin_memcpy(__builtin_assume_aligned(y, 4), o, sizeof(o));
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = o[e];
     }
 }
 
 namespace {
 
-template <I8Mode MODE, int BM, int BN, int WM, int WN, class T>
+template <I8Mode MODE, int BM, int BN, int WM, int WN, int KB, int ST, class T>
 hipError_t launch_tile(I8Args a, hipStream_t st) {
     constexpr int tile_n = MODE == kI8Up ? BN / 2 : BN;
     a.tiles_n = (a.N + tile_n - 1) / tile_n;
-    a.tiles_m = (int)(MODE == kI8Dense ? (a.M + BM - 1) / BM : most_tiles(a.M, a.n_expert, BM));
-    const size_t lds = 2 * (size_t)(BM + BN) * kRowB;
+    a.tiles_m = (int)(MODE == kI8Dense ? (a.M + BM - 1) / BM : plan_tiles(a.M, a.n_expert, BM));
+    constexpr int out = MODE == kI8Up ? BN / WN / 2 : BN / WN;
+    const size_t lds = std::max<size_t>(ST * (size_t)(BM + BN) * KB, (size_t)WM * WN * 32 * (out + 4) * 4);
     const int64_t groups = (int64_t)a.tiles_n * a.tiles_m * a.splits;
-    auto fn = i8_gemm_kernel<MODE, BM, BN, WM, WN, T>;
+    auto fn = i8_gemm_kernel<MODE, BM, BN, WM, WN, KB, ST, T>;
     fn<<<dim3((unsigned)groups), 64 * WM * WN, lds, st>>>(a);
     return hipGetLastError();
 }
@@ -315,23 +369,36 @@ hipError_t launch_tile(I8Args a, hipStream_t st) {
 template <I8Mode MODE, class T>
 hipError_t launch_shape(I8Args a, int shape, hipStream_t st) {
     switch (shape) {
-        case 0: return launch_tile<MODE, 64, 128, 2, 2, T>(a, st);
-        case 1: return launch_tile<MODE, 128, 128, 2, 2, T>(a, st);
-        default: return launch_tile<MODE, 256, 256, 2, 4, T>(a, st);
+        case 0: return launch_tile<MODE, 64, 128, 2, 2, 64, 4, T>(a, st);
+        case 1: return launch_tile<MODE, 128, 128, 2, 2, 64, 4, T>(a, st);
+        case 3: return launch_tile<MODE, 64, 128, 2, 2, 128, 2, T>(a, st);
+        case 4: return launch_tile<MODE, 128, 128, 2, 2, 128, 2, T>(a, st);
+        case 5: return launch_tile<MODE, 128, 128, 2, 2, 64, 2, T>(a, st);
+        case 6: return launch_tile<MODE, 128, 128, 2, 2, 64, 3, T>(a, st);
+        default: return launch_tile<MODE, 256, 256, 2, 4, 128, 2, T>(a, st);
     }
+}
+
+template <class T>
+hipError_t launch_join(const I8Args& a, const void* planes, hipStream_t st) {
+    const int per = a.N % 4 ? 256 : 1024;
+    const dim3 grid((unsigned)((a.N + per - 1) / per * a.M));
+    if (per == 1024) i8_join_kernel<T, 4><<<grid, 256, 0, st>>>(a, static_cast<const int32_t*>(planes));
+    else i8_join_kernel<T, 1><<<grid, 256, 0, st>>>(a, static_cast<const int32_t*>(planes));
+    return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, size_t ws_bytes, hipStream_t st) {
-    const int stages = (a.K + kRowB - 1) / kRowB;
+    const int stages = (a.K + 127) / 128;
     a.splits = 1, a.stps = stages;
     // wide stores need whole dwords
     a.y_wide = ytype == kTypeF32 || (a.y_stride % 2 == 0 && (uintptr_t)a.y % 4 == 0);
     const int forced = knob(Knob::I8Tile);
     if (mode != kI8Dense) {
-        const int64_t mean = a.M / a.n_expert;
-        const int shape = forced >= 0 ? forced : mean >= 192 ? 2 : mean >= 48 ? 1 : 0;
+        const int height = plan_height(a.M, a.n_expert);
+        const int shape = forced >= 0 ? forced : height == 256 ? 2 : height == 128 ? 1 : 0;
         if (mode == kI8Up)
             return ytype == kTypeF16 ? launch_shape<kI8Up, _Float16>(a, shape, st) : launch_shape<kI8Up, float>(a, shape, st);
         return launch_shape<kI8Down, float>(a, shape, st);
@@ -354,10 +421,7 @@ hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, size_t ws_
     p.y = ws, p.y_stride = a.N, p.y_wide = true;
     hipError_t e = launch_shape<kI8Dense, int32_t>(p, shape, st);
     if (e != hipSuccess) return e;
-    const unsigned blocks = (unsigned)std::min<int64_t>((a.M * a.N + 255) / 256, 2048);
-    if (ytype == kTypeF16) i8_join_kernel<_Float16><<<blocks, 256, 0, st>>>(a, static_cast<const int32_t*>(ws));
-    else i8_join_kernel<float><<<blocks, 256, 0, st>>>(a, static_cast<const int32_t*>(ws));
-    return hipGetLastError();
+    return ytype == kTypeF16 ? launch_join<_Float16>(a, ws, st) : launch_join<float>(a, ws, st);
 }
 
 size_t i8_workspace_bytes(int64_t M, int64_t N, int64_t K) {

@@ -1,4 +1,11 @@
 // dcq_i8_rows.hip — products of few int8 rows (a decode step's, or those of an expert) on 16 x 16 int8 MFMA.
+//
+// Every weight is read once for up to 64 rows, so the time is the weights' bytes over the rate of HBM, and what is left to
+// do is to keep enough of them on their way. A wave owns 16 rows of W and a share of K; its operands come through a ring of
+// two stages in LDS that no other wave touches, so that nothing waits for a barrier until the sums are added. Through LDS because
+// an operand's consecutive lanes are in 16 different rows: loaded to registers, every lane's 16 bytes are a request of their own
+// (61 rows x 2560 x 9728: 22.7 us that way, 11.0 with rows of 128 bytes to LDS, 15.2 with rows of 64; one row x 2560 x 9728:
+// 8.1, 6.1 and 6.5).
 #include <algorithm>
 
 #include "dcq_common.h"
@@ -8,33 +15,108 @@
 
 namespace dcq {
 
-// 16 MT rows x 16 NT weight rows to a wave (kI8Up: 16 gate and 16 up rows, NT = 2); KW waves take a chunk of 256 k in
-// turn and add their sums in LDS, NW such groups to a workgroup.
-template <I8Mode MODE, int MT, int NT, int KW, int NW, class T>
+namespace {
+
+constexpr int kStages = 2;
+
+// A wave's sums over its share of K: 16 MT rows of x (x_off: the rows' bytes of the lane's loads, 8 rows a load) times 16 NT
+// rows of weights. Lane l gets column l % 16 of rows 4 (l / 16) + v.
+template <int MT, int NT>
+__device__ __forceinline__ void wave_sums(v4i (&acc)[MT][NT], int8_t* ring, const int8_t* xb, const uint32_t (&x_off)[2 * MT],
+                                          const int8_t* const (&wb)[NT], const uint32_t (&w_off)[2 * NT], int K, int begin, int end) {
+    constexpr int KB = 128, LX = 2 * MT, LW = 2 * NT, L = LX + LW;
+    const int lane = threadIdx.x & 63, l_row = lane / 8;
+    auto issue = [&](int s, int at) {
+        int8_t* S = ring + at * (1024 * L);
+        const int64_t k0 = (int64_t)s * KB;
+        const int pieces = min(8, (K - s * KB) / 16);  // pieces past K are the row's first of the stage
+#pragma unroll
+        for (int i = 0; i < LW; ++i) {
+            const int p = lane % 8 ^ piece_key<KB>(8 * i + l_row);
+            dma16<true>(wb[i / 2] + k0, w_off[i] + (p < pieces ? 16 * p : 0), S + 1024 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < LX; ++i) {
+            const int p = lane % 8 ^ piece_key<KB>(8 * i + l_row);
+            dma16<true>(xb + k0, x_off[i] + (p < pieces ? 16 * p : 0), S + 1024 * (LW + i));
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = (v4i){0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kStages; ++i)
+        if (begin + i < end) issue(begin + i, i);
+    const int r16 = lane & 15, q = lane >> 4;
+    for (int s = begin, at = 0; s < end; ++s) {
+        if (s + 1 < end) counted_wait<L>();  // a wave's loads retire in order: all but the next stage's
+        else __builtin_amdgcn_s_waitcnt(0);
+        const int8_t* S = ring + at * (1024 * L);
+        v4i fw[NT][2], fx[MT][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int fo = r16 * KB + 16 * ((4 * u + q) ^ piece_key<KB>(r16));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) fw[j][u] = *reinterpret_cast<const v4i*>(S + fo + j * 16 * KB);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fx[i][u] = *reinterpret_cast<const v4i*>(S + 1024 * LW + fo + i * 16 * KB);
+        }
+        if (s + kStages < end) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is in registers, its room free
+            issue(s + kStages, at);
+        }
+        at ^= 1;
+        if ((s + 1) * KB > K) {  // x is zero past K
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (s * KB + 64 * u + 16 * q >= K)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) fx[i][u] = (v4i){0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fx[i][u], fw[j][u], acc[i][j], 0, 0, 0);
+    }
+}
+
+// The lane's part of loads of 16 weight rows from n0 on; rows past N are the last one's again.
+__device__ __forceinline__ void weight_rows(uint32_t* w_off, int n0, int N, int64_t w_stride) {
+    const int l_row = (threadIdx.x & 63) / 8;
+    for (int i = 0; i < 2; ++i) w_off[i] = (uint32_t)max(min(8 * i + l_row, N - 1 - n0), 0) * (uint32_t)w_stride;
+}
+
+}  // namespace
+
+// 16 MT rows x 16 outputs to a wave (kI8Up: of 16 gate and 16 up rows). KW waves share K, an equal run of stages each, and add
+// their sums in LDS; NW such groups to a workgroup.
+template <I8Mode MODE, int MT, int KW, int NW, class T>
 __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
     constexpr bool UP = MODE == kI8Up, GROUPED = MODE != kI8Dense;
-    constexpr int TILE_N = UP ? 8 * NT : 16 * NT;  // outputs of a wave group
-    static_assert(!UP || NT == 2, "a gate and an up row to each output");
-    __shared__ int part[NW][KW > 1 ? KW : 1][MT * NT * 4][64];
+    constexpr int NT = UP ? 2 : 1;
+    extern __shared__ __align__(16) uint8_t smem[];
+    int(*part)[KW][MT * NT * 4][64] = reinterpret_cast<int(*)[KW][MT * NT * 4][64]>(smem);  // when the stages are done
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kw = wave % KW, nw = wave / KW;
     const int tile_m = (int)blockIdx.x / a.tiles_n, tile_n = (int)blockIdx.x % a.tiles_n;
-    const int n0 = (tile_n * NW + nw) * TILE_N;
+    const int n0 = (tile_n * NW + nw) * 16;
     int rows_here, expert = 0;
     const int32_t* order = nullptr;
     if constexpr (GROUPED) {
-        const PlanTile t = find_tile(a.plan, a.n_expert, 16 * MT, tile_m);  // each wave for itself
-        expert = __builtin_amdgcn_readfirstlane(t.expert);
-        if (expert < 0) return;
-        rows_here = __builtin_amdgcn_readfirstlane(t.count);
-        order = a.plan + plan_order_at(a.n_expert) + __builtin_amdgcn_readfirstlane(t.begin);
+        const PlanTile t = reinterpret_cast<const PlanTile*>(a.plan + plan_tiles_at(a.n_expert, a.M))[tile_m];
+        if (t.expert < 0) return;
+        expert = t.expert, rows_here = t.count;
+        order = a.plan + plan_order_at(a.n_expert) + t.begin;
         if (expert == a.n_expert) {  // slots of no expert
             if constexpr (UP) {
                 if (kw == 0)
-                    for (int i = lane; i < rows_here * TILE_N; i += 64)
-                        if (n0 + i % TILE_N < a.N)
-                            static_cast<T*>(a.y)[(int64_t)order[i / TILE_N] * a.y_stride + n0 + i % TILE_N] = (T)0.0f;
+                    for (int i = lane; i < rows_here * 16; i += 64)
+                        if (n0 + i % 16 < a.N) static_cast<T*>(a.y)[(int64_t)order[i / 16] * a.y_stride + n0 + i % 16] = (T)0.0f;
             }
             return;
         }
@@ -42,72 +124,27 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
         rows_here = (int)std::min<int64_t>(16 * MT, a.M - (int64_t)tile_m * 16 * MT);
     }
 
-    const int8_t* xp[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int r = min(16 * i + (lane & 15), rows_here - 1);
-        int64_t src;
-        if constexpr (GROUPED) src = UP ? order[r] / a.top : order[r];
-        else src = (int64_t)tile_m * 16 * MT + r;
-        xp[i] = a.x + src * a.x_stride + 16 * (lane >> 4);
-    }
-    const int8_t* wp[NT];
+    uint32_t x_off[2 * MT], w_off[2 * NT];
+    const int8_t* wb[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        const int n = min(UP ? n0 + (lane & 15) : n0 + 16 * j + (lane & 15), a.N - 1);
-        wp[j] = (UP && j ? a.w2 : a.w) + (int64_t)expert * a.w_expert + (int64_t)n * a.w_stride + 16 * (lane >> 4);
+        wb[j] = uniform((j ? a.w2 : a.w) + (int64_t)expert * a.w_expert + (int64_t)min(n0, a.N - 1) * a.w_stride);
+        weight_rows(w_off + 2 * j, n0, a.N, a.w_stride);
     }
+    const int8_t* xb = GROUPED ? a.x : a.x + (int64_t)tile_m * 16 * MT * a.x_stride;
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+        int src = min(8 * i + lane / 8, rows_here - 1);
+        if constexpr (GROUPED) src = UP ? order[src] / a.top : order[src];
+        x_off[i] = (uint32_t)src * (uint32_t)a.x_stride;
+    }
+    const int stages = (a.K + 127) / 128;
     v4i acc[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = (v4i){0, 0, 0, 0};
+    wave_sums<MT, NT>(acc, reinterpret_cast<int8_t*>(smem) + wave * (kStages * 2048 * (MT + NT)), xb, x_off, wb, w_off, a.K,
+                      stages * kw / KW, stages * (kw + 1) / KW);
 
-    v4i fw[2][NT][4];
-    auto load_w = [&](int c, int into) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int k = 256 * c + 64 * u;
-            const int at = k + 16 * (lane >> 4) < a.K ? k : -16 * (lane >> 4);  // past K: the row's first piece
-#pragma unroll
-            for (int j = 0; j < NT; ++j) fw[into][j][u] = *reinterpret_cast<const v4i*>(wp[j] + at);
-        }
-    };
-    auto multiply = [&](int c, int from) {
-        v4i fx[MT][4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int k = 256 * c + 64 * u;
-            const bool in = k + 16 * (lane >> 4) < a.K;
-            const int at = in ? k : -16 * (lane >> 4);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                fx[i][u] = *reinterpret_cast<const v4i*>(xp[i] + at);
-                if (!in) fx[i][u] = (v4i){0, 0, 0, 0};  // x is zero past K
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fx[i][u], fw[from][j][u], acc[i][j], 0, 0, 0);
-    };
-    const int chunks = (a.K + 255) / 256;
-    if (kw < chunks) load_w(kw, 0);
-    for (int c = kw; c < chunks; c += 2 * KW) {
-        if (c + KW < chunks) load_w(c + KW, 1);
-        multiply(c, 0);
-        if (c + KW < chunks) {
-            if (c + 2 * KW < chunks) load_w(c + 2 * KW, 0);
-            multiply(c + KW, 1);
-        }
-    }
-
-    // ---- the waves' sums together; a lane's sums are column lane % 16 of rows 4 (lane / 16) + v ----
-    auto out = [&](int i, int v, int ln, int sum0, int sum1, int j) {
-        const int r = 16 * i + 4 * (ln >> 4) + v, n = n0 + (UP ? 0 : 16 * j) + (ln & 15);
+    auto out = [&](int i, int v, int sum0, int sum1) {
+        const int r = 16 * i + 4 * (lane >> 4) + v, n = n0 + (lane & 15);
         if (r >= rows_here || n >= a.N) return;
         const int64_t row = GROUPED ? (int64_t)order[r] : (int64_t)tile_m * 16 * MT + r;
         const float xs = a.xs[UP ? row / a.top : row];
@@ -121,10 +158,9 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-#pragma unroll
-                for (int j = 0; j < (UP ? 1 : NT); ++j) out(i, v, lane, acc[i][j][v], acc[i][UP ? 1 : 0][v], j);
+            for (int v = 0; v < 4; ++v) out(i, v, acc[i][0][v], acc[i][NT - 1][v]);
     } else {
+        __syncthreads();  // every wave's stages are done
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -132,66 +168,123 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
 #pragma unroll
                 for (int v = 0; v < 4; ++v) part[nw][kw][(i * NT + j) * 4 + v][lane] = acc[i][j][v];
         __syncthreads();
-        // pieces of 64 sums to a wave
-        for (int p = kw; p < MT * 4 * (UP ? 1 : NT); p += KW) {
-            const int v = p % 4, j = UP ? 0 : p / 4 % NT, i = UP ? p / 4 : p / 4 / NT;
+        for (int p = kw; p < MT * 4; p += KW) {  // 64 sums to a wave
+            const int v = p % 4, i = p / 4;
             int s0 = 0, s1 = 0;
 #pragma unroll
             for (int q = 0; q < KW; ++q) {
-                s0 += part[nw][q][(i * NT + j) * 4 + v][lane];
+                s0 += part[nw][q][i * NT * 4 + v][lane];
                 if constexpr (UP) s1 += part[nw][q][(i * NT + 1) * 4 + v][lane];
             }
-            out(i, v, lane, s0, s1, j);
+            out(i, v, s0, s1);
         }
+    }
+}
+
+// A token's 16 outputs of the down products, a slot to a wave: y = R + sum of the slots' products by their weights, in one launch
+// and without a plan's order.
+template <class T>
+__global__ void __launch_bounds__(1024) i8_token_kernel(I8Args a, CombineArgs c) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float part[16][16];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t token = blockIdx.x / a.tiles_n;
+    const int n0 = (int)blockIdx.x % a.tiles_n * 16, n = n0 + (lane & 15);
+    const int64_t slot = token * c.top + wave;
+    const int expert = __builtin_amdgcn_readfirstlane(c.expert[slot]);
+    if (expert >= 0) {
+        uint32_t x_off[2], w_off[2];
+        weight_rows(w_off, n0, a.N, a.w_stride);
+        x_off[0] = x_off[1] = 0;
+        const int8_t* const wb[1] = {uniform(a.w + (int64_t)expert * a.w_expert + (int64_t)n0 * a.w_stride)};
+        v4i acc[1][1];
+        wave_sums<1, 1>(acc, reinterpret_cast<int8_t*>(smem) + wave * (kStages * 4096), uniform(a.x + slot * a.x_stride), x_off, wb,
+                        w_off, a.K, 0, (a.K + 127) / 128);
+        if (lane < 16)  // row 0; the others are the same
+            part[wave][lane] = i8_value(acc[0][0][0], a.ws[(int64_t)expert * a.N + min(n, a.N - 1)], a.xs[slot]);
+    }
+    __syncthreads();
+    if (threadIdx.x < 16 && n < a.N) {
+        float y = 0.0f;
+        for (int j = 0; j < c.top; ++j)
+            if (c.expert[token * c.top + j] >= 0) y = fmaf(c.weights[token * c.top + j], part[j][threadIdx.x], y);
+        if (c.R) y += c.R[token * c.r_stride + n];
+        static_cast<T*>(c.y)[token * c.y_stride + n] = (T)y;
     }
 }
 
 namespace {
 
-template <I8Mode MODE, int MT, int NT, int KW, int NW, class T>
-hipError_t launch_one(I8Args a, hipStream_t st) {
-    constexpr int tile_n = (MODE == kI8Up ? 8 * NT : 16 * NT) * NW;
-    a.tiles_n = (a.N + tile_n - 1) / tile_n;
-    a.tiles_m = (int)(MODE == kI8Dense ? (a.M + 16 * MT - 1) / (16 * MT) : most_tiles(a.M, a.n_expert, 16 * MT));
-    i8_rows_kernel<MODE, MT, NT, KW, NW, T><<<dim3((unsigned)((int64_t)a.tiles_n * a.tiles_m)), 64 * KW * NW, 0, st>>>(a);
+template <I8Mode MODE, int MT, int KW, int NW, class T>
+hipError_t launch_waves(I8Args a, hipStream_t st) {
+    constexpr int NT = MODE == kI8Up ? 2 : 1;
+    a.tiles_n = (a.N + 16 * NW - 1) / (16 * NW);
+    a.tiles_m = (int)(MODE == kI8Dense ? (a.M + 16 * MT - 1) / (16 * MT) : plan_tiles(a.M, a.n_expert, 16 * MT));
+    constexpr size_t lds = std::max<size_t>(KW * NW * kStages * (MT + NT) * 2048, KW * NW * MT * NT * 1024);
+    i8_rows_kernel<MODE, MT, KW, NW, T>
+        <<<dim3((unsigned)((int64_t)a.tiles_n * a.tiles_m)), 64 * KW * NW, lds, st>>>(a);
     return hipGetLastError();
 }
 
-template <I8Mode MODE, int MT, int NT, class T>
-hipError_t launch_waves(const I8Args& a, hipStream_t st) {
-    const int chunks = (a.K + 255) / 256;
-    if (chunks >= 8) return launch_one<MODE, MT, NT, 8, 1, T>(a, st);
-    if (chunks >= 4) return launch_one<MODE, MT, NT, 4, 1, T>(a, st);
-    return launch_one<MODE, MT, NT, 2, 2, T>(a, st);
+// Waves by the rows of K that there are to share (us; one row / 16 rows): 8 waves on K pay where few weight rows leave CUs
+// idle (2560 x 9728: 6.1 against 6.7 with 4; 2048 x 2048 2.7 and 2.8), 4 elsewhere (9728 x 2560 6.3 against 7.0; 4096 x 4096 4.9
+// and 5.1; 151936 x 2560 62.5 and 69.9). Experts' tiles are many and short: 2 waves (5 tokens x 8 of 128, 768 x 2048 gate and up
+// 20.5 against 20.6 with 4 and 30.4 with 8; 48 tokens 57.8, 60.6, 82.3), and one for rows below 1536 (down products of
+// 2048 x 768, 48 tokens: 41.5 against 41.7 with 2 and 50.4 with 4).
+template <I8Mode MODE, int MT, class T>
+hipError_t launch_rows_of(const I8Args& a, hipStream_t st) {
+    if constexpr (MODE == kI8Dense) {
+        if constexpr (MT < 4)
+            if (a.K >= 2048 && a.N < 4096) return launch_waves<MODE, MT, 8, 1, T>(a, st);
+        return a.K >= 512 ? launch_waves<MODE, MT, 4, 1, T>(a, st) : launch_waves<MODE, MT, 1, 4, T>(a, st);
+    } else {
+        return MODE == kI8Up || a.K >= 1536 ? launch_waves<MODE, MT, 2, 1, T>(a, st) : launch_waves<MODE, MT, 1, 2, T>(a, st);
+    }
 }
 
 template <I8Mode MODE, class T>
-hipError_t launch_rows_of(const I8Args& a, int64_t rows, hipStream_t st) {
-    constexpr int NT = MODE == kI8Up ? 2 : 1;
-    if (rows <= 16) return launch_waves<MODE, 1, NT, T>(a, st);
-    if (rows <= 32) return launch_waves<MODE, 2, NT, T>(a, st);
-    return launch_waves<MODE, 4, NT, T>(a, st);
+hipError_t launch_height(const I8Args& a, int64_t rows, hipStream_t st) {
+    if (rows <= 16) return launch_rows_of<MODE, 1, T>(a, st);
+    if (rows <= 32) return launch_rows_of<MODE, 2, T>(a, st);
+    if constexpr (MODE == kI8Dense) return launch_rows_of<MODE, 4, T>(a, st);
+    return hipErrorInvalidValue;  // no plan's tiles are of another height here
 }
 
 }  // namespace
 
-hipError_t launch_i8_rows(I8Mode mode, int ytype, I8Args a, hipStream_t st) {
+hipError_t launch_i8_rows(I8Mode mode, int ytype, const I8Args& a, hipStream_t st) {
     if (mode == kI8Dense)
-        return ytype == kTypeF16 ? launch_rows_of<kI8Dense, _Float16>(a, a.M, st) : launch_rows_of<kI8Dense, float>(a, a.M, st);
+        return ytype == kTypeF16 ? launch_height<kI8Dense, _Float16>(a, a.M, st) : launch_height<kI8Dense, float>(a, a.M, st);
+    const int height = plan_height(a.M, a.n_expert);
     if (mode == kI8Up)
-        return ytype == kTypeF16 ? launch_rows_of<kI8Up, _Float16>(a, 16, st) : launch_rows_of<kI8Up, float>(a, 16, st);
-    return launch_rows_of<kI8Down, float>(a, 16, st);
+        return ytype == kTypeF16 ? launch_height<kI8Up, _Float16>(a, height, st) : launch_height<kI8Up, float>(a, height, st);
+    return launch_height<kI8Down, float>(a, height, st);
 }
 
-hipError_t launch_i8_product(int ytype, I8Args a, void* ws, size_t ws_bytes, hipStream_t st) {
+hipError_t launch_i8_product(int ytype, const I8Args& a, void* ws, size_t ws_bytes, hipStream_t st) {
     const int most = knob(Knob::I8Rows) >= 0 ? knob(Knob::I8Rows) : 64;
     return a.M <= most ? launch_i8_rows(kI8Dense, ytype, a, st) : launch_i8_gemm(kI8Dense, ytype, a, ws, ws_bytes, st);
 }
 
-hipError_t launch_i8_experts(I8Mode mode, int ytype, I8Args a, hipStream_t st) {
-    const int most = knob(Knob::I8Experts) >= 0 ? knob(Knob::I8Experts) : 12;
-    a.splits = 1;
-    return a.M <= (int64_t)most * a.n_expert ? launch_i8_rows(mode, ytype, a, st) : launch_i8_gemm(mode, ytype, a, nullptr, 0, st);
+static hipError_t launch_experts(I8Mode mode, int ytype, const I8Args& a, hipStream_t st) {
+    return plan_height(a.M, a.n_expert) <= 32 ? launch_i8_rows(mode, ytype, a, st) : launch_i8_gemm(mode, ytype, a, nullptr, 0, st);
+}
+
+hipError_t launch_moe_gate_up(int htype, const I8Args& a, hipStream_t st) { return launch_experts(kI8Up, htype, a, st); }
+
+hipError_t launch_moe_down(int ytype, I8Args a, const CombineArgs& c, hipStream_t st) {
+    // One token, or so few slots that hardly two share an expert: no weight is read more often for it.
+    if (c.top <= 16 && (c.rows == 1 || 2 * a.M <= a.n_expert)) {
+        a.tiles_n = (a.N + 15) / 16;
+        const dim3 grid((unsigned)(a.tiles_n * c.rows));
+        const size_t lds = c.top * kStages * 4096;
+        if (ytype == kTypeF16) i8_token_kernel<_Float16><<<grid, 64 * c.top, lds, st>>>(a, c);
+        else i8_token_kernel<float><<<grid, 64 * c.top, lds, st>>>(a, c);
+        return hipGetLastError();
+    }
+    const hipError_t e = launch_experts(kI8Down, kTypeF32, a, st);
+    return e == hipSuccess ? launch_moe_combine(ytype, c, st) : e;
 }
 
 }  // namespace dcq

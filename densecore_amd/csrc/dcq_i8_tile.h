@@ -1,58 +1,45 @@
-// dcq_i8_tile.h — what the int8 products' kernels (dcq_i8_gemm.hip, dcq_i8_rows.hip) share: where an expert's tile of
-// rows is, and how sums become outputs.
+// dcq_i8_tile.h — what the int8 products' kernels (dcq_i8_gemm.hip, dcq_i8_rows.hip) share.
 #pragma once
 
 #include "dcq_common.h"
 #include "dcq_i8.h"
+
+#pragma clang diagnostic ignored "-Winline-asm"  // M0 in the clobber list (see dma16)
 
 namespace dcq {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
-// The tile_at-th tile of `rows` places of a plan's order: tiles do not cross experts, and those of no expert come last.
-// Found by a wave, an equal share of the experts to each lane. expert = n_expert: of no expert; -1: past the last tile.
-struct PlanTile {
-    int expert, begin, count;
-};
-__device__ __forceinline__ PlanTile find_tile(const int32_t* offsets, int n_expert, int rows, int tile_at) {
-    const int lane = threadIdx.x & 63;
-    const int share = (n_expert + 64) / 64;  // of n_expert + 1 groups
-    const int first = lane * share, last = min(first + share, n_expert + 1);
-    int tiles = 0;
-    for (int e = first; e < last; ++e) tiles += (offsets[e + 1] - offsets[e] + rows - 1) / rows;
-    int before = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int v = __shfl_up(before, d, 64);
-        if (lane >= d) before += v;
-    }
-    before -= tiles;
-    PlanTile t = {-1, 0, 0};
-    const uint64_t mine = __ballot(tile_at >= before && tile_at < before + tiles);
-    if (mine) {
-        const int who = __ffsll((unsigned long long)mine) - 1;
-        int left = tile_at - before;
-        if (lane == who) {
-            for (int e = first; e < last; ++e) {
-                const int at = offsets[e], n = offsets[e + 1] - at, k = (n + rows - 1) / rows;
-                if (left < k) {
-                    t.expert = e, t.begin = at + left * rows, t.count = min(rows, n - left * rows);
-                    break;
-                }
-                left -= k;
-            }
-        }
-        t.expert = __shfl(t.expert, who, 64);
-        t.begin = __shfl(t.begin, who, 64);
-        t.count = __shfl(t.count, who, 64);
-    }
-    return t;
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// 16 bytes per lane from a uniform base + per-lane offset to LDS at lds_base + 16 * lane (lds_base uniform, in M0). The
+// compiler does not count these loads: an explicit wait comes before what they bring is read, and before the barrier that
+// publishes it. PRIVATE: to room that only this wave reads.
+template <bool PRIVATE = false>
+__device__ __forceinline__ void dma16(const void* g, uint32_t off, const void* lds_base) {
+    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
+    if constexpr (PRIVATE)
+        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 ; wave-private" ::"v"(off), "s"(g), "s"(m0)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "s"(m0) : "memory", "m0");
 }
-// No more tiles than this, whatever the experts' shares.
-inline int64_t most_tiles(int64_t slots, int n_expert, int rows) {
-    const int64_t groups = slots < n_expert + 1 ? slots : n_expert + 1;
-    return slots / rows + groups;
+// All but the last N loads have landed: "dcq counted wait" tells the assembly's checks so.
+template <int N>
+__device__ __forceinline__ void counted_wait() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\t;dcq counted wait" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ const int8_t* uniform(const int8_t* p) {  // in scalar registers, as dma16's base is to be
+    const uint64_t u = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = __builtin_amdgcn_readfirstlane((int)(u >> 32));
+    return (const int8_t*)((uint64_t)hi << 32 | lo);
+}
+
+// LDS rows of KB bytes: piece p of 16 bytes of row r lies at p ^ key(r), so that 16 rows' pieces p are on all 64 banks.
+template <int KB>
+__device__ __forceinline__ int piece_key(int row) {
+    return KB == 128 ? (row & 7) ^ ((row >> 3) & 1) : (row >> 2) & 3;
 }
 
 // y = sum * ws * xs, the weight's scale first: sum * ws is the product of the row's own unit, so that neither a small

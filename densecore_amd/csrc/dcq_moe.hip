@@ -207,6 +207,15 @@ __global__ void __launch_bounds__(kPlanThreads) moe_plan_kernel(const int32_t* i
         plan[me] = first;
         if (me == n_expert) plan[n_expert + 1] = slots;
     }
+    int all = 0;
+    for (int w = 0; w < W; ++w) all += mine[w];
+    const int height = plan_height(slots, n_expert);
+    const int t0 = (first + me * (height - 1)) / height, t1 = (first + all + (me + 1) * (height - 1)) / height;
+    PlanTile* tiles = reinterpret_cast<PlanTile*>(plan + plan_tiles_at(n_expert, slots));
+    for (int t = t0 + (int)threadIdx.x; t < t1; t += kPlanThreads) {
+        const int done = (t - t0) * height;
+        tiles[t] = done < all ? PlanTile{me, first + done, min(height, all - done), 0} : PlanTile{-1, 0, 0, 0};
+    }
     for (int w = 0; w < wave; ++w) first += mine[w];
     if (same == 0) return;
     for (int at = begin; at < end; at += 64) {
