@@ -73,7 +73,7 @@ struct PlanTile {
 // Rows of a tile: what the products' kernels take at a time, by the rows that an expert has on average.
 __host__ __device__ inline int plan_height(int64_t slots, int n_expert) {
     const int64_t mean = slots / n_expert;
-    return mean <= 12 ? 16 : mean <= 24 ? 32 : mean <= 40 ? 64 : mean <= 384 ? 128 : 256;
+    return mean <= 12 ? 16 : mean <= 112 ? 64 : 128;
 }
 __host__ __device__ inline int64_t plan_tiles(int64_t slots, int n_expert, int height) {
     return (slots + (int64_t)(n_expert + 1) * (height - 1)) / height;

@@ -22,9 +22,10 @@ __device__ __forceinline__ void put(void* y, int64_t at, float v) {
 // A tile of BM rows x BN weight rows per workgroup of WM x WN waves. kI8Up: half of a wave's columns are gate rows and
 // half the same rows of the up matrix, so that a lane holds both products of an output.
 // T: the output's type; int32_t: the sums themselves, to a plane of `splits`.
-template <I8Mode MODE, int BM, int BN, int WM, int WN, int KB, int ST, class T>
+template <I8Mode MODE, int BM, int BN, int WM, int WN, int ST, class T>
 __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     constexpr int W = WM * WN, TM = BM / WM, TN = BN / WN, MI = TM / 32, NJ = TN / 32;
+    constexpr int KB = 128;  // bytes of an LDS row
     constexpr int P = KB / 16, LR = 64 / P;  // 16-byte pieces of an LDS row; rows of a 1 KB load
     constexpr int LA = BM / LR / W, LB = BN / LR / W;  // loads of a wave and stage
     constexpr int Q = KB / 32;  // products' steps of a stage
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
         a_off[i] = (uint32_t)src * (uint32_t)a.x_stride + 16u * (uint32_t)((lane % P) ^ piece_key<KB>(r));
     }
     const int stages = (a.K + KB - 1) / KB;
-    const int stps = a.stps * (128 / KB), s_begin = split * stps, s_end = min(stages, s_begin + stps);
+    const int s_begin = split * a.stps, s_end = min(stages, s_begin + a.stps);
     const int tail_pieces = (a.K % KB) / 16;  // 0: the last stage is whole
 
     // loads from .. to of the wave's LA + LB
@@ -353,30 +354,28 @@ __global__ void __launch_bounds__(256) i8_join_kernel(I8Args a, const int32_t* p
 
 namespace {
 
-template <I8Mode MODE, int BM, int BN, int WM, int WN, int KB, int ST, class T>
+template <I8Mode MODE, int BM, int BN, int WM, int WN, int ST, class T>
 hipError_t launch_tile(I8Args a, hipStream_t st) {
     constexpr int tile_n = MODE == kI8Up ? BN / 2 : BN;
     a.tiles_n = (a.N + tile_n - 1) / tile_n;
     a.tiles_m = (int)(MODE == kI8Dense ? (a.M + BM - 1) / BM : plan_tiles(a.M, a.n_expert, BM));
     constexpr int out = MODE == kI8Up ? BN / WN / 2 : BN / WN;
-    const size_t lds = std::max<size_t>(ST * (size_t)(BM + BN) * KB, (size_t)WM * WN * 32 * (out + 4) * 4);
+    const size_t lds = std::max<size_t>(ST * (size_t)(BM + BN) * 128, (size_t)WM * WN * 32 * (out + 4) * 4);
     const int64_t groups = (int64_t)a.tiles_n * a.tiles_m * a.splits;
-    auto fn = i8_gemm_kernel<MODE, BM, BN, WM, WN, KB, ST, T>;
+    auto fn = i8_gemm_kernel<MODE, BM, BN, WM, WN, ST, T>;
     fn<<<dim3((unsigned)groups), 64 * WM * WN, lds, st>>>(a);
     return hipGetLastError();
 }
 
 template <I8Mode MODE, class T>
 hipError_t launch_shape(I8Args a, int shape, hipStream_t st) {
-    switch (shape) {
-        case 0: return launch_tile<MODE, 64, 128, 2, 2, 64, 4, T>(a, st);
-        case 1: return launch_tile<MODE, 128, 128, 2, 2, 64, 4, T>(a, st);
-        case 3: return launch_tile<MODE, 64, 128, 2, 2, 128, 2, T>(a, st);
-        case 4: return launch_tile<MODE, 128, 128, 2, 2, 128, 2, T>(a, st);
-        case 5: return launch_tile<MODE, 128, 128, 2, 2, 64, 2, T>(a, st);
-        case 6: return launch_tile<MODE, 128, 128, 2, 2, 64, 3, T>(a, st);
-        default: return launch_tile<MODE, 256, 256, 2, 4, 128, 2, T>(a, st);
+    if constexpr (MODE == kI8Dense) {
+        if (shape == 0) return launch_tile<MODE, 64, 64, 2, 2, 4, T>(a, st);
+        if (shape == 3) return launch_tile<MODE, 256, 256, 2, 4, 2, T>(a, st);
+    } else {
+        if (shape == 1) return launch_tile<MODE, 64, 128, 2, 2, 2, T>(a, st);
     }
+    return launch_tile<MODE, 128, 128, 2, 2, 2, T>(a, st);
 }
 
 template <class T>
@@ -398,22 +397,18 @@ hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, size_t ws_
     const int forced = knob(Knob::I8Tile);
     if (mode != kI8Dense) {
         const int height = plan_height(a.M, a.n_expert);
-        const int shape = forced >= 0 ? forced : height == 256 ? 2 : height == 128 ? 1 : 0;
+        const int shape = height == 128 ? 2 : 1;
         if (mode == kI8Up)
             return ytype == kTypeF16 ? launch_shape<kI8Up, _Float16>(a, shape, st) : launch_shape<kI8Up, float>(a, shape, st);
         return launch_shape<kI8Down, float>(a, shape, st);
     }
-    auto tiles = [&](int bm, int bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
-    int shape = forced >= 0 ? forced : tiles(256, 256) >= 200 ? 2 : a.M > 64 ? 1 : 0;
-    const int64_t count = shape == 2 ? tiles(256, 256) : shape == 1 ? tiles(128, 128) : tiles(64, 128);
-    const int forced_split = knob(Knob::I8Split);
+    auto tiles = [&](int64_t bm, int64_t bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
+    const int shape = forced >= 0 ? forced : tiles(256, 256) >= 200 ? 3 : tiles(128, 128) >= 240 ? 2 : 0;
     int splits = 1;
-    if (count < 256) {
-        splits = (int)std::min<int64_t>({512 / count, stages / 4, (int64_t)(ws_bytes / 4) / (a.M * a.N)});
-        splits = std::max(splits, 1);
-    }
-    if (forced_split > 0) splits = std::min<int64_t>(forced_split, std::max<int64_t>(1, (int64_t)(ws_bytes / 4) / (a.M * a.N)));
-    if (splits == 1)
+    if (shape == 0 && stages >= 32) splits = (int)std::max<int64_t>(1, 256 / tiles(64, 64));
+    if (knob(Knob::I8Split) > 0) splits = knob(Knob::I8Split);
+    splits = (int)std::min<int64_t>({splits, stages / 8, (int64_t)(ws_bytes / 4) / (a.M * a.N)});
+    if (splits <= 1)
         return ytype == kTypeF16 ? launch_shape<kI8Dense, _Float16>(a, shape, st) : launch_shape<kI8Dense, float>(a, shape, st);
     a.stps = (stages + splits - 1) / splits;
     a.splits = (stages + a.stps - 1) / a.stps;

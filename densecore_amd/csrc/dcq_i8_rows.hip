@@ -243,32 +243,31 @@ hipError_t launch_rows_of(const I8Args& a, hipStream_t st) {
     }
 }
 
-template <I8Mode MODE, class T>
-hipError_t launch_height(const I8Args& a, int64_t rows, hipStream_t st) {
-    if (rows <= 16) return launch_rows_of<MODE, 1, T>(a, st);
-    if (rows <= 32) return launch_rows_of<MODE, 2, T>(a, st);
-    if constexpr (MODE == kI8Dense) return launch_rows_of<MODE, 4, T>(a, st);
-    return hipErrorInvalidValue;  // no plan's tiles are of another height here
+template <class T>
+hipError_t launch_dense(const I8Args& a, hipStream_t st) {
+    if (a.M <= 16) return launch_rows_of<kI8Dense, 1, T>(a, st);
+    if (a.M <= 32) return launch_rows_of<kI8Dense, 2, T>(a, st);
+    return launch_rows_of<kI8Dense, 4, T>(a, st);
 }
 
 }  // namespace
 
+// Experts' tiles here are of 16 rows (plan_height).
 hipError_t launch_i8_rows(I8Mode mode, int ytype, const I8Args& a, hipStream_t st) {
-    if (mode == kI8Dense)
-        return ytype == kTypeF16 ? launch_height<kI8Dense, _Float16>(a, a.M, st) : launch_height<kI8Dense, float>(a, a.M, st);
-    const int height = plan_height(a.M, a.n_expert);
+    if (mode == kI8Dense) return ytype == kTypeF16 ? launch_dense<_Float16>(a, st) : launch_dense<float>(a, st);
     if (mode == kI8Up)
-        return ytype == kTypeF16 ? launch_height<kI8Up, _Float16>(a, height, st) : launch_height<kI8Up, float>(a, height, st);
-    return launch_height<kI8Down, float>(a, height, st);
+        return ytype == kTypeF16 ? launch_rows_of<kI8Up, 1, _Float16>(a, st) : launch_rows_of<kI8Up, 1, float>(a, st);
+    return launch_rows_of<kI8Down, 1, float>(a, st);
 }
 
 hipError_t launch_i8_product(int ytype, const I8Args& a, void* ws, size_t ws_bytes, hipStream_t st) {
-    const int most = knob(Knob::I8Rows) >= 0 ? knob(Knob::I8Rows) : 64;
-    return a.M <= most ? launch_i8_rows(kI8Dense, ytype, a, st) : launch_i8_gemm(kI8Dense, ytype, a, ws, ws_bytes, st);
+    const bool few = knob(Knob::I8Rows) >= 0 ? a.M <= knob(Knob::I8Rows)
+                                             : a.M <= 32 || (a.M <= 64 && a.N < 65536) || (a.M <= 256 && a.N <= 2048 && a.K <= 4096);
+    return few ? launch_i8_rows(kI8Dense, ytype, a, st) : launch_i8_gemm(kI8Dense, ytype, a, ws, ws_bytes, st);
 }
 
 static hipError_t launch_experts(I8Mode mode, int ytype, const I8Args& a, hipStream_t st) {
-    return plan_height(a.M, a.n_expert) <= 32 ? launch_i8_rows(mode, ytype, a, st) : launch_i8_gemm(mode, ytype, a, nullptr, 0, st);
+    return plan_height(a.M, a.n_expert) == 16 ? launch_i8_rows(mode, ytype, a, st) : launch_i8_gemm(mode, ytype, a, nullptr, 0, st);
 }
 
 hipError_t launch_moe_gate_up(int htype, const I8Args& a, hipStream_t st) { return launch_experts(kI8Up, htype, a, st); }

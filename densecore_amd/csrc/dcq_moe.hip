@@ -13,39 +13,42 @@ __device__ __forceinline__ uint64_t order_key(double v) {
     const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);  // -0 as 0
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
-__device__ __forceinline__ uint64_t dpp64(uint64_t v, int ctrl_at) {
-    const int lo = (int)(uint32_t)v, hi = (int)(uint32_t)(v >> 32);
-    int l, h;
-    switch (ctrl_at) {
-        case 0: l = dpp_mov<0xB1>(lo), h = dpp_mov<0xB1>(hi); break;
-        case 1: l = dpp_mov<0x4E>(lo), h = dpp_mov<0x4E>(hi); break;
-        case 2: l = dpp_mov<0x141>(lo), h = dpp_mov<0x141>(hi); break;
-        case 3: l = dpp_mov<0x140>(lo), h = dpp_mov<0x140>(hi); break;
-        case 4: l = __shfl_xor(lo, 16, 64), h = __shfl_xor(hi, 16, 64); break;
-        default: l = __shfl_xor(lo, 32, 64), h = __shfl_xor(hi, 32, 64); break;
-    }
-    return (uint64_t)(uint32_t)h << 32 | (uint32_t)l;
+constexpr uint64_t kNoKey = 0x000FFFFFFFFFFFFFull;  // order_key(-infinity)
+constexpr uint32_t kNoHigh = (uint32_t)(kNoKey >> 32);
+
+// The largest of a wave's values, in a scalar register: within rows of 16 lanes, then from row to row into lane 63.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x140, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x142, 0xA, 0xF, false));  // row_bcast15: rows 1, 3
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x143, 0xC, 0xF, false));  // row_bcast31: rows 2, 3
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-    for (int i = 0; i < 6; ++i) {
-        const uint64_t o = dpp64(v, i);
-        v = o > v ? o : v;
-    }
-    return v;
+__device__ __forceinline__ double lane_xor(double v, int d) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)u, d, 64), hi = (uint32_t)__shfl_xor((int)(u >> 32), d, 64);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
-    for (int i = 0; i < 6; ++i) v += __longlong_as_double((long long)dpp64((uint64_t)__double_as_longlong(v), i));
+    for (int d = 1; d < 64; d *= 2) v += lane_xor(v, d);
     return v;
 }
-
-constexpr uint64_t kNoKey = 0x000FFFFFFFFFFFFFull;  // order_key(-infinity)
+__device__ __forceinline__ double from_lane(double v, int lane) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane),
+                   hi = (uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
 
 }  // namespace
 
 // A token per wave, expert lane + 64 i in register i. Scores in 64 bits, so that what is chosen is the definition's
-// choice and not that of a rounding; the best are taken one at a time.
+// choice and not that of a rounding. The best are taken one at a time, by the upper half of their keys; the lower halves and
+// the experts' numbers decide between the few that share one.
+// 8192 tokens, 256 experts in 8 groups, best 8: VALU, which 64-bit exponentials and quotients keep busy.
 constexpr int kRouteWaves = 4;
 template <class T, int EPL>
 __global__ void __launch_bounds__(64 * kRouteWaves) moe_route_kernel(RouteArgs a) {
@@ -61,6 +64,9 @@ __global__ void __launch_bounds__(64 * kRouteWaves) moe_route_kernel(RouteArgs a
     for (int i = 0; i < EPL; ++i) {
         const int e = lane + 64 * i;
         v[i] = e < a.n_expert ? (float)x[e] : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
         bad |= !(v[i] < INFINITY);
         top = fmaxf(top, v[i]);
     }
@@ -77,9 +83,9 @@ __global__ void __launch_bounds__(64 * kRouteWaves) moe_route_kernel(RouteArgs a
             score[i] = v[i] == -INFINITY ? 0.0 : exp((double)v[i] - (double)top);
             sum += score[i];
         }
-        sum = wave_sum(sum);
+        const double inv = 1.0 / wave_sum(sum);
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) score[i] = score[i] / sum;
+        for (int i = 0; i < EPL; ++i) score[i] *= inv;
     }
     uint64_t key[EPL];
 #pragma unroll
@@ -97,60 +103,71 @@ __global__ void __launch_bounds__(64 * kRouteWaves) moe_route_kernel(RouteArgs a
         if (a.n_group > 1) shared[wave][e] = c;
     }
     if (a.n_group > 1) {
+        // `share` lanes to a group, each the best two of its part, then of each other's
+        const int per = a.n_expert / a.n_group, bits = 31 - __clz(64 / a.n_group), share = 1 << bits;
+        const int group = lane >> bits;
         __syncthreads();
-        const int per = a.n_expert / a.n_group;
         double b1 = -INFINITY, b2 = -INFINITY;
-        if (lane < a.n_group)
-            for (int e = 0; e < per; ++e) {
-                const double c = shared[wave][lane * per + e];
-                b2 = c > b1 ? b1 : c > b2 ? c : b2;
-                b1 = c > b1 ? c : b1;
+        if (group < a.n_group)
+            for (int e = lane & (share - 1); e < per; e += share) {
+                const double c = shared[wave][group * per + e];
+                b2 = fmax(b2, fmin(b1, c));
+                b1 = fmax(b1, c);
             }
+        for (int d = 1; d < share; d *= 2) {
+            const double o1 = lane_xor(b1, d), o2 = lane_xor(b2, d);
+            b2 = fmax(fmax(b2, o2), fmin(b1, o1));
+            b1 = fmax(b1, o1);
+        }
         const double worth = a.group_best == 2 && b2 > -INFINITY ? b1 + b2 : b1;
-        const uint64_t wk = order_key(worth);
         int ahead = 0;
         for (int g = 0; g < a.n_group; ++g) {
-            const uint64_t o = (uint64_t)(uint32_t)__shfl((int)(uint32_t)(wk >> 32), g, 64) << 32 |
-                               (uint32_t)__shfl((int)(uint32_t)wk, g, 64);
-            ahead += o > wk || (o == wk && g < lane);
+            const double o = from_lane(worth, g << bits);
+            ahead += o > worth || (o == worth && g < group);
         }
-        const uint64_t kept = __ballot(lane < a.n_group && ahead < a.topk_group);
+        const uint64_t kept = __ballot(group < a.n_group && ahead < a.topk_group);  // bit g * share: group g's
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
             const int e = lane + 64 * i;
-            if (e >= a.n_expert || !(kept >> (e / per) & 1)) key[i] = kNoKey;
+            if (e >= a.n_expert || !(kept >> (e / per << bits) & 1)) key[i] = kNoKey;
         }
     }
     int my_id = -1;
     double my_score = 0.0;
     for (int j = 0; j < a.k; ++j) {
-        uint64_t best = key[0];
-        int at = 0;
+        uint32_t best = (uint32_t)(key[0] >> 32);
 #pragma unroll
-        for (int i = 1; i < EPL; ++i)
-            if (key[i] > best) best = key[i], at = i;
-        const uint64_t most = wave_max(best);
-        if (most <= kNoKey) break;
-        uint64_t who = __ballot(best == most);
-        int e = lane + 64 * at;
-        if (who & (who - 1)) {  // equal scores: the lowest expert
-            int low = best == most ? e : 0x7FFFFFFF;
+        for (int i = 1; i < EPL; ++i) best = max(best, (uint32_t)(key[i] >> 32));
+        const uint32_t most = wave_max(best);
+        if (most <= kNoHigh) break;
+        // who has it: usually one lane in one register
+        int e = 0, count = 0;
 #pragma unroll
-            for (int d = 1; d < 64; d *= 2) low = min(low, __shfl_xor(low, d, 64));
-            who = __ballot(best == most && e == low);
+        for (int i = EPL - 1; i >= 0; --i) {
+            const uint64_t who = __ballot((uint32_t)(key[i] >> 32) == most);
+            count += (int)__popcll(who);
+            if (who) e = 64 * i + (int)__builtin_ctzll(who);
         }
-        const int from = __ffsll((unsigned long long)who) - 1;
-        double s = score[0];
-#pragma unroll
-        for (int i = 1; i < EPL; ++i) s = at == i ? score[i] : s;
-        e = __shfl(e, from, 64);
-        s = __shfl(s, from, 64);
-        if (lane == j) my_id = e, my_score = s;
-        if (lane == from) {
+        if (count > 1) {  // the largest lower half, then the lowest expert
+            uint32_t low = 0;
 #pragma unroll
             for (int i = 0; i < EPL; ++i)
-                if (at == i) key[i] = kNoKey;
+                if ((uint32_t)(key[i] >> 32) == most) low = max(low, (uint32_t)key[i]);
+            const uint64_t whole = (uint64_t)most << 32 | wave_max(low);
+#pragma unroll
+            for (int i = EPL - 1; i >= 0; --i) {
+                const uint64_t who = __ballot(key[i] == whole);
+                if (who) e = 64 * i + (int)__builtin_ctzll(who);
+            }
         }
+        double s = score[0];
+#pragma unroll
+        for (int i = 1; i < EPL; ++i) s = e >> 6 == i ? score[i] : s;
+        s = from_lane(s, e & 63);
+        if (lane == j) my_id = e, my_score = s;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i)
+            if (e == lane + 64 * i) key[i] = kNoKey;
     }
     double w = my_id >= 0 ? (double)a.scale * my_score : 0.0;
     if (a.renorm) {
@@ -178,10 +195,11 @@ hipError_t launch_moe_route(int type, const RouteArgs& a, hipStream_t st) {
 }
 
 // A workgroup per expert (and one for the slots of none) looks at all slots: those of lower experts give its place, its
-// own go there in their order. No atomics and no second launch; the slots' numbers come from the caches.
+// own go there in their order. No atomics and no second launch; the slots' numbers come from the caches, 8 loads of a wave
+// on their way at a time (12568 slots of 128 experts: 13.2 us with one).
 constexpr int kPlanThreads = 1024;
 __global__ void __launch_bounds__(kPlanThreads) moe_plan_kernel(const int32_t* ids, int slots, int n_expert, int32_t* plan) {
-    constexpr int W = kPlanThreads / 64;
+    constexpr int W = kPlanThreads / 64, G = 8;
     __shared__ int less[W], mine[W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int me = blockIdx.x;  // n_expert: none
@@ -189,26 +207,43 @@ __global__ void __launch_bounds__(kPlanThreads) moe_plan_kernel(const int32_t* i
     int32_t* expert = plan + plan_expert_at(n_expert, slots);
     // a run of slots to each wave
     const int run = ((slots + W - 1) / W + 63) / 64 * 64, begin = min(wave * run, slots), end = min(begin + run, slots);
+    int e[G];
+    auto load = [&](int at) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int i = at + 64 * g + lane;
+            e[g] = i < end ? ids[i] : 0x7FFFFFFF;
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int i = at + 64 * g + lane;
+            e[g] = i >= end ? 0x7FFFFFFF : e[g] < 0 || e[g] >= n_expert ? n_expert : e[g];
+        }
+    };
     int below = 0, same = 0;
-    for (int at = begin; at < end; at += 64) {
-        const int i = at + lane;
-        int e = i < end ? ids[i] : 0x7FFFFFFF;
-        const bool in = i < end;
-        e = e < 0 || e >= n_expert ? n_expert : e;
-        below += (int)__popcll(__ballot(in && e < me));
-        same += (int)__popcll(__ballot(in && e == me));
-        if (in && at / 64 % (int)gridDim.x == me) expert[i] = e < n_expert ? e : -1;
+    for (int at = begin; at < end; at += 64 * G) {
+        load(at);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            below += (int)__popcll(__ballot(e[g] < me));
+            same += (int)__popcll(__ballot(e[g] == me));
+            const int i = at + 64 * g + lane;
+            if (i < end && (at / 64 + g) % (int)gridDim.x == me) expert[i] = e[g] < n_expert ? e[g] : -1;
+        }
     }
     if (lane == 0) less[wave] = below, mine[wave] = same;
     __syncthreads();
-    int first = 0;
-    for (int w = 0; w < W; ++w) first += less[w];
+    int first = 0, all = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        first += less[w];
+        all += mine[w];
+        before += w < wave ? mine[w] : 0;
+    }
     if (threadIdx.x == 0) {
         plan[me] = first;
         if (me == n_expert) plan[n_expert + 1] = slots;
     }
-    int all = 0;
-    for (int w = 0; w < W; ++w) all += mine[w];
     const int height = plan_height(slots, n_expert);
     const int t0 = (first + me * (height - 1)) / height, t1 = (first + all + (me + 1) * (height - 1)) / height;
     PlanTile* tiles = reinterpret_cast<PlanTile*>(plan + plan_tiles_at(n_expert, slots));
@@ -216,15 +251,16 @@ __global__ void __launch_bounds__(kPlanThreads) moe_plan_kernel(const int32_t* i
         const int done = (t - t0) * height;
         tiles[t] = done < all ? PlanTile{me, first + done, min(height, all - done), 0} : PlanTile{-1, 0, 0, 0};
     }
-    for (int w = 0; w < wave; ++w) first += mine[w];
     if (same == 0) return;
-    for (int at = begin; at < end; at += 64) {
-        const int i = at + lane;
-        int e = i < end ? ids[i] : 0x7FFFFFFF;
-        e = e < 0 || e >= n_expert ? n_expert : e;
-        const uint64_t hit = __ballot(i < end && e == me);
-        if (hit >> lane & 1) order[first + (int)__popcll(hit & ((1ull << lane) - 1))] = i;
-        first += (int)__popcll(hit);
+    first += before;
+    for (int at = begin; at < end; at += 64 * G) {
+        if (run > 64 * G) load(at);  // else what the first pass left
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const uint64_t hit = __ballot(e[g] == me);
+            if (hit >> lane & 1) order[first + (int)__popcll(hit & ((1ull << lane) - 1))] = at + 64 * g + lane;
+            first += (int)__popcll(hit);
+        }
     }
 }
 

@@ -132,7 +132,7 @@ def test_rms_norm_of_zeros_and_of_values_whose_squares_overflow(dev):
 
 # ---------------------------------------------------------------- products
 SHAPES = [(1, 1, 16), (1, 9728, 2560), (1, 33, 131056), (3, 65, 272), (5, 1000, 768), (16, 17, 4096), (17, 300, 528), (31, 2560, 1024),
-          (33, 64, 2048), (48, 513, 1040), (61, 2560, 9728), (64, 129, 112), (65, 100, 256), (100, 2560, 1040), (128, 128, 128),
+          (33, 64, 2048), (48, 513, 1040), (61, 2560, 9728), (40, 65536, 80), (64, 129, 112), (65, 100, 256), (100, 2560, 1040), (90, 200, 5008), (128, 128, 128), (250, 64, 65536),
           (129, 257, 400), (200, 1111, 3088), (256, 2048, 2048), (300, 5000, 656), (513, 770, 144), (700, 9728, 2560),
           (1025, 4096, 2064), (2048, 8192, 2048), (4099, 1500, 272)]
 
@@ -283,7 +283,8 @@ def some_ids(r, m, e, k, kind):
 EXPERTS = [(1, 8, 2, 64, 64, "mixed"), (5, 128, 8, 768, 2048, "mixed"), (1, 1, 1, 17, 16, "mixed"), (7, 16, 3, 100, 272, "padded"),
            (40, 4, 2, 130, 528, "padded"), (33, 8, 4, 65, 144, "one"), (20, 512, 6, 40, 80, "mixed"), (16, 3, 3, 48, 1040, "twice"),
            (9, 8, 2, 33, 64, "none"), (64, 16, 4, 96, 256, "mixed"), (150, 4, 2, 200, 400, "padded"), (300, 2, 2, 257, 144, "mixed"),
-           (513, 8, 1, 64, 128, "mixed"), (700, 60, 4, 80, 160, "padded"), (1000, 3, 2, 300, 272, "mixed"), (260, 2, 2, 128, 2064, "one")]
+           (513, 8, 1, 64, 128, "mixed"), (700, 60, 4, 80, 160, "padded"), (1000, 3, 2, 300, 272, "mixed"), (260, 2, 2, 128, 2064, "one"),
+           (60, 8, 4, 150, 528, "padded"), (130, 4, 1, 300, 1040, "mixed")]
 
 
 @pytest.mark.parametrize("m,e,k,n,width,kind", EXPERTS)
