@@ -13,18 +13,17 @@ __device__ __forceinline__ uint64_t order_key(double v) {
     const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);  // -0 as 0
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
-constexpr uint64_t kNoKey = 0x000FFFFFFFFFFFFFull;  // order_key(-infinity)
-constexpr uint32_t kNoHigh = (uint32_t)(kNoKey >> 32);
+constexpr uint32_t kNoHigh = 0x000FFFFF;  // of order_key(-infinity)
 
-// The largest of a wave's values, in a scalar register: within rows of 16 lanes, then from row to row into lane 63.
+// The largest of a wave's values, in a scalar register: by lanes within rows of 16, then of the four rows.
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xF, 0xF, false));
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xF, 0xF, false));
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xF, 0xF, false));
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x140, 0xF, 0xF, false));
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x142, 0xA, 0xF, false));  // row_bcast15: rows 1, 3
-    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x143, 0xC, 0xF, false));  // row_bcast31: rows 2, 3
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, true));
+    const uint32_t r0 = __builtin_amdgcn_readlane((int)v, 0), r1 = __builtin_amdgcn_readlane((int)v, 16),
+                   r2 = __builtin_amdgcn_readlane((int)v, 32), r3 = __builtin_amdgcn_readlane((int)v, 48);
+    return max(max(r0, r1), max(r2, r3));
 }
 __device__ __forceinline__ double lane_xor(double v, int d) {
     const uint64_t u = (uint64_t)__double_as_longlong(v);
@@ -52,7 +51,7 @@ __device__ __forceinline__ double from_lane(double v, int lane) {
 constexpr int kRouteWaves = 4;
 template <class T, int EPL>
 __global__ void __launch_bounds__(64 * kRouteWaves) moe_route_kernel(RouteArgs a) {
-    __shared__ double shared[kRouteWaves][64 * EPL];
+    __shared__ double shared[kRouteWaves][64 * EPL], scores[kRouteWaves][64 * EPL];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row_at = (int64_t)blockIdx.x * kRouteWaves + wave;
     const int64_t row = row_at < a.rows ? row_at : a.rows - 1;
@@ -87,11 +86,12 @@ __global__ void __launch_bounds__(64 * kRouteWaves) moe_route_kernel(RouteArgs a
 #pragma unroll
         for (int i = 0; i < EPL; ++i) score[i] *= inv;
     }
-    uint64_t key[EPL];
+    uint32_t high[EPL], low[EPL];  // order_key's halves
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
         const int e = lane + 64 * i;
         double c = score[i];
+        scores[wave][e] = c;
         bool out = bad || v[i] == -INFINITY;
         if (a.bias && e < a.n_expert) {
             const float b = a.bias[e];
@@ -99,14 +99,15 @@ __global__ void __launch_bounds__(64 * kRouteWaves) moe_route_kernel(RouteArgs a
             c += (double)b;
         }
         c = out ? -INFINITY : c;
-        key[i] = order_key(c);
+        const uint64_t key = order_key(c);
+        high[i] = (uint32_t)(key >> 32), low[i] = (uint32_t)key;
         if (a.n_group > 1) shared[wave][e] = c;
     }
+    __syncthreads();
     if (a.n_group > 1) {
         // `share` lanes to a group, each the best two of its part, then of each other's
         const int per = a.n_expert / a.n_group, bits = 31 - __clz(64 / a.n_group), share = 1 << bits;
         const int group = lane >> bits;
-        __syncthreads();
         double b1 = -INFINITY, b2 = -INFINITY;
         if (group < a.n_group)
             for (int e = lane & (share - 1); e < per; e += share) {
@@ -129,46 +130,40 @@ __global__ void __launch_bounds__(64 * kRouteWaves) moe_route_kernel(RouteArgs a
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
             const int e = lane + 64 * i;
-            if (e >= a.n_expert || !(kept >> (e / per << bits) & 1)) key[i] = kNoKey;
+            if (e >= a.n_expert || !(kept >> (e / per << bits) & 1)) high[i] = 0;
         }
     }
     int my_id = -1;
-    double my_score = 0.0;
     for (int j = 0; j < a.k; ++j) {
-        uint32_t best = (uint32_t)(key[0] >> 32);
+        uint32_t best = high[0];
 #pragma unroll
-        for (int i = 1; i < EPL; ++i) best = max(best, (uint32_t)(key[i] >> 32));
+        for (int i = 1; i < EPL; ++i) best = max(best, high[i]);
         const uint32_t most = wave_max(best);
         if (most <= kNoHigh) break;
         // who has it: usually one lane in one register
         int e = 0, count = 0;
 #pragma unroll
         for (int i = EPL - 1; i >= 0; --i) {
-            const uint64_t who = __ballot((uint32_t)(key[i] >> 32) == most);
+            const uint64_t who = __ballot(high[i] == most);
             count += (int)__popcll(who);
             if (who) e = 64 * i + (int)__builtin_ctzll(who);
         }
         if (count > 1) {  // the largest lower half, then the lowest expert
-            uint32_t low = 0;
+            uint32_t lower = 0;
 #pragma unroll
-            for (int i = 0; i < EPL; ++i)
-                if ((uint32_t)(key[i] >> 32) == most) low = max(low, (uint32_t)key[i]);
-            const uint64_t whole = (uint64_t)most << 32 | wave_max(low);
+            for (int i = 0; i < EPL; ++i) lower = max(lower, high[i] == most ? low[i] : 0u);
+            lower = wave_max(lower);
 #pragma unroll
             for (int i = EPL - 1; i >= 0; --i) {
-                const uint64_t who = __ballot(key[i] == whole);
+                const uint64_t who = __ballot(high[i] == most && low[i] == lower);
                 if (who) e = 64 * i + (int)__builtin_ctzll(who);
             }
         }
-        double s = score[0];
+        my_id = lane == j ? e : my_id;
 #pragma unroll
-        for (int i = 1; i < EPL; ++i) s = e >> 6 == i ? score[i] : s;
-        s = from_lane(s, e & 63);
-        if (lane == j) my_id = e, my_score = s;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-            if (e == lane + 64 * i) key[i] = kNoKey;
+        for (int i = 0; i < EPL; ++i) high[i] = lane + 64 * i == e ? 0u : high[i];
     }
+    const double my_score = my_id >= 0 ? scores[wave][my_id] : 0.0;
     double w = my_id >= 0 ? (double)a.scale * my_score : 0.0;
     if (a.renorm) {
         const double sum = wave_sum(my_score);
