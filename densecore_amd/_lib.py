@@ -842,25 +842,42 @@ def beam_select(logits, beam_scores, n_out, scores=None, parents=None, tokens=No
 
 
 # ---------------------------------------------------------------- layers in 8-bit integers, dense and of experts
-# int8 rows q with fp32 scales s: element k of row r stands for q[r, k] * s[r].
-def _here(device, *others):
-    """Raise ValueError unless the tensors are all on one device, the current one: a call launches there."""
-    at = device.index
-    if at != _torch.cuda.current_device():
-        raise ValueError(f"tensors on {device}, the current device is cuda:{_torch.cuda.current_device()}")
-    for t in others:
+# int8 rows q with fp32 scales s: element k of row r stands for q[r, k] * s[r]. A call of these has up to a dozen tensors:
+# each is looked at once, and what is made here not at all.
+def _here(stream, *tensors):
+    """The stream to launch on. Raises ValueError unless the tensors are on the current device, where a call launches."""
+    at = _torch._C._cuda_getDevice()
+    for t in tensors:
         if t is not None and t.get_device() != at:
-            raise ValueError(f"tensors on {device} and {t.device}")
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{at}")
+    return _raw_stream() if stream is None else stream
 
 
 def _float_rows(name, t, shape):
-    """Row stride (elements) and type (F32 or F16) of float rows."""
-    half = getattr(t, "dtype", None) is _torch.float16
-    return _rows_of(name, t, _torch.float16 if half else _F32, shape), 1 if half else 0
+    """Row stride in bytes and type (F32 or F16) of float rows."""
+    if getattr(t, "dtype", None) is _torch.float16:
+        return 2 * _rows_of(name, t, _torch.float16, shape), 1
+    return 4 * _rows_of(name, t, _F32, shape), 0
 
 
-def _i8_rows(name, t, shape):
-    return _rows_of(name, t, _torch.int8, shape)
+def _out_rows(name, t, dtype, shape, device, stream):
+    """An output of float rows: (it, its row stride in bytes, its type); a new one is of `dtype`, fp32 unless given."""
+    if t is None:
+        dtype = dtype or _F32
+        if dtype is not _F32 and dtype is not _torch.float16:
+            raise ValueError(f"dtype: {dtype}, expected torch.float32 or torch.float16")
+        t = _new(shape, dtype, device, stream)
+        return t, shape[1] * (4 if dtype is _F32 else 2), 0 if dtype is _F32 else 1
+    return (t, *_float_rows(name, t, shape))
+
+
+def _i8_out(q, s, shape, device, stream):
+    """int8 rows and scales to write: (q, its row stride, s)."""
+    if q is None:
+        q, stride = _new(shape, _torch.int8, device, stream), shape[1]
+    else:
+        stride = _rows_of("q", q, _torch.int8, shape)
+    return q, stride, _made("s", s, _F32, shape[:1], device, stream)
 
 
 def _vector(name, t, n):
@@ -870,34 +887,36 @@ def _vector(name, t, n):
 
 def quantize_i8(x, q=None, s=None, stream=None):
     """x fp32 or fp16 [M, K] -> (q int8 [M, K], s fp32 [M]): s = max |x| / 127 of each row, q the nearest steps."""
-    torch = _torch or _t()
+    _torch or _t()
     m, k = shape = _table_shape("x", x)
     x_stride, typ = _float_rows("x", x, shape)
-    q = _made("q", q, torch.int8, shape, x.device, stream, rows=True)
-    s = _made("s", s, _F32, (m,), x.device, stream)
-    _here(x.device, q, s)
-    _check("dcq_quantize_i8", lib().dcq_quantize_i8(typ, x.data_ptr(), m, k, x_stride * (2 if typ else 4), q.data_ptr(),
-                                                    _i8_rows("q", q, shape), s.data_ptr(), _stream(stream)))
+    q, q_stride, s = _i8_out(q, s, shape, x.device, stream)
+    status = lib().dcq_quantize_i8(typ, x.data_ptr(), m, k, x_stride, q.data_ptr(), q_stride, s.data_ptr(),
+                                   _here(stream, x, q, s))
+    if status:
+        raise DcqError("dcq_quantize_i8", status)
     return q, s
 
 
-def _norm(x, w, eps, r, h, q, s, y, stream):
+def _norm(x, w, eps, r, h, q, q_stride, s, y, stream):
     m, k = shape = _table_shape("x", x)
     x_stride, typ = _float_rows("x", x, shape)
     _vector("w", w, k)
     r_stride = h_stride = 0
     if r is not None:
         r_stride = _rows_of("r", r, _F32, shape)
-        h = _made("h", h, _F32, shape, x.device, stream, rows=True)
-        h_stride = _rows_of("h", h, _F32, shape)
+        if h is None:
+            h, h_stride = _new(shape, _F32, x.device, stream), k
+        else:
+            h_stride = r_stride if h is r else _rows_of("h", h, _F32, shape)
     elif h is not None:
         raise ValueError("h: without r there is no sum to write")
-    q_stride = _i8_rows("q", q, shape) if q is not None else 0
-    y_stride = _rows_of("y", y, _F32, shape) if y is not None else 0
-    _here(x.device, w, r, h, q, s, y)
-    _check("dcq_rms_norm_i8", lib().dcq_rms_norm_i8(
-        typ, x.data_ptr(), x_stride * (2 if typ else 4), _ptr(r), r_stride * 4, _ptr(h), h_stride * 4, w.data_ptr(), eps, m,
-        k, _ptr(q), q_stride, _ptr(s), _ptr(y), y_stride * 4, _stream(stream)))
+    y_stride = 4 * _rows_of("y", y, _F32, shape) if y is not None else 0
+    status = lib().dcq_rms_norm_i8(
+        typ, x.data_ptr(), x_stride, _ptr(r), r_stride * 4, _ptr(h), h_stride * 4, w.data_ptr(), eps, m, k, _ptr(q),
+        q_stride, _ptr(s), _ptr(y), y_stride, _here(stream, x, w, r, h, q, s, y))
+    if status:
+        raise DcqError("dcq_rms_norm_i8", status)
     return h
 
 
@@ -905,18 +924,17 @@ def rms_norm_i8(x, w, eps, r=None, h=None, q=None, s=None, y=None, stream=None):
     """The residual's addition, the RMS norm and the quantization in one call: h = x + r (fp32 [M, K]; h may be r; None without
     r), (q, s) the int8 rows of h * w / sqrt(mean h^2 + eps), and the same in fp32 to y where it is given. x fp32 or fp16.
     Returns (h, q, s)."""
-    torch = _torch or _t()
-    shape = _table_shape("x", x)
-    q = _made("q", q, torch.int8, shape, x.device, stream, rows=True)
-    s = _made("s", s, _F32, shape[:1], x.device, stream)
-    return _norm(x, w, eps, r, h, q, s, y, stream), q, s
+    _torch or _t()
+    q, q_stride, s = _i8_out(q, s, _table_shape("x", x), x.device, stream)
+    return _norm(x, w, eps, r, h, q, q_stride, s, y, stream), q, s
 
 
 def rms_norm(x, w, eps, r=None, h=None, y=None, stream=None):
     """rms_norm_i8 without the int8 rows, for products that take fp32. Returns (h, y)."""
     _torch or _t()
-    y = _made("y", y, _F32, _table_shape("x", x), x.device, stream, rows=True)
-    return _norm(x, w, eps, r, h, None, None, y, stream), y
+    if y is None:
+        y = _new(_table_shape("x", x), _F32, x.device, stream)
+    return _norm(x, w, eps, r, h, None, 0, None, y, stream), y
 
 
 def mul_mat_i8_workspace_size(m, n, k):
@@ -927,28 +945,25 @@ def mul_mat_i8(w, ws, x, xs, r=None, y=None, dtype=None, workspace=None, stream=
     """Y[M, N] = (w x^T, exact) * ws[n] * xs[m] (+ r): w int8 [N, K] and x int8 [M, K] with the scales of their rows; r fp32
     [M, N] (a residual; may be y) or [N] (a bias). y fp32 or fp16 (dtype: of a new one, fp32 unless given)."""
     torch = _torch or _t()
-    n, k = _table_shape("w", w)
+    n, k = shape = _table_shape("w", w)
     m = _table_shape("x", x)[0]
-    w_stride, x_stride = _i8_rows("w", w, (n, k)), _i8_rows("x", x, (m, k))
+    w_stride, x_stride = _rows_of("w", w, torch.int8, shape), _rows_of("x", x, torch.int8, (m, k))
     _vector("ws", ws, n)
     _vector("xs", xs, m)
+    y, y_stride, typ = _out_rows("y", y, dtype, (m, n), x.device, stream)
     r_stride = 0
     if r is not None:
         if getattr(r, "ndim", 0) == 1:
             _vector("r", r, n)
         else:
-            r_stride = _rows_of("r", r, _F32, (m, n))
-    if y is None:
-        y = _new((m, n), dtype or _F32, x.device, stream)
-    y_stride, typ = _float_rows("y", y, (m, n))
+            r_stride = y_stride if r is y and typ == 0 else 4 * _rows_of("r", r, _F32, (m, n))
     if workspace is None:
         need = mul_mat_i8_workspace_size(m, n, k)
         if need:
             workspace = _new(need, _U8, x.device, stream)
-    _here(x.device, w, ws, xs, r, y, workspace)
     status = lib().dcq_mul_mat_i8(
-        w.data_ptr(), ws.data_ptr(), n, k, w_stride, x.data_ptr(), xs.data_ptr(), m, x_stride, _ptr(r), r_stride * 4, typ,
-        y.data_ptr(), y_stride * (2 if typ else 4), *_scratch(workspace), _stream(stream))
+        w.data_ptr(), ws.data_ptr(), n, k, w_stride, x.data_ptr(), xs.data_ptr(), m, x_stride, _ptr(r), r_stride, typ,
+        y.data_ptr(), y_stride, *_scratch(workspace), _here(stream, w, ws, x, xs, r, y, workspace))
     if status:
         raise DcqError("dcq_mul_mat_i8", status)
     return y
@@ -963,7 +978,7 @@ def moe_route(logits, k, scoring="softmax", bias=None, n_group=1, topk_group=1, 
     each [M, k], best first, ties to the lower expert; -1 and 0 where no expert is left. scoring "softmax" or "sigmoid"; bias fp32
     [E] counts for the choice alone; of n_group groups the topk_group best (by the best group_best choices of each) are chosen
     from; weights are scale * score, over the sum of the k with renorm."""
-    torch = _torch or _t()
+    _torch or _t()
     m, e = shape = _table_shape("logits", logits)
     stride, typ = _float_rows("logits", logits, shape)
     if scoring not in MOE_SCORING:
@@ -972,10 +987,9 @@ def moe_route(logits, k, scoring="softmax", bias=None, n_group=1, topk_group=1, 
         _vector("bias", bias, e)
     ids = _made("ids", ids, _I32, (m, k), logits.device, stream)
     weights = _made("weights", weights, _F32, (m, k), logits.device, stream)
-    _here(logits.device, bias, ids, weights)
-    status = lib().dcq_moe_route(typ, logits.data_ptr(), stride * (2 if typ else 4), m, e, MOE_SCORING[scoring], _ptr(bias),
-                                 n_group, topk_group, group_best, k, 1 if renorm else 0, scale, ids.data_ptr(),
-                                 weights.data_ptr(), _stream(stream))
+    status = lib().dcq_moe_route(typ, logits.data_ptr(), stride, m, e, MOE_SCORING[scoring], _ptr(bias), n_group, topk_group,
+                                 group_best, k, 1 if renorm else 0, scale, ids.data_ptr(), weights.data_ptr(),
+                                 _here(stream, logits, bias, ids, weights))
     if status:
         raise DcqError("dcq_moe_route", status)
     return ids, weights
@@ -994,8 +1008,7 @@ def moe_plan(ids, n_expert, plan=None, stream=None):
         _checked("ids", ids, _I32, shape)
     if plan is None:
         plan = _new(max(moe_plan_size(m, k, n_expert), 256), _U8, ids.device, stream)
-    _here(ids.device, plan)
-    status = lib().dcq_moe_plan(ids.data_ptr(), m, k, n_expert, *_scratch(plan), _stream(stream))
+    status = lib().dcq_moe_plan(ids.data_ptr(), m, k, n_expert, *_scratch(plan), _here(stream, ids, plan))
     if status:
         raise DcqError("dcq_moe_plan", status)
     return plan
@@ -1008,10 +1021,11 @@ def _expert_rows(name, t, scales):
     except (AttributeError, ValueError):
         _need(name, t, _torch.int8, (3,))
         raise
-    if not _plain(t, _torch.int8, shape):
-        _checked(name, t, _torch.int8, shape, rows=True)
     if not _plain(scales, _F32, (e, n)):
         _checked(name + "s", scales, _F32, (e, n))
+    if _plain(t, _torch.int8, shape):
+        return e, n, k, k, n * k
+    _checked(name, t, _torch.int8, shape, rows=True)
     row = t.stride(1) if n > 1 else k
     return e, n, k, row, t.stride(0) if e > 1 else row * n
 
@@ -1020,19 +1034,17 @@ def moe_gate_up_i8(plan, wg, wgs, wu, wus, x, xs, k, h=None, dtype=None, stream=
     """h[slot] = silu(wg[e] x) * (wu[e] x) of the M * k slots of a plan: wg, wu int8 [E, N, K] with scales [E, N], x int8
     [M, K] with scales [M], k the slots of a token; zeros for slots of no expert. h fp32 or fp16 [M * k, N]."""
     torch = _torch or _t()
-    e, n, width, row, per = _expert_rows("wg", wg, wgs)
-    if _expert_rows("wu", wu, wus) != (e, n, width, row, per):
+    e, n, width, row, per = sizes = _expert_rows("wg", wg, wgs)
+    if _expert_rows("wu", wu, wus) != sizes:
         raise ValueError("wg and wu must share shape and strides (the ABI takes one)")
     m = _table_shape("x", x)[0]
-    x_stride = _i8_rows("x", x, (m, width))
+    x_stride = _rows_of("x", x, torch.int8, (m, width))
     _vector("xs", xs, m)
-    if h is None:
-        h = _new((m * k, n), dtype or _F32, x.device, stream)
-    h_stride, typ = _float_rows("h", h, (m * k, n))
-    _here(x.device, plan, wg, wgs, wu, wus, xs, h)
+    h, h_stride, typ = _out_rows("h", h, dtype, (m * k, n), x.device, stream)
     status = lib().dcq_moe_gate_up_i8(
         *_scratch(plan), m, k, e, wg.data_ptr(), wgs.data_ptr(), wu.data_ptr(), wus.data_ptr(), n, width, row, per,
-        x.data_ptr(), xs.data_ptr(), x_stride, typ, h.data_ptr(), h_stride * (2 if typ else 4), _stream(stream))
+        x.data_ptr(), xs.data_ptr(), x_stride, typ, h.data_ptr(), h_stride,
+        _here(stream, plan, wg, wgs, wu, wus, x, xs, h))
     if status:
         raise DcqError("dcq_moe_gate_up_i8", status)
     return h
@@ -1047,22 +1059,21 @@ def moe_down_i8(plan, w, ws, h, hs, weights, r=None, y=None, dtype=None, workspa
     scales [E, N], h int8 [M * k, K] with scales [M * k], weights fp32 [M, k], r fp32 [M, N] or None (may be y). y fp32 or fp16."""
     torch = _torch or _t()
     e, n, width, row, per = _expert_rows("w", w, ws)
-    m, k = _table_shape("weights", weights)
-    if not _plain(weights, _F32, (m, k)):
-        _checked("weights", weights, _F32, (m, k))
-    h_stride = _i8_rows("h", h, (m * k, width))
+    m, k = shape = _table_shape("weights", weights)
+    if not _plain(weights, _F32, shape):
+        _checked("weights", weights, _F32, shape)
+    h_stride = _rows_of("h", h, torch.int8, (m * k, width))
     _vector("hs", hs, m * k)
-    r_stride = _rows_of("r", r, _F32, (m, n)) if r is not None else 0
-    if y is None:
-        y = _new((m, n), dtype or _F32, h.device, stream)
-    y_stride, typ = _float_rows("y", y, (m, n))
+    y, y_stride, typ = _out_rows("y", y, dtype, (m, n), h.device, stream)
+    r_stride = 0
+    if r is not None:
+        r_stride = y_stride if r is y and typ == 0 else 4 * _rows_of("r", r, _F32, (m, n))
     if workspace is None:
         workspace = _new(max(moe_down_i8_workspace_size(m, k, n), 256), _U8, h.device, stream)
-    _here(h.device, plan, w, ws, hs, weights, r, y, workspace)
     status = lib().dcq_moe_down_i8(
         *_scratch(plan), m, k, e, w.data_ptr(), ws.data_ptr(), n, width, row, per, h.data_ptr(), hs.data_ptr(), h_stride,
-        weights.data_ptr(), _ptr(r), r_stride * 4, typ, y.data_ptr(), y_stride * (2 if typ else 4), *_scratch(workspace),
-        _stream(stream))
+        weights.data_ptr(), _ptr(r), r_stride, typ, y.data_ptr(), y_stride, *_scratch(workspace),
+        _here(stream, plan, w, ws, h, hs, weights, r, y, workspace))
     if status:
         raise DcqError("dcq_moe_down_i8", status)
     return y
