@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
             }
             T* y = static_cast<T*>(a.y) + (SUMS ? (int64_t)split * a.M * a.N : 0) + row * a.y_stride + n;
             if (left == PER && wide) {
-                __builtin_memcpy(__builtin_assume_aligned(y, 4), o, 16);
+                store_through(y, o);
             } else {
 #pragma unroll
                 for (int e = 0; e < PER; ++e)

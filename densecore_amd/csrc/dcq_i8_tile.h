@@ -42,6 +42,15 @@ __device__ __forceinline__ int piece_key(int row) {
     return KB == 128 ? (row & 7) ^ ((row >> 3) & 1) : (row >> 2) & 3;
 }
 
+// 16 bytes of outputs that nothing reads soon, past the caches' usual places: products whose outputs flow through L2 lose the
+// operands there (4099 x 14336 x 4096, F16 out: 251 -> 229 us; 4096 x 14336 x 2048, F32: 164 -> 141).
+__device__ __forceinline__ void store_through(void* y, const void* v16) {
+    typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+    i32x4 v;
+    __builtin_memcpy(&v, v16, 16);
+    __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(y));
+}
+
 // y = sum * ws * xs, the weight's scale first: sum * ws is the product of the row's own unit, so that neither a small
 // ws * xs is lost nor a large one infinite where the value is not.
 __device__ __forceinline__ float i8_value(int sum, float ws, float xs) { return (float)sum * ws * xs; }
