@@ -138,28 +138,26 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
         if constexpr (GROUPED) src = UP ? order[src] / a.top : order[src];
         x_off[i] = (uint32_t)src * (uint32_t)a.x_stride;
     }
+    // What goes with the sums, on its way before the operands. Pieces of 64 sums, row 16 (p / 4) + 4 (lane / 16) + p % 4 of
+    // column lane % 16, are shared among the KW waves.
+    constexpr int OUT = (MT * 4 + KW - 1) / KW;
+    const int n = min(n0 + (lane & 15), a.N - 1);
+    const int64_t ns = (int64_t)expert * a.N + n;
+    const float ws = a.ws[ns], ws2 = UP ? a.ws2[ns] : 0.0f;
+    float xs[OUT], add[OUT];
+    int64_t row[OUT];
+#pragma unroll
+    for (int t = 0; t < OUT; ++t) {
+        const int p = min(kw + KW * t, MT * 4 - 1), r = min(16 * (p / 4) + 4 * (lane >> 4) + p % 4, rows_here - 1);
+        row[t] = GROUPED ? (int64_t)order[r] : (int64_t)tile_m * 16 * MT + r;
+        xs[t] = a.xs[UP ? row[t] / a.top : row[t]];
+        add[t] = !GROUPED && a.R ? a.R[row[t] * a.r_stride + n] : 0.0f;
+    }
     const int stages = (a.K + 127) / 128;
     v4i acc[MT][NT];
     wave_sums<MT, NT>(acc, reinterpret_cast<int8_t*>(smem) + wave * (kStages * 2048 * (MT + NT)), xb, x_off, wb, w_off, a.K,
                       stages * kw / KW, stages * (kw + 1) / KW);
-
-    auto out = [&](int i, int v, int sum0, int sum1) {
-        const int r = 16 * i + 4 * (lane >> 4) + v, n = n0 + (lane & 15);
-        if (r >= rows_here || n >= a.N) return;
-        const int64_t row = GROUPED ? (int64_t)order[r] : (int64_t)tile_m * 16 * MT + r;
-        const float xs = a.xs[UP ? row / a.top : row];
-        const int64_t ns = (int64_t)expert * a.N + n;
-        float y = i8_value(sum0, a.ws[ns], xs);
-        if constexpr (UP) y = silu(y) * i8_value(sum1, a.ws2[ns], xs);
-        if (!GROUPED && a.R) y += a.R[row * a.r_stride + n];
-        static_cast<T*>(a.y)[row * a.y_stride + n] = (T)y;
-    };
-    if constexpr (KW == 1) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) out(i, v, acc[i][0][v], acc[i][NT - 1][v]);
-    } else {
+    if constexpr (KW > 1) {
         __syncthreads();  // every wave's stages are done
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -168,16 +166,26 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
 #pragma unroll
                 for (int v = 0; v < 4; ++v) part[nw][kw][(i * NT + j) * 4 + v][lane] = acc[i][j][v];
         __syncthreads();
-        for (int p = kw; p < MT * 4; p += KW) {  // 64 sums to a wave
-            const int v = p % 4, i = p / 4;
-            int s0 = 0, s1 = 0;
+    }
+#pragma unroll
+    for (int t = 0; t < OUT; ++t) {
+        const int p = kw + KW * t;
+        if (p >= MT * 4) continue;
+        int s0 = 0, s1 = 0;
+        if constexpr (KW > 1) {
 #pragma unroll
             for (int q = 0; q < KW; ++q) {
-                s0 += part[nw][q][i * NT * 4 + v][lane];
-                if constexpr (UP) s1 += part[nw][q][(i * NT + 1) * 4 + v][lane];
+                s0 += part[nw][q][p / 4 * NT * 4 + p % 4][lane];
+                if constexpr (UP) s1 += part[nw][q][(p / 4 * NT + 1) * 4 + p % 4][lane];
             }
-            out(i, v, s0, s1);
+        } else {  // p is t
+            s0 = acc[t / 4][0][t % 4], s1 = acc[t / 4][NT - 1][t % 4];
         }
+        if (16 * (p / 4) + 4 * (lane >> 4) + p % 4 >= rows_here || n0 + (lane & 15) >= a.N) continue;
+        float y = i8_value(s0, ws, xs[t]);
+        if constexpr (UP) y = silu(y) * i8_value(s1, ws2, xs[t]);
+        if (!GROUPED && a.R) y += add[t];
+        static_cast<T*>(a.y)[row[t] * a.y_stride + n] = (T)y;
     }
 }
 
@@ -247,7 +255,9 @@ template <class T>
 hipError_t launch_dense(const I8Args& a, hipStream_t st) {
     if (a.M <= 16) return launch_rows_of<kI8Dense, 1, T>(a, st);
     if (a.M <= 32) return launch_rows_of<kI8Dense, 2, T>(a, st);
-    return launch_rows_of<kI8Dense, 4, T>(a, st);
+    // up to 64 rows to a tile; few weight rows leave CUs idle then, and pay for being read by two tiles of 32 (61 rows x
+    // 2560 x 9728: 11.1 -> 10.0 us, 2048 x 2048 4.7 -> 3.8, 1024 x 4096 6.2 -> 4.7; but 8192 x 2048 7.3 -> 8.0)
+    return a.N < 4096 ? launch_waves<kI8Dense, 2, 4, 1, T>(a, st) : launch_rows_of<kI8Dense, 4, T>(a, st);
 }
 
 }  // namespace

@@ -273,15 +273,20 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(CombineArgs a) {
     float y[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) y[i] = 0.0f;
-    for (int j = 0; j < a.top; ++j) {
-        const int64_t slot = row * a.top + j;
-        if (a.expert[slot] < 0) continue;
-        const float w = a.weights[slot];
-        const float* p = a.p + slot * a.N + n;
-        float v[V];
-        __builtin_memcpy(v, __builtin_assume_aligned(p, 4 * V), 4 * V);
+    for (int j0 = 0; j0 < a.top; j0 += 4) {  // four slots' loads on their way at a time; those of no expert do not count
+        float v[4][V], w[4];
+        bool in[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = fmaf(w, v[i], y[i]);
+        for (int j = 0; j < 4; ++j) {
+            const int64_t slot = row * a.top + min(j0 + j, a.top - 1);
+            in[j] = j0 + j < a.top && a.expert[slot] >= 0;
+            w[j] = a.weights[slot];
+            __builtin_memcpy(v[j], __builtin_assume_aligned(a.p + slot * a.N + n, 4 * V), 4 * V);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) y[i] = in[j] ? fmaf(w[j], v[j][i], y[i]) : y[i];
     }
     if (a.R) {
         float v[V];
