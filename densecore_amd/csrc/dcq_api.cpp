@@ -1025,7 +1025,8 @@ int dcq_quantize_i8(int type, const void* X, int64_t M, int64_t K, size_t x_stri
 }
 
 static int validate_i8_shape(int64_t M, int64_t N, int64_t K) {
-    return M > 0 && N > 0 && K > 0 && K % 16 == 0 && K <= DCQ_I8_MAX_K && M <= DCQ_I8_MAX_ROWS && N <= DCQ_I8_MAX_ROWS
+    return M > 0 && N > 0 && K > 0 && K % 16 == 0 && K <= DCQ_I8_MAX_K && M <= DCQ_I8_MAX_ROWS && N <= DCQ_I8_MAX_ROWS &&
+                   M * N < (int64_t)1 << 34  // tiles of 64 x 64 below 2^32 threads
                ? DCQ_OK
                : DCQ_ERR_BAD_SHAPE;
 }
@@ -1062,7 +1063,7 @@ int dcq_mul_mat_i8(const int8_t* W, const float* Ws, int64_t N, int64_t K, size_
     a.x = X, a.xs = Xs, a.x_stride = (int64_t)x_stride_bytes, a.M = M;
     a.w = W, a.ws = Ws, a.w_stride = (int64_t)w_stride_bytes, a.N = (int)N, a.K = (int)K;
     a.R = R, a.r_stride = (int64_t)(r_stride_bytes / 4), a.y = Y, a.y_stride = (int64_t)y_stride_bytes / size;
-    return hip_status(launch_i8_product(ytype, a, workspace, workspace ? need : 0, (hipStream_t)stream));
+    return hip_status(launch_i8_product(ytype, a, need ? workspace : nullptr, (hipStream_t)stream));
 }
 
 int dcq_moe_route(int type, const void* logits, size_t stride_bytes, int64_t M, int n_expert, int scoring,
@@ -1119,6 +1120,7 @@ static int validate_experts(const void* plan, size_t plan_size, int64_t M, int k
     int rc = validate_plan(M, k, n_expert);
     if (rc) return rc;
     if ((rc = validate_i8_shape(M * k, N, K))) return rc;
+    if (N > DCQ_MOE_MAX_N || M * k * N >= (int64_t)1 << 31) return DCQ_ERR_BAD_SHAPE;  // of more no launch holds the outputs
     if (!plan || !Xs) return DCQ_ERR_INVALID_ARG;
     if (plan_size < (size_t)plan_bytes(M, k, n_expert)) return DCQ_ERR_WORKSPACE;
     if (expert_stride < w_stride * (size_t)(N - 1) + (size_t)K || expert_stride > ((size_t)1 << 40)) return DCQ_ERR_INVALID_ARG;
@@ -1155,7 +1157,7 @@ int dcq_moe_gate_up_i8(const void* plan, size_t plan_size, int64_t M, int k, int
 }
 
 size_t dcq_moe_down_i8_workspace_size(int64_t M, int k, int64_t N) {
-    if (validate_plan(M, k, 1) || N <= 0 || N > DCQ_I8_MAX_ROWS) return 0;
+    if (validate_plan(M, k, 1) || N <= 0 || N > DCQ_MOE_MAX_N || M * k * N >= (int64_t)1 << 31) return 0;
     return (size_t)round_up(M * k * N * 4, 256);
 }
 

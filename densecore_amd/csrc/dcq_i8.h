@@ -54,13 +54,15 @@ struct I8Args {
     bool y_wide;  // rows of y are of whole dwords
 };
 size_t i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
-hipError_t launch_i8_product(int ytype, const I8Args& a, void* ws, size_t ws_bytes, hipStream_t st);
+// ws: i8_workspace_bytes bytes, or null
+hipError_t launch_i8_product(int ytype, const I8Args& a, void* ws, hipStream_t st);
 hipError_t launch_moe_gate_up(int htype, const I8Args& a, hipStream_t st);
 struct CombineArgs;
 hipError_t launch_moe_down(int ytype, I8Args a, const CombineArgs& c, hipStream_t st);
 // dcq_i8_rows.hip: few rows (of an expert); dcq_i8_gemm.hip: many
 hipError_t launch_i8_rows(I8Mode mode, int ytype, const I8Args& a, hipStream_t st);
-hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, size_t ws_bytes, hipStream_t st);
+hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, hipStream_t st);
+bool i8_few_rows(int64_t M, int64_t N, int64_t K);  // whether a dense product is the former's
 
 // dcq_moe.hip. A plan, in int32: offsets[n_expert + 2] (expert e's slots are places offsets[e] .. offsets[e + 1] - 1 of the
 // order, those of no expert offsets[n_expert] ..); the order: slots sorted by expert; each slot's expert, or -1; and tiles of

@@ -1,5 +1,6 @@
 // dcq_i8_gemm.hip — products of many int8 rows on gfx950 int8 MFMA: dense ones, and those of a plan's experts.
 #include <algorithm>
+#include <cmath>
 
 #include "dcq_common.h"
 #include "dcq_i8.h"
@@ -59,14 +60,14 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     int rows_here, expert = 0;
     const int32_t* order = nullptr;
     if constexpr (GROUPED) {
-        const PlanTile t = reinterpret_cast<const PlanTile*>(a.plan + plan_tiles_at(a.n_expert, a.M))[tile_m];
+        const PlanTile t = plan_tile(a.plan, a.n_expert, a.M, tile_m, BM);
         if (t.expert < 0) return;
         expert = t.expert, rows_here = t.count;
         order = a.plan + plan_order_at(a.n_expert) + t.begin;
         if (expert == a.n_expert) {  // slots of no expert
             if constexpr (UP) {
                 for (int i = tid; i < rows_here * TILE_N; i += 64 * W)
-                    if (n0 + i % TILE_N < a.N) put<T>(a.y, (int64_t)order[i / TILE_N] * a.y_stride + n0 + i % TILE_N, 0.0f);
+                    if (n0 + i % TILE_N < a.N) put<T>(a.y, (int64_t)plan_slot(order, i / TILE_N, a.M) * a.y_stride + n0 + i % TILE_N, 0.0f);
             }
             return;
         }
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     for (int i = 0; i < LA; ++i) {
         const int r = LR * (LA * wave + i) + l_row;
         int src = min(r, rows_here - 1);
-        if constexpr (GROUPED) src = UP ? order[src] / a.top : order[src];
+        if constexpr (GROUPED) src = UP ? plan_slot(order, src, a.M) / a.top : plan_slot(order, src, a.M);
         a_off[i] = (uint32_t)src * (uint32_t)a.x_stride + 16u * (uint32_t)((lane % P) ^ piece_key<KB>(r));
     }
     const int stages = (a.K + KB - 1) / KB;
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     for (int t = 0; t < RT; ++t) {
         const int r = min(tid + 64 * W * t, rows_here - 1);
         if constexpr (GROUPED) {
-            slot[t] = order[r];
+            slot[t] = plan_slot(order, r, a.M);
             rs[t] = a.xs[UP ? slot[t] / a.top : slot[t]];
         } else {
             rs[t] = a.xs[(int64_t)tile_m * BM + r];
@@ -389,40 +390,65 @@ hipError_t launch_join(const I8Args& a, const void* planes, hipStream_t st) {
 
 }  // namespace
 
-hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, size_t ws_bytes, hipStream_t st) {
+// Which tile, and into how many shares of K: the least of the times that the kernels take by their rounds of workgroups,
+// fitted to 64 products of 40 to 1536 rows x 1024 .. 14336 x 1024 .. 14336 (the
+// choice is never more than 13 % behind the best of them, and mostly the best). A round is a + b * stages us, less where half of its workgroups
+// have a CU to themselves; a split adds a launch that reads its planes.
+struct DensePlan {
+    int shape, splits;
+};
+static DensePlan plan_dense(int64_t M, int64_t N, int64_t K, bool may_split) {
+    static const struct {
+        int shape, bm, bn, slots;
+        double a, b, a_half, b_half;
+    } kTiles[] = {{0, 64, 64, 512, 7.5, 0.27, 3.5, 0.28}, {2, 128, 128, 512, 8.0, 0.87, 8.0, 0.52}, {3, 256, 256, 256, 17.0, 1.38, 8.0, 1.2}};
+    const int forced = knob(Knob::I8Tile), forced_split = knob(Knob::I8Split);
+    const int64_t stages = (K + 127) / 128;
+    DensePlan best = {2, 1};
+    double least = INFINITY;
+    for (const auto& t : kTiles) {
+        if (forced >= 0 && forced != t.shape) continue;
+        for (int splits : {1, 2, 3, 4, 6, 8}) {
+            if (splits > 1 && (!may_split || stages / splits < 8 || M * N * splits > (int64_t)1 << 24)) break;
+            if (forced_split > 0 && splits != forced_split) continue;
+            const int64_t groups = (M + t.bm - 1) / t.bm * ((N + t.bn - 1) / t.bn) * splits, rest = groups % t.slots;
+            const double st = (double)((stages + splits - 1) / splits);
+            double us = (double)(groups / t.slots + (rest > t.slots / 2)) * (t.a + t.b * st);
+            if (rest && rest <= t.slots / 2) us += t.a_half + t.b_half * st;
+            if (splits > 1) us += 3.0 + (double)(8 * splits + 4) * (double)(M * N) / 9e6;
+            if (us < least) least = us, best = {t.shape, splits};
+        }
+    }
+    return best;
+}
+
+size_t i8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (i8_few_rows(M, N, K)) return 0;
+    const DensePlan p = plan_dense(M, N, K, true);
+    return p.splits > 1 ? (size_t)round_up(p.splits * M * N * 4, 256) : 0;
+}
+
+hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, hipStream_t st) {
     const int stages = (a.K + 127) / 128;
     a.splits = 1, a.stps = stages;
     // wide stores need whole dwords
     a.y_wide = ytype == kTypeF32 || (a.y_stride % 2 == 0 && (uintptr_t)a.y % 4 == 0);
-    const int forced = knob(Knob::I8Tile);
     if (mode != kI8Dense) {
-        const int height = plan_height(a.M, a.n_expert);
-        const int shape = height == 128 ? 2 : 1;
+        const int shape = plan_height(a.M, a.n_expert) == 128 ? 2 : 1;
         if (mode == kI8Up)
             return ytype == kTypeF16 ? launch_shape<kI8Up, _Float16>(a, shape, st) : launch_shape<kI8Up, float>(a, shape, st);
         return launch_shape<kI8Down, float>(a, shape, st);
     }
-    auto tiles = [&](int64_t bm, int64_t bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
-    const int shape = forced >= 0 ? forced : tiles(256, 256) >= 200 ? 3 : tiles(128, 128) >= 240 ? 2 : 0;
-    int splits = 1;
-    if (shape == 0 && stages >= 32) splits = (int)std::max<int64_t>(1, 256 / tiles(64, 64));
-    if (knob(Knob::I8Split) > 0) splits = knob(Knob::I8Split);
-    splits = (int)std::min<int64_t>({splits, stages / 8, (int64_t)(ws_bytes / 4) / (a.M * a.N)});
-    if (splits <= 1)
-        return ytype == kTypeF16 ? launch_shape<kI8Dense, _Float16>(a, shape, st) : launch_shape<kI8Dense, float>(a, shape, st);
-    a.stps = (stages + splits - 1) / splits;
+    const DensePlan plan = plan_dense(a.M, a.N, a.K, ws != nullptr);
+    if (plan.splits <= 1)
+        return ytype == kTypeF16 ? launch_shape<kI8Dense, _Float16>(a, plan.shape, st) : launch_shape<kI8Dense, float>(a, plan.shape, st);
+    a.stps = (stages + plan.splits - 1) / plan.splits;
     a.splits = (stages + a.stps - 1) / a.stps;
     I8Args p = a;
     p.y = ws, p.y_stride = a.N, p.y_wide = true;
-    hipError_t e = launch_shape<kI8Dense, int32_t>(p, shape, st);
+    const hipError_t e = launch_shape<kI8Dense, int32_t>(p, plan.shape, st);
     if (e != hipSuccess) return e;
     return ytype == kTypeF16 ? launch_join<_Float16>(a, ws, st) : launch_join<float>(a, ws, st);
-}
-
-size_t i8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (K <= 1024 || M * N > (int64_t)1 << 24) return 0;
-    return (size_t)std::min<int64_t>(16, K / 512) * M * N * 4 > ((size_t)64 << 20) ? (size_t)64 << 20
-                                                                                   : (size_t)std::min<int64_t>(16, K / 512) * M * N * 4;
 }
 
 }  // namespace dcq

@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
     int rows_here, expert = 0;
     const int32_t* order = nullptr;
     if constexpr (GROUPED) {
-        const PlanTile t = reinterpret_cast<const PlanTile*>(a.plan + plan_tiles_at(a.n_expert, a.M))[tile_m];
+        const PlanTile t = plan_tile(a.plan, a.n_expert, a.M, tile_m, 16 * MT);
         if (t.expert < 0) return;
         expert = t.expert, rows_here = t.count;
         order = a.plan + plan_order_at(a.n_expert) + t.begin;
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
             if constexpr (UP) {
                 if (kw == 0)
                     for (int i = lane; i < rows_here * 16; i += 64)
-                        if (n0 + i % 16 < a.N) static_cast<T*>(a.y)[(int64_t)order[i / 16] * a.y_stride + n0 + i % 16] = (T)0.0f;
+                        if (n0 + i % 16 < a.N) static_cast<T*>(a.y)[(int64_t)plan_slot(order, i / 16, a.M) * a.y_stride + n0 + i % 16] = (T)0.0f;
             }
             return;
         }
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
         int src = min(8 * i + lane / 8, rows_here - 1);
-        if constexpr (GROUPED) src = UP ? order[src] / a.top : order[src];
+        if constexpr (GROUPED) src = UP ? plan_slot(order, src, a.M) / a.top : plan_slot(order, src, a.M);
         x_off[i] = (uint32_t)src * (uint32_t)a.x_stride;
     }
     // What goes with the sums, on its way before the operands. Pieces of 64 sums, row 16 (p / 4) + 4 (lane / 16) + p % 4 of
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
 #pragma unroll
     for (int t = 0; t < OUT; ++t) {
         const int p = min(kw + KW * t, MT * 4 - 1), r = min(16 * (p / 4) + 4 * (lane >> 4) + p % 4, rows_here - 1);
-        row[t] = GROUPED ? (int64_t)order[r] : (int64_t)tile_m * 16 * MT + r;
+        row[t] = GROUPED ? (int64_t)plan_slot(order, r, a.M) : (int64_t)tile_m * 16 * MT + r;
         xs[t] = a.xs[UP ? row[t] / a.top : row[t]];
         add[t] = !GROUPED && a.R ? a.R[row[t] * a.r_stride + n] : 0.0f;
     }
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(1024) i8_token_kernel(I8Args a, CombineArgs c)
     const int n0 = (int)blockIdx.x % a.tiles_n * 16, n = n0 + (lane & 15);
     const int64_t slot = token * c.top + wave;
     const int expert = __builtin_amdgcn_readfirstlane(c.expert[slot]);
-    if (expert >= 0) {
+    if ((unsigned)expert < (unsigned)a.n_expert) {
         uint32_t x_off[2], w_off[2];
         weight_rows(w_off, n0, a.N, a.w_stride);
         x_off[0] = x_off[1] = 0;
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(1024) i8_token_kernel(I8Args a, CombineArgs c)
     if (threadIdx.x < 16 && n < a.N) {
         float y = 0.0f;
         for (int j = 0; j < c.top; ++j)
-            if (c.expert[token * c.top + j] >= 0) y = fmaf(c.weights[token * c.top + j], part[j][threadIdx.x], y);
+            if ((unsigned)c.expert[token * c.top + j] < (unsigned)a.n_expert) y = fmaf(c.weights[token * c.top + j], part[j][threadIdx.x], y);
         if (c.R) y += c.R[token * c.r_stride + n];
         static_cast<T*>(c.y)[token * c.y_stride + n] = (T)y;
     }
@@ -270,14 +270,22 @@ hipError_t launch_i8_rows(I8Mode mode, int ytype, const I8Args& a, hipStream_t s
     return launch_rows_of<kI8Down, 1, float>(a, st);
 }
 
-hipError_t launch_i8_product(int ytype, const I8Args& a, void* ws, size_t ws_bytes, hipStream_t st) {
-    const bool few = knob(Knob::I8Rows) >= 0 ? a.M <= knob(Knob::I8Rows)
-                                             : a.M <= 32 || (a.M <= 64 && a.N < 65536) || (a.M <= 256 && a.N <= 2048 && a.K <= 4096);
-    return few ? launch_i8_rows(kI8Dense, ytype, a, st) : launch_i8_gemm(kI8Dense, ytype, a, ws, ws_bytes, st);
+// Up to 64 rows, but of tall matrices the 64 x 64 tiles share the weights' and the rows' way through LDS better (20 rows x
+// 151936 x 2560: 90 us here, 78 there; 40 rows x 14336 x 4096 16.0 and 12.4; 40 x 9728 x 2560 9.9 and 9.2); and up to 128 or
+// 256 of small ones, which leave those CUs idle (100 x 4096 x 4096: 9.8 and 12.2, 256 x 2048 x 2048: 6.6 and 7.7; but 100 x
+// 2560 x 9728 16.2 and 14.8, 150 x 4096 x 4096 13.1 and 12.3).
+bool i8_few_rows(int64_t M, int64_t N, int64_t K) {
+    if (knob(Knob::I8Rows) >= 0) return M <= knob(Knob::I8Rows);
+    if (M <= 64) return M <= 16 || (N < 65536 && (M <= 32 || N < 12288));
+    return K <= 4096 && ((M <= 128 && N <= 4096) || (M <= 256 && N <= 2048));
+}
+
+hipError_t launch_i8_product(int ytype, const I8Args& a, void* ws, hipStream_t st) {
+    return i8_few_rows(a.M, a.N, a.K) ? launch_i8_rows(kI8Dense, ytype, a, st) : launch_i8_gemm(kI8Dense, ytype, a, ws, st);
 }
 
 static hipError_t launch_experts(I8Mode mode, int ytype, const I8Args& a, hipStream_t st) {
-    return plan_height(a.M, a.n_expert) == 16 ? launch_i8_rows(mode, ytype, a, st) : launch_i8_gemm(mode, ytype, a, nullptr, 0, st);
+    return plan_height(a.M, a.n_expert) == 16 ? launch_i8_rows(mode, ytype, a, st) : launch_i8_gemm(mode, ytype, a, nullptr, st);
 }
 
 hipError_t launch_moe_gate_up(int htype, const I8Args& a, hipStream_t st) { return launch_experts(kI8Up, htype, a, st); }

@@ -11,6 +11,17 @@ namespace dcq {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
+// A plan's tile, and a place of its order. What a plan of another call holds there reaches no further than this call's arrays.
+__device__ __forceinline__ PlanTile plan_tile(const int32_t* plan, int n_expert, int64_t slots, int at, int height) {
+    PlanTile t = reinterpret_cast<const PlanTile*>(plan + plan_tiles_at(n_expert, slots))[at];
+    if (t.expert > n_expert || t.count <= 0 || t.begin < 0 || t.begin >= slots) t.expert = -1;
+    t.count = min(min(t.count, height), (int)slots - t.begin);
+    return t;
+}
+__device__ __forceinline__ int plan_slot(const int32_t* order, int at, int64_t slots) {
+    return (int)min((uint32_t)order[at], (uint32_t)slots - 1u);
+}
+
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 // 16 bytes per lane from a uniform base + per-lane offset to LDS at lds_base + 16 * lane (lds_base uniform, in M0). The

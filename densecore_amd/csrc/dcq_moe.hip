@@ -190,11 +190,11 @@ hipError_t launch_moe_route(int type, const RouteArgs& a, hipStream_t st) {
 }
 
 // A workgroup per expert (and one for the slots of none) looks at all slots: those of lower experts give its place, its
-// own go there in their order. No atomics and no second launch; the slots' numbers come from the caches, 8 loads of a wave
+// own go there in their order. No atomics and no second launch; the slots' numbers come from the caches, 16 loads of a wave
 // on their way at a time (12568 slots of 128 experts: 13.2 us with one).
 constexpr int kPlanThreads = 1024;
 __global__ void __launch_bounds__(kPlanThreads) moe_plan_kernel(const int32_t* ids, int slots, int n_expert, int32_t* plan) {
-    constexpr int W = kPlanThreads / 64, G = 8;
+    constexpr int W = kPlanThreads / 64, G = 16;
     __shared__ int less[W], mine[W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int me = blockIdx.x;  // n_expert: none

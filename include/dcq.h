@@ -444,13 +444,13 @@ int dcq_beam_select(int type, const void* logits, size_t stride_bytes, int64_t n
  * row of int8 has one fp32 scale: element k of row r stands for q[r][k] * s[r], for weights (a row per output) and
  * for activations (a row per token). Sums over K are exact 32-bit integers, so that results do not depend on
  * how a product is split, nor from run to run. Rows of int8 are 16-byte aligned, K a multiple of 16 up to DCQ_I8_MAX_K,
- * strides up to DCQ_I8_MAX_STRIDE bytes. No output, plan or workspace may share a byte with an input or another of them
- * (DCQ_ERR_INVALID_ARG; rows of one stride may lie between each other's), but where a call says so. Workspaces and plans are
- * 256-byte aligned. A call whose tiles no launch holds (2^32 threads) is DCQ_ERR_BAD_SHAPE. */
+ * strides up to DCQ_I8_MAX_STRIDE bytes, rows up to DCQ_I8_MAX_ROWS, M * N of a product below 2^34 (DCQ_ERR_BAD_SHAPE past
+ * these). No output, plan or workspace may share a byte with an input or another of them (DCQ_ERR_INVALID_ARG; rows of one
+ * stride may lie between each other's), but where a call says so. Workspaces and plans are 256-byte aligned. */
 #define DCQ_I8_MAX_K 131056 /* 128 * 128 * K below 2^31 */
 #define DCQ_I8_MAX_STRIDE ((size_t)1 << 24)
 #define DCQ_I8_MAX_ROWS ((int64_t)1 << 22)
-#define DCQ_I8_MAX_NORM_ROWS ((int64_t)1 << 22)
+#define DCQ_I8_MAX_NORM_ROWS ((int64_t)1 << 22) /* fewer than these */
 
 /* Rows to int8: s = max |x| / 127 rounded to fp32, q = x * (127 / max |x|) in 64 bits, each step rounded, then to the
  * nearest integer, halves to even: -127 .. 127. An all-zero row has s = 0; a row that holds a NaN or an infinity has q = 0 and
@@ -470,8 +470,8 @@ int dcq_rms_norm_i8(int type, const void* X, size_t x_stride_bytes, const float*
 
 /* Y[m][n] = (sum_k W[n][k] X[m][k]) * Ws[n] * Xs[m] (+ R[m][n]), rounded to fp32 after each operation and, with ytype F16,
  * once more at the end. R fp32: rows r_stride_bytes apart (a residual; may be Y itself where Y is F32 with the
- * same stride), or r_stride_bytes 0: one row for all (a bias); NULL: none. Without a workspace (NULL) few large rows run on
- * fewer workgroups; the result is the same. */
+ * same stride), or r_stride_bytes 0: one row for all (a bias); NULL: none. Without a workspace (NULL) K is not
+ * split among workgroups, which is slower where there are few tiles; the result is the same. */
 size_t dcq_mul_mat_i8_workspace_size(int64_t M, int64_t N, int64_t K);
 int dcq_mul_mat_i8(const int8_t* W, const float* Ws, int64_t N, int64_t K, size_t w_stride_bytes, const int8_t* X,
                    const float* Xs, int64_t M, size_t x_stride_bytes, const float* R, size_t r_stride_bytes, int ytype,
@@ -489,19 +489,20 @@ int dcq_mul_mat_i8(const int8_t* W, const float* Ws, int64_t N, int64_t K, size_
 #define DCQ_MOE_SIGMOID 1
 #define DCQ_MOE_MAX_EXPERTS 512
 #define DCQ_MOE_MAX_SLOTS ((int64_t)1 << 22)
+#define DCQ_MOE_MAX_N 131072
 int dcq_moe_route(int type, const void* logits, size_t stride_bytes, int64_t M, int n_expert, int scoring,
                   const float* bias, int n_group, int topk_group, int group_best, int k, int renorm, float scale,
                   int32_t* ids, float* weights, void* stream);
 
 /* The tokens' slots (slot = token * k + place, its expert ids[slot]) sorted by expert, for the two products below, which
- * take the plan of the same M, k and n_expert. A slot whose id is outside 0 .. n_expert - 1 (padding) has no expert. One
+ * take the plan of the same M, k and n_expert (one of others gives wrong results, and no access outside the arrays). A slot whose id is outside 0 .. n_expert - 1 (padding) has no expert. One
  * expert may have several of a token's slots. M * k <= DCQ_MOE_MAX_SLOTS. */
 size_t dcq_moe_plan_size(int64_t M, int k, int n_expert);
 int dcq_moe_plan(const int32_t* ids, int64_t M, int k, int n_expert, void* plan, size_t plan_size, void* stream);
 
 /* H[slot] = silu(Wg[e] x) * (Wu[e] x), silu(g) = g / (1 + e^-g), of each slot's expert e and its token's row x of X; zeros for
  * slots of no expert. Wg, Wu: rows of K, w_stride_bytes apart, experts expert_stride_bytes apart; Wgs, Wus [n_expert][N].
- * H: F32 or F16 (htype), M * k rows. M * x_stride_bytes below 4 GiB. */
+ * H: F32 or F16 (htype), M * k rows. M * x_stride_bytes below 4 GiB, N <= DCQ_MOE_MAX_N, M * k * N below 2^31. */
 int dcq_moe_gate_up_i8(const void* plan, size_t plan_size, int64_t M, int k, int n_expert, const int8_t* Wg,
                        const float* Wgs, const int8_t* Wu, const float* Wus, int64_t N, int64_t K, size_t w_stride_bytes,
                        size_t expert_stride_bytes, const int8_t* X, const float* Xs, size_t x_stride_bytes, int htype, void* H,
@@ -509,7 +510,7 @@ int dcq_moe_gate_up_i8(const void* plan, size_t plan_size, int64_t M, int k, int
 
 /* Y[m] = R[m] + sum_j weights[m][j] * (W[e] h), over the token's slots in their order, h = row m * k + j of Hq (int8, scales
  * Hs) and e its expert; slots of no expert add nothing, whatever their weight. R fp32 rows, or NULL; may be Y itself where Y is F32
- * with the same stride. M * k * h_stride_bytes below 4 GiB. */
+ * with the same stride. M * k * h_stride_bytes below 4 GiB, N and M * k * N as above. The workspace is required. */
 size_t dcq_moe_down_i8_workspace_size(int64_t M, int k, int64_t N);
 int dcq_moe_down_i8(const void* plan, size_t plan_size, int64_t M, int k, int n_expert, const int8_t* W, const float* Ws,
                     int64_t N, int64_t K, size_t w_stride_bytes, size_t expert_stride_bytes, const int8_t* Hq, const float* Hs,
