@@ -165,14 +165,6 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
             for (int j = 0; j < NJ; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[from][j], fa[from][i], acc[i][j], 0, 0, 0);
     };
-    // ---- a ring of ST stages; a wave's loads retire in order, so all but the last n stages' have landed when no more than
-    // n (LA + LB) are on their way ----
-    auto landed = [&](int behind) {
-        if (ST > 3 && behind >= 3) counted_wait<3 * (LA + LB)>();
-        else if (ST > 2 && behind >= 2) counted_wait<2 * (LA + LB)>();
-        else if (behind >= 1) counted_wait<LA + LB>();
-        else __builtin_amdgcn_s_waitcnt(0);
-    };
     // the tile's scales, on their way before the stages, and to LDS after the products
     constexpr int RT = (BM + 64 * W - 1) / (64 * W), CT = (BN + 64 * W - 1) / (64 * W);
     float rs[RT], cs[CT];
@@ -194,10 +186,18 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
         if constexpr (UP) n = i / TN * (TN / 2) + i % (TN / 2);
         cs[t] = (UP && i % TN >= TN / 2 ? a.ws2 : a.ws)[(int64_t)expert * a.N + min(n0 + n, a.N - 1)];
     }
+    // A ring of ST stages. A wave's loads retire in order: all but the last n stages' have landed when no more than n (LA + LB)
+    // are on their way.
+    if (s_end - s_begin >= ST) {
 #pragma unroll
-    for (int i = 0; i < ST; ++i)
-        if (s_begin + i < s_end) issue(s_begin + i, st[i], 0, LA + LB);
-    landed(min(ST, s_end - s_begin) - 1);
+        for (int i = 0; i < ST; ++i) issue(s_begin + i, st[i], 0, LA + LB);
+        counted_wait<(ST - 1) * (LA + LB)>();
+    } else {
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i)
+            if (s_begin + i < s_end) issue(s_begin + i, st[i], 0, LA + LB);
+        __builtin_amdgcn_s_waitcnt(0);
+    }
     clear_tail(s_begin, st[0]);
     __syncthreads();
     read(st[0], 0, 0);
@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
             multiply((q - 1) & 1);
         }
         if (s + 1 < s_end) {
-            landed(min(ST - 2, s_end - 2 - s));
+            counted_wait<(ST - 2) * (LA + LB)>();
+            if (ST > 2 && s + ST > s_end) __builtin_amdgcn_s_waitcnt(0);  // fewer stages are on their way
             clear_tail(s + 1, next);
             __syncthreads();
             read(next, 0, 0);
@@ -225,6 +226,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     // LDS (the stages' room), so that a row's columns go out in wide stores ----
     constexpr bool SUMS = sizeof(T) == 4 && T(0.5f) == T(0);  // int32_t: a plane of sums
     constexpr int OUT = UP ? TN / 2 : TN, PITCH = OUT + 4, PER = 16 / sizeof(T);  // PER: elements of a store
+    __builtin_amdgcn_s_waitcnt(0);  // every stage was waited for: this one makes that plain
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int i = tid + 64 * W * t;
