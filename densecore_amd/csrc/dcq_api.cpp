@@ -101,7 +101,6 @@ int knob(Knob k) {
         "DCQ_Q6K_NO_FUSE",  "DCQ_Q6K_FUSE_NW", "DCQ_Q8_SHAPE", "DCQ_GEMV_GENERIC", "DCQ_GEMV_LG",
         "DCQ_ATTN_NO_MFMA", "DCQ_Q6K_RPW", "DCQ_Q6K_MFMA",     "DCQ_SPLIT_K",    "DCQ_BATCH_MTI",
         "DCQ_GEMM_MT",      "DCQ_GEMM_KQ", "DCQ_I8_TILE",      "DCQ_I8_SPLIT",   "DCQ_I8_ROWS",
-        "DCQ_I8_EXPERTS",   "DCQ_I8_SHAPE",
     };
     static const std::array<int, (int)Knob::kCount> values = [] {
         std::array<int, (int)Knob::kCount> v{};

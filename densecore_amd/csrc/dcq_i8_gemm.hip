@@ -1,4 +1,22 @@
 // dcq_i8_gemm.hip — products of many int8 rows on gfx950 int8 MFMA: dense ones, and those of a plan's experts.
+//
+//   y[m][n] = (sum over k of x[m][k] w[n][k]) ws[n] xs[m] (+ R[m][n]);   experts' gate and up: silu(y_gate) y_up
+//
+// The sums are exact in 32 bits, so that tiles and splits of K are chosen by time alone and change no bit.
+//
+// Large products are bound by the matrix units and the power they draw: 32x32x32 products of random bytes held in registers
+// reach 3.5 POPS (of zeros 4.9: the clock falls with the bits that switch); with their operands through LDS 2.3, at 1.85 GHz with
+// the units busy 61 % of the time (8192 x 8192 x 8192: 479 us). Hence tiles of 256 x 256, each wave 128 x 64 of it, which read
+// the fewest LDS bytes per product (waves of 128 x 128 do not leave registers for operands read ahead: 4 % slower), and nothing
+// else next to the products: loads go straight to LDS, two stages of 128 bytes of K ahead, outputs leave through LDS in
+// 16-byte stores past the caches. Rings of 3 stages and more, stages of 64 bytes, two workgroups of half the size on a CU, raised
+// priorities and fixed orders of reads and products: within 1 % or slower.
+// Small ones are bound by the weights' bytes and by rounds of workgroups: see plan_dense.
+// Experts' products are bound by moving rows: for 1571 tokens x 8 of 128 experts the gate and up products of 768 x 2048 take 112 us,
+// of which their loads to LDS alone, without products and outputs, take 92 (402 MB of weights); the down products of 2048 x 768
+// take 80, and 75. Tiles of 64 x 128 or 128 x 128, as tall as the plan's; a run of tiles to each XCD, whose L2 then holds an
+// expert's weights while its tiles last (tiles interleaved over XCDs, weights asked for ahead of their tile, 64 x 256 and
+// 128 x 256: slower).
 #include <algorithm>
 #include <cmath>
 
@@ -96,33 +114,30 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
         }
         // within the tile's rows: offsets of 32 bits from the tile's first row
         wbase[i] = uniform(wbase[i] + (int64_t)n0 * a.w_stride);
-        b_off[i] = (uint32_t)min(n, a.N - 1 - n0) * (uint32_t)a.w_stride + 16u * (uint32_t)((lane % P) ^ piece_key<KB>(r));
+        b_off[i] = (uint32_t)min(n, a.N - 1 - n0) * (uint32_t)a.w_stride + 16u * (uint32_t)((lane % P) ^ piece_key(r));
     }
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
         const int r = LR * (LA * wave + i) + l_row;
         int src = min(r, rows_here - 1);
         if constexpr (GROUPED) src = UP ? plan_slot(order, src, a.M) / a.top : plan_slot(order, src, a.M);
-        a_off[i] = (uint32_t)src * (uint32_t)a.x_stride + 16u * (uint32_t)((lane % P) ^ piece_key<KB>(r));
+        a_off[i] = (uint32_t)src * (uint32_t)a.x_stride + 16u * (uint32_t)((lane % P) ^ piece_key(r));
     }
     const int stages = (a.K + KB - 1) / KB;
     const int s_begin = split * a.stps, s_end = min(stages, s_begin + a.stps);
     const int tail_pieces = (a.K % KB) / 16;  // 0: the last stage is whole
 
-    // loads from .. to of the wave's LA + LB
-    auto issue = [&](int s, Stage& S, int from, int to) {
+    auto issue = [&](int s, Stage& S) {  // the wave's LA + LB loads
         const bool tail = tail_pieces && s == stages - 1;
         const int64_t k0 = (int64_t)s * KB;
 #pragma unroll
         for (int i = 0; i < LA; ++i) {
-            if (i < from || i >= to) continue;
-            const uint32_t piece = (lane % P) ^ piece_key<KB>(LR * (LA * wave + i) + l_row);
+            const uint32_t piece = (lane % P) ^ piece_key(LR * (LA * wave + i) + l_row);
             dma16(xb + k0, tail && (int)piece >= tail_pieces ? a_off[i] - 16 * piece : a_off[i], S.a + 1024 * (LA * wave + i));
         }
 #pragma unroll
         for (int i = 0; i < LB; ++i) {
-            if (i + LA < from || i + LA >= to) continue;
-            const uint32_t piece = (lane % P) ^ piece_key<KB>(LR * (LB * wave + i) + l_row);
+            const uint32_t piece = (lane % P) ^ piece_key(LR * (LB * wave + i) + l_row);
             dma16(wbase[i] + k0, tail && (int)piece >= tail_pieces ? b_off[i] - 16 * piece : b_off[i],
                   S.b + 1024 * (LB * wave + i));
         }
@@ -132,7 +147,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
         if (!(tail_pieces && s == stages - 1)) return;
 #pragma unroll
         for (int i = 0; i < LA; ++i) {
-            const int piece = (lane % P) ^ piece_key<KB>(LR * (LA * wave + i) + l_row);
+            const int piece = (lane % P) ^ piece_key(LR * (LA * wave + i) + l_row);
             if (piece >= tail_pieces) *reinterpret_cast<uint4*>(S.a + 1024 * (LA * wave + i) + 16 * lane) = make_uint4(0, 0, 0, 0);
         }
     };
@@ -152,7 +167,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     // stage is whole and this one's room free for the stage after it.
     v4i fa[2][MI], fb[2][NJ];
     auto read = [&](const Stage& S, int kb, int into) {
-        const int fo = col * KB + 16 * ((2 * kb + hl) ^ piece_key<KB>(col));
+        const int fo = col * KB + 16 * ((2 * kb + hl) ^ piece_key(col));
 #pragma unroll
         for (int j = 0; j < NJ; ++j) fb[into][j] = *reinterpret_cast<const v4i*>(S.b + fo + (wn + 32 * j) * KB);
 #pragma unroll
@@ -190,12 +205,12 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     // are on their way.
     if (s_end - s_begin >= ST) {
 #pragma unroll
-        for (int i = 0; i < ST; ++i) issue(s_begin + i, st[i], 0, LA + LB);
+        for (int i = 0; i < ST; ++i) issue(s_begin + i, st[i]);
         counted_wait<(ST - 1) * (LA + LB)>();
     } else {
 #pragma unroll
         for (int i = 0; i < ST - 1; ++i)
-            if (s_begin + i < s_end) issue(s_begin + i, st[i], 0, LA + LB);
+            if (s_begin + i < s_end) issue(s_begin + i, st[i]);
         __builtin_amdgcn_s_waitcnt(0);
     }
     clear_tail(s_begin, st[0]);
@@ -217,7 +232,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
             clear_tail(s + 1, next);
             __syncthreads();
             read(next, 0, 0);
-            if (s + ST < s_end) issue(s + ST, S, 0, LA + LB);
+            if (s + ST < s_end) issue(s + ST, S);
         }
         multiply(1);
     }

@@ -32,12 +32,12 @@ __device__ __forceinline__ void wave_sums(v4i (&acc)[MT][NT], int8_t* ring, cons
         const int pieces = min(8, (K - s * KB) / 16);  // pieces past K are the row's first of the stage
 #pragma unroll
         for (int i = 0; i < LW; ++i) {
-            const int p = lane % 8 ^ piece_key<KB>(8 * i + l_row);
+            const int p = lane % 8 ^ piece_key(8 * i + l_row);
             dma16<true>(wb[i / 2] + k0, w_off[i] + (p < pieces ? 16 * p : 0), S + 1024 * i);
         }
 #pragma unroll
         for (int i = 0; i < LX; ++i) {
-            const int p = lane % 8 ^ piece_key<KB>(8 * i + l_row);
+            const int p = lane % 8 ^ piece_key(8 * i + l_row);
             dma16<true>(xb + k0, x_off[i] + (p < pieces ? 16 * p : 0), S + 1024 * (LW + i));
         }
     };
@@ -56,7 +56,7 @@ __device__ __forceinline__ void wave_sums(v4i (&acc)[MT][NT], int8_t* ring, cons
         v4i fw[NT][2], fx[MT][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int fo = r16 * KB + 16 * ((4 * u + q) ^ piece_key<KB>(r16));
+            const int fo = r16 * KB + 16 * ((4 * u + q) ^ piece_key(r16));
 #pragma unroll
             for (int j = 0; j < NT; ++j) fw[j][u] = *reinterpret_cast<const v4i*>(S + fo + j * 16 * KB);
 #pragma unroll

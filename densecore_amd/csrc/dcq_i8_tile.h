@@ -47,11 +47,8 @@ __device__ __forceinline__ const int8_t* uniform(const int8_t* p) {  // in scala
     return (const int8_t*)((uint64_t)hi << 32 | lo);
 }
 
-// LDS rows of KB bytes: piece p of 16 bytes of row r lies at p ^ key(r), so that 16 rows' pieces p are on all 64 banks.
-template <int KB>
-__device__ __forceinline__ int piece_key(int row) {
-    return KB == 128 ? (row & 7) ^ ((row >> 3) & 1) : (row >> 2) & 3;
-}
+// LDS rows of 128 bytes: piece p of 16 bytes of row r lies at p ^ key(r), so that 16 rows' pieces p are on all 64 banks.
+__device__ __forceinline__ int piece_key(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
 // 16 bytes of outputs that nothing reads soon, past the caches' usual places: products whose outputs flow through L2 lose the
 // operands there (4099 x 14336 x 4096, F16 out: 251 -> 229 us; 4096 x 14336 x 2048, F32: 164 -> 141).

@@ -64,12 +64,10 @@ enum class Knob {
     I8Tile,       // DCQ_I8_TILE: force the int8 GEMM's tile (an index into its shapes; -1: rule)
     I8Split,      // DCQ_I8_SPLIT: force its K splits (-1: rule, 1: none)
     I8Rows,       // DCQ_I8_ROWS: rows up to which the few-rows kernel serves a dense int8 product (-1: rule)
-    I8Experts,    // DCQ_I8_EXPERTS: rows of an expert, on average, up to which it serves the experts (-1: rule)
-    I8Shape,      // DCQ_I8_SHAPE: force the few-rows kernel's shape (-1: rule)
     kCount
 };
 // defaults, in Knob order: the launchers' measured rules
-constexpr int kKnobDefault[(int)Knob::kCount] = {-1, 4, 0, 0, 0, 0, -1, -1, 0, -1, 0, -1, 1, -1, -1, -1, -1, -1, -1, -1, -1, -1};
+constexpr int kKnobDefault[(int)Knob::kCount] = {-1, 4, 0, 0, 0, 0, -1, -1, 0, -1, 0, -1, 1, -1, -1, -1, -1, -1, -1, -1};
 #ifdef DCQ_TUNING
 int knob(Knob k);
 #else

@@ -351,6 +351,120 @@ def test_plan(dev, m, e, k):
     assert (plan[at:at + slots] == np.where(flat < e, flat, -1)).all()
 
 
+# ---------------------------------------------------------------- the largest sizes
+def spread_rows(a, dev, stride):
+    """int8 rows as the first columns of rows `stride` bytes apart."""
+    wide = torch.empty((len(a), stride), dtype=torch.int8, device=dev)
+    wide[:, :a.shape[1]] = gpu(a, dev)
+    return wide[:, :a.shape[1]]
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 290, 272), (40, 290, 272), (290, 9, 9728)])
+def test_rows_of_the_largest_stride(dev, m, n, k):
+    """2^24 bytes between rows: the last rows lie more than 2^32 bytes behind the first."""
+    r = rng("spread", m, n, k)
+    w, ws = i8_rows(r, n, k)
+    x, xs = i8_rows(r, m, k)
+    res = r.standard_normal((m, n)).astype(np.float32)
+    wide = torch.empty((m, 1 << 22), device=dev)
+    wide[:, :n] = gpu(res, dev)
+    args = spread_rows(w, dev, 1 << 24), gpu(ws, dev), spread_rows(x, dev, 1 << 24), gpu(xs, dev)
+    check_product(dc.mul_mat_i8(*args, r=wide[:, :n], y=wide[:, :n]), w, ws, x, xs, res)
+
+
+def test_outputs_past_32_bits(dev):
+    """Dense outputs of 5 GiB, and of experts 4.3: rows of every part of them."""
+    r = rng("outputs")
+    m, n, k = 41000, 32768, 32
+    w, ws = i8_rows(r, n, k)
+    x, xs = i8_rows(r, m, k)
+    y = dc.mul_mat_i8(gpu(w, dev), gpu(ws, dev), gpu(x, dev), gpu(xs, dev))
+    at = np.concatenate([[0, m - 1], r.integers(0, m, 60)])
+    check_product(y[torch.from_numpy(at).to(dev)], w, ws, x[at], xs[at])
+    del y
+    m, e, top, n = 8200, 8, 4, 32768
+    ids = some_ids(r, m, e, top, "mixed")
+    wg, wgs = experts(r, e, n, k)
+    wu, wus = experts(r, e, n, k)
+    plan = dc.moe_plan(gpu(ids, dev), e)
+    h = dc.moe_gate_up_i8(plan, gpu(wg, dev), gpu(wgs, dev), gpu(wu, dev), gpu(wus, dev), gpu(x[:m], dev), gpu(xs[:m], dev), top)
+    assert h.numel() * 4 > 2 ** 32
+    at = np.concatenate([[0, m - 1], r.integers(0, m, 20)])
+    got = h.view(m, top, n)[torch.from_numpy(at).to(dev)].reshape(-1, n).double().cpu().numpy()
+    ref, gate, up = I.gate_up(ids[at], e, wg, wgs, wu, wus, x[at], xs[at])
+    assert (np.abs(got - ref) <= (12.1 + 3.01 * np.abs(gate)) * U * np.abs(ref) + 1e-36 * np.abs(up)).all()
+
+
+@pytest.mark.parametrize("m", [1, 6, 60, 400])
+def test_experts_far_apart(dev, m):
+    """2^31 bytes and more between experts, 64 KiB between their rows."""
+    r = rng("far", m)
+    e, top, n, k = 4, 2, 40, 272
+    ids = some_ids(r, m, e, top, "mixed")
+    wg, wgs = experts(r, e, n, k)
+    wu, wus = experts(r, e, n, k)
+    room = torch.empty((2, e, (1 << 31) + 4096), dtype=torch.int8, device=dev)
+    far = [t[:, :n << 16].unflatten(1, (n, 1 << 16))[..., :k] for t in room]
+    for t, v in zip(far, (wg, wu)):
+        t.copy_(gpu(v, dev))
+    x, xs = i8_rows(r, m, k)
+    plan = dc.moe_plan(gpu(ids, dev), e)
+    h = dc.moe_gate_up_i8(plan, far[0], gpu(wgs, dev), far[1], gpu(wus, dev), gpu(x, dev), gpu(xs, dev), top).double().cpu().numpy()
+    ref, gate, up = I.gate_up(ids, e, wg, wgs, wu, wus, x, xs)
+    assert (np.abs(h - ref) <= (12.1 + 3.01 * np.abs(gate)) * U * np.abs(ref) + 1e-36 * np.abs(up)).all()
+    hq, hs = i8_rows(r, m * top, k)
+    weights = r.uniform(0, 1, (m, top)).astype(np.float32)
+    y = dc.moe_down_i8(plan, far[1], gpu(wus, dev), gpu(hq, dev), gpu(hs, dev), gpu(weights, dev)).double().cpu().numpy()
+    ref, size = I.down(ids, e, wu, wus, hq, hs, weights, None)
+    assert (np.abs(y - ref) <= (top + 4.1) * U * size).all()
+
+
+@pytest.mark.parametrize("m,e,k", [(1, 64, 16), (1, 64, 17), (2, 512, 64), (16, 512, 16), (3, 40, 33)])
+def test_many_experts_of_a_token(dev, m, e, k):
+    """Up to 16 slots a token are a workgroup's waves; more go by the plan."""
+    r = rng("many", m, e, k)
+    n, width = 48, 528
+    w, ws = experts(r, e, n, width)
+    h, hs = i8_rows(r, m * k, width)
+    ids = some_ids(r, m, e, k, "mixed")
+    ids[0, k // 2] = -1
+    weights = r.uniform(0, 1, (m, k)).astype(np.float32)
+    plan = dc.moe_plan(gpu(ids, dev), e)
+    y = dc.moe_down_i8(plan, gpu(w, dev), gpu(ws, dev), gpu(h, dev), gpu(hs, dev), gpu(weights, dev))
+    ref, size = I.down(ids, e, w, ws, h, hs, weights, None)
+    assert (np.abs(y.double().cpu().numpy() - ref) <= (k + 4.1) * U * size).all()
+
+
+def test_the_largest_plan_and_routing(dev):
+    """2^22 slots of 512 experts: the plan against a stable sort, the choices of sampled tokens against the oracle's."""
+    r = rng("largest")
+    m, e, k = 1 << 19, 512, 8
+    g = torch.Generator(device=dev)
+    g.manual_seed(5)
+    logits = torch.randn((m, e), generator=g, device=dev, dtype=torch.float16)
+    ids, weights = dc.moe_route(logits, k)
+    at = np.concatenate([[0, m - 1], r.integers(0, m, 500)])
+    ri, rw = I.route(logits[torch.from_numpy(at).to(dev)].cpu().numpy(), k)
+    assert (ids.cpu().numpy()[at] == ri).all() and (np.abs(weights.cpu().numpy()[at] - rw) <= 1.001 * U * rw).all()
+    plan = dc.moe_plan(ids, e).view(torch.int32)
+    flat, order_at = ids.view(-1).long(), -(-(e + 2) // 64) * 64
+    assert torch.equal(plan[order_at:order_at + m * k].long(), torch.sort(flat, stable=True).indices)
+    assert torch.equal(plan[1:e + 1].long(), torch.cumsum(torch.bincount(flat, minlength=e), 0))
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_norm_of_rows_past_32_bits(dev, half):
+    r = rng("norm rows", half)
+    m, k = 300, 2560
+    x, w = hidden(r, m, k, half), (1 + 0.3 * r.standard_normal(k)).astype(np.float32)
+    wide = torch.empty((m, (1 << 24) // x.itemsize), dtype=torch.from_numpy(x).dtype, device=dev)
+    wide[:, :k] = gpu(x, dev)
+    q = torch.empty((m, 1 << 24), dtype=torch.int8, device=dev)[:, :k]
+    _, q, s = dc.rms_norm_i8(wide[:, :k], gpu(w, dev), 1e-5, q=q)
+    _, qr, sr, _ = I.rms_norm(x, w, 1e-5)
+    assert (q.cpu().numpy() == qr).all() and (np.abs(s.cpu().numpy() - sr) <= 1.001 * U * sr).all()
+
+
 # ---------------------------------------------------------------- the calls together, and how programs make them
 def layer_inputs(dev, m, e=16, top=3, hidden=272, width=144, seed=0):
     g = torch.Generator(device=dev)
