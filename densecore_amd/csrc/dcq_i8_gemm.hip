@@ -7,16 +7,16 @@
 // Large products are bound by the matrix units and the power they draw: 32x32x32 products of random bytes held in registers
 // reach 3.5 POPS (of zeros 4.9: the clock falls with the bits that switch); with their operands through LDS 2.3, at 1.85 GHz with
 // the units busy 61 % of the time (8192 x 8192 x 8192: 479 us). Hence tiles of 256 x 256, each wave 128 x 64 of it, which read
-// the fewest LDS bytes per product (waves of 128 x 128 do not leave registers for operands read ahead: 4 % slower), and nothing
+// the fewest LDS bytes per product (waves of 128 x 128 leave no registers for operands read ahead, and are slower), and nothing
 // else next to the products: loads go straight to LDS, two stages of 128 bytes of K ahead, outputs leave through LDS in
 // 16-byte stores past the caches. Rings of 3 stages and more, stages of 64 bytes, two workgroups of half the size on a CU, raised
-// priorities and fixed orders of reads and products: within 1 % or slower.
+// priorities and fixed orders of reads and products: no faster.
 // Small ones are bound by the weights' bytes and by rounds of workgroups: see plan_dense.
-// Experts' products are bound by moving rows: for 1571 tokens x 8 of 128 experts the gate and up products of 768 x 2048 take 112 us,
-// of which their loads to LDS alone, without products and outputs, take 92 (402 MB of weights); the down products of 2048 x 768
-// take 80, and 75. Tiles of 64 x 128 or 128 x 128, as tall as the plan's; a run of tiles to each XCD, whose L2 then holds an
-// expert's weights while its tiles last (tiles interleaved over XCDs, weights asked for ahead of their tile, 64 x 256 and
-// 128 x 256: slower).
+// Experts' products are bound by moving rows: for 1571 tokens x 8 of 128 experts the gate and up products of 768 x 2048 take 111 us,
+// of which their loads to LDS alone, without products and outputs, take 92 (402 MB of weights, 39 of outputs); the down products
+// of 2048 x 768 take 71 (201 MB of weights, 103 of partial rows: 4.3 TB/s). Tiles of 64 x 128 or 128 x 128, as tall as the
+// plan's; a run of tiles to each XCD, whose L2 then holds an expert's weights while its tiles last (tiles interleaved over XCDs,
+// weights asked for ahead of their tile, 64 x 256 and 128 x 256: slower).
 #include <algorithm>
 #include <cmath>
 
@@ -408,9 +408,9 @@ hipError_t launch_join(const I8Args& a, const void* planes, hipStream_t st) {
 }  // namespace
 
 // Which tile, and into how many shares of K: the least of the times that the kernels take by their rounds of workgroups,
-// fitted to 64 products of 40 to 1536 rows x 1024 .. 14336 x 1024 .. 14336 (the
-// choice is never more than 13 % behind the best of them, and mostly the best). A round is a + b * stages us, less where half of its workgroups
-// have a CU to themselves; a split adds a launch that reads its planes.
+// fitted to 64 products of 40 to 1536 rows x 1024 .. 14336 x 1024 .. 14336 (the choice is never more than 13 % behind the
+// best of them, and mostly the best). A round is a + b * stages us, less where its workgroups have a CU to themselves; a
+// split adds a launch that reads its planes.
 struct DensePlan {
     int shape, splits;
 };

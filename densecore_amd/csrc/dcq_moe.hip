@@ -47,7 +47,9 @@ __device__ __forceinline__ double from_lane(double v, int lane) {
 // A token per wave, expert lane + 64 i in register i. Scores in 64 bits, so that what is chosen is the definition's
 // choice and not that of a rounding. The best are taken one at a time, by the upper half of their keys; the lower halves and
 // the experts' numbers decide between the few that share one.
-// 8192 tokens, 256 experts in 8 groups, best 8: VALU, which 64-bit exponentials and quotients keep busy.
+// 8192 tokens, 256 experts in 8 groups, best 8: 15.6 us, 0.5 TB/s. Bound by VALU, 842 instructions a token: 64-bit
+// exponentials and quotients, the groups' best and the choices' steps (18.4 us with the scores' winners followed through every step
+// in place of read back at the end). 5 tokens of 128 experts: 4.3 us, latency.
 constexpr int kRouteWaves = 4;
 template <class T, int EPL>
 __global__ void __launch_bounds__(64 * kRouteWaves) moe_route_kernel(RouteArgs a) {
@@ -191,39 +193,45 @@ hipError_t launch_moe_route(int type, const RouteArgs& a, hipStream_t st) {
 
 // A workgroup per expert (and one for the slots of none) looks at all slots: those of lower experts give its place, its
 // own go there in their order. No atomics and no second launch; the slots' numbers come from the caches, 16 loads of a wave
-// on their way at a time (12568 slots of 128 experts: 13.2 us with one).
+// on their way at a time. 40 slots of 128 experts 3.6 us, which is the launch and two trips to memory; 12568 slots 6.5 (13.2 with
+// one load at a time); 65536 slots of 256 experts 22, by the instructions of every workgroup's look at every slot.
 constexpr int kPlanThreads = 1024;
 __global__ void __launch_bounds__(kPlanThreads) moe_plan_kernel(const int32_t* ids, int slots, int n_expert, int32_t* plan) {
     constexpr int W = kPlanThreads / 64, G = 16;
     __shared__ int less[W], mine[W];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int me = blockIdx.x;  // n_expert: none
     int32_t* order = plan + plan_order_at(n_expert);
     int32_t* expert = plan + plan_expert_at(n_expert, slots);
     // a run of slots to each wave
     const int run = ((slots + W - 1) / W + 63) / 64 * 64, begin = min(wave * run, slots), end = min(begin + run, slots);
     int e[G];
-    auto load = [&](int at) {
+    auto load = [&](int at) {  // numbers out of range, negative ones too, are the least that is too large
+        const uint32_t none = n_expert;
+        if (at + 64 * G <= end) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const int i = at + 64 * g + lane;
-            e[g] = i < end ? ids[i] : 0x7FFFFFFF;
-        }
+            for (int g = 0; g < G; ++g) e[g] = ids[at + 64 * g + lane];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const int i = at + 64 * g + lane;
-            e[g] = i >= end ? 0x7FFFFFFF : e[g] < 0 || e[g] >= n_expert ? n_expert : e[g];
+            for (int g = 0; g < G; ++g) e[g] = (int)min((uint32_t)e[g], none);
+        } else {
+#pragma unroll
+            for (int g = 0; g < G; ++g) e[g] = ids[min(at + 64 * g + lane, end - 1)];
+#pragma unroll
+            for (int g = 0; g < G; ++g) e[g] = at + 64 * g + lane < end ? (int)min((uint32_t)e[g], none) : 0x7FFFFFFF;
         }
     };
+    const int shares = ((slots + 63) / 64 + n_expert) / (n_expert + 1);  // of the slots' experts to write, 64 at a time
+    const int share = me * shares, share_end = share + shares;
     int below = 0, same = 0;
     for (int at = begin; at < end; at += 64 * G) {
         load(at);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
+            if (at + 64 * g >= end) break;
             below += (int)__popcll(__ballot(e[g] < me));
             same += (int)__popcll(__ballot(e[g] == me));
             const int i = at + 64 * g + lane;
-            if (i < end && (at / 64 + g) % (int)gridDim.x == me) expert[i] = e[g] < n_expert ? e[g] : -1;
+            if (at / 64 + g >= share && at / 64 + g < share_end && i < end) expert[i] = e[g] < n_expert ? e[g] : -1;
         }
     }
     if (lane == 0) less[wave] = below, mine[wave] = same;
@@ -252,8 +260,11 @@ __global__ void __launch_bounds__(kPlanThreads) moe_plan_kernel(const int32_t* i
         if (run > 64 * G) load(at);  // else what the first pass left
 #pragma unroll
         for (int g = 0; g < G; ++g) {
+            if (at + 64 * g >= end) break;
             const uint64_t hit = __ballot(e[g] == me);
-            if (hit >> lane & 1) order[first + (int)__popcll(hit & ((1ull << lane) - 1))] = at + 64 * g + lane;
+            if (hit == 0) continue;
+            const int ahead = __builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
+            if (e[g] == me) order[first + ahead] = at + 64 * g + lane;
             first += (int)__popcll(hit);
         }
     }
@@ -264,6 +275,8 @@ hipError_t launch_moe_plan(const int32_t* ids, int64_t slots, int n_expert, int3
     return hipGetLastError();
 }
 
+// y[m] = (R[m] +) sum of the slots' rows by their weights, in the order of a token's slots, in fp32. A thread for V columns of a
+// token. HBM: 1571 tokens x 8 slots x 2048 and the residual, 129 MB, 25.4 us: 5.1 TB/s.
 template <class T, int V>
 __global__ void __launch_bounds__(256) moe_combine_kernel(CombineArgs a) {
     const int blocks = (a.N + 256 * V - 1) / (256 * V);

@@ -5,8 +5,9 @@
 //
 // The norm's factor cancels in q: with p = h w, exact in 64 bits, q = rint(p * (127 / max |p|)), so that no order of a sum
 // decides which step a value next to a border rounds to, and the bytes are the definition's. All of it is 64-bit
-// arithmetic, which costs nothing here: the kernel waits for memory. Sums and the largest are found in one pass over a
-// row that stays in registers, with one barrier. Largest values are compared as bit patterns, where a NaN is above
+// arithmetic, which costs nothing here: the kernel waits for memory (2048 x 4096, F16 x, fp32 r and h: 92 MB in 16.3 us, 5.7 TB/s,
+// the writes past the caches; one row of 2560: 3.2 us with its launch, latency). Sums and the largest are found in one pass
+// over a row that stays in registers, with one barrier. Largest values are compared as bit patterns, where a NaN is above
 // infinity and infinity above all else: a row that holds either has q = 0 and s = NaN, so that what is made of it shows it.
 #include "dcq_common.h"
 #include "dcq_i8.h"
@@ -67,7 +68,7 @@ __device__ __forceinline__ void load8(const _Float16* p, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = half_bits_to_float(d[i / 2] >> (16 * (i % 2)) & 0xFFFFu);
 }
-// h goes past the caches' usual places: the layer's products come before it is read again (2048 x 4096, F16 x: 23.2 -> 17.7 us).
+// h goes past the caches' usual places: the layer's products come before it is read again (2048 x 4096, F16 x: 23.2 -> 17.8 us, before the shapes below).
 __device__ __forceinline__ void store_h8(float* p, const float (&v)[8]) {
     typedef float f32x4 __attribute__((ext_vector_type(4)));
     __builtin_nontemporal_store((f32x4){v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4*>(p));
@@ -223,13 +224,13 @@ template <class T>
 hipError_t launch_norm_type(const NormArgs& a, hipStream_t st) {
     const int pieces = a.width / 8;
     const dim3 grid((unsigned)a.rows);
-    // few rows: a piece to a thread (1 x 2560 3.5 -> 3.1 us, 64 x 4096 4.0 -> 3.7); many: two, for half the barrier's waves
-    const bool few = a.rows <= 512;
+    // The narrowest workgroup that holds a row, a piece to a thread, until its barrier has more than 8 waves: then two pieces
+    // (us, 2048 rows and one: width 2048 8.98 and 2.96, by two pieces 9.69 and 3.41; 4096 16.3 and 3.29, 17.6 and 3.59; but
+    // 8192, where one piece takes 16 waves, 37.1 and 4.03, by one 44.0 and 4.46; 12288 62.9, by four pieces 68.6).
     if (pieces <= 64) norm_row_kernel<T, 64, 1><<<grid, 64, 0, st>>>(a);
+    else if (pieces <= 128) norm_row_kernel<T, 128, 1><<<grid, 128, 0, st>>>(a);
     else if (pieces <= 256) norm_row_kernel<T, 256, 1><<<grid, 256, 0, st>>>(a);
-    else if (pieces <= 512 && few) norm_row_kernel<T, 512, 1><<<grid, 512, 0, st>>>(a);
-    else if (pieces <= 512) norm_row_kernel<T, 256, 2><<<grid, 256, 0, st>>>(a);
-    else if (pieces <= 1024 && few) norm_row_kernel<T, 1024, 1><<<grid, 1024, 0, st>>>(a);
+    else if (pieces <= 512) norm_row_kernel<T, 512, 1><<<grid, 512, 0, st>>>(a);
     else if (pieces <= 1024) norm_row_kernel<T, 512, 2><<<grid, 512, 0, st>>>(a);
     else if (pieces <= 2048) norm_row_kernel<T, 1024, 2><<<grid, 1024, 0, st>>>(a);
     else norm_long_kernel<T><<<grid, 1024, 0, st>>>(a);

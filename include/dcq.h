@@ -480,8 +480,8 @@ int dcq_mul_mat_i8(const int8_t* W, const float* Ws, int64_t N, int64_t K, size_
 /* The k experts of each token, best first, and their weights. A token's scores are the softmax of its logits (F32 or F16,
  * rows stride_bytes apart) or their sigmoid, in 64 bits. The choice goes by score + bias[e] (fp32, or NULL), ties to the
  * lower expert. With n_group > 1 the experts are n_group runs of equal length, a group is worth its best choice
- * (group_best 1) or the sum of its best two (2), and only the experts of the topk_group best groups (ties to the lower) are
- * chosen from. weights are scale * score, without the bias; with renorm, divided by the sum of the k scores (all 0
+ * (group_best 1) or the sum of its best two (2), of those not ruled out, and only the experts of the topk_group best groups
+ * (ties to the lower) are chosen from. weights are scale * score, without the bias; with renorm, divided by the sum of the k scores (all 0
  * where that sum is). A logit of -infinity, or a bias that is not finite, rules an expert out; where fewer than k are
  * left, or the token's logits hold a NaN or +infinity, the rest is -1 with weight 0. n_expert <= DCQ_MOE_MAX_EXPERTS,
  * n_group <= 64, k <= 64. ids, weights [M][k]. */
@@ -495,8 +495,9 @@ int dcq_moe_route(int type, const void* logits, size_t stride_bytes, int64_t M, 
                   int32_t* ids, float* weights, void* stream);
 
 /* The tokens' slots (slot = token * k + place, its expert ids[slot]) sorted by expert, for the two products below, which
- * take the plan of the same M, k and n_expert (one of others gives wrong results, and no access outside the arrays). A slot whose id is outside 0 .. n_expert - 1 (padding) has no expert. One
- * expert may have several of a token's slots. M * k <= DCQ_MOE_MAX_SLOTS. */
+ * take the plan of the same M, k and n_expert (one of others gives wrong results, and no access outside the arrays). A slot
+ * whose id is outside 0 .. n_expert - 1 (padding) has no expert. One expert may have several of a token's slots.
+ * M * k <= DCQ_MOE_MAX_SLOTS, k <= DCQ_MOE_MAX_EXPERTS. */
 size_t dcq_moe_plan_size(int64_t M, int k, int n_expert);
 int dcq_moe_plan(const int32_t* ids, int64_t M, int k, int n_expert, void* plan, size_t plan_size, void* stream);
 
