@@ -237,9 +237,10 @@ hipError_t launch_waves(I8Args a, hipStream_t st) {
 
 // Waves by the rows of K that there are to share (us; one row / 16 rows): 8 waves on K pay where few weight rows leave CUs
 // idle (2560 x 9728: 6.1 against 6.7 with 4; 2048 x 2048 2.7 and 2.8), 4 elsewhere (9728 x 2560 6.3 against 7.0; 4096 x 4096 4.9
-// and 5.1; 151936 x 2560 62.5 and 69.9). Experts' tiles are many and short: 2 waves (5 tokens x 8 of 128, 768 x 2048 gate and up
-// 20.5 against 20.6 with 4 and 30.4 with 8; 48 tokens 57.8, 60.6, 82.3), and one for rows below 1536 (down products of
-// 2048 x 768, 48 tokens: 41.5 against 41.7 with 2 and 50.4 with 4).
+// and 5.1; 151936 x 2560 62.5 and 69.9). Experts' tiles are many, and a wave's share of K short: 1, 2 or 4 waves by K (48 tokens x 8
+// of 128, gate and up of 768 rows, with 1, 2, 4: K 256 10.1, 11.7, 16.4; 1024 33.4, 31.6, 33.2; 2048 61.9, 59.4, 57.8, with 8 79.4;
+// 4096 129.5, 114.1, 112.9; down products of 2048 rows: 512 26.9, 29.2, 40.7; 768 38.0, 38.3, 47.0; 1024 46.1, 44.7, 51.6), but two
+// for the slots of one or two tokens, whose tiles are few (8 slots, K 2048: 9.2, 8.3, 8.7; 24 slots 16.1, 13.6, 13.3).
 template <I8Mode MODE, int MT, class T>
 hipError_t launch_rows_of(const I8Args& a, hipStream_t st) {
     if constexpr (MODE == kI8Dense) {
@@ -247,7 +248,8 @@ hipError_t launch_rows_of(const I8Args& a, hipStream_t st) {
             if (a.K >= 2048 && a.N < 4096) return launch_waves<MODE, MT, 8, 1, T>(a, st);
         return a.K >= 512 ? launch_waves<MODE, MT, 4, 1, T>(a, st) : launch_waves<MODE, MT, 1, 4, T>(a, st);
     } else {
-        return MODE == kI8Up || a.K >= 1536 ? launch_waves<MODE, MT, 2, 1, T>(a, st) : launch_waves<MODE, MT, 1, 2, T>(a, st);
+        if (a.K < 1024) return launch_waves<MODE, MT, 1, 2, T>(a, st);
+        return a.K < 2048 || a.M < 16 ? launch_waves<MODE, MT, 2, 1, T>(a, st) : launch_waves<MODE, MT, 4, 1, T>(a, st);
     }
 }
 
