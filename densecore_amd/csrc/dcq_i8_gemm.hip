@@ -308,11 +308,11 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
                     float u[PER];
                     __builtin_memcpy(u, __builtin_assume_aligned(add, 4), 4 * PER);
 #pragma unroll
-                    for (int e = 0; e < PER; ++e) v[e] += u[e];
+                    for (int e = 0; e < PER; ++e) v[e] = i8_plus(v[e], u[e]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < PER; ++e)
-                        if (e < left) v[e] += add[e];
+                        if (e < left) v[e] = i8_plus(v[e], add[e]);
                 }
             }
             T o[PER];
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(256) i8_join_kernel(I8Args a, const int32_t* p
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         float y = i8_value(sum[e], a.ws[n + e], xs);
-        if (a.R) y += a.R[row * a.r_stride + n + e];
+        if (a.R) y = i8_plus(y, a.R[row * a.r_stride + n + e]);
         o[e] = (T)y;
     }
     T* y = static_cast<T*>(a.y) + row * a.y_stride + n;

@@ -94,17 +94,17 @@ __device__ __forceinline__ void weight_rows(uint32_t* w_off, int n0, int N, int6
 
 // 16 MT rows x 16 outputs to a wave (kI8Up: of 16 gate and 16 up rows). KW waves share K, an equal run of stages each, and add
 // their sums in LDS; NW such groups to a workgroup.
-template <I8Mode MODE, int MT, int KW, int NW, class T>
+template <I8Mode MODE, int MT, int NB, int KW, int NW, class T>
 __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
     constexpr bool UP = MODE == kI8Up, GROUPED = MODE != kI8Dense;
-    constexpr int NT = UP ? 2 : 1;
+    constexpr int NT = UP ? 2 : NB;
     extern __shared__ __align__(16) uint8_t smem[];
     int(*part)[KW][MT * NT * 4][64] = reinterpret_cast<int(*)[KW][MT * NT * 4][64]>(smem);  // when the stages are done
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kw = wave % KW, nw = wave / KW;
     const int tile_m = (int)blockIdx.x / a.tiles_n, tile_n = (int)blockIdx.x % a.tiles_n;
-    const int n0 = (tile_n * NW + nw) * 16;
+    const int n0 = (tile_n * NW + nw) * 16 * NB;
     int rows_here, expert = 0;
     const int32_t* order = nullptr;
     if constexpr (GROUPED) {
@@ -128,8 +128,9 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
     const int8_t* wb[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        wb[j] = uniform((j ? a.w2 : a.w) + (int64_t)expert * a.w_expert + (int64_t)min(n0, a.N - 1) * a.w_stride);
-        weight_rows(w_off + 2 * j, n0, a.N, a.w_stride);
+        const int nj = UP ? n0 : n0 + 16 * j;
+        wb[j] = uniform((UP && j ? a.w2 : a.w) + (int64_t)expert * a.w_expert + (int64_t)min(nj, a.N - 1) * a.w_stride);
+        weight_rows(w_off + 2 * j, nj, a.N, a.w_stride);
     }
     const int8_t* xb = GROUPED ? a.x : a.x + (int64_t)tile_m * 16 * MT * a.x_stride;
 #pragma unroll
@@ -138,20 +139,21 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
         if constexpr (GROUPED) src = UP ? plan_slot(order, src, a.M) / a.top : plan_slot(order, src, a.M);
         x_off[i] = (uint32_t)src * (uint32_t)a.x_stride;
     }
-    // What goes with the sums, on its way before the operands. Pieces of 64 sums, row 16 (p / 4) + 4 (lane / 16) + p % 4 of
-    // column lane % 16, are shared among the KW waves.
-    constexpr int OUT = (MT * 4 + KW - 1) / KW;
-    const int n = min(n0 + (lane & 15), a.N - 1);
-    const int64_t ns = (int64_t)expert * a.N + n;
-    const float ws = a.ws[ns], ws2 = UP ? a.ws2[ns] : 0.0f;
+    // What goes with the sums, on its way before the operands. Pieces of 64 sums, row 16 (p / (4 NB)) + 4 (lane / 16) + p % 4 of
+    // column 16 (p / 4 % NB) + lane % 16, are shared among the KW waves.
+    constexpr int PIECES = MT * NB * 4, OUT = (PIECES + KW - 1) / KW;
+    float ws[NB], ws2 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) ws[j] = a.ws[(int64_t)expert * a.N + min(n0 + 16 * j + (lane & 15), a.N - 1)];
+    if constexpr (UP) ws2 = a.ws2[(int64_t)expert * a.N + min(n0 + (lane & 15), a.N - 1)];
     float xs[OUT], add[OUT];
     int64_t row[OUT];
 #pragma unroll
     for (int t = 0; t < OUT; ++t) {
-        const int p = min(kw + KW * t, MT * 4 - 1), r = min(16 * (p / 4) + 4 * (lane >> 4) + p % 4, rows_here - 1);
+        const int p = min(kw + KW * t, PIECES - 1), r = min(16 * (p / (4 * NB)) + 4 * (lane >> 4) + p % 4, rows_here - 1);
         row[t] = GROUPED ? (int64_t)plan_slot(order, r, a.M) : (int64_t)tile_m * 16 * MT + r;
         xs[t] = a.xs[UP ? row[t] / a.top : row[t]];
-        add[t] = !GROUPED && a.R ? a.R[row[t] * a.r_stride + n] : 0.0f;
+        add[t] = !GROUPED && a.R ? a.R[row[t] * a.r_stride + min(n0 + 16 * (p / 4 % NB) + (lane & 15), a.N - 1)] : 0.0f;
     }
     const int stages = (a.K + 127) / 128;
     v4i acc[MT][NT];
@@ -170,21 +172,26 @@ __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
 #pragma unroll
     for (int t = 0; t < OUT; ++t) {
         const int p = kw + KW * t;
-        if (p >= MT * 4) continue;
+        if (p >= PIECES) continue;
+        const int i = p / (4 * NB), j = p / 4 % NB, at = (i * NT + j) * 4 + p % 4;
         int s0 = 0, s1 = 0;
         if constexpr (KW > 1) {
 #pragma unroll
             for (int q = 0; q < KW; ++q) {
-                s0 += part[nw][q][p / 4 * NT * 4 + p % 4][lane];
-                if constexpr (UP) s1 += part[nw][q][(p / 4 * NT + 1) * 4 + p % 4][lane];
+                s0 += part[nw][q][at][lane];
+                if constexpr (UP) s1 += part[nw][q][at + 4][lane];
             }
         } else {  // p is t
-            s0 = acc[t / 4][0][t % 4], s1 = acc[t / 4][NT - 1][t % 4];
+            s0 = acc[t / (4 * NB)][t / 4 % NB][t % 4], s1 = acc[t / (4 * NB)][NT - 1][t % 4];
         }
-        if (16 * (p / 4) + 4 * (lane >> 4) + p % 4 >= rows_here || n0 + (lane & 15) >= a.N) continue;
-        float y = i8_value(s0, ws, xs[t]);
+        const int n = n0 + 16 * j + (lane & 15);
+        if (16 * i + 4 * (lane >> 4) + p % 4 >= rows_here || n >= a.N) continue;
+        float scale = ws[0];
+#pragma unroll
+        for (int c = 1; c < NB; ++c) scale = j == c ? ws[c] : scale;
+        float y = i8_value(s0, scale, xs[t]);
         if constexpr (UP) y = silu(y) * i8_value(s1, ws2, xs[t]);
-        if (!GROUPED && a.R) y += add[t];
+        if (!GROUPED && a.R) y = i8_plus(y, add[t]);
         static_cast<T*>(a.y)[row[t] * a.y_stride + n] = (T)y;
     }
 }
@@ -224,13 +231,13 @@ __global__ void __launch_bounds__(1024) i8_token_kernel(I8Args a, CombineArgs c)
 
 namespace {
 
-template <I8Mode MODE, int MT, int KW, int NW, class T>
+template <I8Mode MODE, int MT, int NB, int KW, int NW, class T>
 hipError_t launch_waves(I8Args a, hipStream_t st) {
-    constexpr int NT = MODE == kI8Up ? 2 : 1;
-    a.tiles_n = (a.N + 16 * NW - 1) / (16 * NW);
+    constexpr int NT = MODE == kI8Up ? 2 : NB;
+    a.tiles_n = (a.N + 16 * NB * NW - 1) / (16 * NB * NW);
     a.tiles_m = (int)(MODE == kI8Dense ? (a.M + 16 * MT - 1) / (16 * MT) : plan_tiles(a.M, a.n_expert, 16 * MT));
     constexpr size_t lds = std::max<size_t>(KW * NW * kStages * (MT + NT) * 2048, KW * NW * MT * NT * 1024);
-    i8_rows_kernel<MODE, MT, KW, NW, T>
+    i8_rows_kernel<MODE, MT, NB, KW, NW, T>
         <<<dim3((unsigned)((int64_t)a.tiles_n * a.tiles_m)), 64 * KW * NW, lds, st>>>(a);
     return hipGetLastError();
 }
@@ -244,22 +251,48 @@ hipError_t launch_waves(I8Args a, hipStream_t st) {
 template <I8Mode MODE, int MT, class T>
 hipError_t launch_rows_of(const I8Args& a, hipStream_t st) {
     if constexpr (MODE == kI8Dense) {
-        if constexpr (MT < 4)
-            if (a.K >= 2048 && a.N < 4096) return launch_waves<MODE, MT, 8, 1, T>(a, st);
-        return a.K >= 512 ? launch_waves<MODE, MT, 4, 1, T>(a, st) : launch_waves<MODE, MT, 1, 4, T>(a, st);
+        if (a.K >= 2048 && a.N < 4096) return launch_waves<MODE, MT, 1, 8, 1, T>(a, st);
+        return a.K >= 512 ? launch_waves<MODE, MT, 1, 4, 1, T>(a, st) : launch_waves<MODE, MT, 1, 1, 4, T>(a, st);
     } else {
-        if (a.K < 1024) return launch_waves<MODE, MT, 1, 2, T>(a, st);
-        return a.K < 2048 || a.M < 16 ? launch_waves<MODE, MT, 2, 1, T>(a, st) : launch_waves<MODE, MT, 4, 1, T>(a, st);
+        if (a.K < 1024) return launch_waves<MODE, MT, 1, 1, 2, T>(a, st);
+        return a.K < 2048 || a.M < 16 ? launch_waves<MODE, MT, 1, 2, 1, T>(a, st) : launch_waves<MODE, MT, 1, 4, 1, T>(a, st);
     }
+}
+
+// 16 to 48 weight rows a wave: every workgroup takes its rows of x from L2, and more weight rows beside them are fewer such
+// trips, but also fewer workgroups. The least by rounds of a workgroup per CU, each of MT + NB pieces of operands (us, with 16,
+// 32, 48 weight rows: 32 x 9728 x 2560 10.6, 10.7, 9.3; 32 x 14336 x 4096 17.7, 15.3, 17.9; 32 x 8192 x 2048 5.7, 5.5, 6.0;
+// 61 x 9728 x 2560 14.5, 15.6, 11.5; 61 x 8192 x 2048 7.8, 7.2, 8.7; 16 x 151936 x 2560 86.5, 80.3, 80.3). Two workgroups of up to
+// 32 rows share a CU well, though (16 x 8192 x 2048 4.8 with 16 weight rows, 5.1 with 32; 17 rows 5.2 and 5.5).
+template <int MT, class T>
+hipError_t launch_columns(const I8Args& a, hipStream_t st) {
+    const int64_t tiles_m = (a.M + 16 * MT - 1) / (16 * MT);
+    int best = 1;
+    int64_t least = INT64_MAX;
+    const int most = MT <= 2 && (a.N + 15) / 16 * tiles_m <= 512 ? 1 : 3;
+    for (int nb = 1; nb <= most; ++nb) {
+        const int64_t cost = ((a.N + 16 * nb - 1) / (16 * nb) * tiles_m + 255) / 256 * (MT + nb);
+        if (cost < least) least = cost, best = nb;
+    }
+    if (best == 3) return launch_waves<kI8Dense, MT, 3, 4, 1, T>(a, st);
+    if (best == 2) return launch_waves<kI8Dense, MT, 2, 4, 1, T>(a, st);
+    return launch_waves<kI8Dense, MT, 1, 4, 1, T>(a, st);
 }
 
 template <class T>
 hipError_t launch_dense(const I8Args& a, hipStream_t st) {
-    if (a.M <= 16) return launch_rows_of<kI8Dense, 1, T>(a, st);
-    if (a.M <= 32) return launch_rows_of<kI8Dense, 2, T>(a, st);
-    // up to 64 rows to a tile; few weight rows leave CUs idle then, and pay for being read by two tiles of 32 (61 rows x
-    // 2560 x 9728: 11.1 -> 10.0 us, 2048 x 2048 4.7 -> 3.8, 1024 x 4096 6.2 -> 4.7; but 8192 x 2048 7.3 -> 8.0)
-    return a.N < 4096 ? launch_waves<kI8Dense, 2, 4, 1, T>(a, st) : launch_rows_of<kI8Dense, 4, T>(a, st);
+    const bool tall = a.N >= 4096 && a.K >= 512;
+    // (up to 8 rows HBM is what counts: 1 x 9728 x 2560 6.8, 7.7, 6.9, 8 rows 7.4, 8.3, 7.4; 1 x 151936 x 2560 63.1, 64.2, 65.4)
+    if (a.M <= 8 || (a.M <= 16 && !tall)) return launch_rows_of<kI8Dense, 1, T>(a, st);
+    if (a.M <= 16) return launch_columns<1, T>(a, st);
+    if (a.M <= 32) return tall ? launch_columns<2, T>(a, st) : launch_rows_of<kI8Dense, 2, T>(a, st);
+    if (tall) return a.M <= 48 ? launch_columns<3, T>(a, st) : launch_columns<4, T>(a, st);
+    if (a.K < 512) return launch_waves<kI8Dense, 4, 1, 1, 4, T>(a, st);
+    // Few weight rows leave CUs idle, and pay for being read by tiles of 32 rows (61 rows x 2560 x 9728: 15.4 -> 13.3 us,
+    // 2048 x 2048 4.5 -> 3.8); 8 waves then, where a CU gets no second workgroup (2048 x 2048 3.8 -> 3.6, 1024 x 4096
+    // 4.7 -> 4.3; but 2560 x 9728 13.3 -> 14.9).
+    const int64_t groups = (a.N + 15) / 16 * ((a.M + 31) / 32);
+    return groups <= 256 && a.K >= 2048 ? launch_waves<kI8Dense, 2, 1, 8, 1, T>(a, st) : launch_waves<kI8Dense, 2, 1, 4, 1, T>(a, st);
 }
 
 }  // namespace

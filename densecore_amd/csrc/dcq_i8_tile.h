@@ -61,6 +61,14 @@ __device__ __forceinline__ void store_through(void* y, const void* v16) {
 
 // y = sum * ws * xs, the weight's scale first: sum * ws is the product of the row's own unit, so that neither a small
 // ws * xs is lost nor a large one infinite where the value is not.
-__device__ __forceinline__ float i8_value(int sum, float ws, float xs) { return (float)sum * ws * xs; }
+__device__ __forceinline__ float i8_value(int sum, float ws, float xs) {
+#pragma clang fp contract(off)
+    return (float)sum * ws * xs;
+}
+// The addend, after the value's own rounding: not fused with it in one kernel and added in another.
+__device__ __forceinline__ float i8_plus(float v, float r) {
+#pragma clang fp contract(off)
+    return v + r;
+}
 
 }  // namespace dcq

@@ -131,7 +131,8 @@ def test_rms_norm_of_zeros_and_of_values_whose_squares_overflow(dev):
 
 
 # ---------------------------------------------------------------- products
-SHAPES = [(1, 1, 16), (1, 9728, 2560), (1, 33, 131056), (3, 65, 272), (5, 1000, 768), (16, 17, 4096), (17, 300, 528), (31, 2560, 1024),
+SHAPES = [(9, 4097, 512), (16, 8200, 640), (14, 9728, 560), (20, 9730, 528), (30, 14340, 528), (45, 4100, 1040), (48, 9728, 768), (48, 12000, 528),
+          (60, 8192, 656), (61, 9999, 768), (126, 4096, 512), (1, 1, 16), (1, 9728, 2560), (1, 33, 131056), (3, 65, 272), (5, 1000, 768), (16, 17, 4096), (17, 300, 528), (31, 2560, 1024),
           (33, 64, 2048), (48, 513, 1040), (61, 2560, 9728), (40, 65536, 80), (64, 129, 112), (65, 100, 256), (100, 2560, 1040), (90, 200, 5008), (128, 128, 128), (250, 64, 65536),
           (129, 257, 400), (200, 1111, 3088), (256, 2048, 2048), (300, 5000, 656), (513, 770, 144), (700, 9728, 2560),
           (1025, 4096, 2064), (2048, 8192, 2048), (4099, 1500, 272)]
@@ -183,6 +184,19 @@ def test_mul_mat_of_strided_rows_with_an_addend(dev, m, n, k, add, half):
     assert out.data_ptr() == y.data_ptr()
     check_product(out, w, ws, x, xs, res, half)
     assert (y[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("n,k", [(200, 9728), (4100, 4096), (9728, 528), (2048, 2064), (14336, 2048), (1030, 272)])
+def test_mul_mat_bits_do_not_depend_on_the_batch(dev, n, k):
+    """A row's result with a residual or a bias is the same bits whichever kernel, tile or split serves its batch."""
+    r = rng("bits", n, k)
+    w, ws = (gpu(a, dev) for a in i8_rows(r, n, k))
+    x, xs = (gpu(a, dev) for a in i8_rows(r, 700, k))
+    for add in (gpu(r.standard_normal((700, n)).astype(np.float32) * 50, dev), gpu(r.standard_normal(n).astype(np.float32) * 50, dev)):
+        whole = dc.mul_mat_i8(w, ws, x, xs, r=add)
+        for m in (1, 12, 16, 30, 40, 61, 100, 200, 400):
+            part = dc.mul_mat_i8(w, ws, x[:m], xs[:m], r=add if add.ndim == 1 else add[:m])
+            assert torch.equal(part, whole[:m]), m
 
 
 @pytest.mark.parametrize("m", [1, 40, 300])
