@@ -1,7 +1,7 @@
 // dcq_i8_rows.hip — products of few int8 rows (a decode step's, or those of an expert) on 16 x 16 int8 MFMA.
 //
 // Every weight is read once for up to 64 rows, so the time is the weights' bytes over the rate of HBM, and what is left to
-// do is to keep enough of them on their way. A wave owns 16 rows of W and a share of K; its operands come through a ring of
+// do is to keep enough of them on their way. A wave owns 16 to 48 rows of W and a share of K; its operands come through a ring of
 // two stages in LDS that no other wave touches, so that nothing waits for a barrier until the sums are added. Through LDS because
 // an operand's consecutive lanes are in 16 different rows: loaded to registers, every lane's 16 bytes are a request of their own
 // (61 rows x 2560 x 9728: 22.7 us that way, 11.0 with rows of 128 bytes to LDS, 15.2 with rows of 64; one row x 2560 x 9728:
@@ -92,7 +92,7 @@ __device__ __forceinline__ void weight_rows(uint32_t* w_off, int n0, int N, int6
 
 }  // namespace
 
-// 16 MT rows x 16 outputs to a wave (kI8Up: of 16 gate and 16 up rows). KW waves share K, an equal run of stages each, and add
+// 16 MT rows x 16 NB outputs to a wave (kI8Up: of 16 gate and 16 up rows). KW waves share K, an equal run of stages each, and add
 // their sums in LDS; NW such groups to a workgroup.
 template <I8Mode MODE, int MT, int NB, int KW, int NW, class T>
 __global__ void __launch_bounds__(64 * KW * NW) i8_rows_kernel(I8Args a) {
@@ -305,10 +305,10 @@ hipError_t launch_i8_rows(I8Mode mode, int ytype, const I8Args& a, hipStream_t s
     return launch_rows_of<kI8Down, 1, float>(a, st);
 }
 
-// Up to 64 rows, but of tall matrices the 64 x 64 tiles share the weights' and the rows' way through LDS better (20 rows x
-// 151936 x 2560: 90 us here, 78 there; 40 rows x 14336 x 4096 16.0 and 12.4; 40 x 9728 x 2560 9.9 and 9.2); and up to 128 or
-// 256 of small ones, which leave those CUs idle (100 x 4096 x 4096: 9.8 and 12.2, 256 x 2048 x 2048: 6.6 and 7.7; but 100 x
-// 2560 x 9728 16.2 and 14.8, 150 x 4096 x 4096 13.1 and 12.3).
+// Up to 64 rows, but of tall matrices the 64 x 64 tiles share the weights' and the rows' way through LDS better (17 rows x
+// 151936 x 2560: 81 us here, 78 there; 40 x 14336 x 4096 16.3 and 14.1; but 32 x 32000 x 4096 29.0 and 33.5, 40 x 11008 x 4096
+// 11.5 and 13.2, 64 x 8192 x 2048 6.6 and 7.5); and up to 128 or 256 of small ones, which leave those CUs idle (100 x 4096 x 4096:
+// 7.7 and 12.4, 256 x 2048 x 2048: 6.6 and 7.7; but 100 x 2560 x 9728 20.3 and 16.2, 150 x 4096 x 4096 13.1 and 12.3).
 bool i8_few_rows(int64_t M, int64_t N, int64_t K) {
     if (knob(Knob::I8Rows) >= 0) return M <= knob(Knob::I8Rows);
     if (M <= 64) return M <= 16 || (N < 65536 && (M <= 32 || N < 12288));

@@ -443,7 +443,7 @@ int dcq_beam_select(int type, const void* logits, size_t stride_bytes, int64_t n
  * No counterpart in the reference, whose quantized weights all have a scale for every 32 to 256 elements. Here a
  * row of int8 has one fp32 scale: element k of row r stands for q[r][k] * s[r], for weights (a row per output) and
  * for activations (a row per token). Sums over K are exact 32-bit integers, so that results do not depend on
- * how a product is split, nor from run to run. Rows of int8 are 16-byte aligned, K a multiple of 16 up to DCQ_I8_MAX_K,
+ * how a product is split, on the rows beside them, nor from run to run. Rows of int8 are 16-byte aligned, K a multiple of 16 up to DCQ_I8_MAX_K,
  * strides up to DCQ_I8_MAX_STRIDE bytes, rows up to DCQ_I8_MAX_ROWS, M * N of a product below 2^34 (DCQ_ERR_BAD_SHAPE past
  * these). No output, plan or workspace may share a byte with an input or another of them (DCQ_ERR_INVALID_ARG; rows of one
  * stride may lie between each other's), but where a call says so. Workspaces and plans are 256-byte aligned. */

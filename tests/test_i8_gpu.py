@@ -351,6 +351,28 @@ def test_down(dev, m, e, k, n, width, kind, residual, half):
     assert (y[:, n:] == 7).all()
 
 
+@pytest.mark.parametrize("e,k,n,width", [(8, 2, 130, 272), (64, 4, 70, 1040), (3, 3, 257, 2064)])
+def test_experts_bits_do_not_depend_on_the_batch(dev, e, k, n, width):
+    """A token's H rows and Y are the same bits whichever kernel and tiles serve its batch."""
+    r = rng("experts' bits", e, k, n)
+    m = 900
+    wg, wgs, wu, wus = (gpu(a, dev) for a in (*experts(r, e, n, width), *experts(r, e, n, width)))
+    wd, wds = (gpu(a, dev) for a in experts(r, e, n, width))
+    x, xs = (gpu(a, dev) for a in i8_rows(r, m, width))
+    h, hs = (gpu(a, dev) for a in i8_rows(r, m * k, width))
+    ids = gpu(some_ids(r, m, e, k, "mixed"), dev)
+    weights, res = gpu(r.uniform(0, 1, (m, k)).astype(np.float32), dev), gpu(r.standard_normal((m, n)).astype(np.float32), dev)
+
+    def both(m):
+        plan = dc.moe_plan(ids[:m], e)
+        up = dc.moe_gate_up_i8(plan, wg, wgs, wu, wus, x[:m], xs[:m], k)
+        return up, dc.moe_down_i8(plan, wd, wds, h[:m * k], hs[:m * k], weights[:m], r=res[:m])
+    whole = both(m)
+    for part in (1, 2, 8, 30, 100, 300):
+        up, down = both(part)
+        assert torch.equal(up, whole[0][:part * k]) and torch.equal(down, whole[1][:part]), part
+
+
 @pytest.mark.parametrize("m,e,k", [(1, 1, 1), (5, 128, 8), (1000, 512, 7), (4097, 60, 4), (3, 7, 2)])
 def test_plan(dev, m, e, k):
     r = rng("plan", m, e, k)
