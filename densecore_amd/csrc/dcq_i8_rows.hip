@@ -242,57 +242,60 @@ hipError_t launch_waves(I8Args a, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Waves by the rows of K that there are to share (us; one row / 16 rows): 8 waves on K pay where few weight rows leave CUs
-// idle (2560 x 9728: 6.1 against 6.7 with 4; 2048 x 2048 2.7 and 2.8), 4 elsewhere (9728 x 2560 6.3 against 7.0; 4096 x 4096 4.9
-// and 5.1; 151936 x 2560 62.5 and 69.9). Experts' tiles are many, and a wave's share of K short: 1, 2 or 4 waves by K (48 tokens x 8
-// of 128, gate and up of 768 rows, with 1, 2, 4: K 256 10.1, 11.7, 16.4; 1024 33.4, 31.6, 33.2; 2048 61.9, 59.4, 57.8, with 8 79.4;
-// 4096 129.5, 114.1, 112.9; down products of 2048 rows: 512 26.9, 29.2, 40.7; 768 38.0, 38.3, 47.0; 1024 46.1, 44.7, 51.6), but two
-// for the slots of one or two tokens, whose tiles are few (8 slots, K 2048: 9.2, 8.3, 8.7; 24 slots 16.1, 13.6, 13.3).
-template <I8Mode MODE, int MT, class T>
-hipError_t launch_rows_of(const I8Args& a, hipStream_t st) {
-    if constexpr (MODE == kI8Dense) {
-        if (a.K >= 2048 && a.N < 4096) return launch_waves<MODE, MT, 1, 8, 1, T>(a, st);
-        return a.K >= 512 ? launch_waves<MODE, MT, 1, 4, 1, T>(a, st) : launch_waves<MODE, MT, 1, 1, 4, T>(a, st);
-    } else {
-        if (a.K < 1024) return launch_waves<MODE, MT, 1, 1, 2, T>(a, st);
-        return a.K < 2048 || a.M < 16 ? launch_waves<MODE, MT, 1, 2, 1, T>(a, st) : launch_waves<MODE, MT, 1, 4, 1, T>(a, st);
-    }
+// Experts' tiles are many, and a wave's share of K short: 1, 2 or 4 waves by K (48 tokens x 8 of 128, gate and up of 768 rows, with
+// 1, 2, 4: K 256 10.1, 11.7, 16.4 us; 1024 33.4, 31.6, 33.2; 2048 61.9, 59.4, 57.8, with 8 79.4; 4096 129.5, 114.1, 112.9; down
+// products of 2048 rows: 512 26.9, 29.2, 40.7; 768 38.0, 38.3, 47.0; 1024 46.1, 44.7, 51.6), but two for the slots of one or two
+// tokens, whose tiles are few (8 slots, K 2048: 9.2, 8.3, 8.7; 24 slots 16.1, 13.6, 13.3).
+template <I8Mode MODE, class T>
+hipError_t launch_expert_rows(const I8Args& a, hipStream_t st) {
+    if (a.K < 1024) return launch_waves<MODE, 1, 1, 1, 2, T>(a, st);
+    return a.K < 2048 || a.M < 16 ? launch_waves<MODE, 1, 1, 2, 1, T>(a, st) : launch_waves<MODE, 1, 1, 4, 1, T>(a, st);
 }
 
-// 16 to 48 weight rows a wave: every workgroup takes its rows of x from L2, and more weight rows beside them are fewer such
-// trips, but also fewer workgroups. The least by rounds of a workgroup per CU, each of MT + NB pieces of operands (us, with 16,
-// 32, 48 weight rows: 32 x 9728 x 2560 10.6, 10.7, 9.3; 32 x 14336 x 4096 17.7, 15.3, 17.9; 32 x 8192 x 2048 5.7, 5.5, 6.0;
-// 61 x 9728 x 2560 14.5, 15.6, 11.5; 61 x 8192 x 2048 7.8, 7.2, 8.7; 16 x 151936 x 2560 86.5, 80.3, 80.3). Two workgroups of up to
-// 32 rows share a CU well, though (16 x 8192 x 2048 4.8 with 16 weight rows, 5.1 with 32; 17 rows 5.2 and 5.5).
 template <int MT, class T>
-hipError_t launch_columns(const I8Args& a, hipStream_t st) {
-    const int64_t tiles_m = (a.M + 16 * MT - 1) / (16 * MT);
-    int best = 1;
-    int64_t least = INT64_MAX;
-    const int most = MT <= 2 && (a.N + 15) / 16 * tiles_m <= 512 ? 1 : 3;
-    for (int nb = 1; nb <= most; ++nb) {
-        const int64_t cost = ((a.N + 16 * nb - 1) / (16 * nb) * tiles_m + 255) / 256 * (MT + nb);
-        if (cost < least) least = cost, best = nb;
+hipError_t launch_dense_rows(const I8Args& a, int nb, hipStream_t st) {
+    if (a.K < 512) return launch_waves<kI8Dense, MT, 1, 1, 4, T>(a, st);
+    if (nb == 3) return launch_waves<kI8Dense, MT, 3, 4, 1, T>(a, st);
+    if (nb == 2) return launch_waves<kI8Dense, MT, 2, 4, 1, T>(a, st);
+    // 8 waves on K where no CU has a second workgroup and K is long or CUs are idle (us, 4 and 8: 1 x 4096 x 14336 12.7 and 10.6, 24 rows
+    // 14.9 and 14.2; 1 x 2560 x 9728 9.2 and 6.9; 61 x 2048 x 2048 3.8 and 3.6; but 1 x 4096 x 4096 4.5 and 4.8)
+    if constexpr (MT <= 2) {
+        const int64_t groups = (int64_t)((a.N + 15) / 16) * ((a.M + 16 * MT - 1) / (16 * MT));
+        if (groups <= 256 && (a.K >= 8192 || (a.K >= 2048 && a.N < 4096))) return launch_waves<kI8Dense, MT, 1, 8, 1, T>(a, st);
     }
-    if (best == 3) return launch_waves<kI8Dense, MT, 3, 4, 1, T>(a, st);
-    if (best == 2) return launch_waves<kI8Dense, MT, 2, 4, 1, T>(a, st);
     return launch_waves<kI8Dense, MT, 1, 4, 1, T>(a, st);
 }
 
+// 16 mt rows and 16 nb weight rows to a wave. Every workgroup takes its rows of x from L2: more weight rows beside them are fewer
+// such trips, but also fewer workgroups. The least by rounds of a workgroup per CU, each of mt + nb pieces of operands; above 32
+// rows tiles of 32 are a choice, too (us, nb = 1, 2, 3: 32 x 9728 x 2560 10.6, 10.7, 9.3; 32 x 14336 x 4096 17.7, 15.3, 17.9;
+// 24 x 5120 x 8192 15.2, 12.2, 14.6; 61 x 9728 x 2560 14.5, 15.6, 11.5; 61 x 8192 x 2048 7.8, 7.2, 8.7; tiles of 32 for
+// 61 x 3584 x 4096 6.3 -> 6.0, 61 x 4608 x 4096 10.4 -> 8.6).
 template <class T>
 hipError_t launch_dense(const I8Args& a, hipStream_t st) {
-    const bool tall = a.N >= 4096 && a.K >= 512;
-    // (up to 8 rows HBM is what counts: 1 x 9728 x 2560 6.8, 7.7, 6.9, 8 rows 7.4, 8.3, 7.4; 1 x 151936 x 2560 63.1, 64.2, 65.4)
-    if (a.M <= 8 || (a.M <= 16 && !tall)) return launch_rows_of<kI8Dense, 1, T>(a, st);
-    if (a.M <= 16) return launch_columns<1, T>(a, st);
-    if (a.M <= 32) return tall ? launch_columns<2, T>(a, st) : launch_rows_of<kI8Dense, 2, T>(a, st);
-    if (tall) return a.M <= 48 ? launch_columns<3, T>(a, st) : launch_columns<4, T>(a, st);
-    if (a.K < 512) return launch_waves<kI8Dense, 4, 1, 1, 4, T>(a, st);
-    // Few weight rows leave CUs idle, and pay for being read by tiles of 32 rows (61 rows x 2560 x 9728: 15.4 -> 13.3 us,
-    // 2048 x 2048 4.5 -> 3.8); 8 waves then, where a CU gets no second workgroup (2048 x 2048 3.8 -> 3.6, 1024 x 4096
-    // 4.7 -> 4.3; but 2560 x 9728 13.3 -> 14.9).
-    const int64_t groups = (a.N + 15) / 16 * ((a.M + 31) / 32);
-    return groups <= 256 && a.K >= 2048 ? launch_waves<kI8Dense, 2, 1, 8, 1, T>(a, st) : launch_waves<kI8Dense, 2, 1, 4, 1, T>(a, st);
+    const int all = (int)std::min<int64_t>(4, (a.M + 15) / 16);
+    int mt = all, nb = 1;
+    int64_t least = INT64_MAX;
+    auto look = [&](int m, int most) {
+        for (int n = 1; n <= most; ++n) {
+            const int64_t groups = (a.N + 16 * n - 1) / (16 * n) * ((a.M + 16 * m - 1) / (16 * m)), cost = (groups + 255) / 256 * (m + n);
+            if (cost < least) least = cost, mt = m, nb = n;
+        }
+    };
+    // up to 8 rows HBM is what counts (1 x 9728 x 2560 6.8, 7.7, 6.9; 1 x 151936 x 2560 63.1, 64.2, 65.4), and two
+    // workgroups of up to 32 rows with a short K share a CU well (16 x 8192 x 2048 4.8, 5.1; 24 x 7168 x 2048 5.1, 5.2)
+    const bool one = a.M <= 8 || a.K < 512 || (a.M <= 32 && a.K < 4096 && a.N <= 512 * 16);
+    look(all, one ? 1 : 3);
+    if (all > 2 && a.K >= 512) {
+        // (a long K and little more than a workgroup per CU: these share their weights in L2; 61 x 2560 x 9728 13.2, nb = 2 14.1)
+        const bool shared = a.K >= 8192 && (a.N + 15) / 16 * ((a.M + 31) / 32) <= 320;
+        if (shared) least = INT64_MAX;
+        look(2, shared ? 1 : 3);
+    }
+    if (mt == 1) return launch_dense_rows<1, T>(a, nb, st);
+    if (mt == 2) return launch_dense_rows<2, T>(a, nb, st);
+    if (mt == 3) return launch_dense_rows<3, T>(a, nb, st);
+    return launch_dense_rows<4, T>(a, nb, st);
 }
 
 }  // namespace
@@ -301,8 +304,8 @@ hipError_t launch_dense(const I8Args& a, hipStream_t st) {
 hipError_t launch_i8_rows(I8Mode mode, int ytype, const I8Args& a, hipStream_t st) {
     if (mode == kI8Dense) return ytype == kTypeF16 ? launch_dense<_Float16>(a, st) : launch_dense<float>(a, st);
     if (mode == kI8Up)
-        return ytype == kTypeF16 ? launch_rows_of<kI8Up, 1, _Float16>(a, st) : launch_rows_of<kI8Up, 1, float>(a, st);
-    return launch_rows_of<kI8Down, 1, float>(a, st);
+        return ytype == kTypeF16 ? launch_expert_rows<kI8Up, _Float16>(a, st) : launch_expert_rows<kI8Up, float>(a, st);
+    return launch_expert_rows<kI8Down, float>(a, st);
 }
 
 // Up to 64 rows, but of tall matrices the 64 x 64 tiles share the weights' and the rows' way through LDS better (17 rows x
