@@ -132,7 +132,8 @@ def test_rms_norm_of_zeros_and_of_values_whose_squares_overflow(dev):
 
 # ---------------------------------------------------------------- products
 SHAPES = [(9, 4097, 512), (16, 8200, 640), (14, 9728, 560), (20, 9730, 528), (30, 14340, 528), (45, 4100, 1040), (48, 9728, 768), (48, 12000, 528),
-          (60, 8192, 656), (61, 9999, 768), (126, 4096, 512), (1, 1, 16), (1, 9728, 2560), (1, 33, 131056), (3, 65, 272), (5, 1000, 768), (16, 17, 4096), (17, 300, 528), (31, 2560, 1024),
+          (60, 8192, 656), (61, 9999, 768), (126, 4096, 512), (55, 4610, 528), (61, 3600, 528), (5, 4090, 8208), (30, 4096, 8192),
+          (37, 100, 80), (1, 1, 16), (1, 9728, 2560), (1, 33, 131056), (3, 65, 272), (5, 1000, 768), (16, 17, 4096), (17, 300, 528), (31, 2560, 1024),
           (33, 64, 2048), (48, 513, 1040), (61, 2560, 9728), (40, 65536, 80), (64, 129, 112), (65, 100, 256), (100, 2560, 1040), (90, 200, 5008), (128, 128, 128), (250, 64, 65536),
           (129, 257, 400), (200, 1111, 3088), (256, 2048, 2048), (300, 5000, 656), (513, 770, 144), (700, 9728, 2560),
           (1025, 4096, 2064), (2048, 8192, 2048), (4099, 1500, 272)]
