@@ -329,8 +329,12 @@ static hipError_t launch_experts(I8Mode mode, int ytype, const I8Args& a, hipStr
 hipError_t launch_moe_gate_up(int htype, const I8Args& a, hipStream_t st) { return launch_experts(kI8Up, htype, a, st); }
 
 hipError_t launch_moe_down(int ytype, I8Args a, const CombineArgs& c, hipStream_t st) {
-    // One token, or so few slots that hardly two share an expert: no weight is read more often for it.
-    if (c.top <= 16 && (c.rows == 1 || 2 * a.M <= a.n_expert)) {
+    // One token, or so few slots that hardly two share an expert: no weight is read more often for it. Not where one wave on K
+    // keeps too little on its way: a long K beside few slots (us, this way and by the plan with its launch of sums: one token x 8 of 128,
+    // 2048 x 768 6.1 and 9.8; x 8 of 256, 7168 x 2048 24.3 and 42.4; x 4 of 16, 4096 x 4096 14.3 and 15.9; 3 x 6 of 64, 2048 x
+    // 1408 11.5 and 13.5; but x 2 of 8, 4096 x 14336 40.1 and 29.2; x 2 of 4, 2048 x 4096 10.1 and 9.0; 5 x 8 of 128, 2048 x
+    // 768 14.8 and 13.9; 16 x 8 of 256, 7168 x 2048 296 and 223).
+    if (c.top <= 16 && a.M <= 32 && a.K <= 1280 * c.top && (c.rows == 1 || 2 * a.M <= a.n_expert)) {
         a.tiles_n = (a.N + 15) / 16;
         const dim3 grid((unsigned)(a.tiles_n * c.rows));
         const size_t lds = c.top * kStages * 4096;

@@ -299,7 +299,8 @@ EXPERTS = [(1, 8, 2, 64, 64, "mixed"), (5, 128, 8, 768, 2048, "mixed"), (1, 1, 1
            (40, 4, 2, 130, 528, "padded"), (33, 8, 4, 65, 144, "one"), (20, 512, 6, 40, 80, "mixed"), (16, 3, 3, 48, 1040, "twice"),
            (9, 8, 2, 33, 64, "none"), (64, 16, 4, 96, 256, "mixed"), (150, 4, 2, 200, 400, "padded"), (300, 2, 2, 257, 144, "mixed"),
            (513, 8, 1, 64, 128, "mixed"), (700, 60, 4, 80, 160, "padded"), (1000, 3, 2, 300, 272, "mixed"), (260, 2, 2, 128, 2064, "one"),
-           (60, 8, 4, 150, 528, "padded"), (130, 4, 1, 300, 1040, "mixed")]
+           (60, 8, 4, 150, 528, "padded"), (130, 4, 1, 300, 1040, "mixed"), (1, 8, 2, 100, 4112, "mixed"), (3, 64, 4, 70, 144, "padded"),
+           (1, 4, 1, 33, 1296, "mixed")]
 
 
 @pytest.mark.parametrize("m,e,k,n,width,kind", EXPERTS)
@@ -456,7 +457,7 @@ def test_experts_far_apart(dev, m):
     assert (np.abs(y - ref) <= (top + 4.1) * U * size).all()
 
 
-@pytest.mark.parametrize("m,e,k", [(1, 64, 16), (1, 64, 17), (2, 512, 64), (16, 512, 16), (3, 40, 33)])
+@pytest.mark.parametrize("m,e,k", [(1, 64, 16), (1, 64, 17), (2, 512, 16), (2, 512, 64), (16, 512, 16), (3, 40, 33)])
 def test_many_experts_of_a_token(dev, m, e, k):
     """Up to 16 slots a token are a workgroup's waves; more go by the plan."""
     r = rng("many", m, e, k)
