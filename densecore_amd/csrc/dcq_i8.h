@@ -52,6 +52,7 @@ struct I8Args {
     int n_expert, top;
     int tiles_n, tiles_m, splits, stps;  // from here on the launcher's
     bool y_wide;  // rows of y are of whole dwords
+    bool banded;  // experts' tiles in bands of 8 row tiles, as a dense product's are
 };
 size_t i8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 // ws: i8_workspace_bytes bytes, or null
@@ -72,13 +73,14 @@ bool i8_few_rows(int64_t M, int64_t N, int64_t K);  // whether a dense product i
 struct PlanTile {
     int expert, begin, count, unused;
 };
-// Rows of a tile: what the products' kernels take at a time, by the rows that an expert has on average (us, gate and up and down
-// products of 128 experts of 768 and 2048 rows; heights 16, 64, 128: mean 8 68.8 + 45.5, 76.2 + 46.2, 83.8 + 52.2; 12 75.7 + 51.0,
-// 80.2 + 49.6; 16 83.5 + 56.6, 81.8 + 51.7; 48 135.6 + 107.3, 86.7 + 67.9, 96.8 + 73.5; 128 -, 129.3 + 117.1, 127.9 + 120.0; 256 -,
-// 203.5 + 203.8, 190.8 + 202.9).
+// Rows of a tile: what the products' kernels take at a time, by the rows that an expert has on average (us, gate and up + down
+// products. 128 experts of 768 and 2048 rows, heights 16, 64, 128: mean 8 69 + 46, 76 + 46, 84 + 52; 16 84 + 57, 82 + 52; 48 136 + 107,
+// 87 + 68, 97 + 74. Heights 64, 128, 256: mean 128 128 + 117, 125 + 119, 145 + 125; 512 339 + 393, 314 + 389, 323 + 357; 1024 628 +
+// 773, 560 + 761, 545 + 674. 8 experts of 14336 and 4096 rows: mean 64 248 + 134, 251 + 153, 272 + 177; 128 312 + 180, 302 + 162, 332 +
+// 187; 384 634 + 364, 554 + 288, 564 + 374; 1024 1486 + 808, 1242 + 644, 1135 + 619).
 __host__ __device__ inline int plan_height(int64_t slots, int n_expert) {
     const int64_t mean = slots / n_expert;
-    return mean <= 12 ? 16 : mean <= 192 ? 64 : 128;
+    return mean <= 12 ? 16 : mean <= 144 ? 64 : mean <= 480 ? 128 : 256;
 }
 __host__ __device__ inline int64_t plan_tiles(int64_t slots, int n_expert, int height) {
     return (slots + (int64_t)(n_expert + 1) * (height - 1)) / height;

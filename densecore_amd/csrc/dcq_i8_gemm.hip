@@ -14,8 +14,8 @@
 // Small ones are bound by the weights' bytes and by rounds of workgroups: see plan_dense.
 // Experts' products are bound by moving rows: for 1571 tokens x 8 of 128 experts the gate and up products of 768 x 2048 take 111 us,
 // of which their loads to LDS alone, without products and outputs, take 92 (402 MB of weights, 39 of outputs); the down products
-// of 2048 x 768 take 71 (201 MB of weights, 103 of partial rows: 4.3 TB/s). Tiles of 64 x 128 or 128 x 128, as tall as the
-// plan's; a run of tiles to each XCD, whose L2 then holds an expert's weights while its tiles last (tiles interleaved over XCDs,
+// of 2048 x 768 take 71 (201 MB of weights, 103 of partial rows: 4.3 TB/s). Tiles of 64 x 128, 128 x 128 or 256 x 256, as
+// tall as the plan's; a run of tiles to each XCD, whose L2 then holds an expert's weights while its tiles last (tiles interleaved over XCDs,
 // weights asked for ahead of their tile, 64 x 256 and 128 x 256: slower).
 #include <algorithm>
 #include <cmath>
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
     const int xcd = id % kXcds;
     const int at = xcd * (tiles / kXcds) + min(xcd, tiles % kXcds) + id / kXcds;
     int tile_m, tile_n;
-    if constexpr (GROUPED) {
+    if (GROUPED && !a.banded) {
         tile_m = at / a.tiles_n, tile_n = at % a.tiles_n;
     } else {  // bands of 8 row tiles, so that what an XCD's CUs hold at a time is 8 x 4 tiles
         const int band = at / (8 * a.tiles_n), high = min(8, a.tiles_m - 8 * band), in = at - band * 8 * a.tiles_n;
@@ -392,6 +392,7 @@ hipError_t launch_shape(I8Args a, int shape, hipStream_t st) {
         if (shape == 3) return launch_tile<MODE, 256, 256, 2, 4, 2, T>(a, st);
     } else {
         if (shape == 1) return launch_tile<MODE, 64, 128, 2, 2, 2, T>(a, st);
+        if (shape == 3) return launch_tile<MODE, 256, 256, 2, 4, 2, T>(a, st);
     }
     return launch_tile<MODE, 128, 128, 2, 2, 2, T>(a, st);
 }
@@ -451,7 +452,11 @@ hipError_t launch_i8_gemm(I8Mode mode, int ytype, I8Args a, void* ws, hipStream_
     // wide stores need whole dwords
     a.y_wide = ytype == kTypeF32 || (a.y_stride % 2 == 0 && (uintptr_t)a.y % 4 == 0);
     if (mode != kI8Dense) {
-        const int shape = plan_height(a.M, a.n_expert) == 128 ? 2 : 1;
+        // An expert's tiles of all columns for a row tile, then the next row tile's, while its weights stay in an XCD's L2
+        // between the two; else bands (us: 4096 tokens x 8 of 128, gate and up of 768 x 2048 188 so and 209 in bands; but 4096 x 2 of 8,
+        // 14336 x 4096 1671 and 1249).
+        a.banded = (mode == kI8Up ? 2 : 1) * (int64_t)a.N * a.K > (int64_t)8 << 20;
+        const int height = plan_height(a.M, a.n_expert), shape = height == 256 ? 3 : height == 128 ? 2 : 1;
         if (mode == kI8Up)
             return ytype == kTypeF16 ? launch_shape<kI8Up, _Float16>(a, shape, st) : launch_shape<kI8Up, float>(a, shape, st);
         return launch_shape<kI8Down, float>(a, shape, st);

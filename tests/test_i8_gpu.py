@@ -300,7 +300,7 @@ EXPERTS = [(1, 8, 2, 64, 64, "mixed"), (5, 128, 8, 768, 2048, "mixed"), (1, 1, 1
            (9, 8, 2, 33, 64, "none"), (64, 16, 4, 96, 256, "mixed"), (150, 4, 2, 200, 400, "padded"), (300, 2, 2, 257, 144, "mixed"),
            (513, 8, 1, 64, 128, "mixed"), (700, 60, 4, 80, 160, "padded"), (1000, 3, 2, 300, 272, "mixed"), (260, 2, 2, 128, 2064, "one"),
            (60, 8, 4, 150, 528, "padded"), (130, 4, 1, 300, 1040, "mixed"), (1, 8, 2, 100, 4112, "mixed"), (3, 64, 4, 70, 144, "padded"),
-           (1, 4, 1, 33, 1296, "mixed")]
+           (1, 4, 1, 33, 1296, "mixed"), (900, 3, 2, 130, 272, "padded")]
 
 
 @pytest.mark.parametrize("m,e,k,n,width,kind", EXPERTS)
@@ -353,6 +353,29 @@ def test_down(dev, m, e, k, n, width, kind, residual, half):
     assert (y[:, n:] == 7).all()
 
 
+@pytest.mark.parametrize("m", [20, 150, 600, 2200])
+def test_experts_of_large_matrices(dev, m):
+    """Matrices of more than 8 MB, by tiles of every height: sampled tokens."""
+    r = rng("large experts", m)
+    e, k, n, width = 3, 2, 4100, 2064
+    wg, wgs = experts(r, e, n, width)
+    wu, wus = experts(r, e, n, width)
+    x, xs = i8_rows(r, m, width)
+    h, hs = i8_rows(r, m * k, width)
+    ids = some_ids(r, m, e, k, "mixed")
+    ids[m // 2] = -1
+    weights = r.uniform(0, 1, (m, k)).astype(np.float32)
+    plan = dc.moe_plan(gpu(ids, dev), e)
+    up = dc.moe_gate_up_i8(plan, gpu(wg, dev), gpu(wgs, dev), gpu(wu, dev), gpu(wus, dev), gpu(x, dev), gpu(xs, dev), k)
+    y = dc.moe_down_i8(plan, gpu(wg, dev), gpu(wgs, dev), gpu(h, dev), gpu(hs, dev), gpu(weights, dev))
+    at = np.concatenate([[0, m // 2, m - 1], r.integers(0, m, 20)])
+    slots = (at[:, None] * k + np.arange(k)).reshape(-1)
+    ref, gate, lin = I.gate_up(ids[at], e, wg, wgs, wu, wus, x[at], xs[at])
+    assert (np.abs(up.double().cpu().numpy()[slots] - ref) <= (12.1 + 3.01 * np.abs(gate)) * U * np.abs(ref) + 1e-36 * np.abs(lin)).all()
+    ref, size = I.down(ids[at], e, wg, wgs, h[slots], hs[slots], weights[at], None)
+    assert (np.abs(y.double().cpu().numpy()[at] - ref) <= (k + 4.1) * U * size).all()
+
+
 @pytest.mark.parametrize("e,k,n,width", [(8, 2, 130, 272), (64, 4, 70, 1040), (3, 3, 257, 2064)])
 def test_experts_bits_do_not_depend_on_the_batch(dev, e, k, n, width):
     """A token's H rows and Y are the same bits whichever kernel and tiles serve its batch."""
@@ -370,7 +393,7 @@ def test_experts_bits_do_not_depend_on_the_batch(dev, e, k, n, width):
         up = dc.moe_gate_up_i8(plan, wg, wgs, wu, wus, x[:m], xs[:m], k)
         return up, dc.moe_down_i8(plan, wd, wds, h[:m * k], hs[:m * k], weights[:m], r=res[:m])
     whole = both(m)
-    for part in (1, 2, 8, 30, 100, 300):
+    for part in (1, 2, 8, 30, 100, 300, 500):
         up, down = both(part)
         assert torch.equal(up, whole[0][:part * k]) and torch.equal(down, whole[1][:part]), part
 
