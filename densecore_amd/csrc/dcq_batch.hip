@@ -32,8 +32,7 @@
 // launch_sum_splits adds them in order.
 #include "dcq_common.h"
 #include "dcq_kernels.h"
-
-#pragma clang diagnostic ignored "-Winline-asm"  // M0 in the clobber list (see dma16)
+#include "dcq_lds_load.h"
 
 namespace dcq {
 
@@ -42,7 +41,6 @@ namespace {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 constexpr int kWaves = 8;
 // MTI m-tiles of 32 activation rows per workgroup: 2 (64 rows) in general, 1 at M <= 32
@@ -52,16 +50,6 @@ struct BGeo {
     static constexpr int kRegion = kMT * 256 + 1024;    // per-wave LDS: activation + 1 KB scales
 };
 constexpr int kNT = 32;         // weight rows per workgroup
-
-// 16 bytes per lane from global memory straight into LDS at base + 16 * lane (base
-// wave-uniform, in M0). Inline asm: the builtin form makes the compiler wait for every
-// earlier LDS-direct load before the next. The compiler does not count these loads, so
-// they are issued before the ordinary loads they must precede, and the wave waits with
-// an explicit s_waitcnt vmcnt(0) before reading the region. M0 has no other use here.
-__device__ __forceinline__ void dma16(const void* g, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(m0) : "memory", "m0");
-}
 
 __device__ __forceinline__ v16i mfma32(v4i a, v4i b, v16i c) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);

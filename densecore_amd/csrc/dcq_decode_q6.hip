@@ -28,47 +28,16 @@
 // 6-bit values are assembled with one v_bfi_b32 each from the nibble and the qh bit pair.
 #include "dcq_common.h"
 #include "dcq_kernels.h"
+#include "dcq_lds_load.h"
 
 #include <stdlib.h>
-
-#pragma clang diagnostic ignored "-Winline-asm"  // M0 in the clobber list (see dma4)
 
 namespace dcq {
 
 namespace {
 
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-
-// Direct-to-LDS loads: lane l writes base + 4*l (dword) or base + 16*l (dwordx4), base
-// wave-uniform in M0. Inline asm: the builtin form makes the compiler wait for all of them
-// (vmcnt(0)) before any later use of an ordinary load. The compiler does not count these loads;
-// the kernel waits with explicit s_waitcnt. M0 has no other use in the kernel.
-// PRIVATE: the destination is the issuing wave's own row image, read only by that wave after its
-// own counted wait, and the load may stay in flight across a workgroup barrier. The asm carries a
-// "; wave-private" comment so that the assembly scan in tests/test_isa_hazards.py exempts it from
-// the rule that a barrier must follow a wait for every earlier direct-to-LDS load.
-template <bool PRIVATE = false>
-__device__ __forceinline__ void dma4(const void* g, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    if constexpr (PRIVATE)
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off ; wave-private" ::"v"(g), "s"(m0)
-                     : "memory", "m0");
-    else
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(m0) : "memory", "m0");
-}
-// global address 16-byte aligned, base 16-byte aligned
-template <bool PRIVATE = false>
-__device__ __forceinline__ void dma16(const void* g, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    if constexpr (PRIVATE)
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off ; wave-private" ::"v"(g), "s"(m0)
-                     : "memory", "m0");
-    else
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(m0) : "memory", "m0");
-}
-
 // A 16-byte global load the compiler does not track, for loads that must sit in the same
-// in-order queue as the direct-to-LDS loads above: its value may be read only after an explicit
+// in-order queue as the direct-to-LDS loads (dma4, dma16): its value may be read only after an explicit
 // wait that covers it, followed by a sched_barrier (the compiler takes the result as ready).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x4 gload16_untracked(const void* g) {
@@ -446,15 +415,6 @@ __device__ __forceinline__ void lds_spin_until(const int* p, int v) {
     }
 }
 
-// one dword per lane from global memory (uniform base `g` + per-lane offset) into LDS at
-// lds_base + 4 * lane; the base is an SGPR pair, M0 the LDS base. Used for the waves' own tile
-// buffers only ("; wave-private", as dma4<true>).
-__device__ __forceinline__ void dma4s(const void* g, uint32_t off, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1 ; wave-private" ::"v"(off), "s"(g), "s"(m0)
-                 : "memory", "m0");
-}
-
 typedef int v16i_t __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ v16i_t mfma_32x32x16(long a, long b) {
@@ -632,11 +592,11 @@ __global__ void __launch_bounds__(64 * kTallWaves, 1) decode_q6k_mfma_kernel(
         if (rbase + 32 <= n1) {
             const uint8_t* src = W + rbase * w_row_bytes + sboff;
 #pragma unroll 8
-            for (int r = r0; r < r1; ++r) dma4s(src + r * w_row_bytes, dma_off, dst + r * kTallPitch);
+            for (int r = r0; r < r1; ++r) dma4<true>(src + r * w_row_bytes, dma_off, dst + r * kTallPitch);
         } else {
             for (int r = r0; r < r1; ++r) {
                 const int64_t row = rbase + r < n1 ? rbase + r : n1 - 1;
-                dma4s(W + row * w_row_bytes + sboff, dma_off, dst + r * kTallPitch);
+                dma4<true>(W + row * w_row_bytes + sboff, dma_off, dst + r * kTallPitch);
             }
         }
     };

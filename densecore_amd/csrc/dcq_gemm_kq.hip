@@ -35,6 +35,7 @@
 // the up waves pass their sums through LDS and the gate waves store silu(g) * u.
 #include "dcq_common.h"
 #include "dcq_kernels.h"
+#include "dcq_lds_load.h"
 
 namespace dcq {
 
@@ -45,22 +46,8 @@ typedef int v16i __attribute__((ext_vector_type(16)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef unsigned short v2us __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 enum { kQ4 = 0, kQ5 = 1, kQ6 = 2 };
-
-// 16 (4) bytes per lane from global memory (uniform base + per-lane byte offset) into LDS at
-// lds_base + 16 (4) * lane. Inline asm: the compiler's builtin form waits for every earlier LDS-direct
-// load. Not counted by the compiler, so every call precedes the ordinary loads of its superblock (loads
-// retire in order), and the superblock ends with an explicit s_waitcnt vmcnt(0) before the barrier.
-__device__ __forceinline__ void dma16(const void* g, uint32_t off, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "s"(m0) : "memory", "m0");
-}
-__device__ __forceinline__ void dma4(const void* g, uint32_t off, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(g), "s"(m0) : "memory", "m0");
-}
 
 __device__ __forceinline__ uint32_t pk_mul(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, (v2us)(__builtin_bit_cast(v2us, a) * __builtin_bit_cast(v2us, b)));

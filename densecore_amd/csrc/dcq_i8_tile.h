@@ -3,8 +3,7 @@
 
 #include "dcq_common.h"
 #include "dcq_i8.h"
-
-#pragma clang diagnostic ignored "-Winline-asm"  // M0 in the clobber list (see dma16)
+#include "dcq_lds_load.h"
 
 namespace dcq {
 
@@ -22,20 +21,6 @@ __device__ __forceinline__ int plan_slot(const int32_t* order, int at, int64_t s
     return (int)min((uint32_t)order[at], (uint32_t)slots - 1u);
 }
 
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-
-// 16 bytes per lane from a uniform base + per-lane offset to LDS at lds_base + 16 * lane (lds_base uniform, in M0). The
-// compiler does not count these loads: an explicit wait comes before what they bring is read, and before the barrier that
-// publishes it. PRIVATE: to room that only this wave reads.
-template <bool PRIVATE = false>
-__device__ __forceinline__ void dma16(const void* g, uint32_t off, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    if constexpr (PRIVATE)
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 ; wave-private" ::"v"(off), "s"(g), "s"(m0)
-                     : "memory", "m0");
-    else
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "s"(m0) : "memory", "m0");
-}
 // All but the last N loads have landed: "dcq counted wait" tells the assembly's checks so.
 template <int N>
 __device__ __forceinline__ void counted_wait() {

@@ -43,8 +43,7 @@
 // that XCD's L2) walked in m order.
 #include "dcq_common.h"
 #include "dcq_kernels.h"
-
-#pragma clang diagnostic ignored "-Winline-asm"  // M0 in the clobber list (see dma16)
+#include "dcq_lds_load.h"
 
 namespace dcq {
 
@@ -75,28 +74,6 @@ struct __align__(16) Stage {
 // r + 8 collided.
 __device__ __forceinline__ int swz_key(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 __device__ __forceinline__ int swz(int row, int slot) { return row * kRow + 16 * (slot ^ swz_key(row)); }
-
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-
-// 4 bytes per lane from global memory (uniform base `g` + per-lane byte offset `off`) into LDS at
-// lds_base + 4 * lane, as dma16 below.
-__device__ __forceinline__ void dma4(const void* g, uint32_t off, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(g), "s"(m0) : "memory", "m0");
-}
-
-// 16 bytes per lane from global memory (uniform base `g` + per-lane byte offset `off`) straight
-// into LDS at lds_base + 16 * lane (lds_base wave-uniform, in M0): global_load_lds_dwordx4 with an
-// SGPR base, so advancing a stage costs scalar adds only and no registers are held while the load
-// is in flight. Written as inline asm because the compiler's builtin form waits for every earlier
-// LDS-direct load before the next one (it cannot tell the destinations apart). The compiler does
-// not count these loads, so every call precedes the ordinary loads of the same stage (loads retire
-// in order, so its own vmcnt waits stay conservative), and the stage ends with an explicit
-// s_waitcnt vmcnt(0) before the barrier. M0 has no other use in this kernel.
-__device__ __forceinline__ void dma16(const void* g, uint32_t off, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "s"(m0) : "memory", "m0");
-}
 
 __device__ __forceinline__ v16i mfma32(v4i a, v4i b, v16i c) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);

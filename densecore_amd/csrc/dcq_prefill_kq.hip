@@ -42,8 +42,7 @@
 // contiguous band of n tiles, so its weight rows stay in that XCD's L2.
 #include "dcq_common.h"
 #include "dcq_kernels.h"
-
-#pragma clang diagnostic ignored "-Winline-asm"  // M0 in the clobber list (see dma16)
+#include "dcq_lds_load.h"
 
 namespace dcq {
 
@@ -79,19 +78,6 @@ struct __align__(16) StageQ4 {
 };
 
 __device__ __forceinline__ int swz(int row, int slot) { return row * kRow + 16 * (slot ^ (row & 7)); }
-
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-
-// 16 bytes per lane from global memory (uniform base `g` + per-lane byte offset `off`) straight
-// into LDS at lds_base + 16 * lane (lds_base wave-uniform, in M0): global_load_lds_dwordx4 with an
-// SGPR base. Inline asm: the compiler's builtin form waits for every earlier LDS-direct load before
-// the next. The compiler does not count these loads, so they are issued before the ordinary loads
-// of the same stage, and the stage ends with an explicit s_waitcnt vmcnt(0) before the barrier.
-// M0 has no other use in this kernel.
-__device__ __forceinline__ void dma16(const void* g, uint32_t off, const void* lds_base) {
-    const uint32_t m0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(g), "s"(m0) : "memory", "m0");
-}
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 

@@ -41,6 +41,7 @@
 #include "dcq_common.h"
 #include "dcq_kernels.h"
 #include "dcq_kv_row.h"
+#include "dcq_lds_load.h"
 #include "dcq_search.h"
 
 namespace dcq {
@@ -894,16 +895,6 @@ struct __align__(16) TreeBlock {
     static __device__ __forceinline__ int v_swizzle(int r) { return DMA ? (r & 3) << 1 : 0; }
 };
 
-// 16 bytes per lane from global memory (uniform base + per-lane byte offset) into LDS at lds_base + 16 lane.
-// Inline asm: the compiler's builtin form makes LDS reads of any buffer wait for it. Not counted by the compiler;
-// counted_wait below comes before the barrier that publishes the block. M0 is read one instruction after its write
-// at the earliest.
-__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, const void* lds_base) {
-    typedef __attribute__((address_space(3))) const void* LdsPtr;
-    const uint32_t m0 = (uint32_t)(uintptr_t)(LdsPtr)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0)
-                 : "memory", "m0");
-}
 // All loads but the N issued last have landed.
 template <int N>
 __device__ __forceinline__ void counted_wait() {

@@ -1,7 +1,7 @@
 """Assembly checks of the hand-scheduled kernels (CPU: hipcc cross-compiles gfx950; no GPU needed).
 
 Every kernel source that uses MFMAs or direct-to-LDS loads is compiled to gfx950 assembly with the
-library's flags, once per session, and scanned for four hazards the compiler cannot see:
+library's flags, once per session, and scanned for five hazards the compiler cannot see:
 
 1. Inline-asm VALU results read by an MFMA. The compiler inserts the wait states between a VALU
    write and an MFMA read of the written VGPR only for instructions it can see. A value built by
@@ -23,6 +23,10 @@ library's flags, once per session, and scanned for four hazards the compiler can
    operand (the operand's last use). The scan checks the forms in which it does so: the
    accumulator input C is then the inline constant 0, and a register C is either the result range
    itself or disjoint from it (never a partial overlap).
+5. M0 read too early. A direct-to-LDS load takes its LDS base from M0, and the ISA asks for one wait
+   state between a scalar write of M0 and such a load. The compiler inserts it for loads it knows;
+   an inline-asm load gets none unless its text has it. On no control-flow path may a direct-to-LDS
+   load be the next instruction after a write of M0.
 """
 import os
 import re
@@ -221,6 +225,28 @@ def mfma_overlaps(asm_text):
     return n, n_ab, bad
 
 
+def m0_hazards(asm_text):
+    """(direct-to-LDS loads, hits): a hit is a write of M0 with such a load next on some path."""
+    n, hits = 0, []
+    for f, (insts, labels) in functions(asm_text).items():
+        for i, (s, _) in enumerate(insts):
+            n += re.match(r"(global|buffer)_load_lds_", s) is not None
+            if not re.match(r"\w+\s+m0\s*,", s):
+                continue
+            seen, stack = set(), _succ(insts, labels, i)
+            while stack:
+                j = stack.pop()
+                if j in seen:
+                    continue
+                seen.add(j)
+                t = insts[j][0]
+                if t == MARK:  # a comment, which takes no issue slot
+                    stack.extend(_succ(insts, labels, j))
+                elif re.match(r"(global|buffer)_load_lds_", t):
+                    hits.append((f, s, t))
+    return n, hits
+
+
 # ---------------------------------------------------------------- the checkers on known patterns
 def test_scan_flags_the_known_pattern():
     """The checker itself: a v_bfi_b32 from inline asm read as an MFMA operand three slots later."""
@@ -293,6 +319,25 @@ def test_lds_load_scan_on_known_patterns():
     assert load_hazards(private) == (0, 1, [])
 
 
+def test_m0_scan_on_known_patterns():
+    """Planted mistakes: the load right behind the write, with nothing, a label or the marker (a comment) between them. One
+    instruction between them clears it, whichever it is, a branch to the load too."""
+    bad = _DMA
+    assert [h[2] for h in m0_hazards(bad)[1]] == ["global_load_lds_dwordx4 v[18:19], off"]
+    assert len(m0_hazards(bad.replace("s_mov_b32 m0, s43", "v_readfirstlane_b32 m0, v43"))[1]) == 1
+    assert len(m0_hazards(bad.replace("\tglobal_load_lds", "\t;dcq counted wait\n\tglobal_load_lds"))[1]) == 1
+    assert len(m0_hazards(bad.replace("\t;;#ASMSTART\n", ".LBB0_1:\n\t;;#ASMSTART\n", 1))[1]) == 1
+    for between in ("s_nop 0", "v_add_u32_e32 v1, 64, v1", "s_add_u32 s2, s2, 64"):
+        assert m0_hazards(bad.replace("\tglobal_load_lds", f"\t{between}\n\tglobal_load_lds")) == (1, [])
+    # a write at the end of a loop whose head is the load
+    loop = bad.replace("\ts_mov_b32 m0, s43\n", "\ts_mov_b32 m0, s43\n\ts_nop 0\n.LBB0_1:\n")
+    assert m0_hazards(loop) == (1, [])
+    loop = loop.replace("\ts_barrier\n", "\ts_cbranch_scc1 .LBB0_2\n\ts_mov_b32 m0, s44\n\ts_branch .LBB0_1\n.LBB0_2:\n")
+    assert m0_hazards(loop) == (1, [])  # the branch is the instruction between
+    # a read of M0 is no write
+    assert m0_hazards(bad.replace("s_mov_b32 m0, s43", "s_mov_b32 s43, m0")) == (1, [])
+
+
 def test_mfma_overlap_scan_on_known_patterns():
     ok = "\tv_mfma_i32_32x32x32_i8 v[0:15], v[32:35], v[0:3], 0\n\tv_mfma_i32_32x32x32_i8 v[0:15], v[32:35], v[36:39], v[0:15]\n"
     assert mfma_overlaps(ok) == (2, 1, [])
@@ -341,3 +386,11 @@ def test_mfma_operand_overlaps_are_of_the_checked_forms(kernel_asm):
     bad = [(f, s) for f, (_, _, b) in res.items() for s in b]
     assert not bad, f"MFMA operand overlaps outside the checked forms: {bad[:3]}"
     assert sum(n for n, _, _ in res.values()) > 0
+
+
+def test_lds_loads_wait_for_their_base(kernel_asm):
+    res = {f: m0_hazards(text) for f, text in kernel_asm.items()}
+    bad = [(f,) + h for f, (_, hits) in res.items() for h in hits]
+    assert not bad, f"{len(bad)} direct-to-LDS loads right behind a write of M0, e.g. {bad[:3]}"
+    for f in ("dcq_i8_gemm.hip", "dcq_i8_rows.hip", "dcq_tree.hip", "dcq_gemm_kq.hip"):
+        assert res[f][0] > 0, f
