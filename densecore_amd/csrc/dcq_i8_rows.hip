@@ -287,8 +287,14 @@ hipError_t launch_dense(const I8Args& a, hipStream_t st) {
     const bool one = a.M <= 8 || a.K < 512 || (a.M <= 32 && a.K < 4096 && a.N <= 512 * 16);
     look(all, one ? 1 : 3);
     if (all > 2 && a.K >= 512) {
-        // (a long K and little more than a workgroup per CU: these share their weights in L2; 61 x 2560 x 9728 13.2, nb = 2 14.1)
-        const bool shared = a.K >= 8192 && (a.N + 15) / 16 * ((a.M + 31) / 32) <= 320;
+        // Two tiles of 32 rows whose workgroups are up to a third more than CUs: the model counts the second round as a whole one, but a
+        // CU that holds two of them takes little longer. The two read their weights once between them where they are on one XCD (a multiple
+        // of 8 workgroups apart). us, so and by the model, weights from HBM: 48 x 2304 x 4096 7.0, 7.4; 61 x 2304 x 8192 11.4, 11.9; 33 x
+        // 2560 x 9728 12.3, 12.1; 48 rows 12.6, 14.1; 61 rows 13.5, 14.4; 61 x 2688 x 4096 7.6, 7.9; x 12288 16.9, 18.6. But 61 x 2816 (352
+        // workgroups) x 4096 8.7, 7.9; 48 x 2816 x 8192 13.2, 11.8; 61 x 2816 x 12288 20.6, 18.1; 36 x 2576 (322, on two XCDs) x 4096 7.4, 6.9;
+        // x 12288 16.8, 15.8. At K 2048 and 1024 (48 x 2304 5.0, 5.2; 4.1, 4.1) the model stays.
+        const int64_t weight_tiles = (a.N + 15) / 16;
+        const bool shared = a.K >= 4096 && weight_tiles % 8 == 0 && weight_tiles * ((a.M + 31) / 32) <= 336;
         if (shared) least = INT64_MAX;
         look(2, shared ? 1 : 3);
     }

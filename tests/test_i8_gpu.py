@@ -738,3 +738,20 @@ def test_example(dev):
     # int8 activations of 512 and 256 normal values: steps of about 3.2 sigma / 127, a third of one each way, so 0.8 % of a
     # value; through the norm's rows, two products, the gate and the second quantization the layer's own part is off by about 2 %
     assert all(v < 0.06 for v in example.main())
+
+
+@pytest.mark.parametrize("m", [33, 48, 49, 61, 64])
+@pytest.mark.parametrize("n,k", [(2304, 4080), (2304, 4096), (2681, 4112), (2688, 4096), (2690, 4096), (2704, 4096), (2561, 9728)])
+def test_mul_mat_around_a_third_more_workgroups_than_cus(dev, m, n, k):
+    """Two row tiles beside each other, both sides of what chooses them (N to 168 tiles of weight rows, a multiple of 8 of them,
+    K from 4096 on): the sums, and the bits of one row by itself."""
+    r = rng("a third more", m, n, k)
+    w, ws = i8_rows(r, n, k)
+    x, xs = i8_rows(r, m, k)
+    res = r.standard_normal((m, n)).astype(np.float32)
+    t = [gpu(a, dev) for a in (w, ws, x, xs, res)]
+    y = dc.mul_mat_i8(*t[:4], r=t[4])
+    check_product(y, w, ws, x, xs, res)
+    for at in (0, 31, 32, m - 1):
+        row = dc.mul_mat_i8(t[0], t[1], t[2][at:at + 1], t[3][at:at + 1], r=t[4][at:at + 1])
+        assert torch.equal(row[0], y[at]), at
