@@ -73,6 +73,18 @@ bool i8_few_rows(int64_t M, int64_t N, int64_t K);  // whether a dense product i
 struct PlanTile {
     int expert, begin, count, unused;
 };
+// What a plan of another call may hold, brought inside this call's arrays: a tile whose rows are places of the order, or -1
+// for its expert (none), and a slot.
+__host__ __device__ inline PlanTile tile_inside(PlanTile t, int n_expert, int64_t slots, int height) {
+    if (t.expert < 0 || t.expert > n_expert || t.count <= 0 || t.begin < 0 || t.begin >= slots) return {-1, 0, 0, 0};
+    const int left = (int)slots - t.begin, most = left < height ? left : height;
+    t.count = t.count < most ? t.count : most;
+    return t;
+}
+__host__ __device__ inline int slot_inside(int32_t slot, int64_t slots) {
+    const uint32_t last = (uint32_t)slots - 1u;
+    return (int)((uint32_t)slot < last ? (uint32_t)slot : last);
+}
 // Rows of a tile: what the products' kernels take at a time, by the rows that an expert has on average (us, gate and up + down
 // products. 128 experts of 768 and 2048 rows, heights 16, 64, 128: mean 8 69 + 46, 76 + 46, 84 + 52; 16 84 + 57, 82 + 52; 48 136 + 107,
 // 87 + 68, 97 + 74. Heights 64, 128, 256: mean 128 128 + 117, 125 + 119, 145 + 125; 512 339 + 393, 314 + 389, 323 + 357; 1024 628 +

@@ -10,16 +10,11 @@ namespace dcq {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
-// A plan's tile, and a place of its order. What a plan of another call holds there reaches no further than this call's arrays.
+// A plan's tile, and a place of its order.
 __device__ __forceinline__ PlanTile plan_tile(const int32_t* plan, int n_expert, int64_t slots, int at, int height) {
-    PlanTile t = reinterpret_cast<const PlanTile*>(plan + plan_tiles_at(n_expert, slots))[at];
-    if (t.expert > n_expert || t.count <= 0 || t.begin < 0 || t.begin >= slots) t.expert = -1;
-    t.count = min(min(t.count, height), (int)slots - t.begin);
-    return t;
+    return tile_inside(reinterpret_cast<const PlanTile*>(plan + plan_tiles_at(n_expert, slots))[at], n_expert, slots, height);
 }
-__device__ __forceinline__ int plan_slot(const int32_t* order, int at, int64_t slots) {
-    return (int)min((uint32_t)order[at], (uint32_t)slots - 1u);
-}
+__device__ __forceinline__ int plan_slot(const int32_t* order, int at, int64_t slots) { return slot_inside(order[at], slots); }
 
 // All but the last N loads have landed: "dcq counted wait" tells the assembly's checks so.
 template <int N>
