@@ -81,6 +81,7 @@ def main(tokens=6, prompt=200, steps=4, device="cuda"):
     x, r = (torch.randn((tokens, layer.hidden), generator=gen, device=device) for _ in range(2))
     out = torch.empty_like(r)
     stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())  # which still makes the weights and inputs
     with torch.cuda.stream(stream):
         layer.step(x, out.copy_(r))  # once before the capture
     stream.synchronize()
