@@ -2,8 +2,9 @@
 
 Random weights stand for a model's (no checkpoint is needed): what matters is the order of the calls. A layer is the
 residual's addition and norm, the router's product, the choice of experts, their gate and up products, the products'
-quantization, and the down products with the next residual; a dense layer beside it is two products with a norm. The decode step is
-captured into a graph once and replayed: every shape is the step's, and which experts a token goes to stays on the device.
+quantization, and the down products with the next residual. (A dense gate, up and down pair is the same calls with one expert: ids of
+zeros [tokens, 1], weights of 1.) The decode step is captured into a graph once and replayed: every shape is the step's, and which experts
+a token goes to stays on the device.
 
     python examples/moe_decode.py            # on a gfx950 GPU
 """

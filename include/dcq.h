@@ -503,7 +503,8 @@ int dcq_moe_plan(const int32_t* ids, int64_t M, int k, int n_expert, void* plan,
 
 /* H[slot] = silu(Wg[e] x) * (Wu[e] x), silu(g) = g / (1 + e^-g), of each slot's expert e and its token's row x of X; zeros for
  * slots of no expert. Wg, Wu: rows of K, w_stride_bytes apart, experts expert_stride_bytes apart; Wgs, Wus [n_expert][N].
- * H: F32 or F16 (htype), M * k rows. M * x_stride_bytes below 4 GiB, N <= DCQ_MOE_MAX_N, M * k * N below 2^31. */
+ * H: F32 or F16 (htype), M * k rows. A dense layer's pair is one expert: k = 1, n_expert = 1, ids of zeros (and weights of 1 for the down
+ * products, whose result then has dcq_mul_mat_i8's bits). M * x_stride_bytes below 4 GiB, N <= DCQ_MOE_MAX_N, M * k * N below 2^31. */
 int dcq_moe_gate_up_i8(const void* plan, size_t plan_size, int64_t M, int k, int n_expert, const int8_t* Wg,
                        const float* Wgs, const int8_t* Wu, const float* Wus, int64_t N, int64_t K, size_t w_stride_bytes,
                        size_t expert_stride_bytes, const int8_t* X, const float* Xs, size_t x_stride_bytes, int htype, void* H,

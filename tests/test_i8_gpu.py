@@ -755,3 +755,23 @@ def test_mul_mat_around_a_third_more_workgroups_than_cus(dev, m, n, k):
     for at in (0, 31, 32, m - 1):
         row = dc.mul_mat_i8(t[0], t[1], t[2][at:at + 1], t[3][at:at + 1], r=t[4][at:at + 1])
         assert torch.equal(row[0], y[at]), at
+
+
+@pytest.mark.parametrize("m", [1, 12, 13, 100, 300, 700])
+def test_a_dense_pair_is_one_expert(dev, m):
+    """A dense layer's gate, up and down products by the experts' calls: one expert, one slot a token, weight 1. The down product's
+    bits are mul_mat_i8's."""
+    r = rng("one expert", m)
+    n, k = 200, 528
+    (wg, wgs), (wu, wus), (wd, wds) = i8_rows(r, n, k), i8_rows(r, n, k), i8_rows(r, k, n // 16 * 16)
+    x, xs = i8_rows(r, m, k)
+    h, hs = i8_rows(r, m, n // 16 * 16)
+    res = r.standard_normal((m, k)).astype(np.float32)
+    plan = dc.moe_plan(torch.zeros((m, 1), dtype=torch.int32, device=dev), 1)
+    up = dc.moe_gate_up_i8(plan, gpu(wg, dev)[None], gpu(wgs, dev)[None], gpu(wu, dev)[None], gpu(wus, dev)[None], gpu(x, dev), gpu(xs, dev), 1)
+    gate, lin = I.mul_mat(wg, wgs, x, xs), I.mul_mat(wu, wus, x, xs)
+    ref = gate / (1 + np.exp(-gate)) * lin
+    assert (np.abs(up.double().cpu().numpy() - ref) <= (12.1 + 3.01 * np.abs(gate)) * U * np.abs(ref) + 1e-36 * np.abs(lin)).all()
+    t = [gpu(a, dev) for a in (wd, wds, h, hs)]
+    y = dc.moe_down_i8(plan, t[0][None], t[1][None], t[2], t[3], torch.ones((m, 1), device=dev), r=gpu(res, dev))
+    assert torch.equal(y, dc.mul_mat_i8(*t, r=gpu(res, dev)))
