@@ -85,11 +85,17 @@ __host__ __device__ inline int slot_inside(int32_t slot, int64_t slots) {
     const uint32_t last = (uint32_t)slots - 1u;
     return (int)((uint32_t)slot < last ? (uint32_t)slot : last);
 }
-// Rows of a tile: what the products' kernels take at a time, by the rows that an expert has on average (us, gate and up + down
-// products. 128 experts of 768 and 2048 rows, heights 16, 64, 128: mean 8 69 + 46, 76 + 46, 84 + 52; 16 84 + 57, 82 + 52; 48 136 + 107,
-// 87 + 68, 97 + 74. Heights 64, 128, 256: mean 128 128 + 117, 125 + 119, 145 + 125; 512 339 + 393, 314 + 389, 323 + 357; 1024 628 +
-// 773, 560 + 761, 545 + 674. 8 experts of 14336 and 4096 rows: mean 64 248 + 134, 251 + 153, 272 + 177; 128 312 + 180, 302 + 162, 332 +
-// 187; 384 634 + 364, 554 + 288, 564 + 374; 1024 1486 + 808, 1242 + 644, 1135 + 619).
+// Rows of a tile: what the products' kernels take at a time, by the rows that an expert has on average. A plan knows the ids and not
+// the matrices, for which the borders differ; those here lie between them (us, gate and up + down products).
+//   16, 64 rows, 128 experts of 768 x 2048: mean 8 69 + 46, 76 + 46; 16 84 + 57, 82 + 52. One expert with every token costs short tiles
+//     nothing, their weights come from L2 again (96 tokens x 8, mean 6: 70 + 45 with and without it, by 64 rows 82 + 47).
+//   64, 128 rows, gate and up and down together, means 80, 128, 160, 256: 128 experts of 768 x 2048 190, 197; 244, 244; 285, 283; 408, 393. 64 of
+//     1408 x 2048 167, 168; 215, 211; 241, 237; 338, 326. 8 of 14336 x 4096 457, 395; 504, 459; 594, 597; 752, 705. 8 of 4096 x 4096
+//     155, 147; 159, 153; 201, 207; 240, 226. 16 of 1024 x 1024 28, 30; 32, 34; 37, 40; 49, 51.
+//   128, 256 rows, means 384, 480, 576, 768, the same matrices: 552, 536; 669, 640; 785, 742; 1025, 949. 440, 442; 532, 504; 616, 582; 800, 748. 856,
+//     946; 1075, 1058; 1212, 1194; 1527, 1370. 280, 315; 339, 331; 385, 391; 480, 434. 60, 72; 78, 81; 86, 86; 104, 97.
+// Slots of no expert count in the mean, so that a batch mostly of padding has taller tiles than its tokens need (512 tokens x 8 of 128 experts of
+// 768 x 2048 of which 16, 64 or 256 are not padding, with its 64 rows 72 + 44, 87 + 55, 85 + 55; with 16 rows 69 + 37, 87 + 48, 93 + 59).
 __host__ __device__ inline int plan_height(int64_t slots, int n_expert) {
     const int64_t mean = slots / n_expert;
     return mean <= 12 ? 16 : mean <= 144 ? 64 : mean <= 480 ? 128 : 256;

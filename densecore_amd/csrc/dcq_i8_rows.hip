@@ -1,7 +1,9 @@
 // dcq_i8_rows.hip — products of few int8 rows (a decode step's, or those of an expert) on 16 x 16 int8 MFMA.
 //
-// Every weight is read once for up to 64 rows, so the time is the weights' bytes over the rate of HBM, and what is left to
-// do is to keep enough of them on their way. A wave owns 16 to 48 rows of W and a share of K; its operands come through a ring of
+// Weights are read once for a tile of 16 to 64 rows (33 to 64 rows are one such tile or two of 32, up to 256 rows of small matrices
+// four or more), so the time of few rows is the weights' bytes over the rate of HBM, and what is left to do is to keep enough of
+// them on their way; with more rows, what every workgroup takes of x from L2 counts, too (61 x 2560 x 9728: 148 MB of requests to L2, two
+// thirds of them x, for 31 MB from memory). A wave owns 16 to 48 rows of W and a share of K; its operands come through a ring of
 // two stages in LDS that no other wave touches, so that nothing waits for a barrier until the sums are added. Through LDS because
 // an operand's consecutive lanes are in 16 different rows: loaded to registers, every lane's 16 bytes are a request of their own
 // (61 rows x 2560 x 9728: 22.7 us that way, 11.0 with rows of 128 bytes to LDS, 15.2 with rows of 64; one row x 2560 x 9728:

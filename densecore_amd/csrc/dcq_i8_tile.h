@@ -30,8 +30,9 @@ __device__ __forceinline__ const int8_t* uniform(const int8_t* p) {  // in scala
 // LDS rows of 128 bytes: piece p of 16 bytes of row r lies at p ^ key(r), so that 16 rows' pieces p are on all 64 banks.
 __device__ __forceinline__ int piece_key(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
-// 16 bytes of outputs that nothing reads soon, past the caches' usual places: products whose outputs flow through L2 lose the
-// operands there (4099 x 14336 x 4096, F16 out: 251 -> 229 us; 4096 x 14336 x 2048, F32: 164 -> 141).
+// 16 bytes of outputs past the caches' usual places: products whose outputs flow through L2 lose the operands there
+// (4099 x 14336 x 4096, F16 out: 251 -> 229 us; 4096 x 14336 x 2048, F32: 164 -> 141). Down products' rows of slots and the planes of
+// split products go this way, too, though the next launch reads them.
 __device__ __forceinline__ void store_through(void* y, const void* v16) {
     typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
     i32x4 v;
@@ -40,7 +41,8 @@ __device__ __forceinline__ void store_through(void* y, const void* v16) {
 }
 
 // y = sum * ws * xs, the weight's scale first: sum * ws is the product of the row's own unit, so that neither a small
-// ws * xs is lost nor a large one infinite where the value is not.
+// ws * xs is lost nor a large one infinite, as long as sum * ws itself is within fp32's normal range (always for ws from 2^-126 to
+// 2^96, as |sum| < 2^31).
 __device__ __forceinline__ float i8_value(int sum, float ws, float xs) {
 #pragma clang fp contract(off)
     return (float)sum * ws * xs;

@@ -61,7 +61,7 @@ enum class Knob {
     BatchTile,    // DCQ_BATCH_MTI: force the Q4_K batch kernel's 32-row m-tiles per workgroup (1 or 2)
     GemmMt,       // DCQ_GEMM_MT: force the K-quant GEMM's 32-row m-tiles per workgroup (1, 2, 4; -1: rule)
     GemmKq,       // DCQ_GEMM_KQ: 0 keeps K-quant products off the GEMM kernel, 1 forces them on it (-1: rule)
-    I8Tile,       // DCQ_I8_TILE: force the int8 GEMM's tile (an index into its shapes; -1: rule)
+    I8Tile,       // DCQ_I8_TILE: force the dense int8 GEMM's tile (0: 64 x 64, 2: 128 x 128, 3: 256 x 256; -1: rule)
     I8Split,      // DCQ_I8_SPLIT: force its K splits (-1: rule, 1: none)
     I8Rows,       // DCQ_I8_ROWS: rows up to which the few-rows kernel serves a dense int8 product (-1: rule)
     kCount

@@ -5,7 +5,7 @@
 //
 // The norm's factor cancels in q: with p = h w, exact in 64 bits, q = rint(p * (127 / max |p|)), so that no order of a sum
 // decides which step a value next to a border rounds to, and the bytes are the definition's. All of it is 64-bit
-// arithmetic, which costs nothing here: the kernel waits for memory (2048 x 4096, F16 x, fp32 r and h: 92 MB in 16.3 us, 5.7 TB/s,
+// arithmetic, beside the loads (VALU busy 62 %): the kernel waits for memory (2048 x 4096, F16 x, fp32 r and h: 92 MB in 16.3 us, 5.7 TB/s,
 // the writes past the caches; one row of 2560: 3.2 us with its launch, latency). Sums and the largest are found in one pass
 // over a row that stays in registers, with one barrier. Largest values are compared as bit patterns, where a NaN is above
 // infinity and infinity above all else: a row that holds either has q = 0 and s = NaN, so that what is made of it shows it.
