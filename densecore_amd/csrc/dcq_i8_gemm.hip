@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
 #pragma unroll
         for (int i = 0; i < ST - 1; ++i)
             if (s_begin + i < s_end) issue(s_begin + i, st[i]);
-        __builtin_amdgcn_s_waitcnt(0);
+        counted_wait<0>();
     }
     clear_tail(s_begin, st[0]);
     __syncthreads();
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) i8_gemm_kernel(I8Args a) {
         }
         if (s + 1 < s_end) {
             counted_wait<(ST - 2) * (LA + LB)>();
-            if (ST > 2 && s + ST > s_end) __builtin_amdgcn_s_waitcnt(0);  // fewer stages are on their way
+            if (ST > 2 && s + ST > s_end) counted_wait<0>();  // fewer stages are on their way
             clear_tail(s + 1, next);
             __syncthreads();
             read(next, 0, 0);

@@ -53,7 +53,7 @@ __device__ __forceinline__ void wave_sums(v4i (&acc)[MT][NT], int8_t* ring, cons
     const int r16 = lane & 15, q = lane >> 4;
     for (int s = begin, at = 0; s < end; ++s) {
         if (s + 1 < end) counted_wait<L>();  // a wave's loads retire in order: all but the next stage's
-        else __builtin_amdgcn_s_waitcnt(0);
+        else counted_wait<0>();
         const int8_t* S = ring + at * (1024 * L);
         v4i fw[NT][2], fx[MT][2];
 #pragma unroll

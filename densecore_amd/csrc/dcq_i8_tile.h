@@ -16,7 +16,8 @@ __device__ __forceinline__ PlanTile plan_tile(const int32_t* plan, int n_expert,
 }
 __device__ __forceinline__ int plan_slot(const int32_t* order, int at, int64_t slots) { return slot_inside(order[at], slots); }
 
-// All but the last N loads have landed: "dcq counted wait" tells the assembly's checks so.
+// All but the last N loads have landed: "dcq counted wait" tells the assembly's checks so. The clobber keeps the compiler's LDS reads
+// and writes of what has landed behind it, which the builtin wait, as it touches no memory, does not promise.
 template <int N>
 __device__ __forceinline__ void counted_wait() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\t;dcq counted wait" ::"n"(N) : "memory");
